@@ -425,6 +425,52 @@ tb_status tb_probe_mfma(int kind, int64_t blocks, int64_t iters, float* out, hip
  */
 tb_status tb_probe_clock(int64_t blocks, int64_t iters, uint64_t* clocks, float* sink, hipStream_t stream);
 
+/*
+ * Rotary positions with several axes (text: one; images: height and width;
+ * video: time, height and width).
+ *   angle[t, i] = positions[axes[i], t] * inv_freq[i], i = 0 .. R/2 - 1, in 64 bits
+ *   (a, b) -> (a cos - b sin, b cos + a sin) in fp32, rounded once,
+ * for the pairs (x[i], x[i + R/2]) of every head, or (x[2i], x[2i + 1]) when
+ * `interleaved`; channels R .. D - 1 are copied.  `inverse` negates the angles:
+ * the gradient of the rotation.
+ *   q [T, Hq, D], k [T, Hk, D] (dtype 0 = fp32, 1 = fp16, 2 = bf16) at element
+ *   strides st (token) and sh (head), the last dimension contiguous; outputs
+ *   dense.  Hk = 0: no k.  positions int32 [A, T], inv_freq fp32 [R/2], axes
+ *   int32 [R/2] (clamped to 0 .. A - 1; may be null when A = 1).
+ * Requires D even and at most 512, R even and at most D, A at most 8.  T = 0
+ * does nothing.  The outputs must not overlap the inputs.  No counterpart in
+ * the reference's quantised operators.
+ */
+tb_status tb_rotary_axes(const void* q, void* q_out, const void* k, void* k_out, const int32_t* positions,
+                         const float* inv_freq, const int32_t* axes, int64_t T, int64_t Hq, int64_t Hk, int64_t D,
+                         int64_t R, int64_t A, int64_t q_st, int64_t q_sh, int64_t k_st, int64_t k_sh, int dtype,
+                         int interleaved, int inverse, hipStream_t stream);
+
+/*
+ * Appending to a paged key/value cache, the rotation above applied to q and k
+ * on the way.
+ *   k and v of token t go to slot slots[t]: row slots[t] % page_size of page
+ *   slots[t] / page_size of pools [pages, Hkv, page_size, D] at element strides
+ *   c_page, c_head, c_slot (the same for both pools).  Slots outside
+ *   [0, pages * page_size) write nothing; a slot named twice in one call holds
+ *   an unspecified mix of both tokens.  q' goes to q_out, dense [T, Hq, D].
+ *   dtype 1 = fp16, 2 = bf16; cache_dtype the same, or 3: e4m3 codes of
+ *   x / s with s = absmax / 448 over the fp32 row (rotated, not rounded
+ *   before), s in k_scale / v_scale fp32 [pages, Hkv, page_size] at strides
+ *   s_page, s_head, s_slot.  A zero row has s = 0 and zero codes; a row with
+ *   inf or NaN reads back as NaN.
+ * Requires page_size a power of two up to 4096, pages * page_size < 2^31, and
+ * what tb_rotary_axes requires.  Cache offsets are 64-bit.  No counterpart in
+ * the reference's quantised operators.
+ */
+tb_status tb_rope_kv_append(const void* q, const void* k, const void* v, void* q_out, const int32_t* positions,
+                            const float* inv_freq, const int32_t* axes, const int32_t* slots, void* k_cache,
+                            void* v_cache, float* k_scale, float* v_scale, int64_t T, int64_t Hq, int64_t Hkv,
+                            int64_t D, int64_t R, int64_t A, int64_t q_st, int64_t q_sh, int64_t k_st, int64_t k_sh,
+                            int64_t v_st, int64_t v_sh, int64_t pages, int64_t page_size, int64_t c_page,
+                            int64_t c_head, int64_t c_slot, int64_t s_page, int64_t s_head, int64_t s_slot, int dtype,
+                            int cache_dtype, int interleaved, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

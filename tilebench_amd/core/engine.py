@@ -24,7 +24,7 @@ from tilebench_amd.core.timer import DEFAULT_REPEAT, DEFAULT_WARMUP, report_benc
 from tilebench_amd.core.verifier import config_per_output, config_tolerance, verify
 from tilebench_amd.data.tensors import expand_cases, get_generator, infer_problem_size
 from tilebench_amd.hardware import detect_arch
-from tilebench_amd.paths import operator_config
+from tilebench_amd.paths import operator_config, operator_package
 
 HAS_CUDA = torch.cuda.is_available()
 DEFAULT_ENABLED_BACKENDS = BACKEND_ORDER
@@ -54,7 +54,7 @@ def _device_of(inputs):
 def _import_impl(operator_name: str, backend: str):
     """The backend's module, or None (with the reason printed) when it cannot load."""
     try:
-        return importlib.import_module(f"tilebench_amd.benchmarks.operators.{operator_name}.impl_{backend}")
+        return importlib.import_module(f"{operator_package(operator_name)}.impl_{backend}")
     except ImportError as e:
         print(f"  {backend} import skipped: {e}")
         return None
@@ -81,7 +81,7 @@ def run_benchmark_suite(operator_name, benchmark_overrides=None, enabled_backend
         config = yaml.safe_load(f)
     enabled = set(DEFAULT_ENABLED_BACKENDS if enabled_backends is None else enabled_backends)
 
-    impl_torch = importlib.import_module(f"tilebench_amd.benchmarks.operators.{operator_name}.impl_torch")
+    impl_torch = importlib.import_module(f"{operator_package(operator_name)}.impl_torch")
     impls = {}
     for b in BACKEND_ORDER:
         if b in enabled:

@@ -342,6 +342,56 @@ def generate_matmul_fp32_fp16_fp8_inputs(M, N, K, dtype=torch.float32, seed=14, 
     return (a.to(device), b.to(device))
 
 
+# ----------------------------------------------------------------------------- attention path
+
+
+def rotary_frequencies(R: int, axes: int, theta: float):
+    """Inverse frequencies of R / 2 pairs and the axis each follows (runs of about equal size)."""
+    i = torch.arange(R // 2, dtype=torch.float64)
+    return (theta ** (-2.0 * i / R)).float(), (torch.arange(R // 2) * axes // (R // 2)).int()
+
+
+def _rotary_positions(T, axes, g):
+    """Text counts up from anywhere; further axes walk the rows of a grid of 60 x 80."""
+    t = torch.arange(T) + int(torch.randint(0, 30000, (1,), generator=g)) * (axes == 1)
+    return torch.stack([t // 4800, t // 80 % 60, t % 80][-axes:] if axes > 1 else [t]).int()
+
+
+def _fused_heads(T, counts, D, dtype, g, device):
+    """Heads as a fused projection leaves them: views of one [T, heads * D] matrix."""
+    fused = torch.randn(T, sum(counts) * D, generator=g).to(dtype).to(device)
+    return [x.view(T, n, D) for n, x in zip(counts, fused.split([n * D for n in counts], dim=1))]
+
+
+def generate_rotary_axes_inputs(T, axes=1, Hq=32, Hk=8, D=128, dtype=torch.float16, seed=0, device=DEFAULT_DEVICE):
+    g = _gen(seed)
+    q, k, _ = _fused_heads(T, [Hq, Hk, Hk], D, dtype, g, device)
+    inv_freq, ax = rotary_frequencies(D, axes, 10000.0)
+    return q, k, _rotary_positions(T, axes, g).to(device), inv_freq.to(device), ax.to(device)
+
+
+def paged_cache(pages, heads, page, D, dtype, g, e4m3=False, device=DEFAULT_DEVICE):
+    """k and v pools [pages, heads, page, D] full of N(0, 1) values; e4m3 codes and their scales if asked for."""
+    pools = [torch.randn(pages, heads, page, D, generator=g).to(dtype) for _ in range(2)]
+    if not e4m3:
+        return [x.to(device) for x in pools]
+    scales = [x.abs().amax(dim=-1).float() / 448.0 for x in pools]
+    pools = [(x.float() / s[..., None]).to(torch.float8_e4m3fn) for x, s in zip(pools, scales)]
+    return [x.to(device) for x in pools + scales]
+
+
+def generate_rope_kv_append_inputs(T, axes=1, Hq=32, Hkv=8, D=128, page=64, cache="same", dtype=torch.float16, seed=0,
+                                   device=DEFAULT_DEVICE):
+    g = _gen(seed)
+    q, k, v = _fused_heads(T, [Hq, Hkv, Hkv], D, dtype, g, device)
+    inv_freq, ax = rotary_frequencies(D, axes, 500000.0)
+    positions = _rotary_positions(T, axes, g)
+    pages = -(-T // page) + 4
+    slots = torch.randperm(pages * page, generator=g)[:T].int()
+    pools = paged_cache(pages, Hkv, page, D, dtype, g, cache == "e4m3", device)
+    return (q, k, v, positions.to(device), inv_freq.to(device), ax.to(device), slots.to(device), *pools)
+
+
 GENERATORS = {
     "int4_dequant": generate_int4_dequant_inputs,
     "w4a16_gemm": generate_w4a16_gemm_inputs,
@@ -357,6 +407,8 @@ GENERATORS = {
     "fused_moe_w4a16": generate_fused_moe_w4a16_inputs,
     "fp8_act_quant_blocks": generate_fp8_act_quant_blocks_inputs,
     "fp8_block_scaled_gemm": generate_fp8_block_scaled_gemm_inputs,
+    "rotary_axes": generate_rotary_axes_inputs,
+    "rope_kv_append": generate_rope_kv_append_inputs,
 }
 
 
@@ -386,6 +438,10 @@ def infer_problem_size(operator_name, params):
         return 2 * p.get("tokens", 1) * p.get("topk", 1) * p.get("K", 1) * p.get("N", 1)
     if operator_name == "fused_moe_w4a16":
         return 6 * p.get("tokens", 1) * p.get("topk", 1) * p.get("H", 1) * p.get("I", 1)
+    if operator_name == "rotary_axes":
+        return p.get("T", 1) * (p.get("Hq", 1) + p.get("Hk", 0)) * p.get("D", 1)
+    if operator_name == "rope_kv_append":
+        return p.get("T", 1) * (p.get("Hq", 1) + 2 * p.get("Hkv", 1)) * p.get("D", 1)
     size, used = 1, False
     for v in p.values():
         size *= max(1, v)

@@ -12,13 +12,21 @@ PACKAGE_ROOT = Path(__file__).resolve().parent
 DATA_ROOT = PACKAGE_ROOT / "data"
 BENCHMARK_ROOT = PACKAGE_ROOT / "benchmarks"
 OPERATOR_ROOT = BENCHMARK_ROOT / "operators"
+#: operators of the attention path, which read and write a key/value cache that the caller keeps
+SERVING_ROOT = BENCHMARK_ROOT / "serving"
 PEAK_PERFORMANCE_ROOT = DATA_ROOT / "peak_performance"
 REPO_ROOT = Path(os.environ.get("TILEBENCH_REPO_ROOT") or PACKAGE_ROOT.parent).resolve()
 RESULTS_ROOT = REPO_ROOT / "results"
 
 
 def operator_dir(operator_name: str) -> Path:
-    return OPERATOR_ROOT / operator_name
+    serving = SERVING_ROOT / operator_name
+    return serving if serving.is_dir() else OPERATOR_ROOT / operator_name
+
+
+def operator_package(operator_name: str) -> str:
+    """The package that holds the operator's impl_<backend> modules."""
+    return f"tilebench_amd.benchmarks.{operator_dir(operator_name).parent.name}.{operator_name}"
 
 
 def operator_config(operator_name: str) -> Path:
@@ -30,3 +38,7 @@ def operator_config(operator_name: str) -> Path:
 
 def list_operators() -> list[str]:
     return sorted(p.parent.name for p in OPERATOR_ROOT.glob("*/config.yaml"))
+
+
+def list_serving_operators() -> list[str]:
+    return sorted(p.parent.name for p in SERVING_ROOT.glob("*/config.yaml"))

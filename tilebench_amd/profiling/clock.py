@@ -83,12 +83,12 @@ def operator_part(rt, torch, operator: str, rounds: int = 6) -> list[str]:
     from tilebench_amd.core import timer
     from tilebench_amd.core.dtypes import resolve_dtype
     from tilebench_amd.data.tensors import get_generator
-    from tilebench_amd.paths import operator_config
+    from tilebench_amd.paths import operator_config, operator_package
 
     cfg = yaml.safe_load(open(operator_config(operator)))
     params = dict(cfg.get("case_defaults") or {})
     dtype = params.pop("dtype", None) or (cfg.get("case_grid") or {}).get("dtype", ["fp16"])[0]
-    impl = importlib.import_module(f"tilebench_amd.benchmarks.operators.{operator}.impl_hip")
+    impl = importlib.import_module(f"{operator_package(operator)}.impl_hip")
     x = get_generator(operator)(**params, dtype=resolve_dtype(dtype))
     for _ in range(2):
         impl.run(*x)

@@ -39,7 +39,7 @@ import yaml
 
 from tilebench_amd.core.dtypes import resolve_dtype
 from tilebench_amd.data.tensors import expand_cases, get_generator, infer_problem_size
-from tilebench_amd.paths import list_operators, operator_config
+from tilebench_amd.paths import list_operators, operator_config, operator_package
 from tilebench_amd.profiling import kernels as kn
 
 
@@ -81,7 +81,7 @@ def probe_case(impl, op: str, case: dict) -> dict:
 
 
 def probe_operator(op: str, all_cases: bool = False) -> list[dict]:
-    impl = importlib.import_module(f"tilebench_amd.benchmarks.operators.{op}.impl_hip")
+    impl = importlib.import_module(f"{operator_package(op)}.impl_hip")
     with open(operator_config(op)) as fh:
         cfg = yaml.safe_load(fh)
     cases = expand_cases(op, cfg)

@@ -21,6 +21,7 @@ import torch
 from tilebench_amd.profiling.probe import _run_kwargs
 from tilebench_amd.core.dtypes import resolve_dtype
 from tilebench_amd.data.tensors import get_generator
+from tilebench_amd.paths import operator_package
 
 
 def main(argv=None) -> int:
@@ -29,7 +30,7 @@ def main(argv=None) -> int:
         print("usage: workload.py OPERATOR CASE_JSON", file=sys.stderr)
         return 2
     op, case = argv[0], json.loads(argv[1])
-    impl = importlib.import_module(f"tilebench_amd.benchmarks.operators.{op}.impl_hip")
+    impl = importlib.import_module(f"{operator_package(op)}.impl_hip")
     params = {k: v for k, v in case.items() if k not in ("dtype", "block_size")}
     inputs = get_generator(op)(**params, dtype=resolve_dtype(case.get("dtype", "fp32")))
     if not isinstance(inputs, tuple):
