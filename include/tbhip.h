@@ -471,6 +471,48 @@ tb_status tb_rope_kv_append(const void* q, const void* k, const void* v, void* q
                             int64_t c_head, int64_t c_slot, int64_t s_page, int64_t s_head, int64_t s_slot, int dtype,
                             int cache_dtype, int interleaved, hipStream_t stream);
 
+/*
+ * Paged attention of a batch whose sequences share prefixes by groups; a
+ * prefix is read once for all rows of its group (128 at a time).
+ *   q [T, Hq, D] (dtype 1 = fp16, 2 = bf16) at strides q_st, q_sh: the queries of
+ *   sequence b are rows cu_q[b] .. cu_q[b + 1] - 1 (cu_q int32 [B + 1], at most
+ *   max_q of a sequence).  Sequence b's tokens are the prefix of its group, then
+ *   lens[b] own tokens; its queries are the last ones, query i of n_q seeing
+ *   the tokens up to position prefix + lens[b] - n_q + i.
+ *   Caches [n_pages, Hkv, page_size, D] as tb_rope_kv_append writes them; own
+ *   tokens are on pages[b, :] (int32 [B, W]), prefixes on prefix_pages[g, :]
+ *   (int32 [G, Wp]) with prefix_lens int32 [G]; group g holds sequences
+ *   group_offsets[g] .. group_offsets[g + 1] - 1 (int32 [G + 1], ascending, the
+ *   first taken as 0, the last as B).  G = Wp = 0: no prefixes, the three may be
+ *   null.
+ *   out [T, Hq, D] dense = softmax(scale * q k) v, lse fp32 [T, Hq] the natural
+ *   logarithm of the sum.  Rows that see no token, and rows of no sequence, give
+ *   0 and -inf.  Sums are fp32; the weights are rounded to `dtype` before the
+ *   product with the values.
+ * Lengths, offsets and page ids are read on the device and clamped to the
+ * tables and the pool, so malformed ones never address memory outside them.
+ * Needs the workspace reported by tb_shared_prefix_attention_workspace_size
+ * (16-byte aligned, no clearing, not shared by calls that overlap).
+ * Requires D 64 or 128, Hq a multiple of Hkv, page_size a power of two up to
+ * 4096, 16-byte aligned q, caches and out, cache strides in multiples of 16
+ * bytes, q strides in multiples of 8.  No counterpart in the reference's
+ * quantised operators.
+ */
+tb_status tb_shared_prefix_attention(const void* q, const void* k_cache, const void* v_cache, const float* k_scale,
+                                     const float* v_scale, const int32_t* prefix_pages, const int32_t* prefix_lens,
+                                     const int32_t* group_offsets, const int32_t* pages, const int32_t* lens,
+                                     const int32_t* cu_q, void* out, float* lse, int64_t T, int64_t Hq, int64_t Hkv,
+                                     int64_t D, int64_t G, int64_t Wp, int64_t B, int64_t W, int64_t max_q,
+                                     int64_t n_pages, int64_t page_size, int64_t q_st, int64_t q_sh, int64_t c_page,
+                                     int64_t c_head, int64_t c_slot, int64_t s_page, int64_t s_head, int64_t s_slot,
+                                     double scale, int dtype, int cache_dtype, void* workspace,
+                                     int64_t workspace_bytes, hipStream_t stream);
+
+/* Workspace bytes tb_shared_prefix_attention needs for these sizes (0 if none). */
+tb_status tb_shared_prefix_attention_workspace_size(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t G,
+                                                    int64_t Wp, int64_t B, int64_t W, int64_t page_size,
+                                                    int64_t max_q, int64_t* bytes);
+
 #ifdef __cplusplus
 }
 #endif

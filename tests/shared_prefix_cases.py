@@ -1,0 +1,72 @@
+"""Inputs of shared-prefix attention for the tests, and the bounds their results are held to."""
+import torch
+
+from tilebench_amd.benchmarks.serving.shared_prefix_attention import impl_torch
+from tilebench_amd.data.tensors import paged_cache
+
+
+def make(n_q, lens, prefix=(), bounds=(), Hq=8, Hkv=2, D=64, page=16, cache="same", dtype=torch.float16, seed=0, pad=0,
+         spare=0, q_scale=1.0):
+    """CPU inputs in run's order.  pad: rows after the last sequence; spare: unused entries of every page table
+    (which hold ids far outside the pool)."""
+    g = torch.Generator().manual_seed(seed)
+    n_q, lens, prefix = list(n_q), list(lens), list(prefix)
+    need = [-(-n // page) for n in prefix], [-(-n // page) for n in lens]
+    total = max(sum(need[0]) + sum(need[1]), 1)
+    order = torch.randperm(total, generator=g).int()
+    pools = paged_cache(total, Hkv, page, D, dtype, g, cache == "e4m3", "cpu")
+    tables, at = [], 0
+    for counts in need:
+        t = torch.full((len(counts), max(counts + [1]) + spare), 1 << 30, dtype=torch.int32)
+        for i, n in enumerate(counts):
+            t[i, :n] = order[at:at + n]
+            at += n
+        tables.append(t)
+    cu = torch.tensor([sum(n_q[:i]) for i in range(len(n_q) + 1)], dtype=torch.int32)
+    T = int(cu[-1]) + pad
+    q = (torch.randn(T, Hq, D, generator=g) * q_scale).to(dtype)
+    shared = (None, None, None)
+    if prefix:
+        shared = tables[0], torch.tensor(prefix).int(), torch.tensor(list(bounds) or [0, len(n_q)]).int()
+    return [q, pools[0], pools[1], *shared, tables[1], torch.tensor(lens).int(), cu, max(n_q + [0]), None, *pools[2:]]
+
+
+def reference(x):
+    """out, lse and the weighted mean of |v|, in fp64 on the CPU."""
+    out, lse = impl_torch.run(*x, dtype=torch.float64)
+    y = list(x)
+    y[2] = (y[2].view(torch.uint8) & 0x7F).view(y[2].dtype) if y[2].element_size() == 1 else y[2].abs()
+    return out, lse, impl_torch.run(*y, dtype=torch.float64)[0]
+
+
+def check(got, x, ref=None):
+    """Results against fp64.  A weight is rounded to the type (u, half a step) and so is the output; scores are sums
+    of D products in fp32 (D + 8 roundings of sum |q k|), exp2 and the sum over n tokens add n + 16 more;
+    fp16 weights below the normals add 2^-33 of the largest each, with e4m3 values 2^-29 of a code (448 at most)."""
+    q, kc = x[0], x[1]
+    out, lse = got[0].detach().cpu().double(), got[1].detach().cpu().double()
+    want, want_lse, mean = ref if ref is not None else reference(x)
+    u = 2.0 ** -11 if q.dtype == torch.float16 else 2.0 ** -8
+    n = x[6].shape[1] * kc.shape[2] + (x[3].shape[1] * kc.shape[2] if x[3] is not None else 0)
+    D = q.shape[2]
+    k = kc.float()
+    if len(x) > 11:
+        k = k * x[11][..., None]
+    k = torch.where(k.isfinite(), k, torch.zeros_like(k))
+    qk = float(q.float().nan_to_num(0, 0, 0).norm(dim=-1).max()) * float(k.norm(dim=-1).max())
+    e = 2.0 ** -24 * ((D + 8) * qk * (x[10] or D ** -0.5) + n + 16)
+    small = 0.0
+    if q.dtype == torch.float16:
+        small = n * 2.0 ** -29 * 448 if len(x) > 11 else n * 2.0 ** -33 * float(x[2].float().nan_to_num(0, 0, 0).abs().max())
+    bound = 1.01 * (u * (want.abs() + mean) + 2 * e * mean) + small + 2.0 ** -25
+    finite = want.isfinite()
+    assert torch.equal(out.isnan(), want.isnan()), "NaN in other places"
+    assert torch.equal(out[~finite & ~want.isnan()], want[~finite & ~want.isnan()]), "infinities differ"
+    err = (out - want).abs()[finite]
+    over = err - torch.where(mean.isfinite(), bound, torch.full_like(bound, float("inf")))[finite]
+    assert over.numel() == 0 or float(over.max()) <= 0, f"off by {float(err.max())}, over the bound by {float(over.max())}"
+    some = want_lse.isfinite()
+    assert torch.equal(lse[~some & ~want_lse.isnan()], want_lse[~some & ~want_lse.isnan()])
+    assert torch.equal(lse.isnan(), want_lse.isnan())
+    worst = (lse - want_lse).abs()[some] - (2 * e + 2.0 ** -22 * (1 + want_lse.abs()[some]))
+    assert worst.numel() == 0 or float(worst.max()) <= 0, f"lse over the bound by {float(worst.max())}"

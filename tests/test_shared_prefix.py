@@ -1,0 +1,130 @@
+"""Shared-prefix attention on the host: the torch reference against the formula row
+by row, and what the operator refuses before any device is touched."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+from tests.shared_prefix_cases import make, reference
+from tilebench_amd import runtime as rt
+
+
+def by_row(x):
+    """Every row by itself from the formula, fp64."""
+    q, kc, vc, pp, pl, go, pages, lens, cu, max_q, scale = x[:11]
+    ks, vs = (x[11], x[12]) if len(x) > 11 else (None, None)
+    T, Hq, D = q.shape
+    N, Hkv, P, _ = kc.shape
+    out, lse = torch.zeros(T, Hq, D, dtype=torch.float64), torch.full((T, Hq), -math.inf, dtype=torch.float64)
+
+    def token(c, s, ids, j, h):
+        page = min(max(int(ids[j // P]), 0), N - 1)
+        v = c[page, h, j % P].double()
+        return v if s is None else v * float(s[page, h, j % P])
+
+    for b in range(len(lens)):
+        g = 0 if pp is None else max(i for i in range(pp.shape[0]) if int(go[i]) <= b)
+        n = 0 if pp is None else int(pl[g])
+        n_q, own = int(cu[b + 1] - cu[b]), int(lens[b])
+        for i in range(n_q):
+            see = [(pp[g], j) for j in range(n)] + [(pages[b], j) for j in range(own)]
+            see = see[:max(n + own - n_q + i + 1, 0)]
+            for hq in range(Hq):
+                h = hq // (Hq // Hkv)
+                if not see:
+                    continue
+                qq = q[int(cu[b]) + i, hq].double()
+                s = torch.stack([token(kc, ks, ids, j, h) @ qq for ids, j in see]) * (D ** -0.5 if scale is None else scale)
+                v = torch.stack([token(vc, vs, ids, j, h) for ids, j in see])
+                out[int(cu[b]) + i, hq] = torch.softmax(s, dim=0) @ v
+                lse[int(cu[b]) + i, hq] = torch.logsumexp(s, dim=0)
+    return out, lse
+
+
+@pytest.mark.parametrize("kw", [
+    dict(n_q=[1, 1, 1], lens=[3, 17, 1]),
+    dict(n_q=[1, 2, 0, 5], lens=[3, 9, 4, 5], prefix=[7, 0], bounds=[0, 2, 4], page=4, pad=2, spare=1),
+    dict(n_q=[3, 1], lens=[1, 0], prefix=[1], page=2, cache="e4m3", dtype=torch.bfloat16),   # queries before the tokens
+    dict(n_q=[2, 1], lens=[0, 0], page=8),                                                   # rows that see nothing
+])
+def test_reference_is_the_formula(kw):
+    x = make(**kw, Hq=4, Hkv=2, D=64, seed=3)
+    out, lse, _ = reference(x)
+    want, want_lse = by_row(x)
+    torch.testing.assert_close(out, want, rtol=1e-12, atol=1e-12)
+    torch.testing.assert_close(lse, want_lse, rtol=1e-12, atol=1e-12)
+
+
+@pytest.fixture
+def impl():
+    if not rt.LIB_PATH.exists():
+        pytest.skip("libtbhip.so is not built")
+    from tilebench_amd.benchmarks.serving.shared_prefix_attention import impl_hip
+
+    return impl_hip
+
+
+@pytest.mark.parametrize("at,value,error", [
+    (0, lambda v: v[0], ValueError), (0, lambda v: v.float(), TypeError), (0, lambda v: v[:, :3], ValueError),
+    (0, lambda v: v[:, :, :32], ValueError), (1, lambda v: v[:, :1], ValueError), (1, lambda v: v.bfloat16(), TypeError),
+    (3, lambda v: None, ValueError), (3, lambda v: v.long(), TypeError), (3, lambda v: v[0], ValueError),
+    (3, lambda v: v[:, :0], ValueError), (4, lambda v: v.repeat(3), ValueError), (5, lambda v: v[:1], ValueError),
+    (6, lambda v: v.long(), TypeError), (6, lambda v: v[:, :0], ValueError), (7, lambda v: v[:1], ValueError),
+    (8, lambda v: v[:1], ValueError), (8, lambda v: v.long(), TypeError), (9, lambda v: -1, ValueError),
+])
+def test_refusals(impl, at, value, error):
+    x = make([1, 2], [3, 40], prefix=[20], seed=1)
+    assert impl.check(*x) == (3, 8, 2, 64, 1, 2, 2, 3, 6, 16)
+    x[at] = value(x[at])
+    with pytest.raises(error, match="shared_prefix_attention"):
+        impl.check(*x)
+
+
+def test_refusals_of_caches(impl):
+    x = make([1], [3], seed=1)
+    odd = torch.zeros(1, 2, 16, 72, dtype=torch.float16)[..., :64]       # rows of 144 bytes are 16-byte aligned
+    assert impl.check(x[0], odd, odd, *x[3:])
+    for width, shift in ((68, 0), (80, 4)):                               # rows of 136 bytes; rows that start 8 bytes off
+        bad = torch.zeros(1, 2, 16, width, dtype=torch.float16)[..., shift:shift + 64]
+        with pytest.raises(ValueError, match="16-byte"):
+            impl.check(x[0], bad, bad, *x[3:])
+    y = make([1], [3], Hq=4, Hkv=2, D=128, seed=1)
+    y[0] = y[0][:, :, :96]
+    c = [t[..., :96].contiguous() for t in y[1:3]]
+    with pytest.raises(ValueError, match="64 or 128"):
+        impl.check(y[0], *c, *y[3:])
+
+
+def test_entry_point_checks_before_touching_a_device():
+    if not rt.LIB_PATH.exists():
+        pytest.skip("libtbhip.so is not built")
+    lib, fake = rt.load_library(), 1 << 40
+    base = dict(q=fake, kc=fake, ks=None, pp=fake, cu=fake, T=8, Hq=8, Hkv=2, D=64, G=1, Wp=4, B=2, W=4, max_q=4, N=16,
+                P=16, q_st=512, c_slot=64, dtype=1, cache=1, ws=None, wb=0)
+
+    def attend(**kw):
+        a = {**base, **kw}
+        return lib.tb_shared_prefix_attention(
+            a["q"], a["kc"], fake, a["ks"], a["ks"], a["pp"], fake, fake, fake, fake, a["cu"], fake, fake, a["T"],
+            a["Hq"], a["Hkv"], a["D"], a["G"], a["Wp"], a["B"], a["W"], a["max_q"], a["N"], a["P"], a["q_st"], 64, 2048,
+            1024, a["c_slot"], 0, 0, 0, 0.125, a["dtype"], a["cache"], a["ws"], a["wb"], None)
+
+    for kw in (dict(T=-1), dict(Hq=7), dict(Hkv=0), dict(D=96), dict(P=12), dict(P=8192), dict(G=0), dict(Wp=0),
+               dict(B=0), dict(W=0), dict(dtype=0), dict(cache=2), dict(cache=3), dict(ks=fake), dict(N=0),
+               dict(N=1 << 30), dict(q=None), dict(pp=None), dict(cu=None), dict(q_st=510), dict(c_slot=60),
+               dict(T=1 << 30), dict(W=1 << 28), dict(max_q=-1)):
+        assert attend(**kw) == rt.TB_E_INVALID, kw
+        assert "tb_shared_prefix_attention" in lib.tb_last_error().decode()
+    assert attend(q=fake + 8) == rt.TB_E_ALIGN and attend(kc=fake + 8) == rt.TB_E_ALIGN
+    assert attend(T=0) == rt.TB_OK                                   # nothing to do, nothing launched
+    assert attend() == rt.TB_E_WORKSPACE and "workspace" in lib.tb_last_error().decode()
+    need = ctypes.c_int64(-1)
+    size = lib.tb_shared_prefix_attention_workspace_size
+    assert size(8, 8, 2, 64, 1, 4, 2, 4, 16, 4, ctypes.byref(need)) == rt.TB_OK and need.value > 0
+    assert attend(ws=fake, wb=need.value - 1) == rt.TB_E_WORKSPACE
+    assert attend(ws=fake + 4, wb=need.value) == rt.TB_E_ALIGN
+    assert size(0, 8, 2, 64, 1, 4, 2, 4, 16, 4, ctypes.byref(need)) == rt.TB_OK and need.value == 0
+    # no prefix, and enough sequences to fill the device without splits: written directly
+    assert size(512, 8, 8, 64, 0, 0, 512, 64, 16, 1, ctypes.byref(need)) == rt.TB_OK and need.value == 0
+    assert size(8, 8, 2, 64, 1, 4, 2, 4, 16, 4, None) == rt.TB_E_INVALID

@@ -1,0 +1,1117 @@
+// Paged attention of a batch whose sequences share prefixes (decode, drafted
+// tokens and prompt chunks in one call).
+//
+//   out = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale * q . k_j - m),   lse = m + log sum_j p_j
+//
+// over the tokens j of the sequence's group prefix followed by its own tokens,
+// up to the query's own position (the queries are the last n_q tokens).
+//
+// Rows.  The query heads of one key/value head and the queries of one sequence
+// read the same tokens, so they are rows of one product: row r of a run of
+// queries is query r / grp, head r % grp of the group.  Three kinds of work:
+//   tiles   128 rows of a group of more than 32 rows: over the shared prefix, and
+//           on over the own tokens of those sequences that have more than 32 rows
+//   few     the own tokens of one sequence of up to 32 rows, or the prefix of a
+//           group of up to 32 rows: the block's four wavefronts split the tokens
+//   combine joins the partial results of a row (one slot per split) by their maxima
+// so a prefix is read once per 128 rows however many sequences share it.
+//
+// One wavefront's step over TOK tokens in LDS (attend_tile):
+//   S^T = K Q^T    K rows from LDS, Q in registers; a lane holds one row's scores
+//   P^T            exp2 of the scores against the running maximum, in registers; the
+//                  tokens a lane holds are in the order of the next product's operand
+//   O^T = V^T P^T  V^T by transposing LDS reads (ds_read_b64_tr_b16 / _b8) in that order
+// so scores never leave registers, and the maximum, sum and output of a row belong to
+// the lanes that hold the row.  Sums and statistics are fp32.  P is rounded to the
+// inputs' type for the second product (2^-11 or 2^-8 of each weight, unbiased).
+//
+// e4m3 caches: codes are converted exactly to the inputs' type; the keys' scales
+// multiply the scores, the values' scales the weights.
+//
+// Values that a row does not attend to never reach it: masked scores are selected
+// away, and in a tile that some rows see in part infinities and NaN among the
+// values count as zeros in the product and are marked in LDS for the rows that
+// attend to them, to be added at the end.
+#include "tb_common.h"
+
+#include <type_traits>
+
+namespace tb {
+namespace prefix {
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2v __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+enum { F16 = 1, BF16 = 2 };
+constexpr int THREADS = 256, WAVES = 4;
+constexpr int FEW = 32;      // rows of a sequence or group that the token-splitting blocks take
+constexpr int TILE = 128;    // rows of a tile block: 32 a wavefront
+constexpr int TILE_TOK = 64; // tokens of a tile block's step
+constexpr int MAX_SLOTS = 64;
+constexpr float NEG_INF = -__builtin_inff();
+
+struct Args {
+  const void* q;
+  int64_t q_st, q_sh;
+  const char* kc;
+  const char* vc;
+  int64_t c_page, c_head, c_slot;
+  const float* ks;
+  const float* vs;
+  int64_t s_page, s_head, s_slot;
+  const int* prefix_pages;  // [G, Wp]
+  const int* prefix_lens;   // [G]
+  const int* group_offsets; // [G + 1]
+  const int* pages;         // [B, W]
+  const int* lens;          // [B]
+  const int* cu_q;          // [B + 1]
+  void* out;
+  float* lse;
+  float* part_o;  // [slots][T * Hq][D]
+  float2* part_ml;  // [slots][T * Hq]: maximum (log2) and sum; sum -1: the row is final
+  int T, Hq, Hkv, grp, G, Wp, B, W;
+  int n_pages, page_shift;
+  int S1, S2;       // slots of tiles and prefixes, slots of own tokens
+  int direct;       // own tokens in one slot and nothing else: results are final
+  float scale_log2;
+};
+
+template <int DT>
+struct Ty;
+template <>
+struct Ty<F16> {
+  typedef f16x8 v8;
+  typedef _Float16 el;
+  static __device__ __forceinline__ f32x4 mfma(v8 a, v8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x16 mfma(v8 a, v8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t up8(uint32_t w, bool hi) {
+    return hi ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true))
+              : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false));
+  }
+  static constexpr uint32_t EXP = 0x7C00u;  // exponent bits: all ones in infinities and NaN
+};
+template <>
+struct Ty<BF16> {
+  typedef bf16x8 v8;
+  typedef __bf16 el;
+  static __device__ __forceinline__ f32x4 mfma(v8 a, v8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x16 mfma(v8 a, v8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t up8(uint32_t w, bool hi) {
+    return hi ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true))
+              : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false));
+  }
+  static constexpr uint32_t EXP = 0x7F80u;
+};
+
+// ------------------------------------------------------------------ LDS tiles
+//
+// A tile holds rows of RB bytes, one per token; the 16-byte chunk c of row t sits at
+// position c ^ f(t), so that the lanes of one LDS access (16 rows at one chunk for
+// keys, the rows and chunks of one transposing read for values) fall into different
+// banks.  SH is the side of the product's tiles (16 or 32).
+template <int RB>
+__device__ __forceinline__ constexpr int swizzle_k(int t) {
+  return RB == 256 ? (t & 15) : RB == 128 ? ((t >> 1) & 7) : ((t >> 2) & 3);
+}
+template <int RB, int SH, bool E8>
+__device__ __forceinline__ constexpr int swizzle_v(int t) {
+  if (!E8 && SH == 16) return RB == 256 ? (t & 7) << 1 : ((t >> 1) & 3) << 1;
+  if (!E8) return RB == 256 ? (t & 3) << 2 : ((t >> 1) & 1) << 2;
+  if (SH == 16) return RB == 128 ? ((t >> 1) & 3) | ((t >> 4) & 1) << 2 : ((t >> 2) & 1) | ((t >> 4) & 1) << 1;
+  return RB == 128 ? (((t >> 1) & 1) | ((t >> 3) & 1) << 1) << 1 : ((t >> 3) & 1) << 1;
+}
+
+typedef __attribute__((address_space(3))) char lds_char;
+__device__ __forceinline__ uint32_t lds_addr(const void* p) {
+  return (uint32_t)(uintptr_t)(lds_char*)p;
+}
+template <typename V>
+__device__ __forceinline__ V lds_read(uint32_t addr) {
+  return *(const __attribute__((address_space(3))) V*)(uintptr_t)addr;
+}
+
+// 16 (or 4) bytes a lane from global memory to LDS at lds + 16 (4) * lane.
+__device__ __forceinline__ void dma16(uint32_t lds, const char* p) {
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off"
+               :
+               : "s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(p)
+               : "memory", "m0");
+}
+__device__ __forceinline__ void dma4(uint32_t lds, const char* p) {
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off"
+               :
+               : "s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(p)
+               : "memory", "m0");
+}
+// Waits until at most N of this wavefront's vector memory operations are pending.
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+  asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
+}
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory"); }
+
+// The tokens of one prefix or sequence: a row of a page table and a length.
+struct Tokens {
+  const int* table;
+  int width, len;
+};
+
+// 64 consecutive entries of a page table, one a lane (ids outside the pool clamped to it).
+struct Window {
+  int ids = 0, first = 0x7FFFFFFF;
+  __device__ __forceinline__ void cover(const Tokens& s, int lo, int hi, int n_pages) {
+    if (lo >= first && hi < first + 64) return;
+    first = lo;
+    int id = s.table[min(lo + (int)(threadIdx.x & 63), s.width - 1)];
+    id = min(max(id, 0), n_pages - 1);
+    asm volatile("" : "+v"(id));  // the wait for the load belongs here, not at the uses in the loop
+    ids = id;
+  }
+};
+
+// Byte offsets of token rows in the pools.
+template <int TOK, int ESIZE>
+__device__ __forceinline__ int64_t token_offset(const Args& a, const Window& w, const Tokens& s, int t0, int tok) {
+  tok = min(tok, s.len - 1);
+  int page;
+  if ((1 << a.page_shift) >= TOK)  // a step's tokens lie in one page
+    page = __builtin_amdgcn_readlane(w.ids, (t0 >> a.page_shift) - w.first);
+  else
+    page = __builtin_amdgcn_ds_bpermute(((tok >> a.page_shift) - w.first) << 2, w.ids);
+  return (page * a.c_page + (tok & ((1 << a.page_shift) - 1)) * a.c_slot) * ESIZE;
+}
+
+// ------------------------------------------------------------------ one step
+//
+// State of one wavefront: SH rows (lane l: row l % SH), head dimension D.
+template <int DT, bool E8, int D, int SH>
+struct Wave {
+  typedef Ty<DT> Y;
+  typedef typename Y::v8 v8;
+  typedef typename std::conditional<SH == 16, f32x4, f32x16>::type acc_t;
+  static constexpr int RB = D * (E8 ? 1 : 2);
+  static constexpr int NG = 64 / SH;        // lane groups that share the rows
+  static constexpr int KS = 8 * NG;         // depth of one product instruction
+  static constexpr int STEPS = D / KS;      // of S^T
+  static constexpr int DT_N = D / SH;       // output tiles
+  static constexpr int REGS = SH * SH / 64; // accumulator registers of a tile
+
+  // log2 of the largest weight.  fp16: weights down to 2^-32 (2^-28) of the largest are kept; with e4m3 values
+  // their scales are multiplied in, up to 2^12 (a row of fp16 values has at most 2^7.2).
+  static constexpr float LIFT = DT == BF16 ? 0.0f : E8 ? 4.0f : 8.0f;
+
+  v8 q[STEPS];
+  acc_t o[DT_N];
+  float m, l;  // reference of the weights (log2), this lane's part of their sum
+
+  // channel of element 0 of operand `s` in this lane's group
+  static __device__ __forceinline__ int channel(int s, int g) {
+    return E8 ? (s / 2) * NG * 16 + g * 16 + (s % 2) * 8 : s * NG * 8 + g * 8;
+  }
+  __device__ __forceinline__ void init(const typename Y::el* row, bool valid) {
+    const int g = (threadIdx.x & 63) / SH;
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      q[s] = v8{};
+      if (valid) q[s] = *(const v8*)(row + channel(s, g));
+    }
+#pragma unroll
+    for (int d = 0; d < DT_N; ++d) o[d] = acc_t{};
+    m = NEG_INF;
+    l = 0.0f;
+  }
+  // token (within a tile of SH) of accumulator register r
+  static __device__ __forceinline__ int token_of(int r, int g) {
+    return SH == 16 ? g * 4 + r : 8 * (r / 4) + 4 * g + r % 4;
+  }
+  static __device__ __forceinline__ float over_groups_max(float x) {
+    if (SH == 16) x = fmaxf(x, __shfl_xor(x, 16));
+    return fmaxf(x, __shfl_xor(x, 32));
+  }
+  static __device__ __forceinline__ float over_groups_sum(float x) {
+    if (SH == 16) x += __shfl_xor(x, 16);
+    return x + __shfl_xor(x, 32);
+  }
+
+  // S^T of TOK tokens: TOK / SH tiles
+  template <int TOK>
+  __device__ __forceinline__ void scores(uint32_t kbase, acc_t (&s)[TOK / SH]) {
+    const int lane = threadIdx.x & 63, row = lane % SH, g = lane / SH;
+    const uint32_t a0 = kbase + row * RB, x = (uint32_t)(swizzle_k<RB>(row) ^ g) << 4;
+#pragma unroll
+    for (int t = 0; t < TOK / SH; ++t) s[t] = acc_t{};
+    if (E8) {
+#pragma unroll
+      for (int c = 0; c < STEPS / 2; ++c) {
+        const uint32_t at = a0 + (x ^ (uint32_t)(c * NG * 16));
+#pragma unroll
+        for (int t = 0; t < TOK / SH; ++t) {
+          const u32x4 w = lds_read<u32x4>(at + t * SH * RB);
+          u32x4 lo, hi;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            lo[2 * i] = Y::up8(w[i], false);
+            lo[2 * i + 1] = Y::up8(w[i], true);
+            hi[2 * i] = Y::up8(w[2 + i], false);
+            hi[2 * i + 1] = Y::up8(w[2 + i], true);
+          }
+          s[t] = Y::mfma(__builtin_bit_cast(v8, lo), q[2 * c], s[t]);
+          s[t] = Y::mfma(__builtin_bit_cast(v8, hi), q[2 * c + 1], s[t]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < STEPS; ++c) {
+        const uint32_t at = a0 + (x ^ (uint32_t)(c * NG * 16));
+#pragma unroll
+        for (int t = 0; t < TOK / SH; ++t) s[t] = Y::mfma(lds_read<v8>(at + t * SH * RB), q[c], s[t]);
+      }
+    }
+  }
+
+  // scores -> weights, in place of the scores; the running maximum, sum and outputs are brought up to date.
+  // vs: the values' scales of the lane's tokens (e4m3), multiplied into the weights after the sum.
+  // returns the weights as operands of the second product.
+  template <int TOK>
+  __device__ __forceinline__ void weights(acc_t (&s)[TOK / SH], int t0, int limit, bool full, float scale,
+                                          uint32_t sbase, v8 (&p)[TOK / KS]) {
+    const int g = (threadIdx.x & 63) / SH;
+    float top = NEG_INF;
+#pragma unroll
+    for (int t = 0; t < TOK / SH; ++t)
+#pragma unroll
+      for (int r = 0; r < REGS; r += 4) {
+        const int tok = t * SH + token_of(r, g);
+        f32x4 k;
+        if (E8) k = lds_read<f32x4>(sbase + tok * 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float x = s[t][r + i] * (E8 ? k[i] * scale : scale);
+          if (!full) x = t0 + tok + i < limit ? x : NEG_INF;
+          s[t][r + i] = x;
+          top = fmaxf(top, x);
+        }
+      }
+    const float ref = fmaxf(m, over_groups_max(top) - LIFT);
+    const float use = ref == NEG_INF ? 0.0f : ref;
+    const float alpha = __builtin_amdgcn_exp2f(m - use);
+    m = ref;
+    float sum = 0.0f;
+#pragma unroll
+    for (int t = 0; t < TOK / SH; ++t)
+#pragma unroll
+      for (int r = 0; r < REGS; r += 4) {
+        f32x4 v;
+        if (E8) v = lds_read<f32x4>(sbase + (TOK + t * SH + token_of(r, g)) * 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float w = __builtin_amdgcn_exp2f(s[t][r + i] - use);
+          sum += w;
+          s[t][r + i] = !E8 ? w : full || w > 0.0f ? w * v[i] : 0.0f;
+        }
+      }
+    l = l * alpha + sum;
+#pragma unroll
+    for (int d = 0; d < DT_N; ++d)
+#pragma unroll
+      for (int r = 0; r < REGS; ++r) o[d][r] *= alpha;
+#pragma unroll
+    for (int k = 0; k < TOK / KS; ++k)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        p[k][e] = SH == 16 ? (typename Y::el)s[2 * k + e / 4][e % 4]
+                           : (typename Y::el)s[k * 16 / SH][(k % 2) * 8 + e];
+  }
+
+  // V^T of output tile d, tokens of step k, as the first operand.
+  struct Values {
+    uint32_t at, x;  // address of the lane's first row, its swizzled chunk
+    __device__ __forceinline__ explicit Values(uint32_t vbase) {
+      const int lane = threadIdx.x & 63, i = lane & 15;
+      const int gx = lane / SH;                          // the group's four tokens
+      const int sub = SH == 32 ? (lane >> 4) & 1 : 0;    // 16 of a tile's 32 channels
+      if (E8) {
+        const int r = i >> 1, tok = gx * 4 + (r & 3) + (r >> 2) * (KS / 2);
+        at = vbase + tok * RB + (i & 1) * 8;
+        x = (uint32_t)(sub ^ swizzle_v<RB, SH, E8>(tok)) << 4;
+      } else {
+        const int r = i >> 2, b = i & 3, tok = gx * 4 + r;
+        at = vbase + tok * RB + (b & 1) * 8;
+        x = (uint32_t)((sub * 2 + (b >> 1)) ^ swizzle_v<RB, SH, E8>(tok)) << 4;
+      }
+    }
+    __device__ __forceinline__ v8 read(int d, int k) const {
+      if (E8) {
+        const uint32_t p = at + (x ^ (uint32_t)(d * (SH / 16) * 16)) + k * KS * RB;
+        const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2*)(uintptr_t)p);
+        u32x4 u;
+        u[0] = Y::up8((uint32_t)w[0], false);
+        u[1] = Y::up8((uint32_t)w[0], true);
+        u[2] = Y::up8((uint32_t)w[1], false);
+        u[3] = Y::up8((uint32_t)w[1], true);
+        return __builtin_bit_cast(v8, u);
+      }
+      // rows tok and tok + KS / 2: the swizzle of both is the same (it repeats every KS / 2 rows at most)
+      const uint32_t p = at + (x ^ (uint32_t)(d * (SH / 8) * 16)) + k * KS * RB;
+      typedef __attribute__((address_space(3))) s16x4* ptr;
+      struct { s16x4 a, b; } u;
+      u.a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(uintptr_t)p);
+      u.b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(uintptr_t)(p + KS / 2 * RB));
+      return __builtin_bit_cast(v8, u);
+    }
+  };
+
+  // 0xFFFF in the halves of w that are infinities or NaN
+  static __device__ __forceinline__ uint32_t non_finite(uint32_t w) {
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    const uint32_t e = Y::EXP | Y::EXP << 16;
+    const u16x2 other = __builtin_elementwise_min(__builtin_bit_cast(u16x2, (w & e) ^ e), u16x2{1, 1});
+    return __builtin_bit_cast(uint32_t, other - u16x2{1, 1});
+  }
+
+  // O^T += V^T P^T.  A tile that some rows see in part (not `full`): infinities and NaN count as zeros here and are
+  // marked for the rows that attend to their tokens.
+  template <int TOK>
+  __device__ __forceinline__ void values(uint32_t vbase, const v8 (&p)[TOK / KS], int t0, int limit, bool full,
+                                         uint32_t marks) {
+    const Values v(vbase);
+    if (full) {
+#pragma unroll
+      for (int d = 0; d < DT_N; ++d)
+#pragma unroll
+        for (int k = 0; k < TOK / KS; ++k) o[d] = Y::mfma(v.read(d, k), p[k], o[d]);
+      return;
+    }
+    uint32_t bad = 0;
+#pragma unroll
+    for (int d = 0; d < DT_N; ++d)
+#pragma unroll
+      for (int k = 0; k < TOK / KS; ++k) {
+        u32x4 x = __builtin_bit_cast(u32x4, v.read(d, k));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t n = non_finite(x[i]);
+          bad |= n;
+          x[i] &= ~n;
+        }
+        o[d] = Y::mfma(__builtin_bit_cast(v8, x), p[k], o[d]);
+        if (k % 2 == 1) __builtin_amdgcn_sched_barrier(0);  // two operands at a time: more would spill
+      }
+    if (__any(bad != 0)) mark<TOK>(vbase, t0, limit, marks);
+  }
+
+  // Marks of a wavefront: a byte for each of 32 rows and 64 runs of D / 64 channels, four bits a channel
+  // (1: +inf, 2: -inf, 4: NaN among the values that the row attends to).
+  static constexpr int MARKS = 32 * 64;
+  template <int TOK>
+  __device__ __forceinline__ void mark(uint32_t vbase, int t0, int limit, uint32_t marks) {
+    constexpr int PER = D / 64, ESIZE = E8 ? 1 : 2;
+    const int lane = threadIdx.x & 63, at = lane * PER * ESIZE;
+#pragma unroll 1
+    for (int tok = 0; tok < TOK; ++tok) {
+      const uint32_t p = vbase + tok * RB + (((at >> 4) ^ swizzle_v<RB, SH, E8>(tok)) << 4) + (at & 15);
+      uint32_t is = 0;
+#pragma unroll
+      for (int e = 0; e < PER; ++e) {
+        uint32_t x = E8 ? lds_read<uint8_t>(p + e) : lds_read<uint16_t>(p + 2 * e);
+        if (E8) x = (x & 0x7Fu) == 0x7Fu ? 0x7FFFu : 0u;
+        if ((x & Y::EXP) == Y::EXP) is |= ((x & 0x7FFFu) != Y::EXP ? 4u : x & 0x8000u ? 2u : 1u) << (4 * e);
+      }
+      if (!__any(is != 0)) continue;
+#pragma unroll 1
+      for (int r = 0; r < SH; ++r) {
+        if (t0 + tok >= __builtin_amdgcn_readlane(limit, r)) continue;
+        const uint32_t m = marks + r * 64 + lane;
+        *(__attribute__((address_space(3))) uint8_t*)(uintptr_t)m = (uint8_t)(lds_read<uint8_t>(m) | is);
+      }
+    }
+  }
+  static __device__ __forceinline__ void clear_marks(uint32_t marks) {
+    const uint32_t p = marks + (threadIdx.x & 63) * 32;
+    *(__attribute__((address_space(3))) u32x4*)(uintptr_t)p = u32x4{};
+    *(__attribute__((address_space(3))) u32x4*)(uintptr_t)(p + 16) = u32x4{};
+  }
+  // x, or what the marks of row r make of channels c .. c + 3
+  static __device__ __forceinline__ f32x4 marked(f32x4 x, uint32_t marks, int r, int c) {
+    constexpr int PER = D / 64;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t m = (lds_read<uint8_t>(marks + r * 64 + (c + i) / PER) >> (4 * (i % PER))) & 15u;
+      if (m & 1u) x[i] += __builtin_inff();
+      if (m & 2u) x[i] -= __builtin_inff();
+      if (m & 4u) x[i] = __builtin_nanf("");
+    }
+    return x;
+  }
+};
+
+// ------------------------------------------------------------------ rows and lengths
+
+struct Seq {
+  int q0, n_q, own;  // first query, queries, own tokens
+};
+__device__ __forceinline__ int clamp_int(int x, int lo, int hi) { return min(max(x, lo), hi); }
+__device__ __forceinline__ int query_start(const Args& a, int b) { return clamp_int(a.cu_q[b], 0, a.T); }
+__device__ __forceinline__ Seq sequence(const Args& a, int b) {
+  Seq s;
+  s.q0 = query_start(a, b);
+  s.n_q = max(query_start(a, b + 1) - s.q0, 0);
+  s.own = clamp_int(a.lens[b], 0, a.W << a.page_shift);
+  return s;
+}
+struct Group {
+  int b0, b1, q0, rows, len;  // sequences, first query, rows per key/value head, prefix tokens
+};
+__device__ __forceinline__ Group group(const Args& a, int g) {
+  Group r;
+  r.b0 = a.group_offsets && g > 0 ? clamp_int(a.group_offsets[g], 0, a.B) : 0;
+  r.b1 = a.group_offsets && g + 1 < a.G ? clamp_int(a.group_offsets[g + 1], r.b0, a.B) : a.B;
+  r.q0 = query_start(a, r.b0);
+  r.rows = max(query_start(a, r.b1) - r.q0, 0) * a.grp;
+  r.len = a.prefix_lens ? clamp_int(a.prefix_lens[g], 0, a.Wp << a.page_shift) : 0;
+  return r;
+}
+// The sequence of query t among b0 .. b1 - 1 (the last one that starts at or before it).
+__device__ __forceinline__ int sequence_of(const Args& a, int t, int b0, int b1) {
+  int lo = b0, hi = b1;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (a.cu_q[mid] <= t) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+// A row without tokens has the sum 0: its output is 0 and its lse -inf.
+__device__ __forceinline__ float inverse(float sum) { return sum == 0.0f ? 0.0f : 1.0f / sum; }
+__device__ __forceinline__ float natural_lse(float m, float sum) {
+  return sum == 0.0f ? NEG_INF : (m + __builtin_amdgcn_logf(sum)) * 0.69314718055994530942f;
+}
+
+template <typename el>
+__device__ __forceinline__ void store4(el* p, f32x4 x) {
+  struct alignas(8) { el e[4]; } v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v.e[i] = (el)x[i];
+  *(decltype(v)*)p = v;
+}
+
+// ------------------------------------------------------------------ few rows
+
+template <int DT, bool E8, int D>
+struct FewLayout {
+  static constexpr int RB = D * (E8 ? 1 : 2);
+  static constexpr int TOK = RB == 256 ? 32 : 64;  // tokens of a wavefront's step
+  static constexpr int TILE_BYTES = TOK * RB;
+  static constexpr int WAVE_BYTES = 2 * TILE_BYTES + (E8 ? 2 * TOK * 4 : 0);
+  static constexpr int MERGE_ROW = D + 4;  // floats; rows four banks apart
+  static constexpr int MERGE_BYTES = WAVES * FEW * MERGE_ROW * 4 + WAVES * FEW * 8;
+  static constexpr int MARKS = WAVES * WAVE_BYTES > MERGE_BYTES ? WAVES * WAVE_BYTES : MERGE_BYTES;
+  static constexpr int LDS = MARKS + WAVES * 32 * 64;
+};
+
+// Rows 0 .. rows - 1 (at most 32) from query q0 on, key/value head h, tokens of `src`, split `split` of `splits`;
+// results to slot `slot`.
+template <int DT, bool E8, int D, int SH>
+__device__ __forceinline__ void attend_few(const Args& a, char* smem, int h, int q0, int rows, const Tokens& src,
+                                           int base, int split, int splits, int slot, const Seq* seq, int b0, int b1) {
+  typedef FewLayout<DT, E8, D> L;
+  typedef Wave<DT, E8, D, SH> W;
+  typedef typename W::Y::el el;
+  constexpr int TOK = L::TOK, RB = L::RB, RPI = 1024 / RB, NI = TOK / RPI, ESIZE = E8 ? 1 : 2;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int row = lane % SH;
+  const bool valid = row < rows;
+  const int t = q0 + row / a.grp, hq = h * a.grp + row % a.grp;
+
+  // tokens of `src` that the row attends to: its position is that of the last n_q tokens of its sequence.
+  // base: the tokens before src (own tokens), or -1 where src is the prefix
+  int limit = 0x7FFFFFFF;
+  if (valid) {
+    Seq s = seq ? *seq : sequence(a, sequence_of(a, t, b0, b1));
+    const int end = s.own - s.n_q + (t - s.q0) + 1;  // own tokens up to and with the query
+    limit = base < 0 ? clamp_int(src.len + end, 0, src.len) : clamp_int(end, 0, src.len);
+  }
+
+  W w;
+  w.init((const el*)a.q + t * a.q_st + hq * a.q_sh, valid);
+
+  const int tiles = (src.len + TOK - 1) / TOK;
+  const int lo = (int)((int64_t)tiles * split / splits), hi = (int)((int64_t)tiles * (split + 1) / splits);
+  const int n0 = lo + (hi - lo) * wave / WAVES, n1 = lo + (hi - lo) * (wave + 1) / WAVES;
+
+  const uint32_t kbase = lds_addr(smem) + wave * L::WAVE_BYTES, vbase = kbase + L::TILE_BYTES;
+  const uint32_t sbase = vbase + L::TILE_BYTES;
+  const uint32_t marks = lds_addr(smem) + L::MARKS + wave * W::MARKS;
+  W::clear_marks(marks);
+  const char* kp = a.kc + h * a.c_head * ESIZE;
+  const char* vp = a.vc + h * a.c_head * ESIZE;
+  Window win;
+  auto cover = [&](int n) __attribute__((always_inline)) {
+    const int t0 = n * TOK;
+    win.cover(src, t0 >> a.page_shift, min(t0 + TOK - 1, src.len - 1) >> a.page_shift, a.n_pages);
+  };
+  auto fill = [&](int n, bool keys) __attribute__((always_inline)) {
+    const int t0 = n * TOK;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int r = i * RPI + lane / (RB / 16), pos = lane % (RB / 16);
+      const int64_t off = token_offset<TOK, ESIZE>(a, win, src, t0, t0 + r);
+      if (keys)
+        dma16(kbase + i * 1024, kp + off + ((pos ^ swizzle_k<RB>(r)) << 4));
+      else
+        dma16(vbase + i * 1024, vp + off + ((pos ^ swizzle_v<RB, SH, E8>(r)) << 4));
+    }
+  };
+  auto fill_scales = [&](int n) __attribute__((always_inline)) {  // TOK scales of keys, then TOK of values
+    const int t0 = n * TOK;
+    static_assert(TOK == 64 || !E8, "one scale a lane");
+    const int tok = min(t0 + lane, src.len - 1);
+    const int page = __builtin_amdgcn_ds_bpermute(((tok >> a.page_shift) - win.first) << 2, win.ids);
+    const int64_t off = page * a.s_page + h * a.s_head + (tok & ((1 << a.page_shift) - 1)) * a.s_slot;
+    dma4(sbase, (const char*)(a.ks + off));
+    dma4(sbase + TOK * 4, (const char*)(a.vs + off));
+  };
+
+  // Keys and values have one buffer each: the next keys are fetched from when the
+  // scores are done, the next values from when the outputs are.
+  if (n0 < n1) {
+    cover(n0);
+    if (E8) fill_scales(n0);
+    fill(n0, true);
+    fill(n0, false);
+  }
+  for (int n = n0; n < n1; ++n) {
+    const int t0 = n * TOK;
+    const bool full = __all(limit >= t0 + TOK);
+    typename W::acc_t s[TOK / SH];
+    typename W::v8 p[TOK / W::KS];
+    wait_vm<NI>();  // keys (and scales) are there; the values may be on their way
+    w.template scores<TOK>(kbase, s);
+    if (E8) w.template weights<TOK>(s, t0, limit, full, a.scale_log2, sbase, p);
+    wait_lds();
+    if (n + 1 < n1) {
+      cover(n + 1);
+      if (E8) fill_scales(n + 1);
+      fill(n + 1, true);
+    }
+    if (!E8) w.template weights<TOK>(s, t0, limit, full, a.scale_log2, sbase, p);
+    if (n + 1 < n1) wait_vm<NI + (E8 ? 2 : 0)>(); else wait_vm<0>();
+    w.template values<TOK>(vbase, p, t0, limit, full, marks);
+    wait_lds();
+    if (n + 1 < n1) fill(n + 1, false);
+  }
+
+  // join the four wavefronts
+  float l = W::over_groups_sum(w.l);
+  float* merge = (float*)smem;
+  float2* ml = (float2*)(merge + WAVES * FEW * L::MERGE_ROW);
+  __syncthreads();  // every wavefront is done with its tiles
+  if (lane < SH) ml[wave * FEW + row] = float2{w.m, l};
+  __syncthreads();
+  float top = NEG_INF;
+#pragma unroll
+  for (int i = 0; i < WAVES; ++i) top = fmaxf(top, ml[i * FEW + row].x);
+  const float alpha = __builtin_amdgcn_exp2f(w.m - (top == NEG_INF ? 0.0f : top));
+  const int g = lane / SH;
+#pragma unroll
+  for (int d = 0; d < W::DT_N; ++d)
+#pragma unroll
+    for (int r = 0; r < W::REGS; r += 4) {
+      f32x4 x;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = w.o[d][r + i] * alpha;
+      *(f32x4*)(merge + (wave * FEW + row) * L::MERGE_ROW + d * SH + W::token_of(r, g)) = x;
+    }
+  __syncthreads();
+  for (int i = threadIdx.x; i < rows * (D / 4); i += THREADS) {
+    const int r = i / (D / 4), c = (i % (D / 4)) * 4;
+    float m = NEG_INF, sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < WAVES; ++k) m = fmaxf(m, ml[k * FEW + r].x);
+    const float use = m == NEG_INF ? 0.0f : m;
+    f32x4 x{};
+#pragma unroll
+    for (int k = 0; k < WAVES; ++k) {
+      const float2 e = ml[k * FEW + r];
+      sum += e.y * __builtin_amdgcn_exp2f(e.x - use);
+      x += *(const f32x4*)(merge + (k * FEW + r) * L::MERGE_ROW + c);
+    }
+#pragma unroll
+    for (int k = 0; k < WAVES; ++k) x = W::marked(x, lds_addr(smem) + L::MARKS + k * W::MARKS, r, c);
+    const int64_t id = (int64_t)(q0 + r / a.grp) * a.Hq + h * a.grp + r % a.grp;
+    if (a.direct) {
+      store4((el*)a.out + id * D + c, x * inverse(sum));
+      if (c == 0) a.lse[id] = natural_lse(m, sum);
+    } else {
+      *(f32x4*)(a.part_o + ((int64_t)slot * a.T * a.Hq + id) * D + c) = x;
+      if (c == 0) a.part_ml[(int64_t)slot * a.T * a.Hq + id] = float2{m, sum};
+    }
+  }
+}
+
+// Outputs of queries t0 .. t1 - 1 that attend to nothing.
+template <int DT, int D>
+__device__ __forceinline__ void empty_rows(const Args& a, int h, int t0, int t1) {
+  for (int t = t0; t < t1; ++t) {
+    const int64_t id = (int64_t)t * a.Hq + h * a.grp;
+    for (int i = threadIdx.x; i < a.grp * D; i += THREADS) ((typename Ty<DT>::el*)a.out)[id * D + i] = 0;
+    for (int i = threadIdx.x; i < a.grp; i += THREADS) a.lse[id + i] = NEG_INF;
+  }
+}
+
+// Blocks: own tokens of sequence b (b < B), prefix of group b - B; key/value head; split.
+template <int DT, bool E8, int D>
+__global__ void __launch_bounds__(THREADS, 2) few_rows(Args a) {
+  extern __shared__ __align__(16) char smem[];
+  const int unit = blockIdx.x / a.Hkv, h = blockIdx.x % a.Hkv, split = blockIdx.y;
+  constexpr int TOK = FewLayout<DT, E8, D>::TOK;
+  if (unit < a.B) {
+    const int b = unit;
+    if (a.direct && b == 0) {  // rows of no sequence
+      const int first = query_start(a, 0);
+      empty_rows<DT, D>(a, h, 0, first);
+      empty_rows<DT, D>(a, h, max(query_start(a, a.B), first), a.T);
+    }
+    if (split >= a.S2) return;
+    const Seq s = sequence(a, b);
+    const int rows = s.n_q * a.grp;
+    // splits of at least two steps a wavefront
+    const int used = clamp_int((s.own + 8 * TOK - 1) / (8 * TOK), 1, a.S2);
+    if (a.direct && rows > FEW) {  // more queries than max_q announced: nothing was planned for them
+      empty_rows<DT, D>(a, h, s.q0, s.q0 + s.n_q);
+      return;
+    }
+    if (rows > FEW || split >= used) {
+      for (int r = threadIdx.x; r < rows; r += THREADS)
+        a.part_ml[((int64_t)(a.S1 + split) * a.T + s.q0 + r / a.grp) * a.Hq + h * a.grp + r % a.grp] =
+            float2{NEG_INF, 0.0f};
+      return;
+    }
+    if (rows == 0) return;
+    const Tokens src{a.pages + (int64_t)b * a.W, a.W, s.own};
+    if (rows <= 16)
+      attend_few<DT, E8, D, 16>(a, smem, h, s.q0, rows, src, 0, split, used, a.S1 + split, &s, 0, 0);
+    else
+      attend_few<DT, E8, D, 32>(a, smem, h, s.q0, rows, src, 0, split, used, a.S1 + split, &s, 0, 0);
+  } else {
+    const int g = unit - a.B;
+    if (split >= a.S1) return;
+    const Group gr = group(a, g);
+    if (gr.rows > FEW || gr.rows == 0) return;
+    const int used = clamp_int((gr.len + 8 * TOK - 1) / (8 * TOK), 1, a.S1);
+    if (split >= used) {
+      for (int r = threadIdx.x; r < gr.rows; r += THREADS)
+        a.part_ml[((int64_t)split * a.T + gr.q0 + r / a.grp) * a.Hq + h * a.grp + r % a.grp] = float2{NEG_INF, 0.0f};
+      return;
+    }
+    const Tokens src{a.prefix_pages + (int64_t)g * a.Wp, a.Wp, gr.len};
+    if (gr.rows <= 16)
+      attend_few<DT, E8, D, 16>(a, smem, h, gr.q0, gr.rows, src, -1, split, used, split, nullptr, gr.b0, gr.b1);
+    else
+      attend_few<DT, E8, D, 32>(a, smem, h, gr.q0, gr.rows, src, -1, split, used, split, nullptr, gr.b0, gr.b1);
+  }
+}
+
+// ------------------------------------------------------------------ tiles of rows
+
+template <int DT, bool E8, int D>
+struct TileLayout {
+  static constexpr int RB = D * (E8 ? 1 : 2);
+  static constexpr int TILE_BYTES = TILE_TOK * RB;
+  static constexpr int STAGE = 2 * TILE_BYTES + (E8 ? 2 * TILE_TOK * 4 : 0);
+  static constexpr int MARKS = 2 * STAGE;
+  static constexpr int LDS = MARKS + WAVES * 32 * 64;
+};
+
+// The tile (group, row tile) number `index`, or false past the last one.  64 groups at a time.
+__device__ __forceinline__ bool find_tile(const Args& a, int index, int& g, int& tile) {
+  const int lane = threadIdx.x & 63;
+  int seen = 0;
+  for (int x0 = 0; x0 < a.G; x0 += 64) {
+    int n = 0;
+    if (x0 + lane < a.G) {
+      const Group gr = group(a, x0 + lane);
+      n = gr.rows > FEW ? (gr.rows + TILE - 1) / TILE : 0;
+    }
+    int incl = n;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int o = __shfl_up(incl, d);
+      if (lane >= d) incl += o;
+    }
+    const int here = __builtin_amdgcn_readfirstlane(__shfl(incl, 63));
+    if (index < seen + here) {
+      const int l = __builtin_ctzll(__ballot(seen + incl > index));
+      g = __builtin_amdgcn_readfirstlane(x0 + l);
+      tile = __builtin_amdgcn_readfirstlane(index - seen - __shfl(incl - n, l));
+      return true;
+    }
+    seen += here;
+  }
+  return false;
+}
+
+template <int DT, bool E8, int D>
+__global__ void __launch_bounds__(THREADS, 2) row_tiles(Args a) {
+  extern __shared__ __align__(16) char smem[];
+  typedef TileLayout<DT, E8, D> L;
+  constexpr int SH = 32, TOK = TILE_TOK, RB = L::RB, RPI = 1024 / RB, ESIZE = E8 ? 1 : 2;
+  constexpr int NI = TOK / WAVES / RPI;  // copies of a wavefront per tile of keys or values
+  static_assert(NI >= 1, "a wavefront fills 16 rows");
+  typedef Wave<DT, E8, D, SH> W;
+  typedef typename W::Y::el el;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int h = blockIdx.y % a.Hkv, split = blockIdx.y / a.Hkv;
+  int g, tile;
+  if (!find_tile(a, blockIdx.x, g, tile)) return;
+  const Group gr = group(a, g);
+  const int row = tile * TILE + wave * SH + lane % SH;
+  const bool valid = row < gr.rows;
+  const int t = gr.q0 + row / a.grp, hq = h * a.grp + row % a.grp;
+
+  int b = -1, end = 0, own_limit = 0;
+  bool big = false;
+  if (valid) {
+    b = sequence_of(a, t, gr.b0, gr.b1);
+    const Seq s = sequence(a, b);
+    end = s.own - s.n_q + (t - s.q0) + 1;
+    own_limit = clamp_int(end, 0, s.own);
+    big = s.n_q * a.grp > FEW;
+  }
+  const int prefix_limit = valid ? clamp_int(gr.len + end, 0, gr.len) : 0;
+
+  W w;
+  w.init((const el*)a.q + t * a.q_st + hq * a.q_sh, valid);
+
+  // The tile's tokens: the prefix, then the own tokens (as far as a row of the tile sees them) of each of its
+  // sequences with more than 32 rows.  Steps are counted over all of them and shared out to the splits.
+  const int t_first = gr.q0 + tile * TILE / a.grp;
+  const int t_last = gr.q0 + (min((tile + 1) * TILE, gr.rows) - 1) / a.grp;
+  const int b_first = sequence_of(a, t_first, gr.b0, gr.b1), b_last = sequence_of(a, t_last, gr.b0, gr.b1);
+  auto own_tokens = [&](int x) __attribute__((always_inline)) {
+    const Seq s = sequence(a, x);
+    if (s.n_q * a.grp <= FEW) return 0;
+    const int last = min(t_last, s.q0 + s.n_q - 1);
+    return clamp_int(s.own - s.n_q + (last - s.q0) + 1, 0, s.own);
+  };
+  int steps = (gr.len + TOK - 1) / TOK;
+  for (int x = b_first; x <= b_last; ++x) steps += (own_tokens(x) + TOK - 1) / TOK;
+  steps = __builtin_amdgcn_readfirstlane(steps);
+  int skip = (int)((int64_t)steps * split / a.S1);
+  int todo = (int)((int64_t)steps * (split + 1) / a.S1) - skip;
+
+  const uint32_t base = lds_addr(smem), marks = base + L::MARKS + wave * W::MARKS;
+  W::clear_marks(marks);
+  const char* kp = a.kc + h * a.c_head * ESIZE;
+  const char* vp = a.vc + h * a.c_head * ESIZE;
+
+  for (int x = b_first - 1; x <= b_last && todo > 0; ++x) {
+    const bool pre = x < b_first;
+    const int len = __builtin_amdgcn_readfirstlane(pre ? gr.len : own_tokens(x));
+    const int n_all = (len + TOK - 1) / TOK;
+    if (skip >= n_all) {
+      skip -= n_all;
+      continue;
+    }
+    const int n0 = skip, n1 = min(n_all, skip + todo);
+    skip = 0;
+    todo -= n1 - n0;
+    const Tokens src = pre ? Tokens{a.prefix_pages + (int64_t)g * a.Wp, a.Wp, len}
+                           : Tokens{a.pages + (int64_t)x * a.W, a.W, len};
+    int limit = pre ? prefix_limit : b == x ? own_limit : 0;
+    const bool some = valid && limit > 0;
+    if (!valid) limit = 0x7FFFFFFF;
+    Window win;
+    auto fill = [&](int n) __attribute__((always_inline)) {
+      const int t0 = n * TOK;
+      const uint32_t kb = base + (n & 1) * L::STAGE, vb = kb + L::TILE_BYTES, sb = vb + L::TILE_BYTES;
+      win.cover(src, t0 >> a.page_shift, min(t0 + TOK - 1, src.len - 1) >> a.page_shift, a.n_pages);
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const int r = (wave * NI + i) * RPI + lane / (RB / 16), pos = lane % (RB / 16);
+        const int64_t off = token_offset<TOK, ESIZE>(a, win, src, t0, t0 + r);
+        dma16(kb + (wave * NI + i) * 1024, kp + off + ((pos ^ swizzle_k<RB>(r)) << 4));
+        dma16(vb + (wave * NI + i) * 1024, vp + off + ((pos ^ swizzle_v<RB, SH, E8>(r)) << 4));
+      }
+      if (E8 && wave < 2) {
+        const int tok = min(t0 + lane, src.len - 1);
+        const int page = __builtin_amdgcn_ds_bpermute(((tok >> a.page_shift) - win.first) << 2, win.ids);
+        const int64_t off = page * a.s_page + h * a.s_head + (tok & ((1 << a.page_shift) - 1)) * a.s_slot;
+        dma4(sb + wave * TOK * 4, (const char*)((wave ? a.vs : a.ks) + off));
+      }
+    };
+    // both stages may still be read from the segment before
+    __syncthreads();
+    fill(n0);
+    for (int n = n0; n < n1; ++n) {
+      const int t0 = n * TOK;
+      wait_vm<0>();
+      wait_lds();
+      __builtin_amdgcn_s_barrier();  // the step's tokens are there, the other stage is free
+      if (n + 1 < n1) fill(n + 1);
+      if (!__any(some && limit > t0)) continue;
+      const bool full = __all(limit >= t0 + TOK);
+      const uint32_t kb = base + (n & 1) * L::STAGE, vb = kb + L::TILE_BYTES, sb = vb + L::TILE_BYTES;
+      typename W::acc_t s[TOK / SH];
+      typename W::v8 p[TOK / W::KS];
+      w.template scores<TOK>(kb, s);
+      w.template weights<TOK>(s, t0, limit, full, a.scale_log2, sb, p);
+      w.template values<TOK>(vb, p, t0, limit, full, marks);
+    }
+  }
+
+  const float l = W::over_groups_sum(w.l);
+  if (!valid) return;
+  const int gx = lane / SH;
+  const int64_t id = (int64_t)t * a.Hq + hq, slot = (int64_t)split * a.T * a.Hq + id;
+  const bool final = a.S1 == 1 && big;
+  const float inv = final ? inverse(l) : 1.0f;
+#pragma unroll
+  for (int d = 0; d < W::DT_N; ++d)
+#pragma unroll
+    for (int r = 0; r < W::REGS; r += 4) {
+      f32x4 x;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = w.o[d][r + i] * inv;
+      const int c = d * SH + W::token_of(r, gx);
+      x = W::marked(x, marks, lane % SH, c);
+      if (final)
+        store4((el*)a.out + id * D + c, x);
+      else if (!(l == 0.0f))
+        *(f32x4*)(a.part_o + slot * D + c) = x;
+    }
+  if (gx == 0) {
+    a.part_ml[slot] = float2{w.m, final ? -1.0f : l};
+    if (final) a.lse[id] = natural_lse(w.m, l);
+  }
+}
+
+// ------------------------------------------------------------------ combine
+
+// One wavefront a row: lane s reads slot s's maximum and sum, then all lanes add the slots' outputs in order.
+template <int DT, int D>
+__global__ void __launch_bounds__(THREADS) combine(Args a) {
+  typedef typename Ty<DT>::el el;
+  constexpr int PER = D / 64;
+  const int lane = threadIdx.x & 63;
+  const int64_t rows = (int64_t)a.T * a.Hq, id = (int64_t)blockIdx.x * WAVES + (threadIdx.x >> 6);
+  if (id >= rows) return;
+  const int t = (int)(id / a.Hq), first = query_start(a, 0), end = query_start(a, a.B);
+  const int slots = a.S1 + a.S2;
+  float2 ml{NEG_INF, 0.0f};
+  const bool inside = t >= first && t < end;
+  if (inside && lane < slots) ml = a.part_ml[lane * rows + id];
+  if (__any(ml.y < 0.0f)) return;  // written by its tile
+  float top = ml.x;
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+  const float weight = __builtin_amdgcn_exp2f(ml.x - (top == NEG_INF ? 0.0f : top));
+  float sum = weight * ml.y;
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
+  float x[PER] = {};
+  unsigned long long live = __ballot(!(ml.y == 0.0f));  // a NaN counts
+  while (live) {
+    const int s = __builtin_ctzll(live);
+    live &= live - 1;
+    const float w = __shfl(weight, s);
+    const float* p = a.part_o + (s * rows + id) * D + lane * PER;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) x[i] += w * p[i];
+  }
+  const float inv = inverse(sum);
+#pragma unroll
+  for (int i = 0; i < PER; ++i) ((el*)a.out)[id * D + lane * PER + i] = (el)(x[i] * inv);
+  if (lane == 0) a.lse[id] = natural_lse(top, sum);
+}
+
+// ------------------------------------------------------------------ host
+
+struct Plan {
+  int64_t tiles = 0;  // row tiles, an upper bound
+  int S1 = 0, S2 = 1, few_prefix = 0;
+  bool combine = true;
+  int64_t bytes = 0;
+};
+
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Splits: enough blocks for two on each of the 256 CUs, splits of at least 256 tokens.
+inline Plan make_plan(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t G, int64_t Wp, int64_t B, int64_t W,
+                      int64_t page, int64_t max_q) {
+  Plan p;
+  const int64_t grp = Hq / Hkv, rows = T * grp, groups = G > 0 ? G : 1;
+  const bool has_tiles = rows > FEW && (Wp > 0 || max_q * grp > FEW);
+  auto splits = [](int64_t blocks, int64_t tokens) {
+    const int64_t want = 512 / (blocks < 1 ? 1 : blocks), most = ceil_div(tokens, 256);
+    const int64_t s = want < most ? want : most;
+    return (int)(s < 1 ? 1 : s > MAX_SLOTS / 2 ? MAX_SLOTS / 2 : s);
+  };
+  if (has_tiles) {
+    p.tiles = rows / TILE + groups;
+    const int64_t likely = ceil_div(rows, TILE) > groups ? ceil_div(rows, TILE) : groups;
+    p.S1 = splits(likely * Hkv, (Wp + (max_q * grp > FEW ? W : 0)) * page);
+  } else if (Wp > 0) {
+    p.S1 = splits(groups * Hkv, Wp * page);
+  }
+  p.few_prefix = p.S1 > 0 ? (int)groups : 0;
+  p.S2 = splits(B * Hkv, W * page);
+  p.combine = !(p.S1 == 0 && p.S2 == 1);
+  p.bytes = p.combine ? (int64_t)(p.S1 + p.S2) * T * Hq * (D * 4 + 8) : 0;
+  return p;
+}
+
+template <int DT, bool E8, int D>
+tb_status launch(Args& a, const Plan& p, hipStream_t stream, const char* what) {
+  if (p.tiles) {
+    constexpr size_t lds = TileLayout<DT, E8, D>::LDS;
+    if (tb_status s = reserve_lds((const void*)row_tiles<DT, E8, D>, lds, what)) return s;
+    hipLaunchKernelGGL((row_tiles<DT, E8, D>), dim3((unsigned)p.tiles, (unsigned)(p.S1 * a.Hkv)), dim3(THREADS), lds,
+                       stream, a);
+    if (tb_status s = launch_status(what)) return s;
+  }
+  constexpr size_t lds = FewLayout<DT, E8, D>::LDS;
+  if (tb_status s = reserve_lds((const void*)few_rows<DT, E8, D>, lds, what)) return s;
+  const int most = p.few_prefix && p.S1 > p.S2 ? p.S1 : p.S2;
+  hipLaunchKernelGGL((few_rows<DT, E8, D>), dim3((unsigned)((a.B + p.few_prefix) * a.Hkv), (unsigned)most),
+                     dim3(THREADS), lds, stream, a);
+  if (tb_status s = launch_status(what)) return s;
+  if (p.combine) {
+    hipLaunchKernelGGL((combine<DT, D>), dim3((unsigned)ceil_div((int64_t)a.T * a.Hq, WAVES)), dim3(THREADS), 0, stream,
+                       a);
+    return launch_status(what);
+  }
+  return TB_OK;
+}
+
+template <int DT>
+tb_status launch_for(bool e8, int64_t D, Args& a, const Plan& p, hipStream_t stream, const char* what) {
+  if (D == 64) return e8 ? launch<DT, true, 64>(a, p, stream, what) : launch<DT, false, 64>(a, p, stream, what);
+  return e8 ? launch<DT, true, 128>(a, p, stream, what) : launch<DT, false, 128>(a, p, stream, what);
+}
+
+tb_status check_sizes(const char* what, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t G, int64_t Wp, int64_t B,
+                      int64_t W, int64_t page_size, int64_t max_q) {
+  TB_CHECK_ARG(T >= 0 && B >= 0 && G >= 0 && Wp >= 0 && W >= 0 && max_q >= 0, "%s: negative size", what);
+  TB_CHECK_ARG(Hkv >= 1 && Hq >= Hkv && Hq % Hkv == 0 && Hkv <= 65535 / (MAX_SLOTS / 2), "%s: %lld query heads do not share %lld key/value heads",
+               what, (long long)Hq, (long long)Hkv);
+  TB_CHECK_ARG(D == 64 || D == 128, "%s: the head dimension must be 64 or 128 (got %lld)", what, (long long)D);
+  TB_CHECK_ARG(page_size >= 1 && page_size <= 4096 && (page_size & (page_size - 1)) == 0,
+               "%s: the page size must be a power of two up to 4096 (got %lld)", what, (long long)page_size);
+  TB_CHECK_ARG((Wp == 0) == (G == 0), "%s: %lld groups with page tables of %lld", what, (long long)G, (long long)Wp);
+  const int64_t most = (1ll << 31) - 1;
+  // row, token and block numbers are 32-bit in the kernels
+  TB_CHECK_ARG(T * Hq <= most && B * Hkv <= most / 2 && G * Hkv <= most / 4 && W <= most / 2 / page_size &&
+                   Wp <= most / 2 / page_size && max_q * Hq <= most,
+               "%s: sizes past 2^31", what);
+  return TB_OK;
+}
+
+}  // namespace prefix
+}  // namespace tb
+
+extern "C" tb_status tb_shared_prefix_attention_workspace_size(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t G,
+                                                               int64_t Wp, int64_t B, int64_t W, int64_t page_size,
+                                                               int64_t max_q, int64_t* bytes) {
+  using namespace tb::prefix;
+  const char* what = "tb_shared_prefix_attention_workspace_size";
+  TB_CHECK_ARG(bytes, "%s: null pointer", what);
+  if (tb_status s = check_sizes(what, T, Hq, Hkv, D, G, Wp, B, W, page_size, max_q)) return s;
+  *bytes = T == 0 ? 0 : make_plan(T, Hq, Hkv, D, G, Wp, B, W, page_size, max_q).bytes;
+  return TB_OK;
+}
+
+extern "C" tb_status tb_shared_prefix_attention(const void* q, const void* k_cache, const void* v_cache,
+                                                const float* k_scale, const float* v_scale,
+                                                const int32_t* prefix_pages, const int32_t* prefix_lens,
+                                                const int32_t* group_offsets, const int32_t* pages,
+                                                const int32_t* lens, const int32_t* cu_q, void* out, float* lse,
+                                                int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t G, int64_t Wp,
+                                                int64_t B, int64_t W, int64_t max_q, int64_t n_pages,
+                                                int64_t page_size, int64_t q_st, int64_t q_sh, int64_t c_page,
+                                                int64_t c_head, int64_t c_slot, int64_t s_page, int64_t s_head,
+                                                int64_t s_slot, double scale, int dtype, int cache_dtype,
+                                                void* workspace, int64_t workspace_bytes, hipStream_t stream) {
+  using namespace tb::prefix;
+  const char* what = "tb_shared_prefix_attention";
+  if (tb_status s = check_sizes(what, T, Hq, Hkv, D, G, Wp, B, W, page_size, max_q)) return s;
+  TB_CHECK_ARG(dtype == F16 || dtype == BF16, "%s: unknown dtype %d", what, dtype);
+  TB_CHECK_ARG(cache_dtype == dtype || cache_dtype == 3, "%s: the cache holds %d, the queries are %d (3 is e4m3)", what,
+               cache_dtype, dtype);
+  TB_CHECK_ARG((cache_dtype == 3) == (k_scale != nullptr) && (cache_dtype == 3) == (v_scale != nullptr),
+               "%s: scales belong to e4m3 caches, and only to them", what);
+  TB_CHECK_ARG(n_pages >= 1 && n_pages <= ((1ll << 31) - 1) / page_size, "%s: bad number of pages %lld", what,
+               (long long)n_pages);
+  if (T == 0) return TB_OK;
+  TB_CHECK_ARG(B >= 1 && W >= 1, "%s: queries without sequences", what);
+  TB_CHECK_ARG(q && k_cache && v_cache && pages && lens && cu_q && out && lse, "%s: null pointer", what);
+  TB_CHECK_ARG(G == 0 || (prefix_pages && prefix_lens && group_offsets), "%s: null pointer", what);
+  TB_CHECK_ALIGN(q, 16, "q");
+  TB_CHECK_ALIGN(k_cache, 16, "k_cache");
+  TB_CHECK_ALIGN(v_cache, 16, "v_cache");
+  TB_CHECK_ALIGN(out, 16, "out");
+  const int64_t chunk = cache_dtype == 3 ? 16 : 8;  // elements of 16 bytes
+  TB_CHECK_ARG(q_st % 8 == 0 && q_sh % 8 == 0, "%s: q's strides must be multiples of 8 elements", what);
+  TB_CHECK_ARG(c_page % chunk == 0 && c_head % chunk == 0 && c_slot % chunk == 0,
+               "%s: the cache's strides must be multiples of 16 bytes", what);
+  const Plan p = make_plan(T, Hq, Hkv, D, G, Wp, B, W, page_size, max_q);
+  if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes)) {
+    tb::set_error("%s: needs a workspace of %lld bytes, got %lld", what, (long long)p.bytes,
+                  (long long)(workspace ? workspace_bytes : 0));
+    return TB_E_WORKSPACE;
+  }
+  if (p.bytes > 0) TB_CHECK_ALIGN(workspace, 16, "workspace");
+  Args a{};
+  a.q = q;
+  a.q_st = q_st;
+  a.q_sh = q_sh;
+  a.kc = (const char*)k_cache;
+  a.vc = (const char*)v_cache;
+  a.c_page = c_page;
+  a.c_head = c_head;
+  a.c_slot = c_slot;
+  a.ks = k_scale;
+  a.vs = v_scale;
+  a.s_page = s_page;
+  a.s_head = s_head;
+  a.s_slot = s_slot;
+  a.prefix_pages = prefix_pages;
+  a.prefix_lens = G > 0 ? prefix_lens : nullptr;
+  a.group_offsets = G > 0 ? group_offsets : nullptr;
+  a.pages = pages;
+  a.lens = lens;
+  a.cu_q = cu_q;
+  a.out = out;
+  a.lse = lse;
+  a.part_o = (float*)workspace;
+  a.part_ml = (float2*)((char*)workspace + (int64_t)(p.S1 + p.S2) * T * Hq * D * 4);
+  a.T = (int)T;
+  a.Hq = (int)Hq;
+  a.Hkv = (int)Hkv;
+  a.grp = (int)(Hq / Hkv);
+  a.G = G > 0 ? (int)G : 1;
+  a.Wp = (int)Wp;
+  a.B = (int)B;
+  a.W = (int)W;
+  a.n_pages = (int)n_pages;
+  a.page_shift = __builtin_ctzll((unsigned long long)page_size);
+  a.S1 = p.S1;
+  a.S2 = p.S2;
+  a.direct = !p.combine;
+  a.scale_log2 = (float)(scale * 1.44269504088896340736);
+  const bool e8 = cache_dtype == 3;
+  return dtype == F16 ? launch_for<F16>(e8, D, a, p, stream, what) : launch_for<BF16>(e8, D, a, p, stream, what);
+}

@@ -392,6 +392,24 @@ def generate_rope_kv_append_inputs(T, axes=1, Hq=32, Hkv=8, D=128, page=64, cach
     return (q, k, v, positions.to(device), inv_freq.to(device), ax.to(device), slots.to(device), *pools)
 
 
+def generate_shared_prefix_attention_inputs(B, prefix, own, Hq=32, Hkv=8, D=128, page=64, n_q=1, groups=1, cache="same",
+                                            dtype=torch.float16, seed=0, device=DEFAULT_DEVICE):
+    """B sequences of `own` // 2 .. `own` tokens, n_q queries each, behind `groups` prefixes of `prefix` tokens."""
+    g = _gen(seed)
+    lens = torch.randint(max(n_q, own // 2), max(n_q, own) + 1, (B,), generator=g).int()
+    Wp, W = -(-prefix // page), -(-max(n_q, own) // page)
+    order = torch.randperm(groups * Wp + B * W, generator=g).int()
+    pools = paged_cache(order.numel(), Hkv, page, D, dtype, g, cache == "e4m3", device)
+    q = torch.randn(B * n_q, Hq, D, generator=g).to(dtype)
+    bounds = torch.tensor([B * i // groups for i in range(groups + 1)]).int()
+    cu_q = (torch.arange(B + 1) * n_q).int()
+    shared = (None, None, None) if prefix == 0 else tuple(
+        t.to(device) for t in (order[:groups * Wp].view(groups, Wp), torch.full((groups,), prefix).int(), bounds))
+    own_pages = order[groups * Wp:].view(B, W)
+    return (q.to(device), pools[0], pools[1], *shared, own_pages.to(device), lens.to(device), cu_q.to(device), n_q, None,
+            *pools[2:])
+
+
 GENERATORS = {
     "int4_dequant": generate_int4_dequant_inputs,
     "w4a16_gemm": generate_w4a16_gemm_inputs,
@@ -409,6 +427,7 @@ GENERATORS = {
     "fp8_block_scaled_gemm": generate_fp8_block_scaled_gemm_inputs,
     "rotary_axes": generate_rotary_axes_inputs,
     "rope_kv_append": generate_rope_kv_append_inputs,
+    "shared_prefix_attention": generate_shared_prefix_attention_inputs,
 }
 
 
@@ -442,6 +461,8 @@ def infer_problem_size(operator_name, params):
         return p.get("T", 1) * (p.get("Hq", 1) + p.get("Hk", 0)) * p.get("D", 1)
     if operator_name == "rope_kv_append":
         return p.get("T", 1) * (p.get("Hq", 1) + 2 * p.get("Hkv", 1)) * p.get("D", 1)
+    if operator_name == "shared_prefix_attention":
+        return 4 * p.get("B", 1) * p.get("n_q", 1) * (p.get("prefix", 0) + p.get("own", 1)) * p.get("Hq", 1) * p.get("D", 1)
     size, used = 1, False
     for v in p.values():
         size *= max(1, v)
