@@ -9,12 +9,12 @@
 // Rows.  The query heads of one key/value head and the queries of one sequence
 // read the same tokens, so they are rows of one product: row r of a run of
 // queries is query r / grp, head r % grp of the group.  Three kinds of work:
-//   tiles   128 rows of a group of more than 32 rows: over the shared prefix, and
-//           on over the own tokens of those sequences that have more than 32 rows
-//   few     the own tokens of one sequence of up to 32 rows, or the prefix of a
-//           group of up to 32 rows: the block's four wavefronts split the tokens
+//   tiles   64 or 128 rows of a group of more than 16 rows: over the shared prefix, and
+//           on over the own tokens of those sequences that have more than 16 rows
+//   few     the own tokens of one sequence of up to 16 rows, or the prefix of a
+//           group of up to 16 rows: the block's four wavefronts split the tokens
 //   combine joins the partial results of a row (one slot per split) by their maxima
-// so a prefix is read once per 128 rows however many sequences share it.
+// so a prefix is read once per tile however many sequences share it.
 //
 // One wavefront's step over TOK tokens in LDS (attend_tile):
 //   S^T = K Q^T    K rows from LDS, Q in registers; a lane holds one row's scores
@@ -49,10 +49,9 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 enum { F16 = 1, BF16 = 2 };
 constexpr int THREADS = 256, WAVES = 4;
-constexpr int FEW = 32;      // rows of a sequence or group that the token-splitting blocks take
-constexpr int TILE = 128;    // rows of a tile block: 32 a wavefront
-constexpr int TILE_TOK = 64; // tokens of a tile block's step
-constexpr int MAX_SLOTS = 64;
+constexpr int FEW = 16;      // rows of a sequence or group that the token-splitting blocks take
+constexpr int FILL = 512;    // blocks that fill the device: two on each of 256 CUs
+constexpr int MAX_SPLIT = 64;
 constexpr float NEG_INF = -__builtin_inff();
 
 struct Args {
@@ -78,7 +77,10 @@ struct Args {
   int n_pages, page_shift;
   int S1, S2;       // slots of tiles and prefixes, slots of own tokens
   int direct;       // own tokens in one slot and nothing else: results are final
-  float scale_log2;
+  float scale_log2;     // of |scale|, or 1 for a scale of 0
+  uint32_t flip, keep;  // applied to q
+  int big;  // some sequence may have more than FEW rows
+  int tile_blocks;
 };
 
 template <int DT>
@@ -163,6 +165,9 @@ __device__ __forceinline__ void wait_vm() {
 }
 __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory"); }
 
+// e4m3 scales of a tile, for each 32 tokens: 32 of the keys, 32 of the values.
+__device__ __forceinline__ uint32_t scale_at(uint32_t sbase, int tok) { return sbase + (tok >> 5) * 256 + (tok & 31) * 4; }
+
 // The tokens of one prefix or sequence: a row of a page table and a length.
 struct Tokens {
   const int* table;
@@ -194,6 +199,9 @@ __device__ __forceinline__ int64_t token_offset(const Args& a, const Window& w, 
   return (page * a.c_page + (tok & ((1 << a.page_shift) - 1)) * a.c_slot) * ESIZE;
 }
 
+__device__ __forceinline__ uint32_t as_uint(float x) { return __builtin_bit_cast(uint32_t, x); }
+__device__ __forceinline__ float as_float(uint32_t x) { return __builtin_bit_cast(float, x); }
+
 // ------------------------------------------------------------------ one step
 //
 // State of one wavefront: SH rows (lane l: row l % SH), head dimension D.
@@ -209,9 +217,11 @@ struct Wave {
   static constexpr int DT_N = D / SH;       // output tiles
   static constexpr int REGS = SH * SH / 64; // accumulator registers of a tile
 
-  // log2 of the largest weight.  fp16: weights down to 2^-32 (2^-28) of the largest are kept; with e4m3 values
-  // their scales are multiplied in, up to 2^12 (a row of fp16 values has at most 2^7.2).
+  // log2 of the largest weight when m is set, and how far weights may grow past it before m is set again.  fp16:
+  // weights down to 2^-32 (e4m3: 2^-28) of the largest are kept; with e4m3 values their scales are multiplied in, which leaves
+  // room for scales up to 2^10 (a row of fp16 values has at most 146).
   static constexpr float LIFT = DT == BF16 ? 0.0f : E8 ? 4.0f : 8.0f;
+  static constexpr float SLACK = DT == BF16 || !E8 ? 6.0f : 2.0f;
 
   v8 q[STEPS];
   acc_t o[DT_N];
@@ -221,12 +231,16 @@ struct Wave {
   static __device__ __forceinline__ int channel(int s, int g) {
     return E8 ? (s / 2) * NG * 16 + g * 16 + (s % 2) * 8 : s * NG * 8 + g * 8;
   }
-  __device__ __forceinline__ void init(const typename Y::el* row, bool valid) {
+  // flip, keep: the sign bits of a negative scale and nothing of q for a scale of 0 (scale_log2 is positive)
+  __device__ __forceinline__ void init(const typename Y::el* row, bool valid, uint32_t flip, uint32_t keep) {
     const int g = (threadIdx.x & 63) / SH;
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
-      q[s] = v8{};
-      if (valid) q[s] = *(const v8*)(row + channel(s, g));
+      u32x4 x{};
+      if (valid) x = *(const u32x4*)(row + channel(s, g));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = (x[i] & keep) ^ flip;
+      q[s] = __builtin_bit_cast(v8, x);
     }
 #pragma unroll
     for (int d = 0; d < DT_N; ++d) o[d] = acc_t{};
@@ -237,13 +251,22 @@ struct Wave {
   static __device__ __forceinline__ int token_of(int r, int g) {
     return SH == 16 ? g * 4 + r : 8 * (r / 4) + 4 * g + r % 4;
   }
+  // over the lane groups, which hold the same rows (a swap of a value's halves with a copy's gives every lane both)
   static __device__ __forceinline__ float over_groups_max(float x) {
-    if (SH == 16) x = fmaxf(x, __shfl_xor(x, 16));
-    return fmaxf(x, __shfl_xor(x, 32));
+    if (SH == 16) {
+      const auto y = __builtin_amdgcn_permlane16_swap(as_uint(x), as_uint(x), false, false);
+      x = fmaxf(as_float(y[0]), as_float(y[1]));
+    }
+    const auto z = __builtin_amdgcn_permlane32_swap(as_uint(x), as_uint(x), false, false);
+    return fmaxf(as_float(z[0]), as_float(z[1]));
   }
   static __device__ __forceinline__ float over_groups_sum(float x) {
-    if (SH == 16) x += __shfl_xor(x, 16);
-    return x + __shfl_xor(x, 32);
+    if (SH == 16) {
+      const auto y = __builtin_amdgcn_permlane16_swap(as_uint(x), as_uint(x), false, false);
+      x = as_float(y[0]) + as_float(y[1]);
+    }
+    const auto z = __builtin_amdgcn_permlane32_swap(as_uint(x), as_uint(x), false, false);
+    return as_float(z[0]) + as_float(z[1]);
   }
 
   // S^T of TOK tokens: TOK / SH tiles
@@ -282,12 +305,11 @@ struct Wave {
     }
   }
 
-  // scores -> weights, in place of the scores; the running maximum, sum and outputs are brought up to date.
-  // vs: the values' scales of the lane's tokens (e4m3), multiplied into the weights after the sum.
-  // returns the weights as operands of the second product.
+  // Scores -> weights exp2(score - m), the operands of the second product.  m follows the running maximum in steps:
+  // while no row of the wavefront passes its m by 2^SLACK beyond the lift, sums and outputs stay as they are.
   template <int TOK>
   __device__ __forceinline__ void weights(acc_t (&s)[TOK / SH], int t0, int limit, bool full, float scale,
-                                          uint32_t sbase, v8 (&p)[TOK / KS]) {
+                                          uint32_t sbase, int tok0, v8 (&p)[TOK / KS]) {
     const int g = (threadIdx.x & 63) / SH;
     float top = NEG_INF;
 #pragma unroll
@@ -295,39 +317,47 @@ struct Wave {
 #pragma unroll
       for (int r = 0; r < REGS; r += 4) {
         const int tok = t * SH + token_of(r, g);
-        f32x4 k;
-        if (E8) k = lds_read<f32x4>(sbase + tok * 4);
+        if (E8) {
+          const f32x4 k = lds_read<f32x4>(scale_at(sbase, tok0 + tok));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float x = s[t][r + i] * (E8 ? k[i] * scale : scale);
-          if (!full) x = t0 + tok + i < limit ? x : NEG_INF;
-          s[t][r + i] = x;
-          top = fmaxf(top, x);
+          for (int i = 0; i < 4; ++i) s[t][r + i] *= k[i];
         }
+        if (!full) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[t][r + i] = t0 + tok + i < limit ? s[t][r + i] : NEG_INF;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, s[t][r + i]);
+        if (E8 && r % 8 == 4) __builtin_amdgcn_sched_barrier(0);  // all scales at once would spill
       }
-    const float ref = fmaxf(m, over_groups_max(top) - LIFT);
-    const float use = ref == NEG_INF ? 0.0f : ref;
-    const float alpha = __builtin_amdgcn_exp2f(m - use);
-    m = ref;
+    top = over_groups_max(top) * scale;
+    if (__any(top > m + (LIFT + SLACK))) {
+      const float ref = fmaxf(m, top - LIFT);
+      const float alpha = __builtin_amdgcn_exp2f(m - (ref == NEG_INF ? 0.0f : ref));
+      m = ref;
+      l *= alpha;
+#pragma unroll
+      for (int d = 0; d < DT_N; ++d)
+#pragma unroll
+        for (int r = 0; r < REGS; ++r) o[d][r] *= alpha;
+    }
+    const float use = m == NEG_INF ? 0.0f : m;
     float sum = 0.0f;
 #pragma unroll
     for (int t = 0; t < TOK / SH; ++t)
 #pragma unroll
       for (int r = 0; r < REGS; r += 4) {
         f32x4 v;
-        if (E8) v = lds_read<f32x4>(sbase + (TOK + t * SH + token_of(r, g)) * 4);
+        if (E8) v = lds_read<f32x4>(scale_at(sbase, tok0 + t * SH + token_of(r, g)) + 128);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float w = __builtin_amdgcn_exp2f(s[t][r + i] - use);
+          const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r + i], scale, -use));
           sum += w;
           s[t][r + i] = !E8 ? w : full || w > 0.0f ? w * v[i] : 0.0f;
         }
+        if (E8 && r % 8 == 4) __builtin_amdgcn_sched_barrier(0);
       }
-    l = l * alpha + sum;
-#pragma unroll
-    for (int d = 0; d < DT_N; ++d)
-#pragma unroll
-      for (int r = 0; r < REGS; ++r) o[d][r] *= alpha;
+    l += sum;
 #pragma unroll
     for (int k = 0; k < TOK / KS; ++k)
 #pragma unroll
@@ -390,9 +420,9 @@ struct Wave {
     const Values v(vbase);
     if (full) {
 #pragma unroll
-      for (int d = 0; d < DT_N; ++d)
+      for (int k = 0; k < TOK / KS; ++k)
 #pragma unroll
-        for (int k = 0; k < TOK / KS; ++k) o[d] = Y::mfma(v.read(d, k), p[k], o[d]);
+        for (int d = 0; d < DT_N; ++d) o[d] = Y::mfma(v.read(d, k), p[k], o[d]);
       return;
     }
     uint32_t bad = 0;
@@ -522,11 +552,12 @@ struct FewLayout {
   static constexpr int LDS = MARKS + WAVES * 32 * 64;
 };
 
-// Rows 0 .. rows - 1 (at most 32) from query q0 on, key/value head h, tokens of `src`, split `split` of `splits`;
+// Rows 0 .. rows - 1 (at most 16) from query q0 on, key/value head h, tokens of `src`, split `split` of `splits`;
 // results to slot `slot`.
-template <int DT, bool E8, int D, int SH>
+template <int DT, bool E8, int D>
 __device__ __forceinline__ void attend_few(const Args& a, char* smem, int h, int q0, int rows, const Tokens& src,
                                            int base, int split, int splits, int slot, const Seq* seq, int b0, int b1) {
+  constexpr int SH = 16;
   typedef FewLayout<DT, E8, D> L;
   typedef Wave<DT, E8, D, SH> W;
   typedef typename W::Y::el el;
@@ -546,7 +577,7 @@ __device__ __forceinline__ void attend_few(const Args& a, char* smem, int h, int
   }
 
   W w;
-  w.init((const el*)a.q + t * a.q_st + hq * a.q_sh, valid);
+  w.init((const el*)a.q + t * a.q_st + hq * a.q_sh, valid, a.flip, a.keep);
 
   const int tiles = (src.len + TOK - 1) / TOK;
   const int lo = (int)((int64_t)tiles * split / splits), hi = (int)((int64_t)tiles * (split + 1) / splits);
@@ -575,14 +606,14 @@ __device__ __forceinline__ void attend_few(const Args& a, char* smem, int h, int
         dma16(vbase + i * 1024, vp + off + ((pos ^ swizzle_v<RB, SH, E8>(r)) << 4));
     }
   };
-  auto fill_scales = [&](int n) __attribute__((always_inline)) {  // TOK scales of keys, then TOK of values
-    const int t0 = n * TOK;
-    static_assert(TOK == 64 || !E8, "one scale a lane");
-    const int tok = min(t0 + lane, src.len - 1);
-    const int page = __builtin_amdgcn_ds_bpermute(((tok >> a.page_shift) - win.first) << 2, win.ids);
-    const int64_t off = page * a.s_page + h * a.s_head + (tok & ((1 << a.page_shift) - 1)) * a.s_slot;
-    dma4(sbase, (const char*)(a.ks + off));
-    dma4(sbase + TOK * 4, (const char*)(a.vs + off));
+  auto fill_scales = [&](int n) __attribute__((always_inline)) {  // 32 tokens a copy: keys' scales, then values'
+#pragma unroll
+    for (int i = 0; i < TOK / 32; ++i) {
+      const int tok = min(n * TOK + i * 32 + (lane & 31), src.len - 1);
+      const int page = __builtin_amdgcn_ds_bpermute(((tok >> a.page_shift) - win.first) << 2, win.ids);
+      const int64_t off = page * a.s_page + h * a.s_head + (tok & ((1 << a.page_shift) - 1)) * a.s_slot;
+      dma4(sbase + i * 256, (const char*)((lane < 32 ? a.ks : a.vs) + off));
+    }
   };
 
   // Keys and values have one buffer each: the next keys are fetched from when the
@@ -600,15 +631,15 @@ __device__ __forceinline__ void attend_few(const Args& a, char* smem, int h, int
     typename W::v8 p[TOK / W::KS];
     wait_vm<NI>();  // keys (and scales) are there; the values may be on their way
     w.template scores<TOK>(kbase, s);
-    if (E8) w.template weights<TOK>(s, t0, limit, full, a.scale_log2, sbase, p);
+    if (E8) w.template weights<TOK>(s, t0, limit, full, a.scale_log2, sbase, 0, p);
     wait_lds();
     if (n + 1 < n1) {
       cover(n + 1);
       if (E8) fill_scales(n + 1);
       fill(n + 1, true);
     }
-    if (!E8) w.template weights<TOK>(s, t0, limit, full, a.scale_log2, sbase, p);
-    if (n + 1 < n1) wait_vm<NI + (E8 ? 2 : 0)>(); else wait_vm<0>();
+    if (!E8) w.template weights<TOK>(s, t0, limit, full, a.scale_log2, sbase, 0, p);
+    if (n + 1 < n1) wait_vm<NI + (E8 ? TOK / 32 : 0)>(); else wait_vm<0>();
     w.template values<TOK>(vbase, p, t0, limit, full, marks);
     wait_lds();
     if (n + 1 < n1) fill(n + 1, false);
@@ -672,20 +703,18 @@ __device__ __forceinline__ void empty_rows(const Args& a, int h, int t0, int t1)
   }
 }
 
-// Blocks: own tokens of sequence b (b < B), prefix of group b - B; key/value head; split.
+// Block `index`: own tokens of sequence b (b < B) or prefix of group b - B; key/value head; split.
 template <int DT, bool E8, int D>
-__global__ void __launch_bounds__(THREADS, 2) few_rows(Args a) {
-  extern __shared__ __align__(16) char smem[];
-  const int unit = blockIdx.x / a.Hkv, h = blockIdx.x % a.Hkv, split = blockIdx.y;
+__device__ __forceinline__ void few_rows(const Args& a, char* smem, int index) {
   constexpr int TOK = FewLayout<DT, E8, D>::TOK;
-  if (unit < a.B) {
-    const int b = unit;
+  const int own_blocks = a.B * a.Hkv * a.S2;
+  if (index < own_blocks) {
+    const int split = index / (a.B * a.Hkv), unit = index % (a.B * a.Hkv), b = unit / a.Hkv, h = unit % a.Hkv;
     if (a.direct && b == 0) {  // rows of no sequence
       const int first = query_start(a, 0);
       empty_rows<DT, D>(a, h, 0, first);
       empty_rows<DT, D>(a, h, max(query_start(a, a.B), first), a.T);
     }
-    if (split >= a.S2) return;
     const Seq s = sequence(a, b);
     const int rows = s.n_q * a.grp;
     // splits of at least two steps a wavefront
@@ -702,13 +731,10 @@ __global__ void __launch_bounds__(THREADS, 2) few_rows(Args a) {
     }
     if (rows == 0) return;
     const Tokens src{a.pages + (int64_t)b * a.W, a.W, s.own};
-    if (rows <= 16)
-      attend_few<DT, E8, D, 16>(a, smem, h, s.q0, rows, src, 0, split, used, a.S1 + split, &s, 0, 0);
-    else
-      attend_few<DT, E8, D, 32>(a, smem, h, s.q0, rows, src, 0, split, used, a.S1 + split, &s, 0, 0);
+    attend_few<DT, E8, D>(a, smem, h, s.q0, rows, src, 0, split, used, a.S1 + split, &s, 0, 0);
   } else {
-    const int g = unit - a.B;
-    if (split >= a.S1) return;
+    index -= own_blocks;
+    const int split = index / (a.G * a.Hkv), unit = index % (a.G * a.Hkv), g = unit / a.Hkv, h = unit % a.Hkv;
     const Group gr = group(a, g);
     if (gr.rows > FEW || gr.rows == 0) return;
     const int used = clamp_int((gr.len + 8 * TOK - 1) / (8 * TOK), 1, a.S1);
@@ -718,34 +744,66 @@ __global__ void __launch_bounds__(THREADS, 2) few_rows(Args a) {
       return;
     }
     const Tokens src{a.prefix_pages + (int64_t)g * a.Wp, a.Wp, gr.len};
-    if (gr.rows <= 16)
-      attend_few<DT, E8, D, 16>(a, smem, h, gr.q0, gr.rows, src, -1, split, used, split, nullptr, gr.b0, gr.b1);
-    else
-      attend_few<DT, E8, D, 32>(a, smem, h, gr.q0, gr.rows, src, -1, split, used, split, nullptr, gr.b0, gr.b1);
+    attend_few<DT, E8, D>(a, smem, h, gr.q0, gr.rows, src, -1, split, used, split, nullptr, gr.b0, gr.b1);
   }
 }
 
 // ------------------------------------------------------------------ tiles of rows
-
-template <int DT, bool E8, int D>
+//
+// RW wavefronts side by side hold the tile's 32 * RW rows, 4 / RW wavefronts share the tokens of a step.
+template <int DT, bool E8, int D, int RW>
 struct TileLayout {
   static constexpr int RB = D * (E8 ? 1 : 2);
-  static constexpr int TILE_BYTES = TILE_TOK * RB;
-  static constexpr int STAGE = 2 * TILE_BYTES + (E8 ? 2 * TILE_TOK * 4 : 0);
+  static constexpr int ROWS = 32 * RW;
+  static constexpr int TOK = RB == 256 ? 64 : 128;  // tokens of a step
+  static constexpr int TILE_BYTES = TOK * RB;
+  static constexpr int STAGE = 2 * TILE_BYTES + (E8 ? 2 * TOK * 4 : 0);
+  static constexpr int MERGE_ROW = D + 4;
   static constexpr int MARKS = 2 * STAGE;
   static constexpr int LDS = MARKS + WAVES * 32 * 64;
+  static_assert(RW == 4 || MARKS >= ROWS * (MERGE_ROW * 4 + 8), "the merge reuses the stages");
 };
 
-// The tile (group, row tile) number `index`, or false past the last one.  64 groups at a time.
-__device__ __forceinline__ bool find_tile(const Args& a, int index, int& g, int& tile) {
+// Unit (group, row tile, key/value head) and split of tile block `index`; false past the last one.  Units come in
+// rounds of FILL blocks; those of a last, partial round are cut into up to S1 splits that fill the device.  A head's
+// units lie S1 and Hkv apart in block numbers, so with 8 heads they run on one XCD, whose L2 then holds the keys and
+// values that they share.
+struct TileUnit {
+  int g, tile, h, split, splits;
+};
+template <int ROWS>
+__device__ __forceinline__ bool find_tile(const Args& a, int index, TileUnit& u) {
   const int lane = threadIdx.x & 63;
+  auto count = [&](int x) __attribute__((always_inline)) {  // tiles of group x
+    if (x >= a.G) return 0;
+    const Group gr = group(a, x);
+    return gr.rows > FEW ? (gr.rows + ROWS - 1) / ROWS : 0;
+  };
+  int n = 0, total = 0;
+  for (int x0 = (a.G - 1) / 64 * 64; x0 >= 0; x0 -= 64) {  // downwards: ends with the first groups in registers
+    n = count(x0 + lane);
+    total += n;
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) total += __shfl_xor(total, d);
+  const int units = __builtin_amdgcn_readfirstlane(total) * a.Hkv;
+  const int whole = units / FILL * FILL, tail = units - whole;
+  const int splits = tail ? clamp_int(FILL / tail, 1, a.S1) : 1;
+  int unit = index;
+  u.split = 0;
+  u.splits = 1;
+  if (index >= whole) {
+    index -= whole;
+    if (index >= tail * splits) return false;
+    unit = whole + index % tail;
+    u.split = index / tail;
+    u.splits = splits;
+  }
+  u.h = unit % a.Hkv;
+  const int tile = unit / a.Hkv;
   int seen = 0;
   for (int x0 = 0; x0 < a.G; x0 += 64) {
-    int n = 0;
-    if (x0 + lane < a.G) {
-      const Group gr = group(a, x0 + lane);
-      n = gr.rows > FEW ? (gr.rows + TILE - 1) / TILE : 0;
-    }
+    if (x0 > 0) n = count(x0 + lane);
     int incl = n;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -753,10 +811,10 @@ __device__ __forceinline__ bool find_tile(const Args& a, int index, int& g, int&
       if (lane >= d) incl += o;
     }
     const int here = __builtin_amdgcn_readfirstlane(__shfl(incl, 63));
-    if (index < seen + here) {
-      const int l = __builtin_ctzll(__ballot(seen + incl > index));
-      g = __builtin_amdgcn_readfirstlane(x0 + l);
-      tile = __builtin_amdgcn_readfirstlane(index - seen - __shfl(incl - n, l));
+    if (tile < seen + here) {
+      const int l = __builtin_ctzll(__ballot(seen + incl > tile));
+      u.g = __builtin_amdgcn_readfirstlane(x0 + l);
+      u.tile = __builtin_amdgcn_readfirstlane(tile - seen - __shfl(incl - n, l));
       return true;
     }
     seen += here;
@@ -764,21 +822,25 @@ __device__ __forceinline__ bool find_tile(const Args& a, int index, int& g, int&
   return false;
 }
 
-template <int DT, bool E8, int D>
-__global__ void __launch_bounds__(THREADS, 2) row_tiles(Args a) {
-  extern __shared__ __align__(16) char smem[];
-  typedef TileLayout<DT, E8, D> L;
-  constexpr int SH = 32, TOK = TILE_TOK, RB = L::RB, RPI = 1024 / RB, ESIZE = E8 ? 1 : 2;
-  constexpr int NI = TOK / WAVES / RPI;  // copies of a wavefront per tile of keys or values
-  static_assert(NI >= 1, "a wavefront fills 16 rows");
+template <int DT, bool E8, int D, int RW>
+__device__ __forceinline__ void row_tile(const Args& a, char* smem, int index) {
+  typedef TileLayout<DT, E8, D, RW> L;
+  constexpr int SH = 32, TOK = L::TOK, RB = L::RB, RPI = 1024 / RB, ESIZE = E8 ? 1 : 2;
+  constexpr int MINE = TOK / WAVES;            // tokens that a wavefront fetches
+  constexpr int NI = MINE / RPI;               // in copies of 1 KiB
+  constexpr int SHARE = TOK * RW / WAVES;      // tokens that a wavefront attends to
+  constexpr int MOST = E8 ? 32 : 64;           // in steps of so many (e4m3: 64 would spill)
+  constexpr int STEP = SHARE > MOST ? MOST : SHARE;
+  static_assert(NI >= 1, "a wavefront fetches whole copies");
   typedef Wave<DT, E8, D, SH> W;
   typedef typename W::Y::el el;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int h = blockIdx.y % a.Hkv, split = blockIdx.y / a.Hkv;
-  int g, tile;
-  if (!find_tile(a, blockIdx.x, g, tile)) return;
-  const Group gr = group(a, g);
-  const int row = tile * TILE + wave * SH + lane % SH;
+  const int wr = wave % RW, wt = wave / RW;
+  TileUnit u;
+  if (!find_tile<L::ROWS>(a, index, u)) return;
+  const int h = u.h;
+  const Group gr = group(a, u.g);
+  const int row = u.tile * L::ROWS + wr * SH + lane % SH;
   const bool valid = row < gr.rows;
   const int t = gr.q0 + row / a.grp, hq = h * a.grp + row % a.grp;
 
@@ -794,13 +856,16 @@ __global__ void __launch_bounds__(THREADS, 2) row_tiles(Args a) {
   const int prefix_limit = valid ? clamp_int(gr.len + end, 0, gr.len) : 0;
 
   W w;
-  w.init((const el*)a.q + t * a.q_st + hq * a.q_sh, valid);
+  w.init((const el*)a.q + t * a.q_st + hq * a.q_sh, valid, a.flip, a.keep);
 
   // The tile's tokens: the prefix, then the own tokens (as far as a row of the tile sees them) of each of its
-  // sequences with more than 32 rows.  Steps are counted over all of them and shared out to the splits.
-  const int t_first = gr.q0 + tile * TILE / a.grp;
-  const int t_last = gr.q0 + (min((tile + 1) * TILE, gr.rows) - 1) / a.grp;
-  const int b_first = sequence_of(a, t_first, gr.b0, gr.b1), b_last = sequence_of(a, t_last, gr.b0, gr.b1);
+  // sequences with more than 16 rows.  Steps are counted over all of them and shared out to the splits.
+  int b_first = gr.b0, b_last = gr.b0 - 1, t_last = 0;
+  if (a.big) {
+    t_last = gr.q0 + (min((u.tile + 1) * L::ROWS, gr.rows) - 1) / a.grp;
+    b_first = sequence_of(a, gr.q0 + u.tile * L::ROWS / a.grp, gr.b0, gr.b1);
+    b_last = sequence_of(a, t_last, gr.b0, gr.b1);
+  }
   auto own_tokens = [&](int x) __attribute__((always_inline)) {
     const Seq s = sequence(a, x);
     if (s.n_q * a.grp <= FEW) return 0;
@@ -810,8 +875,8 @@ __global__ void __launch_bounds__(THREADS, 2) row_tiles(Args a) {
   int steps = (gr.len + TOK - 1) / TOK;
   for (int x = b_first; x <= b_last; ++x) steps += (own_tokens(x) + TOK - 1) / TOK;
   steps = __builtin_amdgcn_readfirstlane(steps);
-  int skip = (int)((int64_t)steps * split / a.S1);
-  int todo = (int)((int64_t)steps * (split + 1) / a.S1) - skip;
+  int skip = (int)((int64_t)steps * u.split / u.splits);
+  int todo = (int)((int64_t)steps * (u.split + 1) / u.splits) - skip;
 
   const uint32_t base = lds_addr(smem), marks = base + L::MARKS + wave * W::MARKS;
   W::clear_marks(marks);
@@ -829,55 +894,96 @@ __global__ void __launch_bounds__(THREADS, 2) row_tiles(Args a) {
     const int n0 = skip, n1 = min(n_all, skip + todo);
     skip = 0;
     todo -= n1 - n0;
-    const Tokens src = pre ? Tokens{a.prefix_pages + (int64_t)g * a.Wp, a.Wp, len}
+    const Tokens src = pre ? Tokens{a.prefix_pages + (int64_t)u.g * a.Wp, a.Wp, len}
                            : Tokens{a.pages + (int64_t)x * a.W, a.W, len};
     int limit = pre ? prefix_limit : b == x ? own_limit : 0;
     const bool some = valid && limit > 0;
     if (!valid) limit = 0x7FFFFFFF;
     Window win;
     auto fill = [&](int n) __attribute__((always_inline)) {
-      const int t0 = n * TOK;
-      const uint32_t kb = base + (n & 1) * L::STAGE, vb = kb + L::TILE_BYTES, sb = vb + L::TILE_BYTES;
-      win.cover(src, t0 >> a.page_shift, min(t0 + TOK - 1, src.len - 1) >> a.page_shift, a.n_pages);
+      const int t0 = n * TOK + wave * MINE;  // the wavefront's first token
+      const uint32_t kb = base + (n & 1) * L::STAGE + wave * NI * 1024, vb = kb + L::TILE_BYTES;
+      win.cover(src, min(t0, src.len - 1) >> a.page_shift, min(t0 + MINE - 1, src.len - 1) >> a.page_shift, a.n_pages);
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
-        const int r = (wave * NI + i) * RPI + lane / (RB / 16), pos = lane % (RB / 16);
-        const int64_t off = token_offset<TOK, ESIZE>(a, win, src, t0, t0 + r);
-        dma16(kb + (wave * NI + i) * 1024, kp + off + ((pos ^ swizzle_k<RB>(r)) << 4));
-        dma16(vb + (wave * NI + i) * 1024, vp + off + ((pos ^ swizzle_v<RB, SH, E8>(r)) << 4));
+        const int r = i * RPI + lane / (RB / 16), pos = lane % (RB / 16);
+        const int64_t off = token_offset<MINE, ESIZE>(a, win, src, t0, t0 + r);
+        dma16(kb + i * 1024, kp + off + ((pos ^ swizzle_k<RB>(wave * MINE + r)) << 4));
+        dma16(vb + i * 1024, vp + off + ((pos ^ swizzle_v<RB, SH, E8>(wave * MINE + r)) << 4));
       }
-      if (E8 && wave < 2) {
-        const int tok = min(t0 + lane, src.len - 1);
+      if (E8) {
+        static_assert(MINE == 32 || !E8, "the scales of 32 tokens a copy");
+        const int tok = min(t0 + (lane & 31), src.len - 1);
         const int page = __builtin_amdgcn_ds_bpermute(((tok >> a.page_shift) - win.first) << 2, win.ids);
         const int64_t off = page * a.s_page + h * a.s_head + (tok & ((1 << a.page_shift) - 1)) * a.s_slot;
-        dma4(sb + wave * TOK * 4, (const char*)((wave ? a.vs : a.ks) + off));
+        dma4(base + (n & 1) * L::STAGE + 2 * L::TILE_BYTES + wave * 256, (const char*)((lane < 32 ? a.ks : a.vs) + off));
       }
     };
     // both stages may still be read from the segment before
     __syncthreads();
     fill(n0);
     for (int n = n0; n < n1; ++n) {
-      const int t0 = n * TOK;
       wait_vm<0>();
       wait_lds();
       __builtin_amdgcn_s_barrier();  // the step's tokens are there, the other stage is free
       if (n + 1 < n1) fill(n + 1);
-      if (!__any(some && limit > t0)) continue;
-      const bool full = __all(limit >= t0 + TOK);
-      const uint32_t kb = base + (n & 1) * L::STAGE, vb = kb + L::TILE_BYTES, sb = vb + L::TILE_BYTES;
-      typename W::acc_t s[TOK / SH];
-      typename W::v8 p[TOK / W::KS];
-      w.template scores<TOK>(kb, s);
-      w.template weights<TOK>(s, t0, limit, full, a.scale_log2, sb, p);
-      w.template values<TOK>(vb, p, t0, limit, full, marks);
+#pragma unroll
+      for (int c = 0; c < SHARE / STEP; ++c) {
+        const int tok0 = wt * SHARE + c * STEP, t0 = n * TOK + tok0;
+        if (!__any(some && limit > t0)) continue;
+        const bool full = __all(limit >= t0 + STEP);
+        const uint32_t kb = base + (n & 1) * L::STAGE + tok0 * RB, vb = kb + L::TILE_BYTES;
+        const uint32_t sb = base + (n & 1) * L::STAGE + 2 * L::TILE_BYTES;
+        typename W::acc_t s[STEP / SH];
+        typename W::v8 p[STEP / W::KS];
+        w.template scores<STEP>(kb, s);
+        w.template weights<STEP>(s, t0, limit, full, a.scale_log2, sb, tok0, p);
+        w.template values<STEP>(vb, p, t0, limit, full, marks);
+      }
     }
   }
 
-  const float l = W::over_groups_sum(w.l);
-  if (!valid) return;
+  float l = W::over_groups_sum(w.l), alpha = 1.0f;
   const int gx = lane / SH;
-  const int64_t id = (int64_t)t * a.Hq + hq, slot = (int64_t)split * a.T * a.Hq + id;
-  const bool final = a.S1 == 1 && big;
+  float* merge = (float*)smem;
+  float2* ml = (float2*)(merge + L::ROWS * L::MERGE_ROW);
+  if (RW < WAVES) {
+    // the wavefronts that share a row: the second hands its results to the first
+    static_assert(RW == WAVES || RW * 2 == WAVES, "two halves");
+    const int r = wr * SH + lane % SH;
+    __syncthreads();
+    if (wt == 1) {
+#pragma unroll
+      for (int d = 0; d < W::DT_N; ++d)
+#pragma unroll
+        for (int i = 0; i < W::REGS; i += 4) {
+          f32x4 x;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = w.o[d][i + e];
+          *(f32x4*)(merge + r * L::MERGE_ROW + d * SH + W::token_of(i, gx)) = x;
+        }
+      if (gx == 0) ml[r] = float2{w.m, l};
+    }
+    __syncthreads();
+    if (wt == 1) return;
+    const float2 other = ml[r];
+    const float top = fmaxf(w.m, other.x), use = top == NEG_INF ? 0.0f : top;
+    alpha = __builtin_amdgcn_exp2f(w.m - use);
+    const float beta = __builtin_amdgcn_exp2f(other.x - use);
+    l = l * alpha + other.y * beta;
+    w.m = top;
+#pragma unroll
+    for (int d = 0; d < W::DT_N; ++d)
+#pragma unroll
+      for (int i = 0; i < W::REGS; i += 4) {
+        const f32x4 x = *(const f32x4*)(merge + r * L::MERGE_ROW + d * SH + W::token_of(i, gx));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w.o[d][i + e] = w.o[d][i + e] * alpha + x[e] * beta;
+      }
+  }
+  if (!valid) return;
+  const int64_t id = (int64_t)t * a.Hq + hq, slots = (int64_t)a.T * a.Hq, slot = u.split * slots + id;
+  const bool final = u.splits == 1 && big;
   const float inv = final ? inverse(l) : 1.0f;
 #pragma unroll
   for (int d = 0; d < W::DT_N; ++d)
@@ -888,6 +994,7 @@ __global__ void __launch_bounds__(THREADS, 2) row_tiles(Args a) {
       for (int i = 0; i < 4; ++i) x[i] = w.o[d][r + i] * inv;
       const int c = d * SH + W::token_of(r, gx);
       x = W::marked(x, marks, lane % SH, c);
+      if (RW < WAVES) x = W::marked(x, marks + RW * W::MARKS, lane % SH, c);
       if (final)
         store4((el*)a.out + id * D + c, x);
       else if (!(l == 0.0f))
@@ -896,117 +1003,153 @@ __global__ void __launch_bounds__(THREADS, 2) row_tiles(Args a) {
   if (gx == 0) {
     a.part_ml[slot] = float2{w.m, final ? -1.0f : l};
     if (final) a.lse[id] = natural_lse(w.m, l);
+    if (u.split == 0 && !final)  // the slots that other tiles use
+      for (int k = u.splits; k < a.S1; ++k) a.part_ml[k * slots + id] = float2{NEG_INF, 0.0f};
   }
+}
+
+// Tile blocks first (the longest ones), then those of few rows.
+template <int DT, bool E8, int D, int RW>
+__global__ void __launch_bounds__(THREADS, 2) attend(Args a) {
+  extern __shared__ __align__(16) char smem[];
+  const int index = (int)blockIdx.x;
+  if (index < a.tile_blocks)
+    row_tile<DT, E8, D, RW>(a, smem, index);
+  else
+    few_rows<DT, E8, D>(a, smem, index - a.tile_blocks);
 }
 
 // ------------------------------------------------------------------ combine
 
-// One wavefront a row: lane s reads slot s's maximum and sum, then all lanes add the slots' outputs in order.
+// One wavefront a row: lane s reads the maximum and sum of slots s and s + 64, then all lanes add the slots' outputs
+// in order, eight of them in flight.
 template <int DT, int D>
 __global__ void __launch_bounds__(THREADS) combine(Args a) {
   typedef typename Ty<DT>::el el;
-  constexpr int PER = D / 64;
+  constexpr int PER = D / 64, AT_ONCE = 8;
+  struct alignas(4 * PER) Part { float x[PER]; };
+  struct alignas(2 * PER) Out { el x[PER]; };
   const int lane = threadIdx.x & 63;
   const int64_t rows = (int64_t)a.T * a.Hq, id = (int64_t)blockIdx.x * WAVES + (threadIdx.x >> 6);
   if (id >= rows) return;
-  const int t = (int)(id / a.Hq), first = query_start(a, 0), end = query_start(a, a.B);
   const int slots = a.S1 + a.S2;
-  float2 ml{NEG_INF, 0.0f};
-  const bool inside = t >= first && t < end;
-  if (inside && lane < slots) ml = a.part_ml[lane * rows + id];
-  if (__any(ml.y < 0.0f)) return;  // written by its tile
-  float top = ml.x;
+  float2 ml[2] = {float2{NEG_INF, 0.0f}, float2{NEG_INF, 0.0f}};
+  const int t = (int)(id / a.Hq), first = query_start(a, 0), end = query_start(a, a.B);
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (lane + 64 * i < slots) ml[i] = a.part_ml[(lane + 64 * i) * rows + id];
+  if (t < first || t >= end) ml[0] = ml[1] = float2{NEG_INF, 0.0f};  // a row of no sequence
+  if (__any(ml[0].y < 0.0f)) return;  // written by its tile
+  float top = fmaxf(ml[0].x, ml[1].x);
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
-  const float weight = __builtin_amdgcn_exp2f(ml.x - (top == NEG_INF ? 0.0f : top));
-  float sum = weight * ml.y;
+  float weight[2], sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    weight[i] = __builtin_amdgcn_exp2f(ml[i].x - (top == NEG_INF ? 0.0f : top));
+    sum += weight[i] * ml[i].y;
+  }
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
   float x[PER] = {};
-  unsigned long long live = __ballot(!(ml.y == 0.0f));  // a NaN counts
-  while (live) {
-    const int s = __builtin_ctzll(live);
-    live &= live - 1;
-    const float w = __shfl(weight, s);
-    const float* p = a.part_o + (s * rows + id) * D + lane * PER;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) x[i] += w * p[i];
+  for (int i = 0; i < 2; ++i) {
+    unsigned long long live = __ballot(!(ml[i].y == 0.0f));  // a NaN counts
+    while (live) {
+      Part p[AT_ONCE];
+      float w[AT_ONCE];
+#pragma unroll
+      for (int k = 0; k < AT_ONCE; ++k) {
+        const int s = live ? __builtin_ctzll(live) : 0;
+        w[k] = live ? __shfl(weight[i], s) : 0.0f;
+        p[k] = Part{};
+        if (live) p[k] = *(const Part*)(a.part_o + ((s + 64 * i) * rows + id) * D + lane * PER);
+        live &= live - 1;
+      }
+#pragma unroll
+      for (int k = 0; k < AT_ONCE; ++k)
+#pragma unroll
+        for (int e = 0; e < PER; ++e) x[e] += w[k] * p[k].x[e];
+    }
   }
   const float inv = inverse(sum);
+  Out o;
 #pragma unroll
-  for (int i = 0; i < PER; ++i) ((el*)a.out)[id * D + lane * PER + i] = (el)(x[i] * inv);
+  for (int e = 0; e < PER; ++e) o.x[e] = (el)(x[e] * inv);
+  *(Out*)((el*)a.out + id * D + lane * PER) = o;
   if (lane == 0) a.lse[id] = natural_lse(top, sum);
 }
 
 // ------------------------------------------------------------------ host
 
 struct Plan {
-  int64_t tiles = 0;  // row tiles, an upper bound
-  int S1 = 0, S2 = 1, few_prefix = 0;
+  int64_t tile_blocks = 0;  // an upper bound
+  int row_waves = 2;        // tiles of 64 or 128 rows
+  int S1 = 0, S2 = 1;
+  int64_t few_blocks = 0;
   bool combine = true;
   int64_t bytes = 0;
 };
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+inline int64_t between(int64_t x, int64_t lo, int64_t hi) { return x < lo ? lo : x > hi ? hi : x; }
 
-// Splits: enough blocks for two on each of the 256 CUs, splits of at least 256 tokens.
+// Tiles of 128 rows where they fill the device by themselves, else of 64 (fewer splits, so fewer partial results).
+// Splits of at least 256 tokens.
 inline Plan make_plan(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t G, int64_t Wp, int64_t B, int64_t W,
                       int64_t page, int64_t max_q) {
   Plan p;
   const int64_t grp = Hq / Hkv, rows = T * grp, groups = G > 0 ? G : 1;
-  const bool has_tiles = rows > FEW && (Wp > 0 || max_q * grp > FEW);
-  auto splits = [](int64_t blocks, int64_t tokens) {
-    const int64_t want = 512 / (blocks < 1 ? 1 : blocks), most = ceil_div(tokens, 256);
-    const int64_t s = want < most ? want : most;
-    return (int)(s < 1 ? 1 : s > MAX_SLOTS / 2 ? MAX_SLOTS / 2 : s);
-  };
-  if (has_tiles) {
-    p.tiles = rows / TILE + groups;
-    const int64_t likely = ceil_div(rows, TILE) > groups ? ceil_div(rows, TILE) : groups;
-    p.S1 = splits(likely * Hkv, (Wp + (max_q * grp > FEW ? W : 0)) * page);
+  const bool big = max_q * grp > FEW;
+  if (rows > FEW && (Wp > 0 || big)) {
+    p.row_waves = ceil_div(rows, 128) * Hkv >= FILL ? 4 : 2;
+    const int64_t tile = 32 * p.row_waves;
+    const int64_t tokens = (Wp + (big ? W : 0)) * page;
+    // a last round of `tail` units is cut into FILL / tail splits; with one group the number of tiles is known
+    const int64_t units = ceil_div(rows, tile) * Hkv, tail = units % FILL;
+    const int64_t most = groups == 1 ? (units < FILL ? FILL / units : tail ? FILL / tail : 1) : FILL / Hkv;
+    p.S1 = (int)between(most, 1, between(ceil_div(tokens, 256), 1, units < FILL ? MAX_SPLIT : 8));
+    p.tile_blocks = (rows / tile + groups) * Hkv + FILL;
   } else if (Wp > 0) {
-    p.S1 = splits(groups * Hkv, Wp * page);
+    p.S1 = (int)between(FILL / (groups * Hkv), 1, between(ceil_div(Wp * page, 256), 1, MAX_SPLIT));
   }
-  p.few_prefix = p.S1 > 0 ? (int)groups : 0;
-  p.S2 = splits(B * Hkv, W * page);
+  p.S2 = (int)between(FILL / (B * Hkv), p.S1 > 0 ? 4 : 1, between(ceil_div(W * page, 256), 1, MAX_SPLIT));
+  if (p.S2 > ceil_div(W * page, 256)) p.S2 = (int)ceil_div(W * page, 256);
+  p.few_blocks = B * Hkv * p.S2 + (p.S1 > 0 ? groups * Hkv * p.S1 : 0);
   p.combine = !(p.S1 == 0 && p.S2 == 1);
   p.bytes = p.combine ? (int64_t)(p.S1 + p.S2) * T * Hq * (D * 4 + 8) : 0;
   return p;
 }
 
-template <int DT, bool E8, int D>
+template <int DT, bool E8, int D, int RW>
 tb_status launch(Args& a, const Plan& p, hipStream_t stream, const char* what) {
-  if (p.tiles) {
-    constexpr size_t lds = TileLayout<DT, E8, D>::LDS;
-    if (tb_status s = reserve_lds((const void*)row_tiles<DT, E8, D>, lds, what)) return s;
-    hipLaunchKernelGGL((row_tiles<DT, E8, D>), dim3((unsigned)p.tiles, (unsigned)(p.S1 * a.Hkv)), dim3(THREADS), lds,
-                       stream, a);
-    if (tb_status s = launch_status(what)) return s;
-  }
-  constexpr size_t lds = FewLayout<DT, E8, D>::LDS;
-  if (tb_status s = reserve_lds((const void*)few_rows<DT, E8, D>, lds, what)) return s;
-  const int most = p.few_prefix && p.S1 > p.S2 ? p.S1 : p.S2;
-  hipLaunchKernelGGL((few_rows<DT, E8, D>), dim3((unsigned)((a.B + p.few_prefix) * a.Hkv), (unsigned)most),
-                     dim3(THREADS), lds, stream, a);
+  constexpr int few = FewLayout<DT, E8, D>::LDS, tile = TileLayout<DT, E8, D, RW>::LDS;
+  constexpr size_t lds = few > tile ? few : tile;
+  static_assert(lds <= 81920, "two blocks a CU");
+  if (tb_status s = reserve_lds((const void*)attend<DT, E8, D, RW>, lds, what)) return s;
+  hipLaunchKernelGGL((attend<DT, E8, D, RW>), dim3((unsigned)(p.tile_blocks + p.few_blocks)), dim3(THREADS), lds, stream,
+                     a);
   if (tb_status s = launch_status(what)) return s;
-  if (p.combine) {
-    hipLaunchKernelGGL((combine<DT, D>), dim3((unsigned)ceil_div((int64_t)a.T * a.Hq, WAVES)), dim3(THREADS), 0, stream,
-                       a);
-    return launch_status(what);
-  }
-  return TB_OK;
+  if (!p.combine) return TB_OK;
+  hipLaunchKernelGGL((combine<DT, D>), dim3((unsigned)ceil_div((int64_t)a.T * a.Hq, WAVES)), dim3(THREADS), 0, stream, a);
+  return launch_status(what);
+}
+
+template <int DT, bool E8, int D>
+tb_status launch_rows(Args& a, const Plan& p, hipStream_t stream, const char* what) {
+  return p.row_waves == 4 ? launch<DT, E8, D, 4>(a, p, stream, what) : launch<DT, E8, D, 2>(a, p, stream, what);
 }
 
 template <int DT>
 tb_status launch_for(bool e8, int64_t D, Args& a, const Plan& p, hipStream_t stream, const char* what) {
-  if (D == 64) return e8 ? launch<DT, true, 64>(a, p, stream, what) : launch<DT, false, 64>(a, p, stream, what);
-  return e8 ? launch<DT, true, 128>(a, p, stream, what) : launch<DT, false, 128>(a, p, stream, what);
+  if (D == 64) return e8 ? launch_rows<DT, true, 64>(a, p, stream, what) : launch_rows<DT, false, 64>(a, p, stream, what);
+  return e8 ? launch_rows<DT, true, 128>(a, p, stream, what) : launch_rows<DT, false, 128>(a, p, stream, what);
 }
 
 tb_status check_sizes(const char* what, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t G, int64_t Wp, int64_t B,
                       int64_t W, int64_t page_size, int64_t max_q) {
   TB_CHECK_ARG(T >= 0 && B >= 0 && G >= 0 && Wp >= 0 && W >= 0 && max_q >= 0, "%s: negative size", what);
-  TB_CHECK_ARG(Hkv >= 1 && Hq >= Hkv && Hq % Hkv == 0 && Hkv <= 65535 / (MAX_SLOTS / 2), "%s: %lld query heads do not share %lld key/value heads",
+  TB_CHECK_ARG(Hkv >= 1 && Hq >= Hkv && Hq % Hkv == 0, "%s: %lld query heads do not share %lld key/value heads",
                what, (long long)Hq, (long long)Hkv);
   TB_CHECK_ARG(D == 64 || D == 128, "%s: the head dimension must be 64 or 128 (got %lld)", what, (long long)D);
   TB_CHECK_ARG(page_size >= 1 && page_size <= 4096 && (page_size & (page_size - 1)) == 0,
@@ -1014,7 +1157,7 @@ tb_status check_sizes(const char* what, int64_t T, int64_t Hq, int64_t Hkv, int6
   TB_CHECK_ARG((Wp == 0) == (G == 0), "%s: %lld groups with page tables of %lld", what, (long long)G, (long long)Wp);
   const int64_t most = (1ll << 31) - 1;
   // row, token and block numbers are 32-bit in the kernels
-  TB_CHECK_ARG(T * Hq <= most && B * Hkv <= most / 2 && G * Hkv <= most / 4 && W <= most / 2 / page_size &&
+  TB_CHECK_ARG(T * Hq <= most && B * Hkv <= most / MAX_SPLIT / 4 && G * Hkv <= most / MAX_SPLIT / 4 && W <= most / 2 / page_size &&
                    Wp <= most / 2 / page_size && max_q * Hq <= most,
                "%s: sizes past 2^31", what);
   return TB_OK;
@@ -1053,6 +1196,7 @@ extern "C" tb_status tb_shared_prefix_attention(const void* q, const void* k_cac
                cache_dtype, dtype);
   TB_CHECK_ARG((cache_dtype == 3) == (k_scale != nullptr) && (cache_dtype == 3) == (v_scale != nullptr),
                "%s: scales belong to e4m3 caches, and only to them", what);
+  TB_CHECK_ARG(scale - scale == 0.0, "%s: the scale must be finite", what);
   TB_CHECK_ARG(n_pages >= 1 && n_pages <= ((1ll << 31) - 1) / page_size, "%s: bad number of pages %lld", what,
                (long long)n_pages);
   if (T == 0) return TB_OK;
@@ -1111,7 +1255,11 @@ extern "C" tb_status tb_shared_prefix_attention(const void* q, const void* k_cac
   a.S1 = p.S1;
   a.S2 = p.S2;
   a.direct = !p.combine;
-  a.scale_log2 = (float)(scale * 1.44269504088896340736);
+  a.scale_log2 = scale == 0.0 ? 1.0f : (float)((scale < 0.0 ? -scale : scale) * 1.44269504088896340736);
+  a.flip = scale < 0.0 ? 0x80008000u : 0u;
+  a.keep = scale == 0.0 ? 0u : ~0u;
+  a.big = max_q * a.grp > FEW;
+  a.tile_blocks = (int)p.tile_blocks;
   const bool e8 = cache_dtype == 3;
   return dtype == F16 ? launch_for<F16>(e8, D, a, p, stream, what) : launch_for<BF16>(e8, D, a, p, stream, what);
 }
