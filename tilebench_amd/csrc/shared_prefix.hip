@@ -79,6 +79,7 @@ struct Args {
   int direct;       // own tokens in one slot and nothing else: results are final
   float scale_log2;     // of |scale|, or 1 for a scale of 0
   uint32_t flip, keep;  // applied to q
+  int near;  // 64 slots of a page lie within 2 GiB
   int big;  // some sequence may have more than FEW rows
   int tile_blocks;
 };
@@ -152,6 +153,16 @@ __device__ __forceinline__ void dma16(uint32_t lds, const char* p) {
                : "s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(p)
                : "memory", "m0");
 }
+// the same from a uniform address plus a 32-bit offset of each lane
+__device__ __forceinline__ void dma16(uint32_t lds, const char* p, uint32_t off) {
+  const uint64_t u = (uint64_t)(uintptr_t)p;
+  const uint64_t base = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)u) |
+                        (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(u >> 32)) << 32;
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2"
+               :
+               : "s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(off), "s"(base)
+               : "memory", "m0");
+}
 __device__ __forceinline__ void dma4(uint32_t lds, const char* p) {
   asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off"
                :
@@ -187,17 +198,35 @@ struct Window {
   }
 };
 
-// Byte offsets of token rows in the pools.
-template <int TOK, int ESIZE>
-__device__ __forceinline__ int64_t token_offset(const Args& a, const Window& w, const Tokens& s, int t0, int tok) {
-  tok = min(tok, s.len - 1);
-  int page;
-  if ((1 << a.page_shift) >= TOK)  // a step's tokens lie in one page
-    page = __builtin_amdgcn_readlane(w.ids, (t0 >> a.page_shift) - w.first);
-  else
-    page = __builtin_amdgcn_ds_bpermute(((tok >> a.page_shift) - w.first) << 2, w.ids);
-  return (page * a.c_page + (tok & ((1 << a.page_shift) - 1)) * a.c_slot) * ESIZE;
-}
+// Copies of NI KiB of token rows into a tile: rows lane / (RB / 16) + i * RPI from token t0 on, the 16-byte chunk of a
+// lane at its swizzled place.
+template <int RB, int NI>
+struct Copier {
+  static constexpr int LANES = RB / 16, RPI = 64 / LANES, ROWS = NI * RPI;
+  // swizzle(r) is linear in the bits of r: that of the lane's row and that of the copy's first row
+  template <typename Swizzle>
+  static __device__ __forceinline__ void run(const Args& a, const Window& w, const Tokens& s, const char* pool,
+                                             uint32_t lds, int t0, int esize, Swizzle swizzle) {
+    const int lane = threadIdx.x & 63, r = lane / LANES, chunk = (lane % LANES) ^ swizzle(r);
+    const int mask = (1 << a.page_shift) - 1;
+    if (a.near && mask + 1 >= ROWS && t0 + ROWS <= s.len) {  // whole and in one page
+      const int page = __builtin_amdgcn_readlane(w.ids, (t0 >> a.page_shift) - w.first);
+      const char* p = pool + (page * a.c_page + (t0 & mask) * a.c_slot) * esize;
+      const uint32_t row = (uint32_t)(r * (int)a.c_slot * esize);
+      const int64_t step = RPI * a.c_slot * esize;
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+        dma16(lds + i * 1024, p + i * step, row + (uint32_t)((chunk ^ swizzle(i * RPI)) << 4));
+      return;
+    }
+#pragma unroll 1
+    for (int i = 0; i < NI; ++i) {
+      const int tok = min(t0 + r + i * RPI, s.len - 1);  // past the end: the last token again (masked)
+      const int page = __builtin_amdgcn_ds_bpermute(((tok >> a.page_shift) - w.first) << 2, w.ids);
+      dma16(lds + i * 1024, pool + (page * a.c_page + (tok & mask) * a.c_slot) * esize + ((chunk ^ swizzle(i * RPI)) << 4));
+    }
+  }
+};
 
 __device__ __forceinline__ uint32_t as_uint(float x) { return __builtin_bit_cast(uint32_t, x); }
 __device__ __forceinline__ float as_float(uint32_t x) { return __builtin_bit_cast(float, x); }
@@ -305,6 +334,18 @@ struct Wave {
     }
   }
 
+  // Scores of the tokens that a row does not see: -inf.  left: tokens up to the row's limit, from the lane group's first.
+  template <int TOK>
+  static __device__ __forceinline__ void hide(acc_t (&s)[TOK / SH], int left) {
+    __builtin_amdgcn_sched_barrier(0);  // comparisons hoisted over the products would take all scalar registers
+#pragma unroll
+    for (int t = 0; t < TOK / SH; ++t) {
+#pragma unroll
+      for (int r = 0; r < REGS; ++r) s[t][r] = t * SH + token_of(r, 0) < left ? s[t][r] : NEG_INF;
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+
   // Scores -> weights exp2(score - m), the operands of the second product.  m follows the running maximum in steps:
   // while no row of the wavefront passes its m by 2^SLACK beyond the lift, sums and outputs stay as they are.
   template <int TOK>
@@ -312,6 +353,7 @@ struct Wave {
                                           uint32_t sbase, int tok0, v8 (&p)[TOK / KS]) {
     const int g = (threadIdx.x & 63) / SH;
     float top = NEG_INF;
+    if (!full) hide<TOK>(s, limit - t0 - 4 * g);
 #pragma unroll
     for (int t = 0; t < TOK / SH; ++t)
 #pragma unroll
@@ -320,11 +362,7 @@ struct Wave {
         if (E8) {
           const f32x4 k = lds_read<f32x4>(scale_at(sbase, tok0 + tok));
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[t][r + i] *= k[i];
-        }
-        if (!full) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[t][r + i] = t0 + tok + i < limit ? s[t][r + i] : NEG_INF;
+          for (int i = 0; i < 4; ++i) s[t][r + i] *= full || s[t][r + i] > NEG_INF ? k[i] : 1.0f;
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) top = fmaxf(top, s[t][r + i]);
@@ -404,75 +442,59 @@ struct Wave {
     }
   };
 
-  // 0xFFFF in the halves of w that are infinities or NaN
-  static __device__ __forceinline__ uint32_t non_finite(uint32_t w) {
-    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-    const uint32_t e = Y::EXP | Y::EXP << 16;
-    const u16x2 other = __builtin_elementwise_min(__builtin_bit_cast(u16x2, (w & e) ^ e), u16x2{1, 1});
-    return __builtin_bit_cast(uint32_t, other - u16x2{1, 1});
-  }
-
-  // O^T += V^T P^T.  A tile that some rows see in part (not `full`): infinities and NaN count as zeros here and are
-  // marked for the rows that attend to their tokens.
+  // O^T += V^T P^T
   template <int TOK>
-  __device__ __forceinline__ void values(uint32_t vbase, const v8 (&p)[TOK / KS], int t0, int limit, bool full,
-                                         uint32_t marks) {
+  __device__ __forceinline__ void values(uint32_t vbase, const v8 (&p)[TOK / KS]) {
     const Values v(vbase);
-    if (full) {
 #pragma unroll
-      for (int k = 0; k < TOK / KS; ++k)
+    for (int k = 0; k < TOK / KS; ++k)
 #pragma unroll
-        for (int d = 0; d < DT_N; ++d) o[d] = Y::mfma(v.read(d, k), p[k], o[d]);
-      return;
-    }
-    uint32_t bad = 0;
-#pragma unroll
-    for (int d = 0; d < DT_N; ++d)
-#pragma unroll
-      for (int k = 0; k < TOK / KS; ++k) {
-        u32x4 x = __builtin_bit_cast(u32x4, v.read(d, k));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t n = non_finite(x[i]);
-          bad |= n;
-          x[i] &= ~n;
-        }
-        o[d] = Y::mfma(__builtin_bit_cast(v8, x), p[k], o[d]);
-        if (k % 2 == 1) __builtin_amdgcn_sched_barrier(0);  // two operands at a time: more would spill
-      }
-    if (__any(bad != 0)) mark<TOK>(vbase, t0, limit, marks);
+      for (int d = 0; d < DT_N; ++d) o[d] = Y::mfma(v.read(d, k), p[k], o[d]);
   }
 
-  // Marks of a wavefront: a byte for each of 32 rows and 64 runs of D / 64 channels, four bits a channel
-  // (1: +inf, 2: -inf, 4: NaN among the values that the row attends to).
-  static constexpr int MARKS = 32 * 64;
-  template <int TOK>
-  __device__ __forceinline__ void mark(uint32_t vbase, int t0, int limit, uint32_t marks) {
+  // Infinities and NaN among the values of tokens that some rows do not see.  They are replaced by zeros in the tile
+  // and marked for the rows that see their token: a byte for each row and each run of D / 64 channels, four bits a
+  // channel (1: +inf, 2: -inf, 4: NaN), added to the row's output at the end.
+  //
+  // Tokens tok0 .. tok0 + ROWS - 1 of the tile at vbase, t0 being the tile's first token; limit_of(r): the limit of row r.
+  template <int ROWS, typename Limit>
+  static __device__ __forceinline__ void set_apart(uint32_t vbase, int tok0, int t0, int rows, uint32_t marks,
+                                                   Limit limit_of) {
+    const int lane = threadIdx.x & 63;
+    const uint32_t exps = E8 ? 0x7F7F7F7Fu : Y::EXP | Y::EXP << 16, ones = E8 ? 0x7F7F7F7Fu : 0x7FFF7FFFu;
+    uint32_t good = ~0u;  // the top bit of an element: not (all exponent bits, or the NaN code)
+#pragma unroll
+    for (int i = 0; i < ROWS * RB / 1024; ++i) {
+      const u32x4 x = lds_read<u32x4>(vbase + tok0 * RB + i * 1024 + lane * 16);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) good &= exps - (x[e] & exps) + ones;
+    }
+    if (!__any((~good & ~ones) != 0)) return;
     constexpr int PER = D / 64, ESIZE = E8 ? 1 : 2;
-    const int lane = threadIdx.x & 63, at = lane * PER * ESIZE;
+    const int at = lane * PER * ESIZE;
 #pragma unroll 1
-    for (int tok = 0; tok < TOK; ++tok) {
+    for (int tok = tok0; tok < tok0 + ROWS; ++tok) {
       const uint32_t p = vbase + tok * RB + (((at >> 4) ^ swizzle_v<RB, SH, E8>(tok)) << 4) + (at & 15);
       uint32_t is = 0;
 #pragma unroll
       for (int e = 0; e < PER; ++e) {
         uint32_t x = E8 ? lds_read<uint8_t>(p + e) : lds_read<uint16_t>(p + 2 * e);
         if (E8) x = (x & 0x7Fu) == 0x7Fu ? 0x7FFFu : 0u;
-        if ((x & Y::EXP) == Y::EXP) is |= ((x & 0x7FFFu) != Y::EXP ? 4u : x & 0x8000u ? 2u : 1u) << (4 * e);
+        if ((x & Y::EXP) != Y::EXP) continue;
+        is |= ((x & 0x7FFFu) != Y::EXP ? 4u : x & 0x8000u ? 2u : 1u) << (4 * e);
+        if (E8)
+          *(__attribute__((address_space(3))) uint8_t*)(uintptr_t)(p + e) = 0;
+        else
+          *(__attribute__((address_space(3))) uint16_t*)(uintptr_t)(p + 2 * e) = 0;
       }
       if (!__any(is != 0)) continue;
 #pragma unroll 1
-      for (int r = 0; r < SH; ++r) {
-        if (t0 + tok >= __builtin_amdgcn_readlane(limit, r)) continue;
-        const uint32_t m = marks + r * 64 + lane;
-        *(__attribute__((address_space(3))) uint8_t*)(uintptr_t)m = (uint8_t)(lds_read<uint8_t>(m) | is);
+      for (int r = 0; r < rows; ++r) {
+        if (t0 + tok >= limit_of(r) || is == 0) continue;
+        __hip_atomic_fetch_or((__attribute__((address_space(3))) uint32_t*)(uintptr_t)(marks + r * 64 + (lane & ~3)),
+                              is << (8 * (lane & 3)), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
       }
     }
-  }
-  static __device__ __forceinline__ void clear_marks(uint32_t marks) {
-    const uint32_t p = marks + (threadIdx.x & 63) * 32;
-    *(__attribute__((address_space(3))) u32x4*)(uintptr_t)p = u32x4{};
-    *(__attribute__((address_space(3))) u32x4*)(uintptr_t)(p + 16) = u32x4{};
   }
   // x, or what the marks of row r make of channels c .. c + 3
   static __device__ __forceinline__ f32x4 marked(f32x4 x, uint32_t marks, int r, int c) {
@@ -549,44 +571,54 @@ struct FewLayout {
   static constexpr int MERGE_ROW = D + 4;  // floats; rows four banks apart
   static constexpr int MERGE_BYTES = WAVES * FEW * MERGE_ROW * 4 + WAVES * FEW * 8;
   static constexpr int MARKS = WAVES * WAVE_BYTES > MERGE_BYTES ? WAVES * WAVE_BYTES : MERGE_BYTES;
-  static constexpr int LDS = MARKS + WAVES * 32 * 64;
+  static constexpr int LIMITS = MARKS + FEW * 64;
+  static constexpr int LDS = LIMITS + FEW * 4;
 };
 
-// Rows 0 .. rows - 1 (at most 16) from query q0 on, key/value head h, tokens of `src`, split `split` of `splits`;
-// results to slot `slot`.
+// What a block of few rows does: rows 0 .. rows - 1 (at most 16) from query q0 on over the tokens of `src`, of which it
+// takes split `split` of `splits`; results to slot `slot`.
+struct FewTask {
+  int h, q0, rows, split, splits, slot;
+  Tokens src;
+  bool own;    // own tokens of the sequence `seq`, or the prefix of sequences b0 .. b1 - 1
+  Seq seq;
+  int b0, b1;
+};
+
 template <int DT, bool E8, int D>
-__device__ __forceinline__ void attend_few(const Args& a, char* smem, int h, int q0, int rows, const Tokens& src,
-                                           int base, int split, int splits, int slot, const Seq* seq, int b0, int b1) {
+__device__ __forceinline__ void attend_few(const Args& a, char* smem, const FewTask& f) {
   constexpr int SH = 16;
   typedef FewLayout<DT, E8, D> L;
   typedef Wave<DT, E8, D, SH> W;
   typedef typename W::Y::el el;
-  constexpr int TOK = L::TOK, RB = L::RB, RPI = 1024 / RB, NI = TOK / RPI, ESIZE = E8 ? 1 : 2;
+  constexpr int TOK = L::TOK, RB = L::RB, NI = TOK * RB / 1024, ESIZE = E8 ? 1 : 2;
+  typedef Copier<RB, NI> Copy;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int row = lane % SH;
-  const bool valid = row < rows;
-  const int t = q0 + row / a.grp, hq = h * a.grp + row % a.grp;
+  const int row = lane % SH, h = f.h;
+  const Tokens src = f.src;
+  const bool valid = row < f.rows;
+  const int t = f.q0 + row / a.grp, hq = h * a.grp + row % a.grp;
 
-  // tokens of `src` that the row attends to: its position is that of the last n_q tokens of its sequence.
-  // base: the tokens before src (own tokens), or -1 where src is the prefix
+  // tokens of `src` that the row attends to: its position is that of the last n_q tokens of its sequence
   int limit = 0x7FFFFFFF;
   if (valid) {
-    Seq s = seq ? *seq : sequence(a, sequence_of(a, t, b0, b1));
+    const Seq s = f.own ? f.seq : sequence(a, sequence_of(a, t, f.b0, f.b1));
     const int end = s.own - s.n_q + (t - s.q0) + 1;  // own tokens up to and with the query
-    limit = base < 0 ? clamp_int(src.len + end, 0, src.len) : clamp_int(end, 0, src.len);
+    limit = clamp_int(f.own ? end : src.len + end, 0, src.len);
   }
 
   W w;
   w.init((const el*)a.q + t * a.q_st + hq * a.q_sh, valid, a.flip, a.keep);
 
   const int tiles = (src.len + TOK - 1) / TOK;
-  const int lo = (int)((int64_t)tiles * split / splits), hi = (int)((int64_t)tiles * (split + 1) / splits);
+  const int lo = (int)((int64_t)tiles * f.split / f.splits), hi = (int)((int64_t)tiles * (f.split + 1) / f.splits);
   const int n0 = lo + (hi - lo) * wave / WAVES, n1 = lo + (hi - lo) * (wave + 1) / WAVES;
 
   const uint32_t kbase = lds_addr(smem) + wave * L::WAVE_BYTES, vbase = kbase + L::TILE_BYTES;
-  const uint32_t sbase = vbase + L::TILE_BYTES;
-  const uint32_t marks = lds_addr(smem) + L::MARKS + wave * W::MARKS;
-  W::clear_marks(marks);
+  const uint32_t sbase = vbase + L::TILE_BYTES, marks = lds_addr(smem) + L::MARKS, limits = lds_addr(smem) + L::LIMITS;
+  for (int i = threadIdx.x; i < FEW * 16; i += THREADS) *(uint32_t*)(smem + L::MARKS + 4 * i) = 0;
+  if (wave == 0 && lane < SH) *(int*)(smem + L::LIMITS + 4 * lane) = limit;
+  __syncthreads();
   const char* kp = a.kc + h * a.c_head * ESIZE;
   const char* vp = a.vc + h * a.c_head * ESIZE;
   Window win;
@@ -594,17 +626,11 @@ __device__ __forceinline__ void attend_few(const Args& a, char* smem, int h, int
     const int t0 = n * TOK;
     win.cover(src, t0 >> a.page_shift, min(t0 + TOK - 1, src.len - 1) >> a.page_shift, a.n_pages);
   };
-  auto fill = [&](int n, bool keys) __attribute__((always_inline)) {
-    const int t0 = n * TOK;
-#pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      const int r = i * RPI + lane / (RB / 16), pos = lane % (RB / 16);
-      const int64_t off = token_offset<TOK, ESIZE>(a, win, src, t0, t0 + r);
-      if (keys)
-        dma16(kbase + i * 1024, kp + off + ((pos ^ swizzle_k<RB>(r)) << 4));
-      else
-        dma16(vbase + i * 1024, vp + off + ((pos ^ swizzle_v<RB, SH, E8>(r)) << 4));
-    }
+  auto fill_keys = [&](int n) __attribute__((always_inline)) {
+    Copy::run(a, win, src, kp, kbase, n * TOK, ESIZE, [](int r) { return swizzle_k<RB>(r); });
+  };
+  auto fill_values = [&](int n) __attribute__((always_inline)) {
+    Copy::run(a, win, src, vp, vbase, n * TOK, ESIZE, [](int r) { return swizzle_v<RB, SH, E8>(r); });
   };
   auto fill_scales = [&](int n) __attribute__((always_inline)) {  // 32 tokens a copy: keys' scales, then values'
 #pragma unroll
@@ -621,8 +647,8 @@ __device__ __forceinline__ void attend_few(const Args& a, char* smem, int h, int
   if (n0 < n1) {
     cover(n0);
     if (E8) fill_scales(n0);
-    fill(n0, true);
-    fill(n0, false);
+    fill_keys(n0);
+    fill_values(n0);
   }
   for (int n = n0; n < n1; ++n) {
     const int t0 = n * TOK;
@@ -636,13 +662,17 @@ __device__ __forceinline__ void attend_few(const Args& a, char* smem, int h, int
     if (n + 1 < n1) {
       cover(n + 1);
       if (E8) fill_scales(n + 1);
-      fill(n + 1, true);
+      fill_keys(n + 1);
     }
     if (!E8) w.template weights<TOK>(s, t0, limit, full, a.scale_log2, sbase, 0, p);
     if (n + 1 < n1) wait_vm<NI + (E8 ? TOK / 32 : 0)>(); else wait_vm<0>();
-    w.template values<TOK>(vbase, p, t0, limit, full, marks);
+    if (!full) {
+      W::template set_apart<TOK>(vbase, 0, t0, f.rows, marks, [&](int r) { return lds_read<int>(limits + 4 * r); });
+      wait_lds();
+    }
+    w.template values<TOK>(vbase, p);
     wait_lds();
-    if (n + 1 < n1) fill(n + 1, false);
+    if (n + 1 < n1) fill_values(n + 1);
   }
 
   // join the four wavefronts
@@ -667,7 +697,7 @@ __device__ __forceinline__ void attend_few(const Args& a, char* smem, int h, int
       *(f32x4*)(merge + (wave * FEW + row) * L::MERGE_ROW + d * SH + W::token_of(r, g)) = x;
     }
   __syncthreads();
-  for (int i = threadIdx.x; i < rows * (D / 4); i += THREADS) {
+  for (int i = threadIdx.x; i < f.rows * (D / 4); i += THREADS) {
     const int r = i / (D / 4), c = (i % (D / 4)) * 4;
     float m = NEG_INF, sum = 0.0f;
 #pragma unroll
@@ -680,15 +710,14 @@ __device__ __forceinline__ void attend_few(const Args& a, char* smem, int h, int
       sum += e.y * __builtin_amdgcn_exp2f(e.x - use);
       x += *(const f32x4*)(merge + (k * FEW + r) * L::MERGE_ROW + c);
     }
-#pragma unroll
-    for (int k = 0; k < WAVES; ++k) x = W::marked(x, lds_addr(smem) + L::MARKS + k * W::MARKS, r, c);
-    const int64_t id = (int64_t)(q0 + r / a.grp) * a.Hq + h * a.grp + r % a.grp;
+    x = W::marked(x, marks, r, c);
+    const int64_t id = (int64_t)(f.q0 + r / a.grp) * a.Hq + h * a.grp + r % a.grp;
     if (a.direct) {
       store4((el*)a.out + id * D + c, x * inverse(sum));
       if (c == 0) a.lse[id] = natural_lse(m, sum);
     } else {
-      *(f32x4*)(a.part_o + ((int64_t)slot * a.T * a.Hq + id) * D + c) = x;
-      if (c == 0) a.part_ml[(int64_t)slot * a.T * a.Hq + id] = float2{m, sum};
+      *(f32x4*)(a.part_o + ((int64_t)f.slot * a.T * a.Hq + id) * D + c) = x;
+      if (c == 0) a.part_ml[(int64_t)f.slot * a.T * a.Hq + id] = float2{m, sum};
     }
   }
 }
@@ -708,44 +737,44 @@ template <int DT, bool E8, int D>
 __device__ __forceinline__ void few_rows(const Args& a, char* smem, int index) {
   constexpr int TOK = FewLayout<DT, E8, D>::TOK;
   const int own_blocks = a.B * a.Hkv * a.S2;
-  if (index < own_blocks) {
-    const int split = index / (a.B * a.Hkv), unit = index % (a.B * a.Hkv), b = unit / a.Hkv, h = unit % a.Hkv;
+  FewTask f;
+  f.own = index < own_blocks;
+  if (!f.own) index -= own_blocks;
+  const int heads = (f.own ? a.B : a.G) * a.Hkv, unit = index % heads, b = unit / a.Hkv;
+  f.h = unit % a.Hkv;
+  f.split = index / heads;
+  f.slot = f.own ? a.S1 + f.split : f.split;
+  if (f.own) {
     if (a.direct && b == 0) {  // rows of no sequence
       const int first = query_start(a, 0);
-      empty_rows<DT, D>(a, h, 0, first);
-      empty_rows<DT, D>(a, h, max(query_start(a, a.B), first), a.T);
+      empty_rows<DT, D>(a, f.h, 0, first);
+      empty_rows<DT, D>(a, f.h, max(query_start(a, a.B), first), a.T);
     }
-    const Seq s = sequence(a, b);
-    const int rows = s.n_q * a.grp;
-    // splits of at least two steps a wavefront
-    const int used = clamp_int((s.own + 8 * TOK - 1) / (8 * TOK), 1, a.S2);
-    if (a.direct && rows > FEW) {  // more queries than max_q announced: nothing was planned for them
-      empty_rows<DT, D>(a, h, s.q0, s.q0 + s.n_q);
+    f.seq = sequence(a, b);
+    f.q0 = f.seq.q0;
+    f.rows = f.seq.n_q * a.grp;
+    f.src = Tokens{a.pages + (int64_t)b * a.W, a.W, f.seq.own};
+    if (a.direct && f.rows > FEW) {  // more queries than max_q announced: nothing was planned for them
+      empty_rows<DT, D>(a, f.h, f.q0, f.q0 + f.seq.n_q);
       return;
     }
-    if (rows > FEW || split >= used) {
-      for (int r = threadIdx.x; r < rows; r += THREADS)
-        a.part_ml[((int64_t)(a.S1 + split) * a.T + s.q0 + r / a.grp) * a.Hq + h * a.grp + r % a.grp] =
-            float2{NEG_INF, 0.0f};
-      return;
-    }
-    if (rows == 0) return;
-    const Tokens src{a.pages + (int64_t)b * a.W, a.W, s.own};
-    attend_few<DT, E8, D>(a, smem, h, s.q0, rows, src, 0, split, used, a.S1 + split, &s, 0, 0);
   } else {
-    index -= own_blocks;
-    const int split = index / (a.G * a.Hkv), unit = index % (a.G * a.Hkv), g = unit / a.Hkv, h = unit % a.Hkv;
-    const Group gr = group(a, g);
-    if (gr.rows > FEW || gr.rows == 0) return;
-    const int used = clamp_int((gr.len + 8 * TOK - 1) / (8 * TOK), 1, a.S1);
-    if (split >= used) {
-      for (int r = threadIdx.x; r < gr.rows; r += THREADS)
-        a.part_ml[((int64_t)split * a.T + gr.q0 + r / a.grp) * a.Hq + h * a.grp + r % a.grp] = float2{NEG_INF, 0.0f};
-      return;
-    }
-    const Tokens src{a.prefix_pages + (int64_t)g * a.Wp, a.Wp, gr.len};
-    attend_few<DT, E8, D>(a, smem, h, gr.q0, gr.rows, src, -1, split, used, split, nullptr, gr.b0, gr.b1);
+    const Group gr = group(a, b);
+    f.q0 = gr.q0;
+    f.rows = gr.rows;
+    f.src = Tokens{a.prefix_pages + (int64_t)b * a.Wp, a.Wp, gr.len};
+    f.b0 = gr.b0;
+    f.b1 = gr.b1;
+    if (f.rows > FEW) return;  // its tiles write these slots
   }
+  // splits of at least two steps a wavefront
+  f.splits = clamp_int((f.src.len + 8 * TOK - 1) / (8 * TOK), 1, f.own ? a.S2 : a.S1);
+  if (f.rows > FEW || f.split >= f.splits) {
+    for (int r = threadIdx.x; r < f.rows; r += THREADS)
+      a.part_ml[((int64_t)f.slot * a.T + f.q0 + r / a.grp) * a.Hq + f.h * a.grp + r % a.grp] = float2{NEG_INF, 0.0f};
+    return;
+  }
+  if (f.rows > 0) attend_few<DT, E8, D>(a, smem, f);
 }
 
 // ------------------------------------------------------------------ tiles of rows
@@ -760,7 +789,8 @@ struct TileLayout {
   static constexpr int STAGE = 2 * TILE_BYTES + (E8 ? 2 * TOK * 4 : 0);
   static constexpr int MERGE_ROW = D + 4;
   static constexpr int MARKS = 2 * STAGE;
-  static constexpr int LDS = MARKS + WAVES * 32 * 64;
+  static constexpr int ROW_INFO = MARKS + ROWS * 64;
+  static constexpr int LDS = ROW_INFO + ROWS * 12;
   static_assert(RW == 4 || MARKS >= ROWS * (MERGE_ROW * 4 + 8), "the merge reuses the stages");
 };
 
@@ -825,9 +855,10 @@ __device__ __forceinline__ bool find_tile(const Args& a, int index, TileUnit& u)
 template <int DT, bool E8, int D, int RW>
 __device__ __forceinline__ void row_tile(const Args& a, char* smem, int index) {
   typedef TileLayout<DT, E8, D, RW> L;
-  constexpr int SH = 32, TOK = L::TOK, RB = L::RB, RPI = 1024 / RB, ESIZE = E8 ? 1 : 2;
+  constexpr int SH = 32, TOK = L::TOK, RB = L::RB, ESIZE = E8 ? 1 : 2;
   constexpr int MINE = TOK / WAVES;            // tokens that a wavefront fetches
-  constexpr int NI = MINE / RPI;               // in copies of 1 KiB
+  constexpr int NI = MINE * RB / 1024;         // in copies of 1 KiB
+  typedef Copier<RB, NI> Copy;
   constexpr int SHARE = TOK * RW / WAVES;      // tokens that a wavefront attends to
   constexpr int MOST = E8 ? 32 : 64;           // in steps of so many (e4m3: 64 would spill)
   constexpr int STEP = SHARE > MOST ? MOST : SHARE;
@@ -878,8 +909,15 @@ __device__ __forceinline__ void row_tile(const Args& a, char* smem, int index) {
   int skip = (int)((int64_t)steps * u.split / u.splits);
   int todo = (int)((int64_t)steps * (u.split + 1) / u.splits) - skip;
 
-  const uint32_t base = lds_addr(smem), marks = base + L::MARKS + wave * W::MARKS;
-  W::clear_marks(marks);
+  const uint32_t base = lds_addr(smem), marks = base + L::MARKS, info = base + L::ROW_INFO;
+  for (int i = threadIdx.x; i < L::ROWS * 16; i += THREADS) *(uint32_t*)(smem + L::MARKS + 4 * i) = 0;
+  // of every row, for the marks: sequence (-1: no row), prefix tokens and own tokens that it sees
+  if (wt == 0 && lane < SH) {
+    int* p = (int*)(smem + L::ROW_INFO) + wr * SH + lane;
+    p[0] = b;
+    p[L::ROWS] = prefix_limit;
+    p[2 * L::ROWS] = own_limit;
+  }
   const char* kp = a.kc + h * a.c_head * ESIZE;
   const char* vp = a.vc + h * a.c_head * ESIZE;
 
@@ -902,15 +940,10 @@ __device__ __forceinline__ void row_tile(const Args& a, char* smem, int index) {
     Window win;
     auto fill = [&](int n) __attribute__((always_inline)) {
       const int t0 = n * TOK + wave * MINE;  // the wavefront's first token
-      const uint32_t kb = base + (n & 1) * L::STAGE + wave * NI * 1024, vb = kb + L::TILE_BYTES;
+      const uint32_t kb = base + (n & 1) * L::STAGE + wave * MINE * RB;
       win.cover(src, min(t0, src.len - 1) >> a.page_shift, min(t0 + MINE - 1, src.len - 1) >> a.page_shift, a.n_pages);
-#pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        const int r = i * RPI + lane / (RB / 16), pos = lane % (RB / 16);
-        const int64_t off = token_offset<MINE, ESIZE>(a, win, src, t0, t0 + r);
-        dma16(kb + i * 1024, kp + off + ((pos ^ swizzle_k<RB>(wave * MINE + r)) << 4));
-        dma16(vb + i * 1024, vp + off + ((pos ^ swizzle_v<RB, SH, E8>(wave * MINE + r)) << 4));
-      }
+      Copy::run(a, win, src, kp, kb, t0, ESIZE, [](int r) { return swizzle_k<RB>(r); });
+      Copy::run(a, win, src, vp, kb + L::TILE_BYTES, t0, ESIZE, [](int r) { return swizzle_v<RB, SH, E8>(r); });
       if (E8) {
         static_assert(MINE == 32 || !E8, "the scales of 32 tokens a copy");
         const int tok = min(t0 + (lane & 31), src.len - 1);
@@ -919,11 +952,26 @@ __device__ __forceinline__ void row_tile(const Args& a, char* smem, int index) {
         dma4(base + (n & 1) * L::STAGE + 2 * L::TILE_BYTES + wave * 256, (const char*)((lane < 32 ? a.ks : a.vs) + off));
       }
     };
-    // both stages may still be read from the segment before
+    // both stages may still be read from the segment before; the rows' limits are there after this
     __syncthreads();
     fill(n0);
+    auto limit_of = [&](int r) {
+      const int rb = lds_read<int>(info + 4 * r);
+      return rb < 0 ? 0 : pre ? lds_read<int>(info + 4 * (L::ROWS + r))
+                              : rb == x ? lds_read<int>(info + 4 * (2 * L::ROWS + r)) : 0;
+    };
+    int seen_by_all = 0x7FFFFFFF;  // tokens that every row of the tile sees
+#pragma unroll
+    for (int r = 0; r < L::ROWS; r += 64)
+      if (lds_read<int>(info + 4 * (r + lane)) >= 0) seen_by_all = min(seen_by_all, limit_of(r + lane));
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) seen_by_all = min(seen_by_all, __shfl_xor(seen_by_all, d));
+    seen_by_all = __builtin_amdgcn_readfirstlane(seen_by_all);
     for (int n = n0; n < n1; ++n) {
+      const uint32_t stage = base + (n & 1) * L::STAGE;
       wait_vm<0>();
+      if ((n + 1) * TOK > seen_by_all)  // each wavefront looks at the tokens it has fetched
+        W::template set_apart<MINE>(stage + L::TILE_BYTES, wave * MINE, n * TOK, L::ROWS, marks, limit_of);
       wait_lds();
       __builtin_amdgcn_s_barrier();  // the step's tokens are there, the other stage is free
       if (n + 1 < n1) fill(n + 1);
@@ -932,13 +980,12 @@ __device__ __forceinline__ void row_tile(const Args& a, char* smem, int index) {
         const int tok0 = wt * SHARE + c * STEP, t0 = n * TOK + tok0;
         if (!__any(some && limit > t0)) continue;
         const bool full = __all(limit >= t0 + STEP);
-        const uint32_t kb = base + (n & 1) * L::STAGE + tok0 * RB, vb = kb + L::TILE_BYTES;
-        const uint32_t sb = base + (n & 1) * L::STAGE + 2 * L::TILE_BYTES;
+        const uint32_t kb = stage + tok0 * RB;
         typename W::acc_t s[STEP / SH];
         typename W::v8 p[STEP / W::KS];
         w.template scores<STEP>(kb, s);
-        w.template weights<STEP>(s, t0, limit, full, a.scale_log2, sb, tok0, p);
-        w.template values<STEP>(vb, p, t0, limit, full, marks);
+        w.template weights<STEP>(s, t0, limit, full, a.scale_log2, stage + 2 * L::TILE_BYTES, tok0, p);
+        w.template values<STEP>(kb + L::TILE_BYTES, p);
       }
     }
   }
@@ -947,11 +994,11 @@ __device__ __forceinline__ void row_tile(const Args& a, char* smem, int index) {
   const int gx = lane / SH;
   float* merge = (float*)smem;
   float2* ml = (float2*)(merge + L::ROWS * L::MERGE_ROW);
+  __syncthreads();  // all marks are made
   if (RW < WAVES) {
     // the wavefronts that share a row: the second hands its results to the first
     static_assert(RW == WAVES || RW * 2 == WAVES, "two halves");
     const int r = wr * SH + lane % SH;
-    __syncthreads();
     if (wt == 1) {
 #pragma unroll
       for (int d = 0; d < W::DT_N; ++d)
@@ -993,8 +1040,7 @@ __device__ __forceinline__ void row_tile(const Args& a, char* smem, int index) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) x[i] = w.o[d][r + i] * inv;
       const int c = d * SH + W::token_of(r, gx);
-      x = W::marked(x, marks, lane % SH, c);
-      if (RW < WAVES) x = W::marked(x, marks + RW * W::MARKS, lane % SH, c);
+      x = W::marked(x, marks, wr * SH + lane % SH, c);
       if (final)
         store4((el*)a.out + id * D + c, x);
       else if (!(l == 0.0f))
@@ -1258,6 +1304,7 @@ extern "C" tb_status tb_shared_prefix_attention(const void* q, const void* k_cac
   a.scale_log2 = scale == 0.0 ? 1.0f : (float)((scale < 0.0 ? -scale : scale) * 1.44269504088896340736);
   a.flip = scale < 0.0 ? 0x80008000u : 0u;
   a.keep = scale == 0.0 ? 0u : ~0u;
+  a.near = c_slot >= 0 && c_slot < (1 << 23);
   a.big = max_q * a.grp > FEW;
   a.tile_blocks = (int)p.tile_blocks;
   const bool e8 = cache_dtype == 3;
