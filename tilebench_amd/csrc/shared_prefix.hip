@@ -84,6 +84,15 @@ struct Args {
   int tile_blocks;
 };
 
+// The kernel's arguments, read again from memory.  Epilogues and other code off the loops take theirs from here: fields
+// that are only needed there would hold scalar registers through the loops, which then spill.
+__device__ __forceinline__ Args reload() {
+  typedef const __attribute__((address_space(4))) Args* ptr;
+  ptr p = (ptr)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const Args*)p;
+}
+
 template <int DT>
 struct Ty;
 template <>
@@ -697,6 +706,7 @@ __device__ __forceinline__ void attend_few(const Args& a, char* smem, const FewT
       *(f32x4*)(merge + (wave * FEW + row) * L::MERGE_ROW + d * SH + W::token_of(r, g)) = x;
     }
   __syncthreads();
+  const Args b = reload();
   for (int i = threadIdx.x; i < f.rows * (D / 4); i += THREADS) {
     const int r = i / (D / 4), c = (i % (D / 4)) * 4;
     float m = NEG_INF, sum = 0.0f;
@@ -711,13 +721,13 @@ __device__ __forceinline__ void attend_few(const Args& a, char* smem, const FewT
       x += *(const f32x4*)(merge + (k * FEW + r) * L::MERGE_ROW + c);
     }
     x = W::marked(x, marks, r, c);
-    const int64_t id = (int64_t)(f.q0 + r / a.grp) * a.Hq + h * a.grp + r % a.grp;
-    if (a.direct) {
-      store4((el*)a.out + id * D + c, x * inverse(sum));
-      if (c == 0) a.lse[id] = natural_lse(m, sum);
+    const int64_t id = (int64_t)(f.q0 + r / b.grp) * b.Hq + h * b.grp + r % b.grp;
+    if (b.direct) {
+      store4((el*)b.out + id * D + c, x * inverse(sum));
+      if (c == 0) b.lse[id] = natural_lse(m, sum);
     } else {
-      *(f32x4*)(a.part_o + ((int64_t)f.slot * a.T * a.Hq + id) * D + c) = x;
-      if (c == 0) a.part_ml[(int64_t)f.slot * a.T * a.Hq + id] = float2{m, sum};
+      *(f32x4*)(b.part_o + ((int64_t)f.slot * b.T * b.Hq + id) * D + c) = x;
+      if (c == 0) b.part_ml[(int64_t)f.slot * b.T * b.Hq + id] = float2{m, sum};
     }
   }
 }
@@ -898,8 +908,9 @@ __device__ __forceinline__ void row_tile(const Args& a, char* smem, int index) {
     b_last = sequence_of(a, t_last, gr.b0, gr.b1);
   }
   auto own_tokens = [&](int x) __attribute__((always_inline)) {
-    const Seq s = sequence(a, x);
-    if (s.n_q * a.grp <= FEW) return 0;
+    const Args again = reload();
+    const Seq s = sequence(again, x);
+    if (s.n_q * again.grp <= FEW) return 0;
     const int last = min(t_last, s.q0 + s.n_q - 1);
     return clamp_int(s.own - s.n_q + (last - s.q0) + 1, 0, s.own);
   };
@@ -932,8 +943,9 @@ __device__ __forceinline__ void row_tile(const Args& a, char* smem, int index) {
     const int n0 = skip, n1 = min(n_all, skip + todo);
     skip = 0;
     todo -= n1 - n0;
-    const Tokens src = pre ? Tokens{a.prefix_pages + (int64_t)u.g * a.Wp, a.Wp, len}
-                           : Tokens{a.pages + (int64_t)x * a.W, a.W, len};
+    const Args again = reload();
+    const Tokens src = pre ? Tokens{again.prefix_pages + (int64_t)u.g * again.Wp, again.Wp, len}
+                           : Tokens{again.pages + (int64_t)x * again.W, again.W, len};
     int limit = pre ? prefix_limit : b == x ? own_limit : 0;
     const bool some = valid && limit > 0;
     if (!valid) limit = 0x7FFFFFFF;
@@ -1029,7 +1041,8 @@ __device__ __forceinline__ void row_tile(const Args& a, char* smem, int index) {
       }
   }
   if (!valid) return;
-  const int64_t id = (int64_t)t * a.Hq + hq, slots = (int64_t)a.T * a.Hq, slot = u.split * slots + id;
+  const Args e = reload();
+  const int64_t id = (int64_t)t * e.Hq + hq, slots = (int64_t)e.T * e.Hq, slot = u.split * slots + id;
   const bool final = u.splits == 1 && big;
   const float inv = final ? inverse(l) : 1.0f;
 #pragma unroll
@@ -1042,15 +1055,15 @@ __device__ __forceinline__ void row_tile(const Args& a, char* smem, int index) {
       const int c = d * SH + W::token_of(r, gx);
       x = W::marked(x, marks, wr * SH + lane % SH, c);
       if (final)
-        store4((el*)a.out + id * D + c, x);
+        store4((el*)e.out + id * D + c, x);
       else if (!(l == 0.0f))
-        *(f32x4*)(a.part_o + slot * D + c) = x;
+        *(f32x4*)(e.part_o + slot * D + c) = x;
     }
   if (gx == 0) {
-    a.part_ml[slot] = float2{w.m, final ? -1.0f : l};
-    if (final) a.lse[id] = natural_lse(w.m, l);
+    e.part_ml[slot] = float2{w.m, final ? -1.0f : l};
+    if (final) e.lse[id] = natural_lse(w.m, l);
     if (u.split == 0 && !final)  // the slots that other tiles use
-      for (int k = u.splits; k < a.S1; ++k) a.part_ml[k * slots + id] = float2{NEG_INF, 0.0f};
+      for (int k = u.splits; k < e.S1; ++k) e.part_ml[k * slots + id] = float2{NEG_INF, 0.0f};
   }
 }
 
