@@ -38,6 +38,16 @@ CASES = {
     # few rows: groups of up to 32 rows
     "rows_16": dict(n_q=[4, 4], lens=[50, 4], prefix=[100], page=32),
     "rows_32": dict(n_q=[2, 2, 4], lens=[50, 2, 90], prefix=[300], D=128, page=64),
+    "rows_16_long": dict(n_q=[2, 2], lens=[50, 4], prefix=[1500], page=32, pad=1),
+    "rows_12_groups": dict(n_q=[1, 1, 1, 2, 1], lens=[50, 4, 0, 300, 7], prefix=[1500, 0, 900], bounds=[0, 2, 3, 5],
+                           D=128, page=32),
+    "joint_groups": dict(n_q=[1, 1, 1, 2, 1, 0], lens=[50, 4, 0, 300, 7, 2], prefix=[150, 0, 500], bounds=[0, 2, 3, 6],
+                         page=32, pad=2),
+    "many_groups": dict(n_q=[1] * 150, lens=[(5 * i) % 40 for i in range(150)], prefix=[(17 * i) % 300 for i in range(75)],
+                        bounds=[2 * i for i in range(76)], Hq=20, Hkv=2, page=8),
+    "many_in_a_group": dict(n_q=[1] * 150, lens=[(5 * i) % 40 for i in range(150)], prefix=[1100], page=16),
+    "many_mixed": dict(n_q=[1 + 7 * (i % 5 == 0) for i in range(150)], lens=[9 + (5 * i) % 40 for i in range(150)],
+                       prefix=[100], page=16),
     "mqa_20_rows": dict(n_q=[1, 1], lens=[30, 200], prefix=[500], Hq=20, Hkv=1, D=128),
     # row tiles
     "tile_ragged": dict(n_q=ONES, lens=[(11 * i) % 70 + 1 for i in range(40)], prefix=[1000], page=32),
@@ -95,9 +105,9 @@ def test_splits_of_long_prefixes_and_scales(gpu):
 
 
 @pytest.mark.parametrize("kw", [
-    dict(n_q=[1, 1], lens=[20, 70], prefix=[40]), dict(n_q=ONES, lens=[20] * 40, prefix=[90], D=128),
+    dict(n_q=[1, 1], lens=[20, 70], prefix=[40]), dict(n_q=[1, 2], lens=[20, 70], prefix=[1100]), dict(n_q=ONES, lens=[20] * 40, prefix=[90], D=128),
     dict(n_q=[70, 3], lens=[80, 20], prefix=[30], D=128), dict(n_q=[4, 2, 1], lens=[40, 3, 9])],
-    ids=["few", "tile", "chunk", "drafts"])
+    ids=["joint", "few", "tile", "chunk", "drafts"])
 @pytest.mark.parametrize("cache", ["same", "e4m3"])
 def test_values_outside_a_row_s_tokens_leave_no_trace(gpu, kw, cache):
     """NaN and infinities in unused slots and pages; in tokens after a query's own;

@@ -100,7 +100,7 @@ def test_entry_point_checks_before_touching_a_device():
     if not rt.LIB_PATH.exists():
         pytest.skip("libtbhip.so is not built")
     lib, fake = rt.load_library(), 1 << 40
-    base = dict(q=fake, kc=fake, ks=None, pp=fake, cu=fake, T=8, Hq=8, Hkv=2, D=64, G=1, Wp=4, B=2, W=4, max_q=4, N=16,
+    base = dict(q=fake, kc=fake, ks=None, pp=fake, cu=fake, T=8, Hq=8, Hkv=2, D=64, G=1, Wp=90, B=2, W=4, max_q=4, N=16,
                 P=16, q_st=512, c_slot=64, dtype=1, cache=1, ws=None, wb=0)
 
     def attend(**kw):
@@ -121,10 +121,12 @@ def test_entry_point_checks_before_touching_a_device():
     assert attend() == rt.TB_E_WORKSPACE and "workspace" in lib.tb_last_error().decode()
     need = ctypes.c_int64(-1)
     size = lib.tb_shared_prefix_attention_workspace_size
-    assert size(8, 8, 2, 64, 1, 4, 2, 4, 16, 4, ctypes.byref(need)) == rt.TB_OK and need.value > 0
+    assert size(8, 8, 2, 64, 1, 90, 2, 4, 16, 4, ctypes.byref(need)) == rt.TB_OK and need.value > 0
     assert attend(ws=fake, wb=need.value - 1) == rt.TB_E_WORKSPACE
     assert attend(ws=fake + 4, wb=need.value) == rt.TB_E_ALIGN
     assert size(0, 8, 2, 64, 1, 4, 2, 4, 16, 4, ctypes.byref(need)) == rt.TB_OK and need.value == 0
     # no prefix, and enough sequences to fill the device without splits: written directly
     assert size(512, 8, 8, 64, 0, 0, 512, 64, 16, 1, ctypes.byref(need)) == rt.TB_OK and need.value == 0
+    # short prefixes: every sequence reads its own
+    assert size(8, 8, 2, 64, 1, 4, 2, 4, 16, 4, ctypes.byref(need)) == rt.TB_OK and need.value == 0
     assert size(8, 8, 2, 64, 1, 4, 2, 4, 16, 4, None) == rt.TB_E_INVALID

@@ -9,10 +9,10 @@
 // Rows.  The query heads of one key/value head and the queries of one sequence
 // read the same tokens, so they are rows of one product: row r of a run of
 // queries is query r / grp, head r % grp of the group.  Three kinds of work:
-//   tiles   64 or 128 rows of a group of more than 16 rows: over the shared prefix, and
-//           on over the own tokens of those sequences that have more than 16 rows
-//   few     the own tokens of one sequence of up to 16 rows, or the prefix of a
-//           group of up to 16 rows: the block's four wavefronts split the tokens
+//   tiles   64 or 128 rows of a group: over the shared prefix, and on over the own
+//           tokens of those sequences that have more than 16 rows
+//   few     the own tokens of one sequence of up to 16 rows (in short calls with its
+//           prefix): the block's four wavefronts split the tokens
 //   combine joins the partial results of a row (one slot per split) by their maxima
 // so a prefix is read once per tile however many sequences share it.
 //
@@ -46,13 +46,26 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 enum { F16 = 1, BF16 = 2 };
 constexpr int THREADS = 256, WAVES = 4;
-constexpr int FEW = 16;      // rows of a sequence or group that the token-splitting blocks take
+constexpr int FEW = 16;      // rows of a sequence that the token-splitting blocks take
 constexpr int FILL = 512;    // blocks that fill the device: two on each of 256 CUs
 constexpr int MAX_SPLIT = 64;
 constexpr float NEG_INF = -__builtin_inff();
+
+// Division of n < 2^31 by a divisor that the host knows: n / d = (umulhi(n, mul) + n) >> shift.
+struct Divisor {
+  uint32_t d = 1, mul = 0, shift = 0;
+  Divisor() = default;
+  explicit Divisor(uint32_t by) : d(by) {
+    while ((1ull << shift) < by) ++shift;
+    mul = (uint32_t)((((1ull << shift) - by) << 32) / by + 1);
+  }
+  __device__ __forceinline__ int divide(int n) const { return (int)((__umulhi((uint32_t)n, mul) + (uint32_t)n) >> shift); }
+  __device__ __forceinline__ int rest(int n, int quotient) const { return n - quotient * (int)d; }
+};
 
 struct Args {
   const void* q;
@@ -74,23 +87,45 @@ struct Args {
   float* part_o;  // [slots][T * Hq][D]
   float2* part_ml;  // [slots][T * Hq]: maximum (log2) and sum; sum -1: the row is final
   int T, Hq, Hkv, grp, G, Wp, B, W;
+  Divisor by_grp, by_heads;  // grp, Hkv
   int n_pages, page_shift;
-  int S1, S2;       // slots of tiles and prefixes, slots of own tokens
+  int S1, S2;       // slots of tiles, slots of own tokens
+  int tile_fill;    // blocks that the tiles are shared out to
+  int spread;       // own tokens are shared out to 2 * FILL more blocks than there are sequences and heads
   int direct;       // own tokens in one slot and nothing else: results are final
   float scale_log2;     // of |scale|, or 1 for a scale of 0
   uint32_t flip, keep;  // applied to q
+  int joint;   // sequences read their prefix themselves
+  int rounds;  // at least FILL units of tiles
   int near;  // 64 slots of a page lie within 2 GiB
   int big;  // some sequence may have more than FEW rows
   int tile_blocks;
 };
 
-// The kernel's arguments, read again from memory.  Epilogues and other code off the loops take theirs from here: fields
-// that are only needed there would hold scalar registers through the loops, which then spill.
-__device__ __forceinline__ Args reload() {
-  typedef const __attribute__((address_space(4))) Args* ptr;
-  ptr p = (ptr)__builtin_amdgcn_kernarg_segment_ptr();
-  asm volatile("" : "+s"(p));
-  return *(const Args*)p;
+// The kernel's arguments once more, from LDS.  Epilogues and other code off the loops take theirs from here: fields that
+// are only needed there would hold scalar registers through the loops, which then spill, and reading the argument
+// segment again takes 2 us.
+constexpr int ARG_WORDS = sizeof(Args) / 4;
+static_assert(ARG_WORDS <= THREADS && sizeof(Args) % 4 == 0, "a word a thread");
+__device__ __forceinline__ uint32_t argument_word() {
+  const __attribute__((address_space(4))) uint32_t* p =
+      (const __attribute__((address_space(4))) uint32_t*)__builtin_amdgcn_kernarg_segment_ptr();
+  return p[min((int)threadIdx.x, ARG_WORDS - 1)];
+}
+template <typename V>
+__device__ __forceinline__ V lds_read(uint32_t addr);
+__device__ __forceinline__ Args saved_args(uint32_t at) {
+  struct {
+    uint32_t w[ARG_WORDS];
+  } x;
+#pragma unroll
+  for (int i = 0; i < ARG_WORDS; ++i) x.w[i] = lds_read<uint32_t>(at + 4 * i);
+  return __builtin_bit_cast(Args, x);
+}
+__device__ __forceinline__ const int* uniform(const int* p) {
+  const uint64_t u = (uint64_t)(uintptr_t)p;
+  return (const int*)(uintptr_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)u) |
+                                 (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(u >> 32)) << 32);
 }
 
 template <int DT>
@@ -183,6 +218,10 @@ template <int N>
 __device__ __forceinline__ void wait_vm() {
   asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
 }
+// A barrier for LDS contents that leaves vector memory operations pending (__syncthreads waits for them).
+__device__ __forceinline__ void block_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory");
+}
 __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory"); }
 
 // e4m3 scales of a tile, for each 32 tokens: 32 of the keys, 32 of the values.
@@ -197,8 +236,9 @@ struct Tokens {
 // 64 consecutive entries of a page table, one a lane (ids outside the pool clamped to it).
 struct Window {
   int ids = 0, first = 0x7FFFFFFF;
+  __device__ __forceinline__ void reset() { first = 0x7FFFFFFF; }
   __device__ __forceinline__ void cover(const Tokens& s, int lo, int hi, int n_pages) {
-    if (lo >= first && hi < first + 64) return;
+    if (lo >= first && hi - 64 < first) return;
     first = lo;
     int id = s.table[min(lo + (int)(threadIdx.x & 63), s.width - 1)];
     id = min(max(id, 0), n_pages - 1);
@@ -243,12 +283,13 @@ __device__ __forceinline__ float as_float(uint32_t x) { return __builtin_bit_cas
 // ------------------------------------------------------------------ one step
 //
 // State of one wavefront: SH rows (lane l: row l % SH), head dimension D.
-template <int DT, bool E8, int D, int SH>
+// E8: the tiles hold e4m3 codes (else 16-bit values); SC: keys and values have scales.
+template <int DT, bool E8, int D, int SH, bool SC = E8>
 struct Wave {
   typedef Ty<DT> Y;
   typedef typename Y::v8 v8;
   typedef typename std::conditional<SH == 16, f32x4, f32x16>::type acc_t;
-  static constexpr int RB = D * (E8 ? 1 : 2);
+  static constexpr int RB = D * (E8 ? 1 : 2), SIDE = SH;
   static constexpr int NG = 64 / SH;        // lane groups that share the rows
   static constexpr int KS = 8 * NG;         // depth of one product instruction
   static constexpr int STEPS = D / KS;      // of S^T
@@ -258,8 +299,8 @@ struct Wave {
   // log2 of the largest weight when m is set, and how far weights may grow past it before m is set again.  fp16:
   // weights down to 2^-32 (e4m3: 2^-28) of the largest are kept; with e4m3 values their scales are multiplied in, which leaves
   // room for scales up to 2^10 (a row of fp16 values has at most 146).
-  static constexpr float LIFT = DT == BF16 ? 0.0f : E8 ? 4.0f : 8.0f;
-  static constexpr float SLACK = DT == BF16 || !E8 ? 6.0f : 2.0f;
+  static constexpr float LIFT = DT == BF16 ? 0.0f : SC ? 4.0f : 8.0f;
+  static constexpr float SLACK = DT == BF16 || !SC ? 6.0f : 2.0f;
 
   v8 q[STEPS];
   acc_t o[DT_N];
@@ -368,14 +409,14 @@ struct Wave {
 #pragma unroll
       for (int r = 0; r < REGS; r += 4) {
         const int tok = t * SH + token_of(r, g);
-        if (E8) {
+        if (SC) {
           const f32x4 k = lds_read<f32x4>(scale_at(sbase, tok0 + tok));
 #pragma unroll
           for (int i = 0; i < 4; ++i) s[t][r + i] *= full || s[t][r + i] > NEG_INF ? k[i] : 1.0f;
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) top = fmaxf(top, s[t][r + i]);
-        if (E8 && r % 8 == 4) __builtin_amdgcn_sched_barrier(0);  // all scales at once would spill
+        if (SC && r % 8 == 4) __builtin_amdgcn_sched_barrier(0);  // all scales at once would spill
       }
     top = over_groups_max(top) * scale;
     if (__any(top > m + (LIFT + SLACK))) {
@@ -395,14 +436,14 @@ struct Wave {
 #pragma unroll
       for (int r = 0; r < REGS; r += 4) {
         f32x4 v;
-        if (E8) v = lds_read<f32x4>(scale_at(sbase, tok0 + t * SH + token_of(r, g)) + 128);
+        if (SC) v = lds_read<f32x4>(scale_at(sbase, tok0 + t * SH + token_of(r, g)) + 128);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r + i], scale, -use));
           sum += w;
-          s[t][r + i] = !E8 ? w : full || w > 0.0f ? w * v[i] : 0.0f;
+          s[t][r + i] = !SC ? w : full || w > 0.0f ? w * v[i] : 0.0f;
         }
-        if (E8 && r % 8 == 4) __builtin_amdgcn_sched_barrier(0);
+        if (SC && r % 8 == 4) __builtin_amdgcn_sched_barrier(0);
       }
     l += sum;
 #pragma unroll
@@ -465,10 +506,11 @@ struct Wave {
   // and marked for the rows that see their token: a byte for each row and each run of D / 64 channels, four bits a
   // channel (1: +inf, 2: -inf, 4: NaN), added to the row's output at the end.
   //
-  // Tokens tok0 .. tok0 + ROWS - 1 of the tile at vbase, t0 being the tile's first token; limit_of(r): the limit of row r.
+  // Tokens tok0 .. tok0 + ROWS - 1 of the tile at vbase, t0 being the tile's first token; limit_of(r): the limit of row
+  // r; the word `any` is set if there are any.
   template <int ROWS, typename Limit>
   static __device__ __forceinline__ void set_apart(uint32_t vbase, int tok0, int t0, int rows, uint32_t marks,
-                                                   Limit limit_of) {
+                                                   uint32_t any, Limit limit_of) {
     const int lane = threadIdx.x & 63;
     const uint32_t exps = E8 ? 0x7F7F7F7Fu : Y::EXP | Y::EXP << 16, ones = E8 ? 0x7F7F7F7Fu : 0x7FFF7FFFu;
     uint32_t good = ~0u;  // the top bit of an element: not (all exponent bits, or the NaN code)
@@ -479,6 +521,7 @@ struct Wave {
       for (int e = 0; e < 4; ++e) good &= exps - (x[e] & exps) + ones;
     }
     if (!__any((~good & ~ones) != 0)) return;
+    *(__attribute__((address_space(3))) int*)(uintptr_t)any = 1;
     constexpr int PER = D / 64, ESIZE = E8 ? 1 : 2;
     const int at = lane * PER * ESIZE;
 #pragma unroll 1
@@ -533,6 +576,9 @@ __device__ __forceinline__ Seq sequence(const Args& a, int b) {
   s.own = clamp_int(a.lens[b], 0, a.W << a.page_shift);
   return s;
 }
+__device__ __forceinline__ int prefix_length(const Args& a, int g) {
+  return a.prefix_lens ? clamp_int(a.prefix_lens[g], 0, a.Wp << a.page_shift) : 0;
+}
 struct Group {
   int b0, b1, q0, rows, len;  // sequences, first query, rows per key/value head, prefix tokens
 };
@@ -542,7 +588,7 @@ __device__ __forceinline__ Group group(const Args& a, int g) {
   r.b1 = a.group_offsets && g + 1 < a.G ? clamp_int(a.group_offsets[g + 1], r.b0, a.B) : a.B;
   r.q0 = query_start(a, r.b0);
   r.rows = max(query_start(a, r.b1) - r.q0, 0) * a.grp;
-  r.len = a.prefix_lens ? clamp_int(a.prefix_lens[g], 0, a.Wp << a.page_shift) : 0;
+  r.len = prefix_length(a, g);
   return r;
 }
 // The sequence of query t among b0 .. b1 - 1 (the last one that starts at or before it).
@@ -554,6 +600,41 @@ __device__ __forceinline__ int sequence_of(const Args& a, int t, int b0, int b1)
   }
   return lo;
 }
+
+// The sequences of a group: up to 64 of them are held one a lane (one round of loads, then shuffles), more are looked
+// up in memory.
+struct SeqTable {
+  int b0, n, start = 0x7FFFFFFF, next = 0x7FFFFFFF, own = 0;
+  __device__ __forceinline__ void load(const Args& a, int first, int last) {
+    const int lane = threadIdx.x & 63;
+    b0 = first;
+    n = last - first;
+    if (n <= 64 && lane < n) {
+      start = query_start(a, b0 + lane);
+      next = query_start(a, b0 + lane + 1);
+      own = clamp_int(a.lens[b0 + lane], 0, a.W << a.page_shift);
+    }
+  }
+  // number (from b0) of the sequence of query t; every lane takes part
+  __device__ __forceinline__ int find(const Args& a, int t) const {
+    if (n > 64) return sequence_of(a, t, b0, b0 + n) - b0;
+    int at = 0;
+#pragma unroll
+    for (int step = 32; step > 0; step >>= 1) {
+      const int c = __shfl(start, at + step);
+      if (at + step < n && c <= t) at += step;
+    }
+    return at;
+  }
+  __device__ __forceinline__ Seq get(const Args& a, int i) const {
+    if (n > 64) return sequence(a, b0 + i);
+    Seq s;
+    s.q0 = __shfl(start, i);
+    s.n_q = max(__shfl(next, i) - s.q0, 0);
+    s.own = __shfl(own, i);
+    return s;
+  }
+};
 
 // A row without tokens has the sum 0: its output is 0 and its lse -inf.
 __device__ __forceinline__ float inverse(float sum) { return sum == 0.0f ? 0.0f : 1.0f / sum; }
@@ -569,6 +650,77 @@ __device__ __forceinline__ void store4(el* p, f32x4 x) {
   *(decltype(v)*)p = v;
 }
 
+// ------------------------------------------------------------------ results of a block
+//
+// Layout in LDS at the end: the outputs of PARTS wavefronts for each of ROWS rows (fp32, 16-byte chunks swizzled by the
+// row), their references and sums, the marks.  Threads then take runs of four channels: whole rows are stored at once,
+// by a short loop (unrolled over a wavefront's registers it took 4 us, most of it fetching instructions).
+template <int D>
+__device__ __forceinline__ uint32_t out_at(uint32_t base, int part_row, int chunk) {
+  return base + part_row * D * 4 + ((chunk ^ (part_row & 15)) << 4);
+}
+template <typename W, int D>
+__device__ __forceinline__ void stash(const W& w, uint32_t outs, uint32_t stats, int part_row) {
+  const float l = W::over_groups_sum(w.l);
+  const int g = (threadIdx.x & 63) / W::SIDE;
+#pragma unroll
+  for (int d = 0; d < W::DT_N; ++d)
+#pragma unroll
+    for (int r = 0; r < W::REGS; r += 4) {
+      f32x4 x;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = w.o[d][r + i];
+      *(__attribute__((address_space(3))) f32x4*)(uintptr_t)out_at<D>(outs, part_row, (d * W::SIDE + W::token_of(r, g)) / 4) = x;
+    }
+  if (g == 0) *(__attribute__((address_space(3))) f32x2*)(uintptr_t)(stats + part_row * 8) = f32x2{w.m, l};
+}
+// rows: how many; q0: query of row `first`; final_row(r): its result is complete; unused: slots from this one on to mark
+// empty (S1 or S2 of them in all, from `slot0`).
+template <typename W, int D, int ROWS, int PARTS, typename Final>
+__device__ __forceinline__ void finish(uint32_t args, uint32_t outs, uint32_t stats, uint32_t marks, uint32_t any,
+                                       int rows, int q0, int first, int h, int slot, int empty0, int empty1, Final final_row) {
+  const Args a = saved_args(args);
+  const bool marked = lds_read<int>(any) != 0;
+  const int64_t all = (int64_t)a.T * a.Hq;
+  typedef typename W::Y::el el;
+#pragma unroll 1
+  for (int i = threadIdx.x; i < rows * (D / 4); i += THREADS) {
+    const int r = i / (D / 4), c = i % (D / 4);
+    f32x4 x = lds_read<f32x4>(out_at<D>(outs, r, c));
+    f32x2 ml = lds_read<f32x2>(stats + r * 8);  // reference, sum
+    if (PARTS > 1) {
+      float m = ml[0], sum = 0.0f;
+#pragma unroll
+      for (int k = 1; k < PARTS; ++k) m = fmaxf(m, lds_read<f32x2>(stats + (k * ROWS + r) * 8)[0]);
+      const float use = m == NEG_INF ? 0.0f : m;
+      f32x4 y{};
+#pragma unroll
+      for (int k = 0; k < PARTS; ++k) {
+        const f32x2 e = lds_read<f32x2>(stats + (k * ROWS + r) * 8);
+        const float f = __builtin_amdgcn_exp2f(e[0] - use);
+        sum += e[1] * f;
+        y += lds_read<f32x4>(out_at<D>(outs, k * ROWS + r, c)) * f;
+      }
+      x = y;
+      ml = f32x2{m, sum};
+    }
+    if (marked) x = W::marked(x, marks, r, c * 4);
+    const int qi = a.by_grp.divide(first + r);
+    const int64_t id = (int64_t)(q0 + qi) * a.Hq + h * a.grp + a.by_grp.rest(first + r, qi);
+    const bool final = final_row(r);
+    if (final)
+      store4((el*)a.out + id * D + c * 4, x * inverse(ml[1]));
+    else if (!(ml[1] == 0.0f))
+      *(f32x4*)(a.part_o + (slot * all + id) * D + c * 4) = x;
+    if (c == 0) {
+      if (final) a.lse[id] = natural_lse(ml[0], ml[1]);
+      if (!a.direct) a.part_ml[slot * all + id] = float2{ml[0], final ? -1.0f : ml[1]};
+      if (!final)
+        for (int k = empty0; k < empty1; ++k) a.part_ml[k * all + id] = float2{NEG_INF, 0.0f};
+    }
+  }
+}
+
 // ------------------------------------------------------------------ few rows
 
 template <int DT, bool E8, int D>
@@ -577,25 +729,22 @@ struct FewLayout {
   static constexpr int TOK = RB == 256 ? 32 : 64;  // tokens of a wavefront's step
   static constexpr int TILE_BYTES = TOK * RB;
   static constexpr int WAVE_BYTES = 2 * TILE_BYTES + (E8 ? 2 * TOK * 4 : 0);
-  static constexpr int MERGE_ROW = D + 4;  // floats; rows four banks apart
-  static constexpr int MERGE_BYTES = WAVES * FEW * MERGE_ROW * 4 + WAVES * FEW * 8;
-  static constexpr int MARKS = WAVES * WAVE_BYTES > MERGE_BYTES ? WAVES * WAVE_BYTES : MERGE_BYTES;
-  static constexpr int LIMITS = MARKS + FEW * 64;
-  static constexpr int LDS = LIMITS + FEW * 4;
+  static constexpr int OUT_BYTES = WAVES * FEW * D * 4;
+  static constexpr int MARKS = WAVES * WAVE_BYTES > OUT_BYTES ? WAVES * WAVE_BYTES : OUT_BYTES;
+  static constexpr int LIMITS = MARKS + FEW * 64, STATS = LIMITS + 2 * FEW * 4, ANY = STATS + WAVES * FEW * 8;
+  static constexpr int ARGS = ANY + 16, LDS = ARGS + sizeof(Args);
 };
 
-// What a block of few rows does: rows 0 .. rows - 1 (at most 16) from query q0 on over the tokens of `src`, of which it
-// takes split `split` of `splits`; results to slot `slot`.
+// What a block of few rows does: rows 0 .. rows - 1 (at most 16) from query q0 on, over prefix tokens and then own tokens
+// (either may be none), of which it takes split `split` of `splits`; results to slot `slot`.
 struct FewTask {
-  int h, q0, rows, split, splits, slot;
-  Tokens src;
-  bool own;    // own tokens of the sequence `seq`, or the prefix of sequences b0 .. b1 - 1
-  Seq seq;
-  int b0, b1;
+  int h, q0, rows, split, splits;
+  Tokens prefix, own;
+  int n_q, seen;  // queries of the sequence, its own tokens
 };
 
 template <int DT, bool E8, int D>
-__device__ __forceinline__ void attend_few(const Args& a, char* smem, const FewTask& f) {
+__device__ __forceinline__ void attend_few(const Args& a, char* smem, const FewTask& f, uint32_t arg_word) {
   constexpr int SH = 16;
   typedef FewLayout<DT, E8, D> L;
   typedef Wave<DT, E8, D, SH> W;
@@ -604,47 +753,41 @@ __device__ __forceinline__ void attend_few(const Args& a, char* smem, const FewT
   typedef Copier<RB, NI> Copy;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int row = lane % SH, h = f.h;
-  const Tokens src = f.src;
   const bool valid = row < f.rows;
-  const int t = f.q0 + row / a.grp, hq = h * a.grp + row % a.grp;
-
-  // tokens of `src` that the row attends to: its position is that of the last n_q tokens of its sequence
-  int limit = 0x7FFFFFFF;
-  if (valid) {
-    const Seq s = f.own ? f.seq : sequence(a, sequence_of(a, t, f.b0, f.b1));
-    const int end = s.own - s.n_q + (t - s.q0) + 1;  // own tokens up to and with the query
-    limit = clamp_int(f.own ? end : src.len + end, 0, src.len);
-  }
+  const int qi = a.by_grp.divide(row), hq = h * a.grp + a.by_grp.rest(row, qi), t = f.q0 + qi;
 
   W w;
   w.init((const el*)a.q + t * a.q_st + hq * a.q_sh, valid, a.flip, a.keep);
 
-  const int tiles = (src.len + TOK - 1) / TOK;
+  const int pre = (f.prefix.len + TOK - 1) / TOK, tiles = pre + (f.own.len + TOK - 1) / TOK;
   const int lo = (int)((int64_t)tiles * f.split / f.splits), hi = (int)((int64_t)tiles * (f.split + 1) / f.splits);
   const int n0 = lo + (hi - lo) * wave / WAVES, n1 = lo + (hi - lo) * (wave + 1) / WAVES;
 
   const uint32_t kbase = lds_addr(smem) + wave * L::WAVE_BYTES, vbase = kbase + L::TILE_BYTES;
   const uint32_t sbase = vbase + L::TILE_BYTES, marks = lds_addr(smem) + L::MARKS, limits = lds_addr(smem) + L::LIMITS;
-  for (int i = threadIdx.x; i < FEW * 16; i += THREADS) *(uint32_t*)(smem + L::MARKS + 4 * i) = 0;
-  if (wave == 0 && lane < SH) *(int*)(smem + L::LIMITS + 4 * lane) = limit;
-  __syncthreads();
   const char* kp = a.kc + h * a.c_head * ESIZE;
   const char* vp = a.vc + h * a.c_head * ESIZE;
+  // step n: of the prefix while n < pre, then of the own tokens
+  auto source = [&](int n) __attribute__((always_inline)) { return n < pre ? f.prefix : f.own; };
+  auto first_token = [&](int n) __attribute__((always_inline)) { return (n < pre ? n : n - pre) * TOK; };
   Window win;
   auto cover = [&](int n) __attribute__((always_inline)) {
-    const int t0 = n * TOK;
+    if (n == pre) win.reset();
+    const Tokens src = source(n);
+    const int t0 = first_token(n);
     win.cover(src, t0 >> a.page_shift, min(t0 + TOK - 1, src.len - 1) >> a.page_shift, a.n_pages);
   };
   auto fill_keys = [&](int n) __attribute__((always_inline)) {
-    Copy::run(a, win, src, kp, kbase, n * TOK, ESIZE, [](int r) { return swizzle_k<RB>(r); });
+    Copy::run(a, win, source(n), kp, kbase, first_token(n), ESIZE, [](int r) { return swizzle_k<RB>(r); });
   };
   auto fill_values = [&](int n) __attribute__((always_inline)) {
-    Copy::run(a, win, src, vp, vbase, n * TOK, ESIZE, [](int r) { return swizzle_v<RB, SH, E8>(r); });
+    Copy::run(a, win, source(n), vp, vbase, first_token(n), ESIZE, [](int r) { return swizzle_v<RB, SH, E8>(r); });
   };
   auto fill_scales = [&](int n) __attribute__((always_inline)) {  // 32 tokens a copy: keys' scales, then values'
+    const Tokens src = source(n);
 #pragma unroll
     for (int i = 0; i < TOK / 32; ++i) {
-      const int tok = min(n * TOK + i * 32 + (lane & 31), src.len - 1);
+      const int tok = min(first_token(n) + i * 32 + (lane & 31), src.len - 1);
       const int page = __builtin_amdgcn_ds_bpermute(((tok >> a.page_shift) - win.first) << 2, win.ids);
       const int64_t off = page * a.s_page + h * a.s_head + (tok & ((1 << a.page_shift) - 1)) * a.s_slot;
       dma4(sbase + i * 256, (const char*)((lane < 32 ? a.ks : a.vs) + off));
@@ -659,8 +802,26 @@ __device__ __forceinline__ void attend_few(const Args& a, char* smem, const FewT
     fill_keys(n0);
     fill_values(n0);
   }
+
+  // Tokens that the row attends to (its position is that of the last n_q tokens of its sequence), worked out while
+  // the first ones are on their way.
+  int prefix_limit = 0x7FFFFFFF, own_limit = 0x7FFFFFFF;
+  if (valid) {
+    const int end = f.seen - f.n_q + qi + 1;  // own tokens up to and with the query
+    prefix_limit = clamp_int(f.prefix.len + end, 0, f.prefix.len);
+    own_limit = clamp_int(end, 0, f.own.len);
+  }
+  for (int i = threadIdx.x; i < FEW * 16; i += THREADS) *(uint32_t*)(smem + L::MARKS + 4 * i) = 0;
+  if (threadIdx.x < ARG_WORDS) *(uint32_t*)(smem + L::ARGS + 4 * threadIdx.x) = arg_word;
+  if (wave == 0 && lane < SH) {
+    ((int*)(smem + L::LIMITS))[lane] = prefix_limit;
+    ((int*)(smem + L::LIMITS))[FEW + lane] = own_limit;
+    if (lane == 0) *(int*)(smem + L::ANY) = 0;
+  }
+  block_barrier();
+
   for (int n = n0; n < n1; ++n) {
-    const int t0 = n * TOK;
+    const int t0 = first_token(n), limit = n < pre ? prefix_limit : own_limit;
     const bool full = __all(limit >= t0 + TOK);
     typename W::acc_t s[TOK / SH];
     typename W::v8 p[TOK / W::KS];
@@ -676,7 +837,8 @@ __device__ __forceinline__ void attend_few(const Args& a, char* smem, const FewT
     if (!E8) w.template weights<TOK>(s, t0, limit, full, a.scale_log2, sbase, 0, p);
     if (n + 1 < n1) wait_vm<NI + (E8 ? TOK / 32 : 0)>(); else wait_vm<0>();
     if (!full) {
-      W::template set_apart<TOK>(vbase, 0, t0, f.rows, marks, [&](int r) { return lds_read<int>(limits + 4 * r); });
+      const uint32_t at = limits + (n < pre ? 0 : 4 * FEW);
+      W::template set_apart<TOK>(vbase, 0, t0, f.rows, marks, lds_addr(smem) + L::ANY, [&](int r) { return lds_read<int>(at + 4 * r); });
       wait_lds();
     }
     w.template values<TOK>(vbase, p);
@@ -684,52 +846,14 @@ __device__ __forceinline__ void attend_few(const Args& a, char* smem, const FewT
     if (n + 1 < n1) fill_values(n + 1);
   }
 
-  // join the four wavefronts
-  float l = W::over_groups_sum(w.l);
-  float* merge = (float*)smem;
-  float2* ml = (float2*)(merge + WAVES * FEW * L::MERGE_ROW);
-  __syncthreads();  // every wavefront is done with its tiles
-  if (lane < SH) ml[wave * FEW + row] = float2{w.m, l};
-  __syncthreads();
-  float top = NEG_INF;
-#pragma unroll
-  for (int i = 0; i < WAVES; ++i) top = fmaxf(top, ml[i * FEW + row].x);
-  const float alpha = __builtin_amdgcn_exp2f(w.m - (top == NEG_INF ? 0.0f : top));
-  const int g = lane / SH;
-#pragma unroll
-  for (int d = 0; d < W::DT_N; ++d)
-#pragma unroll
-    for (int r = 0; r < W::REGS; r += 4) {
-      f32x4 x;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = w.o[d][r + i] * alpha;
-      *(f32x4*)(merge + (wave * FEW + row) * L::MERGE_ROW + d * SH + W::token_of(r, g)) = x;
-    }
-  __syncthreads();
-  const Args b = reload();
-  for (int i = threadIdx.x; i < f.rows * (D / 4); i += THREADS) {
-    const int r = i / (D / 4), c = (i % (D / 4)) * 4;
-    float m = NEG_INF, sum = 0.0f;
-#pragma unroll
-    for (int k = 0; k < WAVES; ++k) m = fmaxf(m, ml[k * FEW + r].x);
-    const float use = m == NEG_INF ? 0.0f : m;
-    f32x4 x{};
-#pragma unroll
-    for (int k = 0; k < WAVES; ++k) {
-      const float2 e = ml[k * FEW + r];
-      sum += e.y * __builtin_amdgcn_exp2f(e.x - use);
-      x += *(const f32x4*)(merge + (k * FEW + r) * L::MERGE_ROW + c);
-    }
-    x = W::marked(x, marks, r, c);
-    const int64_t id = (int64_t)(f.q0 + r / b.grp) * b.Hq + h * b.grp + r % b.grp;
-    if (b.direct) {
-      store4((el*)b.out + id * D + c, x * inverse(sum));
-      if (c == 0) b.lse[id] = natural_lse(m, sum);
-    } else {
-      *(f32x4*)(b.part_o + ((int64_t)f.slot * b.T * b.Hq + id) * D + c) = x;
-      if (c == 0) b.part_ml[(int64_t)f.slot * b.T * b.Hq + id] = float2{m, sum};
-    }
-  }
+  block_barrier();  // every wavefront is done with its tiles
+  const uint32_t outs = lds_addr(smem), stats = outs + L::STATS;
+  stash<W, D>(w, outs, stats, wave * FEW + row);
+  block_barrier();
+  const bool direct = a.direct;
+  finish<W, D, FEW, WAVES>(outs + L::ARGS, outs, stats, marks, outs + L::ANY, f.rows, f.q0, 0, h, a.S1 + f.split,
+                           f.split == 0 ? a.S1 + f.splits : 0, f.split == 0 ? a.S1 + a.S2 : 0,
+                           [&](int) { return direct; });
 }
 
 // Outputs of queries t0 .. t1 - 1 that attend to nothing.
@@ -742,119 +866,61 @@ __device__ __forceinline__ void empty_rows(const Args& a, int h, int t0, int t1)
   }
 }
 
-// Block `index`: own tokens of sequence b (b < B) or prefix of group b - B; key/value head; split.
-template <int DT, bool E8, int D>
-__device__ __forceinline__ void few_rows(const Args& a, char* smem, int index) {
-  constexpr int TOK = FewLayout<DT, E8, D>::TOK;
-  const int own_blocks = a.B * a.Hkv * a.S2;
-  FewTask f;
-  f.own = index < own_blocks;
-  if (!f.own) index -= own_blocks;
-  const int heads = (f.own ? a.B : a.G) * a.Hkv, unit = index % heads, b = unit / a.Hkv;
-  f.h = unit % a.Hkv;
-  f.split = index / heads;
-  f.slot = f.own ? a.S1 + f.split : f.split;
-  if (f.own) {
-    if (a.direct && b == 0) {  // rows of no sequence
-      const int first = query_start(a, 0);
-      empty_rows<DT, D>(a, f.h, 0, first);
-      empty_rows<DT, D>(a, f.h, max(query_start(a, a.B), first), a.T);
-    }
-    f.seq = sequence(a, b);
-    f.q0 = f.seq.q0;
-    f.rows = f.seq.n_q * a.grp;
-    f.src = Tokens{a.pages + (int64_t)b * a.W, a.W, f.seq.own};
-    if (a.direct && f.rows > FEW) {  // more queries than max_q announced: nothing was planned for them
-      empty_rows<DT, D>(a, f.h, f.q0, f.q0 + f.seq.n_q);
-      return;
-    }
-  } else {
-    const Group gr = group(a, b);
-    f.q0 = gr.q0;
-    f.rows = gr.rows;
-    f.src = Tokens{a.prefix_pages + (int64_t)b * a.Wp, a.Wp, gr.len};
-    f.b0 = gr.b0;
-    f.b1 = gr.b1;
-    if (f.rows > FEW) return;  // its tiles write these slots
-  }
-  // splits of at least two steps a wavefront
-  f.splits = clamp_int((f.src.len + 8 * TOK - 1) / (8 * TOK), 1, f.own ? a.S2 : a.S1);
-  if (f.rows > FEW || f.split >= f.splits) {
-    for (int r = threadIdx.x; r < f.rows; r += THREADS)
-      a.part_ml[((int64_t)f.slot * a.T + f.q0 + r / a.grp) * a.Hq + f.h * a.grp + r % a.grp] = float2{NEG_INF, 0.0f};
-    return;
-  }
-  if (f.rows > 0) attend_few<DT, E8, D>(a, smem, f);
-}
-
-// ------------------------------------------------------------------ tiles of rows
-//
-// RW wavefronts side by side hold the tile's 32 * RW rows, 4 / RW wavefronts share the tokens of a step.
-template <int DT, bool E8, int D, int RW>
-struct TileLayout {
-  static constexpr int RB = D * (E8 ? 1 : 2);
-  static constexpr int ROWS = 32 * RW;
-  static constexpr int TOK = RB == 256 ? 64 : 128;  // tokens of a step
-  static constexpr int TILE_BYTES = TOK * RB;
-  static constexpr int STAGE = 2 * TILE_BYTES + (E8 ? 2 * TOK * 4 : 0);
-  static constexpr int MERGE_ROW = D + 4;
-  static constexpr int MARKS = 2 * STAGE;
-  static constexpr int ROW_INFO = MARKS + ROWS * 64;
-  static constexpr int LDS = ROW_INFO + ROWS * 12;
-  static_assert(RW == 4 || MARKS >= ROWS * (MERGE_ROW * 4 + 8), "the merge reuses the stages");
+// Which entry (group or sequence) block `index` works for, which of its units and which split of that.  Entries have
+// `units` units of `steps` steps (set by count(entry), an entry a lane, 64 at a time); a unit is cut into splits of
+// about the same number of steps, `fill` blocks in all at most (units beside: an entry's last split may be short), of
+// `least` steps at least and `most` splits at most.
+struct Unit {
+  int entry, lane, at, split, splits;
 };
-
-// Unit (group, row tile, key/value head) and split of tile block `index`; false past the last one.  Units come in
-// rounds of FILL blocks; those of a last, partial round are cut into up to S1 splits that fill the device.  A head's
-// units lie S1 and Hkv apart in block numbers, so with 8 heads they run on one XCD, whose L2 then holds the keys and
-// values that they share.
-struct TileUnit {
-  int g, tile, h, split, splits;
-};
-template <int ROWS>
-__device__ __forceinline__ bool find_tile(const Args& a, int index, TileUnit& u) {
+template <typename Count>
+__device__ __forceinline__ bool share_out(int entries, int index, int fill, int least, int most, Unit& u, int& total,
+                                          Count count) {
   const int lane = threadIdx.x & 63;
-  auto count = [&](int x) __attribute__((always_inline)) {  // tiles of group x
-    if (x >= a.G) return 0;
-    const Group gr = group(a, x);
-    return gr.rows > FEW ? (gr.rows + ROWS - 1) / ROWS : 0;
-  };
-  int n = 0, total = 0;
-  for (int x0 = (a.G - 1) / 64 * 64; x0 >= 0; x0 -= 64) {  // downwards: ends with the first groups in registers
-    n = count(x0 + lane);
-    total += n;
+  int units = 0, steps = 0;
+  total = 0;
+  float all = 0.0f;
+  for (int x0 = (entries - 1) / 64 * 64; x0 >= 0; x0 -= 64) {  // downwards: ends with the first entries in registers
+    count(x0 + lane, units, steps);
+    total += units;
+    all += (float)units * (float)steps;
   }
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) total += __shfl_xor(total, d);
-  const int units = __builtin_amdgcn_readfirstlane(total) * a.Hkv;
-  const int whole = units / FILL * FILL, tail = units - whole;
-  const int splits = tail ? clamp_int(FILL / tail, 1, a.S1) : 1;
-  int unit = index;
-  u.split = 0;
-  u.splits = 1;
-  if (index >= whole) {
-    index -= whole;
-    if (index >= tail * splits) return false;
-    unit = whole + index % tail;
-    u.split = index / tail;
-    u.splits = splits;
-  }
-  u.h = unit % a.Hkv;
-  const int tile = unit / a.Hkv;
-  int seen = 0;
-  for (int x0 = 0; x0 < a.G; x0 += 64) {
-    if (x0 > 0) n = count(x0 + lane);
-    int incl = n;
+  if (entries > 1) {
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-      const int o = __shfl_up(incl, d);
-      if (lane >= d) incl += o;
+      total += __shfl_xor(total, d);
+      all += __shfl_xor(all, d);
     }
-    const int here = __builtin_amdgcn_readfirstlane(__shfl(incl, 63));
-    if (tile < seen + here) {
-      const int l = __builtin_ctzll(__ballot(seen + incl > tile));
-      u.g = __builtin_amdgcn_readfirstlane(x0 + l);
-      u.tile = __builtin_amdgcn_readfirstlane(tile - seen - __shfl(incl - n, l));
+  }
+  total = __builtin_amdgcn_readfirstlane(total);
+  if (index >= total + fill) return false;
+  // steps of a split: sum of units * ceil(steps / share) <= sum of units * (steps / share + 1) <= fill
+  const int room = max(fill - total, fill / 4);
+  const float share = fmaxf(as_float(__builtin_amdgcn_readfirstlane(as_uint(all))) / (float)room, (float)least);
+  int seen = 0;
+  for (int x0 = 0; x0 < entries; x0 += 64) {
+    if (entries > 64) count(x0 + lane, units, steps);
+    int cuts = (int)ceilf((float)steps / share);
+    if (entries == 1) cuts = min(fill / max(units, 1), (steps + least - 1) / least);
+    cuts = clamp_int(cuts, 1, most);
+    int incl = units * cuts;
+    const int n = incl;
+    if (entries > 1) {
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(incl, d);
+        if (lane >= d) incl += o;
+      }
+    }
+    const int here = __builtin_amdgcn_readlane(incl, entries > 1 ? 63 : 0);
+    if (index < seen + here) {
+      u.lane = entries > 1 ? __builtin_ctzll(__ballot(seen + incl > index)) : 0;
+      const int at = index - seen - __builtin_amdgcn_readlane(incl - n, u.lane);
+      const int of = __builtin_amdgcn_readlane(units, u.lane);
+      u.entry = x0 + u.lane;
+      u.splits = __builtin_amdgcn_readlane(cuts, u.lane);
+      u.split = (int)((uint32_t)at / (uint32_t)of);
+      u.at = at - u.split * of;
       return true;
     }
     seen += here;
@@ -862,115 +928,322 @@ __device__ __forceinline__ bool find_tile(const Args& a, int index, TileUnit& u)
   return false;
 }
 
+// Block `index` of the own tokens: sequence, key/value head, split (with the sequence's prefix where the call is
+// `joint`).
+template <int DT, bool E8, int D>
+__device__ __forceinline__ void few_rows(const Args& a, char* smem, int index, uint32_t arg_word) {
+  constexpr int TOK = FewLayout<DT, E8, D>::TOK;
+  Seq s;
+  FewTask f;
+  int b;
+  if (a.spread) {
+    Seq of_lane;
+    Unit u;
+    int total;
+    auto count = [&](int x, int& units, int& steps) __attribute__((always_inline)) {
+      units = steps = 0;
+      if (x >= a.B) return;
+      of_lane = sequence(a, x);
+      const int rows = of_lane.n_q * a.grp;
+      units = rows > 0 ? a.Hkv : 0;
+      steps = rows > FEW ? 0 : (of_lane.own + TOK - 1) / TOK;
+    };
+    if (!share_out(a.B, index, 2 * FILL, 8, a.S2, u, total, count)) return;  // two steps a wavefront at least
+    b = u.entry;
+    f.h = u.at;
+    f.split = u.split;
+    f.splits = u.splits;
+    s.q0 = __builtin_amdgcn_readlane(of_lane.q0, u.lane);
+    s.n_q = __builtin_amdgcn_readlane(of_lane.n_q, u.lane);
+    s.own = __builtin_amdgcn_readlane(of_lane.own, u.lane);
+  } else {
+    b = a.by_heads.divide(index);
+    f.h = a.by_heads.rest(index, b);
+    f.split = 0;
+    f.splits = 1;
+    s = sequence(a, b);
+    if (a.direct && b == 0) {  // rows of no sequence
+      const int first = query_start(a, 0);
+      empty_rows<DT, D>(a, f.h, 0, first);
+      empty_rows<DT, D>(a, f.h, max(query_start(a, a.B), first), a.T);
+    }
+  }
+  f.q0 = s.q0;
+  f.n_q = s.n_q;
+  f.rows = s.n_q * a.grp;
+  f.seen = s.own;
+  f.own = Tokens{a.pages + (int64_t)b * a.W, a.W, s.own};
+  f.prefix = Tokens{nullptr, 0, 0};
+  if (a.joint) {
+    int lo = 0, hi = a.G;  // the last group that starts at or before the sequence
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (a.group_offsets[mid] <= b) lo = mid; else hi = mid;
+    }
+    f.prefix = Tokens{a.prefix_pages + (int64_t)lo * a.Wp, a.Wp, prefix_length(a, lo)};
+  }
+  if (f.rows > FEW) {
+    if (a.direct) {  // more queries than max_q announced: nothing was planned for them
+      empty_rows<DT, D>(a, f.h, f.q0, f.q0 + s.n_q);
+      return;
+    }
+    const int64_t all = (int64_t)a.T * a.Hq;  // their tiles take the own tokens
+    for (int r = threadIdx.x; r < f.rows; r += THREADS) {
+      const int qi = a.by_grp.divide(r);
+      const int64_t id = (int64_t)(f.q0 + qi) * a.Hq + f.h * a.grp + a.by_grp.rest(r, qi);
+      for (int k = 0; k < a.S2; ++k) a.part_ml[(a.S1 + k) * all + id] = float2{NEG_INF, 0.0f};
+    }
+    return;
+  }
+  if (f.rows > 0) attend_few<DT, E8, D>(a, smem, f, arg_word);
+}
+
+// ------------------------------------------------------------------ tiles of rows
+//
+// RW wavefronts side by side hold the tile's 32 * RW rows, 4 / RW wavefronts share the tokens of a step.
 template <int DT, bool E8, int D, int RW>
-__device__ __forceinline__ void row_tile(const Args& a, char* smem, int index) {
+struct TileLayout {
+  static constexpr int RB = D * 2;  // the tiles hold 16-bit values; e4m3 codes are converted on the way
+  static constexpr int ROWS = 32 * RW;
+  static constexpr int TOK = RB == 256 ? 64 : 128;  // tokens of a step
+  static constexpr int TILE_BYTES = TOK * RB;
+  static constexpr int STAGE = 2 * TILE_BYTES + (E8 ? 2 * TOK * 4 : 0);
+  static constexpr int MARKS = 2 * STAGE;
+  static constexpr int ROW_INFO = MARKS + ROWS * 64, STATS = ROW_INFO + ROWS * 12, ANY = STATS + WAVES * 32 * 8;
+  static constexpr int ARGS = ANY + 16, LDS = ARGS + sizeof(Args);
+  static_assert(MARKS >= WAVES * 32 * D * 4, "the outputs reuse the stages");
+};
+
+// Unit (group, row tile, key/value head) and split of tile block `index`; false past the last one.
+//
+// At least FILL units: rounds of FILL whole units, then those of a last, partial round cut into splits that fill the
+// device.  Fewer are shared out by their steps.  A head's units lie Hkv apart in block numbers, so with 8 heads they
+// run on one XCD, whose L2 then holds the keys and values that they share.
+struct TileUnit {
+  Group gr;
+  int g, tile, h, split, splits;
+};
+template <int ROWS, int TOK>
+__device__ __forceinline__ bool find_tile(const Args& a, int index, TileUnit& t) {
+  Group gr;
+  auto count = [&](int x, int& units, int& steps) __attribute__((always_inline)) {
+    units = steps = 0;
+    if (x >= a.G) return;
+    gr = group(a, x);
+    units = (gr.rows + ROWS - 1) / ROWS * a.Hkv;
+    steps = (gr.len + (a.big ? a.W << a.page_shift : 0) + TOK - 1) / TOK;  // own tokens: the most there may be
+  };
+  Unit u;
+  int total, split = 0, splits = 0;
+  if (a.rounds) {
+    // units in order, uncut: of the count of units, which of them this block takes
+    if (a.G == 1) {
+      int steps;
+      count(0, total, steps);
+    } else {
+      total = 0;
+      for (int x0 = 0; x0 < a.G; x0 += 64) {
+        int units, steps;
+        count(x0 + (threadIdx.x & 63), units, steps);
+        total += units;
+      }
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) total += __shfl_xor(total, d);
+    }
+    total = __builtin_amdgcn_readfirstlane(total);
+    const int whole = total / FILL * FILL, tail = total - whole;
+    splits = 1;
+    if (index >= whole) {
+      if (tail == 0) return false;
+      splits = clamp_int(FILL / tail, 1, a.S1);
+      index -= whole;
+      if (index >= tail * splits) return false;
+      split = index / tail;
+      index = whole + index - split * tail;
+    }
+  }
+  if (!share_out(a.G, index, a.tile_fill, 256 / TOK, a.rounds ? 1 : a.S1, u, total, count)) return false;
+  t.split = a.rounds ? split : u.split;
+  t.splits = a.rounds ? splits : u.splits;
+  t.g = u.entry;
+  t.tile = a.by_heads.divide(u.at);
+  t.h = a.by_heads.rest(u.at, t.tile);
+  t.gr.b0 = __builtin_amdgcn_readlane(gr.b0, u.lane);
+  t.gr.b1 = __builtin_amdgcn_readlane(gr.b1, u.lane);
+  t.gr.q0 = __builtin_amdgcn_readlane(gr.q0, u.lane);
+  t.gr.rows = __builtin_amdgcn_readlane(gr.rows, u.lane);
+  t.gr.len = __builtin_amdgcn_readlane(gr.len, u.lane);
+  return true;
+}
+
+template <int DT, bool E8, int D, int RW>
+__device__ __forceinline__ void row_tile(const Args& a, char* smem, int index, uint32_t arg_word) {
   typedef TileLayout<DT, E8, D, RW> L;
   constexpr int SH = 32, TOK = L::TOK, RB = L::RB, ESIZE = E8 ? 1 : 2;
   constexpr int MINE = TOK / WAVES;            // tokens that a wavefront fetches
-  constexpr int NI = MINE * RB / 1024;         // in copies of 1 KiB
-  typedef Copier<RB, NI> Copy;
-  constexpr int SHARE = TOK * RW / WAVES;      // tokens that a wavefront attends to
-  constexpr int MOST = E8 ? 32 : 64;           // in steps of so many (e4m3: 64 would spill)
-  constexpr int STEP = SHARE > MOST ? MOST : SHARE;
+  constexpr int NI = MINE * D * ESIZE / 1024;  // in copies of 1 KiB
+  constexpr int SHARE = TOK * RW / WAVES;      // tokens of a step that a wavefront attends to
+  constexpr int BIG = 1 << 30;                 // on a row's sequence number: it has more than 16 rows
+  constexpr int STEP = SHARE > 64 ? 64 : SHARE;
   static_assert(NI >= 1, "a wavefront fetches whole copies");
-  typedef Wave<DT, E8, D, SH> W;
+  typedef Copier<RB, NI> Copy;
+  typedef Wave<DT, false, D, SH, E8> W;
   typedef typename W::Y::el el;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int wr = wave % RW, wt = wave / RW;
   TileUnit u;
-  if (!find_tile<L::ROWS>(a, index, u)) return;
+  if (!find_tile<L::ROWS, TOK>(a, index, u)) return;
   const int h = u.h;
-  const Group gr = group(a, u.g);
+  const Group gr = u.gr;
   const int row = u.tile * L::ROWS + wr * SH + lane % SH;
   const bool valid = row < gr.rows;
-  const int t = gr.q0 + row / a.grp, hq = h * a.grp + row % a.grp;
+  const int qi = a.by_grp.divide(row), hq = h * a.grp + a.by_grp.rest(row, qi), t = gr.q0 + qi;
 
-  int b = -1, end = 0, own_limit = 0;
-  bool big = false;
-  if (valid) {
-    b = sequence_of(a, t, gr.b0, gr.b1);
-    const Seq s = sequence(a, b);
-    end = s.own - s.n_q + (t - s.q0) + 1;
-    own_limit = clamp_int(end, 0, s.own);
-    big = s.n_q * a.grp > FEW;
-  }
-  const int prefix_limit = valid ? clamp_int(gr.len + end, 0, gr.len) : 0;
-
+  SeqTable table;
+  table.load(a, gr.b0, gr.b1);
   W w;
   w.init((const el*)a.q + t * a.q_st + hq * a.q_sh, valid, a.flip, a.keep);
 
   // The tile's tokens: the prefix, then the own tokens (as far as a row of the tile sees them) of each of its
   // sequences with more than 16 rows.  Steps are counted over all of them and shared out to the splits.
-  int b_first = gr.b0, b_last = gr.b0 - 1, t_last = 0;
+  int x_first = 0, x_last = -1, t_last = 0;  // sequences, from the group's first
   if (a.big) {
-    t_last = gr.q0 + (min((u.tile + 1) * L::ROWS, gr.rows) - 1) / a.grp;
-    b_first = sequence_of(a, gr.q0 + u.tile * L::ROWS / a.grp, gr.b0, gr.b1);
-    b_last = sequence_of(a, t_last, gr.b0, gr.b1);
+    t_last = gr.q0 + a.by_grp.divide(min((u.tile + 1) * L::ROWS, gr.rows) - 1);
+    x_first = __builtin_amdgcn_readfirstlane(table.find(a, gr.q0 + a.by_grp.divide(u.tile * L::ROWS)));
+    x_last = __builtin_amdgcn_readfirstlane(table.find(a, t_last));
   }
-  auto own_tokens = [&](int x) __attribute__((always_inline)) {
-    const Args again = reload();
-    const Seq s = sequence(again, x);
-    if (s.n_q * again.grp <= FEW) return 0;
+  auto own_tokens = [&](const Args& a, int x) __attribute__((always_inline)) {
+    const Seq s = table.get(a, x);
     const int last = min(t_last, s.q0 + s.n_q - 1);
-    return clamp_int(s.own - s.n_q + (last - s.q0) + 1, 0, s.own);
+    return __builtin_amdgcn_readfirstlane(
+        s.n_q * a.grp <= FEW ? 0 : clamp_int(s.own - s.n_q + (last - s.q0) + 1, 0, s.own));
   };
   int steps = (gr.len + TOK - 1) / TOK;
-  for (int x = b_first; x <= b_last; ++x) steps += (own_tokens(x) + TOK - 1) / TOK;
+  for (int x = x_first; x <= x_last; ++x) steps += (own_tokens(a, x) + TOK - 1) / TOK;
   steps = __builtin_amdgcn_readfirstlane(steps);
   int skip = (int)((int64_t)steps * u.split / u.splits);
   int todo = (int)((int64_t)steps * (u.split + 1) / u.splits) - skip;
 
-  const uint32_t base = lds_addr(smem), marks = base + L::MARKS, info = base + L::ROW_INFO;
-  for (int i = threadIdx.x; i < L::ROWS * 16; i += THREADS) *(uint32_t*)(smem + L::MARKS + 4 * i) = 0;
-  // of every row, for the marks: sequence (-1: no row), prefix tokens and own tokens that it sees
-  if (wt == 0 && lane < SH) {
-    int* p = (int*)(smem + L::ROW_INFO) + wr * SH + lane;
-    p[0] = b;
-    p[L::ROWS] = prefix_limit;
-    p[2 * L::ROWS] = own_limit;
-  }
+  const uint32_t base = lds_addr(smem), marks = base + L::MARKS, info = base + L::ROW_INFO, any = base + L::ANY;
   const char* kp = a.kc + h * a.c_head * ESIZE;
   const char* vp = a.vc + h * a.c_head * ESIZE;
 
-  for (int x = b_first - 1; x <= b_last && todo > 0; ++x) {
-    const bool pre = x < b_first;
-    const int len = __builtin_amdgcn_readfirstlane(pre ? gr.len : own_tokens(x));
-    const int n_all = (len + TOK - 1) / TOK;
-    if (skip >= n_all) {
-      skip -= n_all;
-      continue;
+  // the run of steps at hand: steps n0 .. n1 - 1 of the prefix (x < x_first) or of sequence x
+  int x = x_first - 2, n0 = 0, n1 = 0;
+  Tokens src{nullptr, 0, 0};
+  Window win;
+  auto next_run = [&](const Args& a) __attribute__((always_inline)) {
+    while (todo > 0 && x < x_last) {
+      ++x;
+      const int len = x < x_first ? gr.len : own_tokens(a, x);
+      const int all = (len + TOK - 1) / TOK;
+      if (skip >= all) {
+        skip -= all;
+        continue;
+      }
+      n0 = skip;
+      n1 = min(all, skip + todo);
+      skip = 0;
+      todo -= n1 - n0;
+      src.table = uniform(x < x_first ? a.prefix_pages + (int64_t)u.g * a.Wp : a.pages + (int64_t)(gr.b0 + x) * a.W);
+      src.width = __builtin_amdgcn_readfirstlane(x < x_first ? a.Wp : a.W);
+      src.len = len;
+      win.reset();
+      return true;
     }
-    const int n0 = skip, n1 = min(n_all, skip + todo);
-    skip = 0;
-    todo -= n1 - n0;
-    const Args again = reload();
-    const Tokens src = pre ? Tokens{again.prefix_pages + (int64_t)u.g * again.Wp, again.Wp, len}
-                           : Tokens{again.pages + (int64_t)x * again.W, again.W, len};
-    int limit = pre ? prefix_limit : b == x ? own_limit : 0;
+    return false;
+  };
+  // e4m3 codes pass through registers: rows lane / LANES + i * (64 / LANES), 16 codes a lane, and one scale a lane (of
+  // the keys of the wavefront's tokens, then of their values).
+  constexpr int LANES = D / 16;
+  u32x4 codes[2][E8 ? NI : 1];
+  float scale = 0.0f;
+  auto fetch = [&](int n) __attribute__((always_inline)) {
+    const int t0 = n * TOK + wave * MINE;  // the wavefront's first token
+    win.cover(src, min(t0, src.len - 1) >> a.page_shift, min(t0 + MINE - 1, src.len - 1) >> a.page_shift, a.n_pages);
+    if (!E8) {
+      const uint32_t kb = base + (n & 1) * L::STAGE + wave * MINE * RB;
+      Copy::run(a, win, src, kp, kb, t0, ESIZE, [](int r) { return swizzle_k<RB>(r); });
+      Copy::run(a, win, src, vp, kb + L::TILE_BYTES, t0, ESIZE, [](int r) { return swizzle_v<RB, SH, false>(r); });
+      return;
+    }
+    const int mask = (1 << a.page_shift) - 1;
+    auto offset = [&](int r, int64_t page_stride, int64_t slot_stride) __attribute__((always_inline)) {
+      const int tok = min(t0 + r, src.len - 1);
+      const int page = __builtin_amdgcn_ds_bpermute(((tok >> a.page_shift) - win.first) << 2, win.ids);
+      return page * page_stride + (tok & mask) * slot_stride;
+    };
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int64_t off = offset(lane / LANES + i * (64 / LANES), a.c_page, a.c_slot) + (lane % LANES) * 16;
+      codes[0][i] = *(const u32x4*)(kp + off);
+      codes[1][i] = *(const u32x4*)(vp + off);
+    }
+    const int64_t off = offset(lane % MINE, a.s_page, a.s_slot) + h * a.s_head;
+    scale = ((lane / MINE) & 1 ? a.vs : a.ks)[off];
+  };
+  auto place = [&](int n) __attribute__((always_inline)) {
+    if (!E8) return;
+    const uint32_t stage = base + (n & 1) * L::STAGE;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int r = wave * MINE + lane / LANES + i * (64 / LANES);
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+        const uint32_t row = stage + kv * L::TILE_BYTES + r * RB;
+        const int swizzle = kv ? swizzle_v<RB, SH, false>(r) : swizzle_k<RB>(r);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          u32x4 x;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = W::Y::up8(codes[kv][i][half * 2 + e / 2], e & 1);
+          *(__attribute__((address_space(3))) u32x4*)(uintptr_t)(row + ((((lane % LANES) * 2 + half) ^ swizzle) << 4)) = x;
+        }
+      }
+    }
+    if (lane < 2 * MINE)
+      *(__attribute__((address_space(3))) float*)(uintptr_t)(
+          scale_at(stage + 2 * L::TILE_BYTES, wave * MINE + lane % MINE) + (lane / MINE) * 128) = scale;
+  };
+  bool have = next_run(a);
+  if (have) fetch(n0);
+
+  // What the rows see, worked out while the first tokens are on their way.
+  int mine = -1, prefix_limit = 0, own_limit = 0;  // sequence from the group's first
+  bool big = false;
+  {
+    const int i = table.find(a, t);
+    const Seq s = table.get(a, i);
+    if (valid) {
+      const int end = s.own - s.n_q + (t - s.q0) + 1;  // own tokens up to and with the query
+      mine = i;
+      prefix_limit = clamp_int(gr.len + end, 0, gr.len);
+      own_limit = clamp_int(end, 0, s.own);
+      big = s.n_q * a.grp > FEW;
+    }
+  }
+  for (int i = threadIdx.x; i < L::ROWS * 16; i += THREADS) *(uint32_t*)(smem + L::MARKS + 4 * i) = 0;
+  if (threadIdx.x < ARG_WORDS) *(uint32_t*)(smem + L::ARGS + 4 * threadIdx.x) = arg_word;
+  // of every row, for the marks: sequence (-1: no row), prefix tokens and own tokens that it sees
+  if (wt == 0 && lane < SH) {
+    int* p = (int*)(smem + L::ROW_INFO) + wr * SH + lane;
+    p[0] = big ? mine | BIG : mine;
+    p[L::ROWS] = prefix_limit;
+    p[2 * L::ROWS] = own_limit;
+    if (wr == 0 && lane == 0) *(int*)(smem + L::ANY) = 0;
+  }
+  if (have) place(n0);
+  block_barrier();
+
+  while (have) {
+    const bool pre = x < x_first;
+    int limit = pre ? prefix_limit : mine == x ? own_limit : 0;
     const bool some = valid && limit > 0;
     if (!valid) limit = 0x7FFFFFFF;
-    Window win;
-    auto fill = [&](int n) __attribute__((always_inline)) {
-      const int t0 = n * TOK + wave * MINE;  // the wavefront's first token
-      const uint32_t kb = base + (n & 1) * L::STAGE + wave * MINE * RB;
-      win.cover(src, min(t0, src.len - 1) >> a.page_shift, min(t0 + MINE - 1, src.len - 1) >> a.page_shift, a.n_pages);
-      Copy::run(a, win, src, kp, kb, t0, ESIZE, [](int r) { return swizzle_k<RB>(r); });
-      Copy::run(a, win, src, vp, kb + L::TILE_BYTES, t0, ESIZE, [](int r) { return swizzle_v<RB, SH, E8>(r); });
-      if (E8) {
-        static_assert(MINE == 32 || !E8, "the scales of 32 tokens a copy");
-        const int tok = min(t0 + (lane & 31), src.len - 1);
-        const int page = __builtin_amdgcn_ds_bpermute(((tok >> a.page_shift) - win.first) << 2, win.ids);
-        const int64_t off = page * a.s_page + h * a.s_head + (tok & ((1 << a.page_shift) - 1)) * a.s_slot;
-        dma4(base + (n & 1) * L::STAGE + 2 * L::TILE_BYTES + wave * 256, (const char*)((lane < 32 ? a.ks : a.vs) + off));
-      }
-    };
-    // both stages may still be read from the segment before; the rows' limits are there after this
-    __syncthreads();
-    fill(n0);
     auto limit_of = [&](int r) {
-      const int rb = lds_read<int>(info + 4 * r);
+      const int rb = lds_read<int>(info + 4 * r);  // (a sequence whose own tokens are read here has the BIG bit)
       return rb < 0 ? 0 : pre ? lds_read<int>(info + 4 * (L::ROWS + r))
-                              : rb == x ? lds_read<int>(info + 4 * (2 * L::ROWS + r)) : 0;
+                              : rb == (x | BIG) ? lds_read<int>(info + 4 * (2 * L::ROWS + r)) : 0;
     };
     int seen_by_all = 0x7FFFFFFF;  // tokens that every row of the tile sees
 #pragma unroll
@@ -983,10 +1256,9 @@ __device__ __forceinline__ void row_tile(const Args& a, char* smem, int index) {
       const uint32_t stage = base + (n & 1) * L::STAGE;
       wait_vm<0>();
       if ((n + 1) * TOK > seen_by_all)  // each wavefront looks at the tokens it has fetched
-        W::template set_apart<MINE>(stage + L::TILE_BYTES, wave * MINE, n * TOK, L::ROWS, marks, limit_of);
-      wait_lds();
-      __builtin_amdgcn_s_barrier();  // the step's tokens are there, the other stage is free
-      if (n + 1 < n1) fill(n + 1);
+        W::template set_apart<MINE>(stage + L::TILE_BYTES, wave * MINE, n * TOK, L::ROWS, marks, any, limit_of);
+      block_barrier();  // the step's tokens are there, the other stage is free
+      if (n + 1 < n1) fetch(n + 1);
 #pragma unroll
       for (int c = 0; c < SHARE / STEP; ++c) {
         const int tok0 = wt * SHARE + c * STEP, t0 = n * TOK + tok0;
@@ -999,72 +1271,29 @@ __device__ __forceinline__ void row_tile(const Args& a, char* smem, int index) {
         w.template weights<STEP>(s, t0, limit, full, a.scale_log2, stage + 2 * L::TILE_BYTES, tok0, p);
         w.template values<STEP>(kb + L::TILE_BYTES, p);
       }
+      if (n + 1 < n1) place(n + 1);
+    }
+    if (todo > 0) {
+      have = next_run(saved_args(base + L::ARGS));
+      if (have) {
+        block_barrier();  // both stages may still be read
+        fetch(n0);
+        place(n0);
+      }
+    } else {
+      have = false;
     }
   }
 
-  float l = W::over_groups_sum(w.l), alpha = 1.0f;
-  const int gx = lane / SH;
-  float* merge = (float*)smem;
-  float2* ml = (float2*)(merge + L::ROWS * L::MERGE_ROW);
-  __syncthreads();  // all marks are made
-  if (RW < WAVES) {
-    // the wavefronts that share a row: the second hands its results to the first
-    static_assert(RW == WAVES || RW * 2 == WAVES, "two halves");
-    const int r = wr * SH + lane % SH;
-    if (wt == 1) {
-#pragma unroll
-      for (int d = 0; d < W::DT_N; ++d)
-#pragma unroll
-        for (int i = 0; i < W::REGS; i += 4) {
-          f32x4 x;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] = w.o[d][i + e];
-          *(f32x4*)(merge + r * L::MERGE_ROW + d * SH + W::token_of(i, gx)) = x;
-        }
-      if (gx == 0) ml[r] = float2{w.m, l};
-    }
-    __syncthreads();
-    if (wt == 1) return;
-    const float2 other = ml[r];
-    const float top = fmaxf(w.m, other.x), use = top == NEG_INF ? 0.0f : top;
-    alpha = __builtin_amdgcn_exp2f(w.m - use);
-    const float beta = __builtin_amdgcn_exp2f(other.x - use);
-    l = l * alpha + other.y * beta;
-    w.m = top;
-#pragma unroll
-    for (int d = 0; d < W::DT_N; ++d)
-#pragma unroll
-      for (int i = 0; i < W::REGS; i += 4) {
-        const f32x4 x = *(const f32x4*)(merge + r * L::MERGE_ROW + d * SH + W::token_of(i, gx));
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w.o[d][i + e] = w.o[d][i + e] * alpha + x[e] * beta;
-      }
-  }
-  if (!valid) return;
-  const Args e = reload();
-  const int64_t id = (int64_t)t * e.Hq + hq, slots = (int64_t)e.T * e.Hq, slot = u.split * slots + id;
-  const bool final = u.splits == 1 && big;
-  const float inv = final ? inverse(l) : 1.0f;
-#pragma unroll
-  for (int d = 0; d < W::DT_N; ++d)
-#pragma unroll
-    for (int r = 0; r < W::REGS; r += 4) {
-      f32x4 x;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = w.o[d][r + i] * inv;
-      const int c = d * SH + W::token_of(r, gx);
-      x = W::marked(x, marks, wr * SH + lane % SH, c);
-      if (final)
-        store4((el*)e.out + id * D + c, x);
-      else if (!(l == 0.0f))
-        *(f32x4*)(e.part_o + slot * D + c) = x;
-    }
-  if (gx == 0) {
-    e.part_ml[slot] = float2{w.m, final ? -1.0f : l};
-    if (final) e.lse[id] = natural_lse(w.m, l);
-    if (u.split == 0 && !final)  // the slots that other tiles use
-      for (int k = u.splits; k < e.S1; ++k) e.part_ml[k * slots + id] = float2{NEG_INF, 0.0f};
-  }
+  block_barrier();  // all marks are made, the stages are free
+  stash<W, D>(w, base, base + L::STATS, wave * SH + lane % SH);
+  block_barrier();
+  const int first = u.tile * L::ROWS;
+  finish<W, D, L::ROWS, WAVES / RW>(base + L::ARGS, base, base + L::STATS, marks, any, min(gr.rows - first, L::ROWS), gr.q0, first, h,
+                                    u.split, u.split == 0 ? u.splits : 0, u.split == 0 ? a.S1 : 0, [&](int r) {
+                                      return u.splits == 1 && (lds_read<int>(info + 4 * r) & BIG) &&
+                                             lds_read<int>(info + 4 * r) >= 0;
+                                    });
 }
 
 // Tile blocks first (the longest ones), then those of few rows.
@@ -1072,109 +1301,180 @@ template <int DT, bool E8, int D, int RW>
 __global__ void __launch_bounds__(THREADS, 2) attend(Args a) {
   extern __shared__ __align__(16) char smem[];
   const int index = (int)blockIdx.x;
+  const uint32_t arg_word = argument_word();
   if (index < a.tile_blocks)
-    row_tile<DT, E8, D, RW>(a, smem, index);
+    row_tile<DT, E8, D, RW>(a, smem, index, arg_word);
   else
-    few_rows<DT, E8, D>(a, smem, index - a.tile_blocks);
+    few_rows<DT, E8, D>(a, smem, index - a.tile_blocks, arg_word);
 }
 
 // ------------------------------------------------------------------ combine
 
 // One wavefront a row: lane s reads the maximum and sum of slots s and s + 64, then all lanes add the slots' outputs
-// in order, eight of them in flight.
+// in order, eight of them in flight.  A wavefront looks through `run` rows for those that their tile has not written
+// already (most of a prompt's).
 template <int DT, int D>
-__global__ void __launch_bounds__(THREADS) combine(Args a) {
+__global__ void __launch_bounds__(THREADS) combine(Args a, int run) {
   typedef typename Ty<DT>::el el;
   constexpr int PER = D / 64, AT_ONCE = 8;
   struct alignas(4 * PER) Part { float x[PER]; };
   struct alignas(2 * PER) Out { el x[PER]; };
   const int lane = threadIdx.x & 63;
-  const int64_t rows = (int64_t)a.T * a.Hq, id = (int64_t)blockIdx.x * WAVES + (threadIdx.x >> 6);
-  if (id >= rows) return;
+  const int64_t rows = (int64_t)a.T * a.Hq, id0 = ((int64_t)blockIdx.x * WAVES + (threadIdx.x >> 6)) * run;
+  if (id0 >= rows) return;
+  const int slots = a.S1 + a.S2, first = query_start(a, 0), end = query_start(a, a.B);
+  // rows to write: not final ones, and those of no sequence
+  bool open = lane < run && id0 + lane < rows;
+  if (open && run > 1) {
+    const int t = (int)((id0 + lane) / a.Hq);
+    open = t < first || t >= end || !(a.part_ml[id0 + lane].y < 0.0f);
+  }
+  for (unsigned long long rest = __ballot(open); rest; rest &= rest - 1) {
+    const int64_t id = id0 + __builtin_ctzll(rest);
+    const int t = (int)(id / a.Hq);
+    float2 ml[2] = {float2{NEG_INF, 0.0f}, float2{NEG_INF, 0.0f}};
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (lane + 64 * i < slots) ml[i] = a.part_ml[(lane + 64 * i) * rows + id];
+    if (t < first || t >= end) ml[0] = ml[1] = float2{NEG_INF, 0.0f};  // a row of no sequence
+    if (__any(ml[0].y < 0.0f)) continue;
+    float top = fmaxf(ml[0].x, ml[1].x);
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+    float weight[2], sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      weight[i] = __builtin_amdgcn_exp2f(ml[i].x - (top == NEG_INF ? 0.0f : top));
+      sum += weight[i] * ml[i].y;
+    }
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
+    float x[PER] = {};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      unsigned long long live = __ballot(!(ml[i].y == 0.0f));  // a NaN counts
+      while (live) {
+        Part p[AT_ONCE];
+        float w[AT_ONCE];
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; ++k) {
+          const int s = live ? __builtin_ctzll(live) : 0;
+          w[k] = live ? __shfl(weight[i], s) : 0.0f;
+          p[k] = Part{};
+          if (live) p[k] = *(const Part*)(a.part_o + ((s + 64 * i) * rows + id) * D + lane * PER);
+          live &= live - 1;
+        }
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; ++k)
+#pragma unroll
+          for (int e = 0; e < PER; ++e) x[e] += w[k] * p[k].x[e];
+      }
+    }
+    const float inv = inverse(sum);
+    Out o;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) o.x[e] = (el)(x[e] * inv);
+    *(Out*)((el*)a.out + id * D + lane * PER) = o;
+    if (lane == 0) a.lse[id] = natural_lse(top, sum);
+  }
+}
+
+// The same with a block a row, for many slots: lanes 0 .. 31 and 32 .. 63 of each wavefront read a slot's output each.
+template <int DT, int D>
+__global__ void __launch_bounds__(THREADS) combine_many(Args a) {
+  typedef typename Ty<DT>::el el;
+  constexpr int PER = D / 32, HALVES = 2 * WAVES;
+  struct alignas(4 * PER) Part { float x[PER]; };
+  __shared__ float joined[HALVES][D];
+  const int lane = threadIdx.x & 63, half = (int)threadIdx.x >> 5, at = lane & 31;
+  const int64_t rows = (int64_t)a.T * a.Hq, id = blockIdx.x;
   const int slots = a.S1 + a.S2;
   float2 ml[2] = {float2{NEG_INF, 0.0f}, float2{NEG_INF, 0.0f}};
-  const int t = (int)(id / a.Hq), first = query_start(a, 0), end = query_start(a, a.B);
 #pragma unroll
   for (int i = 0; i < 2; ++i)
     if (lane + 64 * i < slots) ml[i] = a.part_ml[(lane + 64 * i) * rows + id];
+  const int t = (int)(id / a.Hq), first = query_start(a, 0), end = query_start(a, a.B);
   if (t < first || t >= end) ml[0] = ml[1] = float2{NEG_INF, 0.0f};  // a row of no sequence
-  if (__any(ml[0].y < 0.0f)) return;  // written by its tile
+  if (__any(ml[0].y < 0.0f)) return;                                // written by its tile
   float top = fmaxf(ml[0].x, ml[1].x);
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
   float weight[2], sum = 0.0f;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    weight[i] = __builtin_amdgcn_exp2f(ml[i].x - (top == NEG_INF ? 0.0f : top));
+    weight[i] = ml[i].y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(ml[i].x - (top == NEG_INF ? 0.0f : top));
     sum += weight[i] * ml[i].y;
   }
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
   float x[PER] = {};
+#pragma unroll 8
+  for (int s0 = 0; s0 < slots; s0 += HALVES) {  // all lanes take part: the shuffles read any lane
+    const int s = s0 + half;
+    const float w0 = __shfl(weight[0], s & 63), w1 = __shfl(weight[1], s & 63);
+    const float l0 = __shfl(ml[0].y, s & 63), l1 = __shfl(ml[1].y, s & 63);
+    const float w = s < 64 ? w0 : w1, l = s < 64 ? l0 : l1;
+    Part p{};
+    if (s < slots && !(l == 0.0f)) p = *(const Part*)(a.part_o + (s * rows + id) * D + at * PER);  // an empty one is not there
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    unsigned long long live = __ballot(!(ml[i].y == 0.0f));  // a NaN counts
-    while (live) {
-      Part p[AT_ONCE];
-      float w[AT_ONCE];
-#pragma unroll
-      for (int k = 0; k < AT_ONCE; ++k) {
-        const int s = live ? __builtin_ctzll(live) : 0;
-        w[k] = live ? __shfl(weight[i], s) : 0.0f;
-        p[k] = Part{};
-        if (live) p[k] = *(const Part*)(a.part_o + ((s + 64 * i) * rows + id) * D + lane * PER);
-        live &= live - 1;
-      }
-#pragma unroll
-      for (int k = 0; k < AT_ONCE; ++k)
-#pragma unroll
-        for (int e = 0; e < PER; ++e) x[e] += w[k] * p[k].x[e];
-    }
+    for (int k = 0; k < PER; ++k) x[k] += w * p.x[k];
   }
-  const float inv = inverse(sum);
-  Out o;
 #pragma unroll
-  for (int e = 0; e < PER; ++e) o.x[e] = (el)(x[e] * inv);
-  *(Out*)((el*)a.out + id * D + lane * PER) = o;
-  if (lane == 0) a.lse[id] = natural_lse(top, sum);
+  for (int k = 0; k < PER; ++k) joined[half][at * PER + k] = x[k];
+  __syncthreads();
+  for (int c = threadIdx.x; c < D; c += THREADS) {
+    float y = 0.0f;
+#pragma unroll
+    for (int k = 0; k < HALVES; ++k) y += joined[k][c];
+    ((el*)a.out)[id * D + c] = (el)(y * inverse(sum));
+  }
+  if (threadIdx.x == 0) a.lse[id] = natural_lse(top, sum);
 }
 
 // ------------------------------------------------------------------ host
 
 struct Plan {
-  int64_t tile_blocks = 0;  // an upper bound
-  int row_waves = 2;        // tiles of 64 or 128 rows
+  int64_t tile_blocks = 0, few_blocks = 0;  // upper bounds
+  int row_waves = 2;                        // tiles of 64 or 128 rows
+  int tile_fill = FILL;
   int S1 = 0, S2 = 1;
-  int64_t few_blocks = 0;
-  bool combine = true;
+  bool joint = false, rounds = false, spread = false, combine = true;
   int64_t bytes = 0;
 };
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline int64_t between(int64_t x, int64_t lo, int64_t hi) { return x < lo ? lo : x > hi ? hi : x; }
 
-// Tiles of 128 rows where they fill the device by themselves, else of 64 (fewer splits, so fewer partial results).
-// Splits of at least 256 tokens.
+// Short calls: every block reads its sequence's prefix itself, which saves the combine (a second launch and the
+// partial results, about 5 us) for at most 16 MB more reads.  Otherwise tiles of 128 rows, or of 64 where groups have
+// no more; splits of at least 256 tokens.
 inline Plan make_plan(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t G, int64_t Wp, int64_t B, int64_t W,
                       int64_t page, int64_t max_q) {
   Plan p;
   const int64_t grp = Hq / Hkv, rows = T * grp, groups = G > 0 ? G : 1;
   const bool big = max_q * grp > FEW;
-  if (rows > FEW && (Wp > 0 || big)) {
-    p.row_waves = ceil_div(rows, 128) * Hkv >= FILL ? 4 : 2;
-    const int64_t tile = 32 * p.row_waves;
-    const int64_t tokens = (Wp + (big ? W : 0)) * page;
-    // a last round of `tail` units is cut into FILL / tail splits; with one group the number of tiles is known
-    const int64_t units = ceil_div(rows, tile) * Hkv, tail = units % FILL;
-    const int64_t most = groups == 1 ? (units < FILL ? FILL / units : tail ? FILL / tail : 1) : FILL / Hkv;
-    p.S1 = (int)between(most, 1, between(ceil_div(tokens, 256), 1, units < FILL ? MAX_SPLIT : 8));
+  p.joint = Wp > 0 && !big && (Wp + W) * page <= 1024 && B * Hkv * Wp * page * D * 4 <= (16 << 20);
+  if (!p.joint && (Wp > 0 || big)) {
+    // a group's rows padded to tiles, those of 64 counted 5 / 4 (they read each token twice as often)
+    const int64_t each = ceil_div(rows, groups);
+    p.row_waves = ceil_div(each, 128) * 128 <= ceil_div(each, 64) * 80 ? 4 : 2;
+    const int64_t tile = 32 * p.row_waves, units = ceil_div(rows, tile) * Hkv;
+    const int64_t tokens = (Wp + (big ? W : 0)) * page, cuts = ceil_div(tokens, 256);
+    p.rounds = units >= FILL;
+    // where there is much else to read, tiles leave every CU's second place to it
+    p.tile_fill = !big && B * W > groups * Wp ? FILL / 2 : FILL;
+    // partial results of up to 512 MB where only a last round of tiles is split
+    const int64_t room = (512 << 20) / (T * Hq * (D * 4 + 8));
+    p.S1 = (int)between(cuts, 1, p.rounds ? between(room, 1, 8) : MAX_SPLIT);
+    if (groups == 1 && !p.rounds) p.S1 = (int)between(p.tile_fill / between(units, 1, FILL), 1, p.S1);
     p.tile_blocks = (rows / tile + groups) * Hkv + FILL;
-  } else if (Wp > 0) {
-    p.S1 = (int)between(FILL / (groups * Hkv), 1, between(ceil_div(Wp * page, 256), 1, MAX_SPLIT));
   }
-  p.S2 = (int)between(FILL / (B * Hkv), p.S1 > 0 ? 4 : 1, between(ceil_div(W * page, 256), 1, MAX_SPLIT));
-  if (p.S2 > ceil_div(W * page, 256)) p.S2 = (int)ceil_div(W * page, 256);
-  p.few_blocks = B * Hkv * p.S2 + (p.S1 > 0 ? groups * Hkv * p.S1 : 0);
+  const int64_t units = B * Hkv;
+  p.spread = !p.joint && B <= 128 && units < 2 * FILL && (p.S1 > 0 || units < FILL) && W * page > 256;
+  p.S2 = p.spread ? (int)between(ceil_div(W * page, 256), 1, MAX_SPLIT) : 1;
+  if (p.spread && B == 1) p.S2 = (int)between(2 * FILL / Hkv, 1, p.S2);
+  p.spread = p.S2 > 1;
+  p.few_blocks = units + (p.spread ? 2 * FILL : 0);
   p.combine = !(p.S1 == 0 && p.S2 == 1);
   p.bytes = p.combine ? (int64_t)(p.S1 + p.S2) * T * Hq * (D * 4 + 8) : 0;
   return p;
@@ -1190,7 +1490,12 @@ tb_status launch(Args& a, const Plan& p, hipStream_t stream, const char* what) {
                      a);
   if (tb_status s = launch_status(what)) return s;
   if (!p.combine) return TB_OK;
-  hipLaunchKernelGGL((combine<DT, D>), dim3((unsigned)ceil_div((int64_t)a.T * a.Hq, WAVES)), dim3(THREADS), 0, stream, a);
+  const int64_t rows = (int64_t)a.T * a.Hq, run = a.big && rows >= 32768 ? 16 : 1;
+  if (a.S1 + a.S2 > 16 && rows <= 16384) {  // 69 slots: 8.0 us by wavefronts
+    hipLaunchKernelGGL((combine_many<DT, D>), dim3((unsigned)rows), dim3(THREADS), 0, stream, a);
+    return launch_status(what);
+  }
+  hipLaunchKernelGGL((combine<DT, D>), dim3((unsigned)ceil_div(rows, WAVES * run)), dim3(THREADS), 0, stream, a, (int)run);
   return launch_status(what);
 }
 
@@ -1317,6 +1622,12 @@ extern "C" tb_status tb_shared_prefix_attention(const void* q, const void* k_cac
   a.scale_log2 = scale == 0.0 ? 1.0f : (float)((scale < 0.0 ? -scale : scale) * 1.44269504088896340736);
   a.flip = scale < 0.0 ? 0x80008000u : 0u;
   a.keep = scale == 0.0 ? 0u : ~0u;
+  a.joint = p.joint;
+  a.rounds = p.rounds;
+  a.spread = p.spread;
+  a.tile_fill = p.tile_fill;
+  a.by_grp = Divisor((uint32_t)a.grp);
+  a.by_heads = Divisor((uint32_t)Hkv);
   a.near = c_slot >= 0 && c_slot < (1 << 23);
   a.big = max_q * a.grp > FEW;
   a.tile_blocks = (int)p.tile_blocks;
