@@ -511,7 +511,7 @@ tb_status tb_shared_prefix_attention(const void* q, const void* k_cache, const v
 /* Workspace bytes tb_shared_prefix_attention needs for these sizes (0 if none). */
 tb_status tb_shared_prefix_attention_workspace_size(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t G,
                                                     int64_t Wp, int64_t B, int64_t W, int64_t page_size,
-                                                    int64_t max_q, int64_t* bytes);
+                                                    int64_t max_q, int cache_dtype, int64_t* bytes);
 
 #ifdef __cplusplus
 }

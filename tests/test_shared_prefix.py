@@ -121,12 +121,12 @@ def test_entry_point_checks_before_touching_a_device():
     assert attend() == rt.TB_E_WORKSPACE and "workspace" in lib.tb_last_error().decode()
     need = ctypes.c_int64(-1)
     size = lib.tb_shared_prefix_attention_workspace_size
-    assert size(8, 8, 2, 64, 1, 90, 2, 4, 16, 4, ctypes.byref(need)) == rt.TB_OK and need.value > 0
+    assert size(8, 8, 2, 64, 1, 90, 2, 4, 16, 4, 1, ctypes.byref(need)) == rt.TB_OK and need.value > 0
     assert attend(ws=fake, wb=need.value - 1) == rt.TB_E_WORKSPACE
     assert attend(ws=fake + 4, wb=need.value) == rt.TB_E_ALIGN
-    assert size(0, 8, 2, 64, 1, 4, 2, 4, 16, 4, ctypes.byref(need)) == rt.TB_OK and need.value == 0
+    assert size(0, 8, 2, 64, 1, 4, 2, 4, 16, 4, 1, ctypes.byref(need)) == rt.TB_OK and need.value == 0
     # no prefix, and enough sequences to fill the device without splits: written directly
-    assert size(512, 8, 8, 64, 0, 0, 512, 64, 16, 1, ctypes.byref(need)) == rt.TB_OK and need.value == 0
+    assert size(512, 8, 8, 64, 0, 0, 512, 64, 16, 1, 1, ctypes.byref(need)) == rt.TB_OK and need.value == 0
     # short prefixes: every sequence reads its own
-    assert size(8, 8, 2, 64, 1, 4, 2, 4, 16, 4, ctypes.byref(need)) == rt.TB_OK and need.value == 0
-    assert size(8, 8, 2, 64, 1, 4, 2, 4, 16, 4, None) == rt.TB_E_INVALID
+    assert size(8, 8, 2, 64, 1, 4, 2, 4, 16, 4, 1, ctypes.byref(need)) == rt.TB_OK and need.value == 0
+    assert size(8, 8, 2, 64, 1, 4, 2, 4, 16, 4, 1, None) == rt.TB_E_INVALID

@@ -90,7 +90,8 @@ def run(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, prefix_pa
     out = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device)
     lse = torch.empty((T, Hq), dtype=torch.float32, device=q.device)
     need = ctypes.c_int64(0)
-    rt.call("tb_shared_prefix_attention_workspace_size", T, Hq, Hkv, D, G, Wp, B, W, page, max_q, ctypes.byref(need))
+    rt.call("tb_shared_prefix_attention_workspace_size", T, Hq, Hkv, D, G, Wp, B, W, page, max_q,
+            paged.DTYPES[k_cache.dtype], ctypes.byref(need))
     ws = torch.empty(need.value, dtype=torch.uint8, device=q.device) if need.value else None
     cs = k_cache.stride()
     ss = (0, 0, 0) if k_scale is None else k_scale.stride()
@@ -99,7 +100,7 @@ def run(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, prefix_pa
             lens.data_ptr(), cu_q.data_ptr(), out.data_ptr(), lse.data_ptr(), T, Hq, Hkv, D, G, Wp, B, W, max_q,
             n_pages, page, q.stride(0), q.stride(1), cs[0], cs[1], cs[2], *ss, D ** -0.5 if scale is None else scale,
             paged.DTYPES[q.dtype], paged.DTYPES[k_cache.dtype], rt.ptr(ws), need.value, rt.stream_handle(q.device))
-    _last_config = {"kernels": ["row_tiles", "few_rows", "combine"], "workspace_bytes": need.value}
+    _last_config = {"kernels": ["attend", "combine"] if need.value else ["attend_each"], "workspace_bytes": need.value}
     return (out, lse)
 
 

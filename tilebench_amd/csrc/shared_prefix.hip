@@ -11,9 +11,10 @@
 // queries is query r / grp, head r % grp of the group.  Three kinds of work:
 //   tiles   64 or 128 rows of a group: over the shared prefix, and on over the own
 //           tokens of those sequences that have more than 16 rows
-//   few     the own tokens of one sequence of up to 16 rows (in short calls with its
-//           prefix): the block's four wavefronts split the tokens
+//   streams the own tokens of the sequences of up to 16 rows, laid end to end and
+//           shared out evenly to the wavefronts
 //   combine joins the partial results of a row (one slot per split) by their maxima
+// Short calls are done by a block for each sequence and head (attend_each).
 // so a prefix is read once per tile however many sequences share it.
 //
 // One wavefront's step over TOK tokens in LDS (attend_tile):
@@ -85,14 +86,16 @@ struct Args {
   void* out;
   float* lse;
   float* part_o;  // [slots][T * Hq][D]
-  float2* part_ml;  // [slots][T * Hq]: maximum (log2) and sum; sum -1: the row is final
+  float2* part_ml;  // [slots][T * Hq]: maximum (log2) and sum
+  int* n_tile;      // [T * Hq]: slots 0 .. that the row's tiles used, -1 where its result is final
+  int* n_own;       // [T * Hq]: slots S1 .. that its own tokens used
   int T, Hq, Hkv, grp, G, Wp, B, W;
   Divisor by_grp, by_heads;  // grp, Hkv
   int n_pages, page_shift;
   int S1, S2;       // slots of tiles, slots of own tokens
   int tile_fill;    // blocks that the tiles are shared out to
-  int spread;       // own tokens are shared out to 2 * FILL more blocks than there are sequences and heads
-  int direct;       // own tokens in one slot and nothing else: results are final
+  int streams;      // wavefronts that the own tokens are shared out to
+  int stream_least; // steps of one of them at least
   float scale_log2;     // of |scale|, or 1 for a scale of 0
   uint32_t flip, keep;  // applied to q
   int joint;   // sequences read their prefix themselves
@@ -674,16 +677,15 @@ __device__ __forceinline__ void stash(const W& w, uint32_t outs, uint32_t stats,
     }
   if (g == 0) *(__attribute__((address_space(3))) f32x2*)(uintptr_t)(stats + part_row * 8) = f32x2{w.m, l};
 }
-// rows: how many; q0: query of row `first`; final_row(r): its result is complete; unused: slots from this one on to mark
-// empty (S1 or S2 of them in all, from `slot0`).
-template <typename W, int D, int ROWS, int PARTS, typename Final>
+// rows: how many; q0: query of row `first`.  big(r): its result is complete if the unit was not split.
+template <typename W, int D, int ROWS, int PARTS, bool TILES, typename Big>
 __device__ __forceinline__ void finish(uint32_t args, uint32_t outs, uint32_t stats, uint32_t marks, uint32_t any,
-                                       int rows, int q0, int first, int h, int slot, int empty0, int empty1, Final final_row) {
+                                       int rows, int q0, int first, int h, int split, int splits, Big big) {
   const Args a = saved_args(args);
   const bool marked = lds_read<int>(any) != 0;
   const int64_t all = (int64_t)a.T * a.Hq;
   typedef typename W::Y::el el;
-#pragma unroll 1
+#pragma unroll 2
   for (int i = threadIdx.x; i < rows * (D / 4); i += THREADS) {
     const int r = i / (D / 4), c = i % (D / 4);
     f32x4 x = lds_read<f32x4>(out_at<D>(outs, r, c));
@@ -707,16 +709,18 @@ __device__ __forceinline__ void finish(uint32_t args, uint32_t outs, uint32_t st
     if (marked) x = W::marked(x, marks, r, c * 4);
     const int qi = a.by_grp.divide(first + r);
     const int64_t id = (int64_t)(q0 + qi) * a.Hq + h * a.grp + a.by_grp.rest(first + r, qi);
-    const bool final = final_row(r);
+    const bool own_here = !TILES || big(r), final = own_here && splits == 1;
     if (final)
       store4((el*)a.out + id * D + c * 4, x * inverse(ml[1]));
     else if (!(ml[1] == 0.0f))
-      *(f32x4*)(a.part_o + (slot * all + id) * D + c * 4) = x;
+      *(f32x4*)(a.part_o + (split * all + id) * D + c * 4) = x;
     if (c == 0) {
       if (final) a.lse[id] = natural_lse(ml[0], ml[1]);
-      if (!a.direct) a.part_ml[slot * all + id] = float2{ml[0], final ? -1.0f : ml[1]};
-      if (!final)
-        for (int k = empty0; k < empty1; ++k) a.part_ml[k * all + id] = float2{NEG_INF, 0.0f};
+      if (TILES && !final) a.part_ml[split * all + id] = float2{ml[0], ml[1]};
+      if (TILES && split == 0) {
+        a.n_tile[id] = final ? -1 : splits;
+        if (own_here) a.n_own[id] = 0;
+      }
     }
   }
 }
@@ -736,9 +740,9 @@ struct FewLayout {
 };
 
 // What a block of few rows does: rows 0 .. rows - 1 (at most 16) from query q0 on, over prefix tokens and then own tokens
-// (either may be none), of which it takes split `split` of `splits`; results to slot `slot`.
+// (either may be none).
 struct FewTask {
-  int h, q0, rows, split, splits;
+  int h, q0, rows;
   Tokens prefix, own;
   int n_q, seen;  // queries of the sequence, its own tokens
 };
@@ -760,8 +764,7 @@ __device__ __forceinline__ void attend_few(const Args& a, char* smem, const FewT
   w.init((const el*)a.q + t * a.q_st + hq * a.q_sh, valid, a.flip, a.keep);
 
   const int pre = (f.prefix.len + TOK - 1) / TOK, tiles = pre + (f.own.len + TOK - 1) / TOK;
-  const int lo = (int)((int64_t)tiles * f.split / f.splits), hi = (int)((int64_t)tiles * (f.split + 1) / f.splits);
-  const int n0 = lo + (hi - lo) * wave / WAVES, n1 = lo + (hi - lo) * (wave + 1) / WAVES;
+  const int n0 = tiles * wave / WAVES, n1 = tiles * (wave + 1) / WAVES;
 
   const uint32_t kbase = lds_addr(smem) + wave * L::WAVE_BYTES, vbase = kbase + L::TILE_BYTES;
   const uint32_t sbase = vbase + L::TILE_BYTES, marks = lds_addr(smem) + L::MARKS, limits = lds_addr(smem) + L::LIMITS;
@@ -850,10 +853,8 @@ __device__ __forceinline__ void attend_few(const Args& a, char* smem, const FewT
   const uint32_t outs = lds_addr(smem), stats = outs + L::STATS;
   stash<W, D>(w, outs, stats, wave * FEW + row);
   block_barrier();
-  const bool direct = a.direct;
-  finish<W, D, FEW, WAVES>(outs + L::ARGS, outs, stats, marks, outs + L::ANY, f.rows, f.q0, 0, h, a.S1 + f.split,
-                           f.split == 0 ? a.S1 + f.splits : 0, f.split == 0 ? a.S1 + a.S2 : 0,
-                           [&](int) { return direct; });
+  finish<W, D, FEW, WAVES, false>(outs + L::ARGS, outs, stats, marks, outs + L::ANY, f.rows, f.q0, 0, h, 0, 1,
+                                  [](int) { return true; });
 }
 
 // Outputs of queries t0 .. t1 - 1 that attend to nothing.
@@ -866,7 +867,305 @@ __device__ __forceinline__ void empty_rows(const Args& a, int h, int t0, int t1)
   }
 }
 
-// Which entry (group or sequence) block `index` works for, which of its units and which split of that.  Entries have
+// A block for each sequence and key/value head (with the sequence's prefix where the call is `joint`); results are final.
+template <int DT, bool E8, int D>
+__global__ void __launch_bounds__(THREADS, 2) attend_each(Args a) {
+  extern __shared__ __align__(16) char smem[];
+  const uint32_t arg_word = argument_word();
+  const int b = a.by_heads.divide((int)blockIdx.x);
+  FewTask f;
+  f.h = a.by_heads.rest((int)blockIdx.x, b);
+  if (b == 0) {  // rows of no sequence
+    const int first = query_start(a, 0);
+    empty_rows<DT, D>(a, f.h, 0, first);
+    empty_rows<DT, D>(a, f.h, max(query_start(a, a.B), first), a.T);
+  }
+  const Seq s = sequence(a, b);
+  f.q0 = s.q0;
+  f.n_q = s.n_q;
+  f.rows = s.n_q * a.grp;
+  f.seen = s.own;
+  f.own = Tokens{a.pages + (int64_t)b * a.W, a.W, s.own};
+  f.prefix = Tokens{nullptr, 0, 0};
+  if (a.joint) {
+    int lo = 0, hi = a.G;  // the last group that starts at or before the sequence
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (a.group_offsets[mid] <= b) lo = mid; else hi = mid;
+    }
+    f.prefix = Tokens{a.prefix_pages + (int64_t)lo * a.Wp, a.Wp, prefix_length(a, lo)};
+  }
+  if (f.rows > FEW)  // more queries than max_q announced: nothing was planned for them
+    empty_rows<DT, D>(a, f.h, f.q0, f.q0 + s.n_q);
+  else if (f.rows > 0)
+    attend_few<DT, E8, D>(a, smem, f, arg_word);
+}
+
+// ------------------------------------------------------------------ own tokens in streams
+//
+// Units are the sequences of up to 16 rows, once for each key/value head; their steps of TOK tokens, laid end to end,
+// are shared out evenly to all wavefronts.  A wavefront runs through its share without a pause where one unit ends and
+// the next begins: the next unit's first keys are fetched while the last values of the one before are used.  Unit by
+// unit its results go to a slot, the n-th of those wavefronts that the unit's steps fall to.  (A block for each unit,
+// its wavefronts joined at the end, left the memory idle for half of its 11 us at 400 tokens.)
+template <int DT, bool E8, int D>
+struct StreamLayout {
+  static constexpr int RB = D * (E8 ? 1 : 2);
+  static constexpr int TOK = RB == 256 ? 32 : 64;  // tokens of a step
+  static constexpr int TILE_BYTES = TOK * RB;
+  static constexpr int WAVE_BYTES = 2 * TILE_BYTES + (E8 ? 2 * TOK * 4 : 0);
+  static constexpr int MARKS = WAVES * WAVE_BYTES, MARK_BYTES = FEW * 64 + FEW * 4 + 16;  // marks, limits, any
+  static constexpr int ARGS = MARKS + WAVES * MARK_BYTES, LDS = ARGS + sizeof(Args);
+};
+
+template <int DT, bool E8, int D>
+__device__ __forceinline__ void stream_rows(const Args& a, char* smem, int index, uint32_t arg_word) {
+  constexpr int SH = 16;
+  typedef StreamLayout<DT, E8, D> L;
+  typedef Wave<DT, E8, D, SH> W;
+  typedef typename W::Y::el el;
+  constexpr int TOK = L::TOK, RB = L::RB, NI = TOK * RB / 1024, ESIZE = E8 ? 1 : 2;
+  typedef Copier<RB, NI> Copy;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int row = lane % SH, qi = a.by_grp.divide(row), head = a.by_grp.rest(row, qi);
+
+  if (threadIdx.x < ARG_WORDS) *(uint32_t*)(smem + L::ARGS + 4 * threadIdx.x) = arg_word;
+  block_barrier();  // the only one: the wavefronts go their own ways from here
+
+  // Steps of sequence x0 + lane, 64 sequences at a time.  Sequences of more than 16 rows have none (their tiles take
+  // their tokens; without tiles an empty one, which marks them empty); without own tokens one, an empty one.
+  Seq s;
+  int steps = 0;
+  auto count = [&](int x) __attribute__((always_inline)) {
+    steps = 0;
+    s = Seq{0, 0, 0};
+    if (x >= a.B) return;
+    s = sequence(a, x);
+    const int rows = s.n_q * a.grp;
+    if (rows > FEW) s.own = 0;
+    steps = rows == 0 || (rows > FEW && a.big) ? 0 : max((s.own + TOK - 1) / TOK, 1);
+  };
+  int total = 0;
+  for (int x0 = (a.B - 1) / 64 * 64; x0 >= 0; x0 -= 64) {  // downwards: ends with the first sequences in registers
+    count(x0 + lane);
+    total += steps;
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) total += __shfl_xor(total, d);
+  total = __builtin_amdgcn_readfirstlane(total) * a.Hkv;
+  const int per = max((total + a.streams - 1) / a.streams, a.stream_least);
+  const int mine = index * WAVES + wave;
+  int left = min(per, total - mine * per);  // steps to do (mine * per < streams * per < 2^31: see the plan)
+  if (left <= 0) return;
+
+  // the unit that the first step belongs to: sequence x0 + at, head h, step n; `start` is its first step of all
+  int x0 = 0, at = 0, h = 0, n = 0, start = 0;
+  {
+    const int want = mine * per;
+    int seen = 0;
+    for (;; x0 += 64) {
+      if (a.B > 64) count(x0 + lane);
+      int incl = steps * a.Hkv;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(incl, d);
+        if (lane >= d) incl += o;
+      }
+      const int here = __builtin_amdgcn_readlane(incl, 63);
+      if (want < seen + here) {
+        at = __builtin_ctzll(__ballot(seen + incl > want));
+        const int each = __builtin_amdgcn_readlane(steps, at);
+        start = seen + __builtin_amdgcn_readlane(incl, at) - each * a.Hkv;
+        h = (int)((uint32_t)(want - start) / (uint32_t)each);
+        start += h * each;
+        n = want - start;
+        break;
+      }
+      seen += here;
+    }
+  }
+
+  struct UnitOf {
+    int q0, n_q, own, h, slot, last;  // last: its steps
+    Tokens src;
+  };
+  auto unit_here = [&](const Args& a) __attribute__((always_inline)) {
+    UnitOf u;
+    u.q0 = __builtin_amdgcn_readlane(s.q0, at);
+    u.n_q = __builtin_amdgcn_readlane(s.n_q, at);
+    u.own = __builtin_amdgcn_readlane(s.own, at);
+    u.last = __builtin_amdgcn_readlane(steps, at);
+    u.h = h;
+    u.slot = mine - (int)((uint32_t)start / (uint32_t)per);
+    u.src = Tokens{uniform(a.pages + (int64_t)(x0 + at) * a.W), __builtin_amdgcn_readfirstlane(a.W), u.own};
+    return u;
+  };
+  // on to the next unit (there is one: steps are left)
+  auto next_unit = [&]() __attribute__((always_inline)) {
+    start += __builtin_amdgcn_readlane(steps, at);
+    n = 0;
+    if (++h < a.Hkv) return;
+    h = 0;
+    for (;;) {
+      if (++at == 64) {
+        at = 0;
+        x0 += 64;
+        count(x0 + lane);
+      }
+      const unsigned long long some = __ballot(steps > 0) >> at;
+      if (some) {
+        at += __builtin_ctzll(some);
+        return;
+      }
+      at = 63;
+    }
+  };
+
+  const uint32_t kbase = lds_addr(smem) + wave * L::WAVE_BYTES, vbase = kbase + L::TILE_BYTES;
+  const uint32_t sbase = vbase + L::TILE_BYTES;
+  const uint32_t marks = lds_addr(smem) + L::MARKS + wave * L::MARK_BYTES, limits = marks + FEW * 64, any = limits + FEW * 4;
+  auto clear_marks = [&]() __attribute__((always_inline)) {
+    *(__attribute__((address_space(3))) u32x4*)(uintptr_t)(marks + lane * 16) = u32x4{};
+    if (lane == 0) *(__attribute__((address_space(3))) int*)(uintptr_t)any = 0;
+  };
+  static_assert(FEW * 64 == 64 * 16, "16 bytes a lane");
+  clear_marks();
+
+  Window win;
+  auto cover = [&](const Tokens& src, int n) __attribute__((always_inline)) {
+    win.cover(src, n * TOK >> a.page_shift, min(n * TOK + TOK - 1, src.len - 1) >> a.page_shift, a.n_pages);
+  };
+  auto fill_scales = [&](const UnitOf& u, int n) __attribute__((always_inline)) {  // 32 tokens a copy
+#pragma unroll
+    for (int i = 0; i < TOK / 32; ++i) {
+      const int tok = min(n * TOK + i * 32 + (lane & 31), u.src.len - 1);
+      const int page = __builtin_amdgcn_ds_bpermute(((tok >> a.page_shift) - win.first) << 2, win.ids);
+      const int64_t off = page * a.s_page + u.h * a.s_head + (tok & ((1 << a.page_shift) - 1)) * a.s_slot;
+      dma4(sbase + i * 256, (const char*)((lane < 32 ? a.ks : a.vs) + off));
+    }
+  };
+  auto fill_keys = [&](const UnitOf& u, int n) __attribute__((always_inline)) {
+    if (u.src.len == 0) return;
+    cover(u.src, n);
+    if (E8) fill_scales(u, n);
+    Copy::run(a, win, u.src, a.kc + u.h * a.c_head * ESIZE, kbase, n * TOK, ESIZE, [](int r) { return swizzle_k<RB>(r); });
+  };
+  auto fill_values = [&](const UnitOf& u, int n) __attribute__((always_inline)) {
+    if (u.src.len == 0) return;
+    Copy::run(a, win, u.src, a.vc + u.h * a.c_head * ESIZE, vbase, n * TOK, ESIZE,
+              [](int r) { return swizzle_v<RB, SH, E8>(r); });
+  };
+  auto queries = [&](W& w, const UnitOf& u) __attribute__((always_inline)) {
+    const bool valid = row < u.n_q * a.grp;
+    w.init((const el*)a.q + (u.q0 + qi) * a.q_st + (u.h * a.grp + head) * a.q_sh, valid, a.flip, a.keep);
+  };
+
+  UnitOf u = unit_here(a);
+  W w;
+  queries(w, u);
+  fill_keys(u, n);
+  fill_values(u, n);
+  int limit = 0;
+  auto set_limits = [&]() __attribute__((always_inline)) {
+    const bool valid = row < u.n_q * a.grp;
+    limit = valid ? clamp_int(u.own - u.n_q + qi + 1, 0, u.own) : 0x7FFFFFFF;
+    if (lane < SH) *(__attribute__((address_space(3))) int*)(uintptr_t)(limits + 4 * lane) = limit;
+  };
+  set_limits();
+
+  for (;;) {
+    const int t0 = n * TOK;
+    const bool ends = n + 1 == u.last, more = left > 1;
+    UnitOf v = u;   // the next step's unit
+    W next;         // its queries
+    int n_next = n + 1;
+    typename W::acc_t s2[TOK / SH];
+    typename W::v8 p[TOK / W::KS];
+    const bool full = __all(limit >= t0 + TOK), nothing = u.src.len == 0;
+    if (!nothing) {
+      wait_vm<NI>();  // keys (and scales) are there; the values may be on their way
+      w.template scores<TOK>(kbase, s2);
+      if (E8) w.template weights<TOK>(s2, t0, limit, full, a.scale_log2, sbase, 0, p);
+      wait_lds();
+    }
+    if (more) {
+      if (ends) {
+        next_unit();
+        n_next = 0;
+        v = unit_here(saved_args(lds_addr(smem) + L::ARGS));
+        queries(next, v);
+        win.reset();
+      }
+      fill_keys(v, n_next);
+    }
+    if (!nothing) {
+      if (!E8) w.template weights<TOK>(s2, t0, limit, full, a.scale_log2, sbase, 0, p);
+      if (more && v.src.len > 0) wait_vm<NI + (E8 ? TOK / 32 : 0)>(); else wait_vm<0>();
+      if (!full) {
+        W::template set_apart<TOK>(vbase, 0, t0, min(u.n_q * a.grp, FEW), marks, any,
+                                   [&](int r) { return lds_read<int>(limits + 4 * r); });
+        wait_lds();
+      }
+      w.template values<TOK>(vbase, p);
+      wait_lds();
+    }
+    if (ends || !more) {
+      // this unit's results
+      const Args b = saved_args(lds_addr(smem) + L::ARGS);
+      const float l = W::over_groups_sum(w.l);
+      const int64_t all = (int64_t)b.T * b.Hq;
+      const bool marked = lds_read<int>(any) != 0;
+      const int g = lane / SH, rows = u.n_q * b.grp;
+      if (row < rows && rows <= FEW) {
+        const int64_t id = (int64_t)(u.q0 + qi) * b.Hq + u.h * b.grp + head, slot = (b.S1 + u.slot) * all + id;
+        if (!(l == 0.0f)) {
+#pragma unroll
+          for (int d = 0; d < W::DT_N; ++d) {
+            f32x4 x = w.o[d];
+            const int c = d * SH + W::token_of(0, g);
+            if (marked) x = W::marked(x, marks, row, c);
+            *(f32x4*)(b.part_o + slot * D + c) = x;
+          }
+        }
+        if (g == 0) {
+          b.part_ml[slot] = float2{w.m, l};
+          if (ends) b.n_own[id] = u.slot + 1;
+        }
+      }
+      if (rows > FEW)  // more queries than max_q announced: nothing was planned for them
+        for (int r = lane; r < rows; r += 64) {
+          const int q = b.by_grp.divide(r);
+          b.n_own[(int64_t)(u.q0 + q) * b.Hq + u.h * b.grp + b.by_grp.rest(r, q)] = 0;
+        }
+      if (!more) return;
+      if (marked) clear_marks();
+      u = v;
+      w = next;
+      set_limits();
+    }
+    n = n_next;
+    --left;
+    fill_values(v, n);
+  }
+}
+
+// ------------------------------------------------------------------ tiles of rows
+//
+// RW wavefronts side by side hold the tile's 32 * RW rows, 4 / RW wavefronts share the tokens of a step.
+template <int DT, bool E8, int D, int RW>
+struct TileLayout {
+  static constexpr int RB = D * 2;  // the tiles hold 16-bit values; e4m3 codes are converted on the way
+  static constexpr int ROWS = 32 * RW;
+  static constexpr int TOK = RB == 256 ? 64 : 128;  // tokens of a step
+  static constexpr int TILE_BYTES = TOK * RB;
+  static constexpr int STAGE = 2 * TILE_BYTES + (E8 ? 2 * TOK * 4 : 0);
+  static constexpr int MARKS = 2 * STAGE;
+  static constexpr int ROW_INFO = MARKS + ROWS * 64, STATS = ROW_INFO + ROWS * 12, ANY = STATS + WAVES * 32 * 8;
+  static constexpr int ARGS = ANY + 16, LDS = ARGS + sizeof(Args);
+  static_assert(MARKS >= WAVES * 32 * D * 4, "the outputs reuse the stages");
+};
+
+// Which entry (group) block `index` works for, which of its units and which split of that.  Entries have
 // `units` units of `steps` steps (set by count(entry), an entry a lane, 64 at a time); a unit is cut into splits of
 // about the same number of steps, `fill` blocks in all at most (units beside: an entry's last split may be short), of
 // `least` steps at least and `most` splits at most.
@@ -927,92 +1226,6 @@ __device__ __forceinline__ bool share_out(int entries, int index, int fill, int 
   }
   return false;
 }
-
-// Block `index` of the own tokens: sequence, key/value head, split (with the sequence's prefix where the call is
-// `joint`).
-template <int DT, bool E8, int D>
-__device__ __forceinline__ void few_rows(const Args& a, char* smem, int index, uint32_t arg_word) {
-  constexpr int TOK = FewLayout<DT, E8, D>::TOK;
-  Seq s;
-  FewTask f;
-  int b;
-  if (a.spread) {
-    Seq of_lane;
-    Unit u;
-    int total;
-    auto count = [&](int x, int& units, int& steps) __attribute__((always_inline)) {
-      units = steps = 0;
-      if (x >= a.B) return;
-      of_lane = sequence(a, x);
-      const int rows = of_lane.n_q * a.grp;
-      units = rows > 0 ? a.Hkv : 0;
-      steps = rows > FEW ? 0 : (of_lane.own + TOK - 1) / TOK;
-    };
-    if (!share_out(a.B, index, 2 * FILL, 8, a.S2, u, total, count)) return;  // two steps a wavefront at least
-    b = u.entry;
-    f.h = u.at;
-    f.split = u.split;
-    f.splits = u.splits;
-    s.q0 = __builtin_amdgcn_readlane(of_lane.q0, u.lane);
-    s.n_q = __builtin_amdgcn_readlane(of_lane.n_q, u.lane);
-    s.own = __builtin_amdgcn_readlane(of_lane.own, u.lane);
-  } else {
-    b = a.by_heads.divide(index);
-    f.h = a.by_heads.rest(index, b);
-    f.split = 0;
-    f.splits = 1;
-    s = sequence(a, b);
-    if (a.direct && b == 0) {  // rows of no sequence
-      const int first = query_start(a, 0);
-      empty_rows<DT, D>(a, f.h, 0, first);
-      empty_rows<DT, D>(a, f.h, max(query_start(a, a.B), first), a.T);
-    }
-  }
-  f.q0 = s.q0;
-  f.n_q = s.n_q;
-  f.rows = s.n_q * a.grp;
-  f.seen = s.own;
-  f.own = Tokens{a.pages + (int64_t)b * a.W, a.W, s.own};
-  f.prefix = Tokens{nullptr, 0, 0};
-  if (a.joint) {
-    int lo = 0, hi = a.G;  // the last group that starts at or before the sequence
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (a.group_offsets[mid] <= b) lo = mid; else hi = mid;
-    }
-    f.prefix = Tokens{a.prefix_pages + (int64_t)lo * a.Wp, a.Wp, prefix_length(a, lo)};
-  }
-  if (f.rows > FEW) {
-    if (a.direct) {  // more queries than max_q announced: nothing was planned for them
-      empty_rows<DT, D>(a, f.h, f.q0, f.q0 + s.n_q);
-      return;
-    }
-    const int64_t all = (int64_t)a.T * a.Hq;  // their tiles take the own tokens
-    for (int r = threadIdx.x; r < f.rows; r += THREADS) {
-      const int qi = a.by_grp.divide(r);
-      const int64_t id = (int64_t)(f.q0 + qi) * a.Hq + f.h * a.grp + a.by_grp.rest(r, qi);
-      for (int k = 0; k < a.S2; ++k) a.part_ml[(a.S1 + k) * all + id] = float2{NEG_INF, 0.0f};
-    }
-    return;
-  }
-  if (f.rows > 0) attend_few<DT, E8, D>(a, smem, f, arg_word);
-}
-
-// ------------------------------------------------------------------ tiles of rows
-//
-// RW wavefronts side by side hold the tile's 32 * RW rows, 4 / RW wavefronts share the tokens of a step.
-template <int DT, bool E8, int D, int RW>
-struct TileLayout {
-  static constexpr int RB = D * 2;  // the tiles hold 16-bit values; e4m3 codes are converted on the way
-  static constexpr int ROWS = 32 * RW;
-  static constexpr int TOK = RB == 256 ? 64 : 128;  // tokens of a step
-  static constexpr int TILE_BYTES = TOK * RB;
-  static constexpr int STAGE = 2 * TILE_BYTES + (E8 ? 2 * TOK * 4 : 0);
-  static constexpr int MARKS = 2 * STAGE;
-  static constexpr int ROW_INFO = MARKS + ROWS * 64, STATS = ROW_INFO + ROWS * 12, ANY = STATS + WAVES * 32 * 8;
-  static constexpr int ARGS = ANY + 16, LDS = ARGS + sizeof(Args);
-  static_assert(MARKS >= WAVES * 32 * D * 4, "the outputs reuse the stages");
-};
 
 // Unit (group, row tile, key/value head) and split of tile block `index`; false past the last one.
 //
@@ -1289,14 +1502,12 @@ __device__ __forceinline__ void row_tile(const Args& a, char* smem, int index, u
   stash<W, D>(w, base, base + L::STATS, wave * SH + lane % SH);
   block_barrier();
   const int first = u.tile * L::ROWS;
-  finish<W, D, L::ROWS, WAVES / RW>(base + L::ARGS, base, base + L::STATS, marks, any, min(gr.rows - first, L::ROWS), gr.q0, first, h,
-                                    u.split, u.split == 0 ? u.splits : 0, u.split == 0 ? a.S1 : 0, [&](int r) {
-                                      return u.splits == 1 && (lds_read<int>(info + 4 * r) & BIG) &&
-                                             lds_read<int>(info + 4 * r) >= 0;
-                                    });
+  finish<W, D, L::ROWS, WAVES / RW, true>(
+      base + L::ARGS, base, base + L::STATS, marks, any, min(gr.rows - first, L::ROWS), gr.q0, first, h, u.split, u.splits,
+      [&](int r) { return lds_read<int>(info + 4 * r) >= 0 && (lds_read<int>(info + 4 * r) & BIG); });
 }
 
-// Tile blocks first (the longest ones), then those of few rows.
+// Tile blocks first, then streams.
 template <int DT, bool E8, int D, int RW>
 __global__ void __launch_bounds__(THREADS, 2) attend(Args a) {
   extern __shared__ __align__(16) char smem[];
@@ -1305,14 +1516,27 @@ __global__ void __launch_bounds__(THREADS, 2) attend(Args a) {
   if (index < a.tile_blocks)
     row_tile<DT, E8, D, RW>(a, smem, index, arg_word);
   else
-    few_rows<DT, E8, D>(a, smem, index - a.tile_blocks, arg_word);
+    stream_rows<DT, E8, D>(a, smem, index - a.tile_blocks, arg_word);
 }
 
 // ------------------------------------------------------------------ combine
 
-// One wavefront a row: lane s reads the maximum and sum of slots s and s + 64, then all lanes add the slots' outputs
-// in order, eight of them in flight.  A wavefront looks through `run` rows for those that their tile has not written
-// already (most of a prompt's).
+// The slots of a row: the first n_tile of the tiles', the first n_own of the streams'; n-th of both: slot_of(n).
+struct Slots {
+  int tile, own;
+  __device__ __forceinline__ Slots(const Args& a, int64_t id, int first, int end) {
+    const int t = (int)(id / a.Hq);
+    const bool inside = t >= first && t < end;  // else a row of no sequence
+    tile = inside && a.S1 > 0 ? min(a.n_tile[id], a.S1) : 0;
+    own = inside && tile >= 0 ? clamp_int(a.n_own[id], 0, a.S2) : 0;
+  }
+  __device__ __forceinline__ int count() const { return tile + own; }
+  __device__ __forceinline__ int slot_of(const Args& a, int n) const { return n < tile ? n : a.S1 + n - tile; }
+};
+
+// One wavefront a row: lane n reads the maximum and sum of the row's slots n and n + 64, then all lanes add the slots'
+// outputs in order, eight of them in flight.  A wavefront looks through `run` rows for those that their tile has not
+// written already (most of a prompt's).
 template <int DT, int D>
 __global__ void __launch_bounds__(THREADS) combine(Args a, int run) {
   typedef typename Ty<DT>::el el;
@@ -1322,22 +1546,18 @@ __global__ void __launch_bounds__(THREADS) combine(Args a, int run) {
   const int lane = threadIdx.x & 63;
   const int64_t rows = (int64_t)a.T * a.Hq, id0 = ((int64_t)blockIdx.x * WAVES + (threadIdx.x >> 6)) * run;
   if (id0 >= rows) return;
-  const int slots = a.S1 + a.S2, first = query_start(a, 0), end = query_start(a, a.B);
-  // rows to write: not final ones, and those of no sequence
+  const int first = query_start(a, 0), end = query_start(a, a.B);
   bool open = lane < run && id0 + lane < rows;
-  if (open && run > 1) {
-    const int t = (int)((id0 + lane) / a.Hq);
-    open = t < first || t >= end || !(a.part_ml[id0 + lane].y < 0.0f);
-  }
+  if (open && run > 1) open = Slots(a, id0 + lane, first, end).tile >= 0;
   for (unsigned long long rest = __ballot(open); rest; rest &= rest - 1) {
     const int64_t id = id0 + __builtin_ctzll(rest);
-    const int t = (int)(id / a.Hq);
+    const Slots slots(a, id, first, end);
+    if (slots.tile < 0) continue;
+    const int n = __builtin_amdgcn_readfirstlane(slots.count());
     float2 ml[2] = {float2{NEG_INF, 0.0f}, float2{NEG_INF, 0.0f}};
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-      if (lane + 64 * i < slots) ml[i] = a.part_ml[(lane + 64 * i) * rows + id];
-    if (t < first || t >= end) ml[0] = ml[1] = float2{NEG_INF, 0.0f};  // a row of no sequence
-    if (__any(ml[0].y < 0.0f)) continue;
+      if (lane + 64 * i < n) ml[i] = a.part_ml[slots.slot_of(a, lane + 64 * i) * rows + id];
     float top = fmaxf(ml[0].x, ml[1].x);
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
@@ -1352,7 +1572,7 @@ __global__ void __launch_bounds__(THREADS) combine(Args a, int run) {
     float x[PER] = {};
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      unsigned long long live = __ballot(!(ml[i].y == 0.0f));  // a NaN counts
+      unsigned long long live = __ballot(!(ml[i].y == 0.0f));  // an empty slot's output is not there; a NaN counts
       while (live) {
         Part p[AT_ONCE];
         float w[AT_ONCE];
@@ -1361,7 +1581,7 @@ __global__ void __launch_bounds__(THREADS) combine(Args a, int run) {
           const int s = live ? __builtin_ctzll(live) : 0;
           w[k] = live ? __shfl(weight[i], s) : 0.0f;
           p[k] = Part{};
-          if (live) p[k] = *(const Part*)(a.part_o + ((s + 64 * i) * rows + id) * D + lane * PER);
+          if (live) p[k] = *(const Part*)(a.part_o + (slots.slot_of(a, s + 64 * i) * rows + id) * D + lane * PER);
           live &= live - 1;
         }
 #pragma unroll
@@ -1388,14 +1608,13 @@ __global__ void __launch_bounds__(THREADS) combine_many(Args a) {
   __shared__ float joined[HALVES][D];
   const int lane = threadIdx.x & 63, half = (int)threadIdx.x >> 5, at = lane & 31;
   const int64_t rows = (int64_t)a.T * a.Hq, id = blockIdx.x;
-  const int slots = a.S1 + a.S2;
+  const Slots slots(a, id, query_start(a, 0), query_start(a, a.B));
+  if (slots.tile < 0) return;  // written by its tile
+  const int n = slots.count();
   float2 ml[2] = {float2{NEG_INF, 0.0f}, float2{NEG_INF, 0.0f}};
 #pragma unroll
   for (int i = 0; i < 2; ++i)
-    if (lane + 64 * i < slots) ml[i] = a.part_ml[(lane + 64 * i) * rows + id];
-  const int t = (int)(id / a.Hq), first = query_start(a, 0), end = query_start(a, a.B);
-  if (t < first || t >= end) ml[0] = ml[1] = float2{NEG_INF, 0.0f};  // a row of no sequence
-  if (__any(ml[0].y < 0.0f)) return;                                // written by its tile
+    if (lane + 64 * i < n) ml[i] = a.part_ml[slots.slot_of(a, lane + 64 * i) * rows + id];
   float top = fmaxf(ml[0].x, ml[1].x);
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
@@ -1409,13 +1628,14 @@ __global__ void __launch_bounds__(THREADS) combine_many(Args a) {
   for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
   float x[PER] = {};
 #pragma unroll 8
-  for (int s0 = 0; s0 < slots; s0 += HALVES) {  // all lanes take part: the shuffles read any lane
+  for (int s0 = 0; s0 < n; s0 += HALVES) {  // all lanes take part: the shuffles read any lane
     const int s = s0 + half;
     const float w0 = __shfl(weight[0], s & 63), w1 = __shfl(weight[1], s & 63);
     const float l0 = __shfl(ml[0].y, s & 63), l1 = __shfl(ml[1].y, s & 63);
     const float w = s < 64 ? w0 : w1, l = s < 64 ? l0 : l1;
     Part p{};
-    if (s < slots && !(l == 0.0f)) p = *(const Part*)(a.part_o + (s * rows + id) * D + at * PER);  // an empty one is not there
+    if (s < n && !(l == 0.0f))  // an empty slot's output is not there
+      p = *(const Part*)(a.part_o + (slots.slot_of(a, s) * rows + id) * D + at * PER);
 #pragma unroll
     for (int k = 0; k < PER; ++k) x[k] += w * p.x[k];
   }
@@ -1434,27 +1654,31 @@ __global__ void __launch_bounds__(THREADS) combine_many(Args a) {
 // ------------------------------------------------------------------ host
 
 struct Plan {
-  int64_t tile_blocks = 0, few_blocks = 0;  // upper bounds
-  int row_waves = 2;                        // tiles of 64 or 128 rows
+  int64_t tile_blocks = 0, stream_blocks = 0, each_blocks = 0;  // upper bounds
+  int row_waves = 2;                                            // tiles of 64 or 128 rows
   int tile_fill = FILL;
-  int S1 = 0, S2 = 1;
-  bool joint = false, rounds = false, spread = false, combine = true;
+  int S1 = 0, S2 = 0, stream_least = 0;
+  bool joint = false, rounds = false;
   int64_t bytes = 0;
 };
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline int64_t between(int64_t x, int64_t lo, int64_t hi) { return x < lo ? lo : x > hi ? hi : x; }
 
-// Short calls: every block reads its sequence's prefix itself, which saves the combine (a second launch and the
-// partial results, about 5 us) for at most 16 MB more reads.  Otherwise tiles of 128 rows, or of 64 where groups have
-// no more; splits of at least 256 tokens.
+// Short calls, and calls of many sequences without prefixes: a block for each sequence and head, which saves the combine
+// (a second launch and the partial results, about 5 us) for at most 16 MB of prefixes read again.  Otherwise tiles of
+// 128 rows, or of 64 where groups have few; splits of at least 256 tokens; the own tokens in streams.
 inline Plan make_plan(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t G, int64_t Wp, int64_t B, int64_t W,
-                      int64_t page, int64_t max_q) {
+                      int64_t page, int64_t max_q, bool e8) {
   Plan p;
   const int64_t grp = Hq / Hkv, rows = T * grp, groups = G > 0 ? G : 1;
   const bool big = max_q * grp > FEW;
   p.joint = Wp > 0 && !big && (Wp + W) * page <= 1024 && B * Hkv * Wp * page * D * 4 <= (16 << 20);
-  if (!p.joint && (Wp > 0 || big)) {
+  if (p.joint || (Wp == 0 && !big && (B * Hkv >= 2 * FILL || W * page <= 512))) {
+    p.each_blocks = B * Hkv;
+    return p;
+  }
+  if (Wp > 0 || big) {
     // a group's rows padded to tiles, those of 64 counted 5 / 4 (they read each token twice as often)
     const int64_t each = ceil_div(rows, groups);
     p.row_waves = ceil_div(each, 128) * 128 <= ceil_div(each, 64) * 80 ? 4 : 2;
@@ -1469,38 +1693,44 @@ inline Plan make_plan(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t G, 
     if (groups == 1 && !p.rounds) p.S1 = (int)between(p.tile_fill / between(units, 1, FILL), 1, p.S1);
     p.tile_blocks = (rows / tile + groups) * Hkv + FILL;
   }
-  const int64_t units = B * Hkv;
-  p.spread = !p.joint && B <= 128 && units < 2 * FILL && (p.S1 > 0 || units < FILL) && W * page > 256;
-  p.S2 = p.spread ? (int)between(ceil_div(W * page, 256), 1, MAX_SPLIT) : 1;
-  if (p.spread && B == 1) p.S2 = (int)between(2 * FILL / Hkv, 1, p.S2);
-  p.spread = p.S2 > 1;
-  p.few_blocks = units + (p.spread ? 2 * FILL : 0);
-  p.combine = !(p.S1 == 0 && p.S2 == 1);
-  p.bytes = p.combine ? (int64_t)(p.S1 + p.S2) * T * Hq * (D * 4 + 8) : 0;
+  // streams of at least four steps, of so many that a sequence falls to at most 63 of them
+  const int64_t tok = (e8 || D == 64) ? 64 : 32, most = ceil_div(W * page, tok);
+  p.stream_least = (int)between(ceil_div(most, MAX_SPLIT - 2), 4, 1 << 30);
+  p.S2 = (int)(ceil_div(most, p.stream_least) + 1);
+  p.stream_blocks = between(ceil_div(B * Hkv * most, WAVES * p.stream_least), 1, p.S1 > 0 && !p.rounds ? FILL / 2 : FILL);
+  p.bytes = (int64_t)(p.S1 + p.S2) * T * Hq * (D * 4 + 8) + 2 * T * Hq * 4;
   return p;
 }
 
 template <int DT, bool E8, int D, int RW>
 tb_status launch(Args& a, const Plan& p, hipStream_t stream, const char* what) {
-  constexpr int few = FewLayout<DT, E8, D>::LDS, tile = TileLayout<DT, E8, D, RW>::LDS;
-  constexpr size_t lds = few > tile ? few : tile;
+  constexpr int own = StreamLayout<DT, E8, D>::LDS, tile = TileLayout<DT, E8, D, RW>::LDS;
+  constexpr size_t lds = own > tile ? own : tile;
   static_assert(lds <= 81920, "two blocks a CU");
   if (tb_status s = reserve_lds((const void*)attend<DT, E8, D, RW>, lds, what)) return s;
-  hipLaunchKernelGGL((attend<DT, E8, D, RW>), dim3((unsigned)(p.tile_blocks + p.few_blocks)), dim3(THREADS), lds, stream,
+  hipLaunchKernelGGL((attend<DT, E8, D, RW>), dim3((unsigned)(p.tile_blocks + p.stream_blocks)), dim3(THREADS), lds, stream,
                      a);
   if (tb_status s = launch_status(what)) return s;
-  if (!p.combine) return TB_OK;
   const int64_t rows = (int64_t)a.T * a.Hq, run = a.big && rows >= 32768 ? 16 : 1;
-  if (a.S1 + a.S2 > 16 && rows <= 16384) {  // 69 slots: 8.0 us by wavefronts
+  if (a.S1 + a.S2 > 16 && rows <= 16384)  // 69 slots: 8.0 us by wavefronts, 5.0 by blocks
     hipLaunchKernelGGL((combine_many<DT, D>), dim3((unsigned)rows), dim3(THREADS), 0, stream, a);
-    return launch_status(what);
-  }
-  hipLaunchKernelGGL((combine<DT, D>), dim3((unsigned)ceil_div(rows, WAVES * run)), dim3(THREADS), 0, stream, a, (int)run);
+  else
+    hipLaunchKernelGGL((combine<DT, D>), dim3((unsigned)ceil_div(rows, WAVES * run)), dim3(THREADS), 0, stream, a, (int)run);
+  return launch_status(what);
+}
+
+template <int DT, bool E8, int D>
+tb_status launch_each(Args& a, const Plan& p, hipStream_t stream, const char* what) {
+  constexpr size_t lds = FewLayout<DT, E8, D>::LDS;
+  static_assert(lds <= 81920, "two blocks a CU");
+  if (tb_status s = reserve_lds((const void*)attend_each<DT, E8, D>, lds, what)) return s;
+  hipLaunchKernelGGL((attend_each<DT, E8, D>), dim3((unsigned)p.each_blocks), dim3(THREADS), lds, stream, a);
   return launch_status(what);
 }
 
 template <int DT, bool E8, int D>
 tb_status launch_rows(Args& a, const Plan& p, hipStream_t stream, const char* what) {
+  if (p.each_blocks) return launch_each<DT, E8, D>(a, p, stream, what);
   return p.row_waves == 4 ? launch<DT, E8, D, 4>(a, p, stream, what) : launch<DT, E8, D, 2>(a, p, stream, what);
 }
 
@@ -1524,6 +1754,7 @@ tb_status check_sizes(const char* what, int64_t T, int64_t Hq, int64_t Hkv, int6
   TB_CHECK_ARG(T * Hq <= most && B * Hkv <= most / MAX_SPLIT / 4 && G * Hkv <= most / MAX_SPLIT / 4 && W <= most / 2 / page_size &&
                    Wp <= most / 2 / page_size && max_q * Hq <= most,
                "%s: sizes past 2^31", what);
+  TB_CHECK_ARG(B == 0 || W == 0 || Hkv * B <= (1ll << 30) / ceil_div(W * page_size, 32), "%s: sizes past 2^31", what);
   return TB_OK;
 }
 
@@ -1532,12 +1763,12 @@ tb_status check_sizes(const char* what, int64_t T, int64_t Hq, int64_t Hkv, int6
 
 extern "C" tb_status tb_shared_prefix_attention_workspace_size(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t G,
                                                                int64_t Wp, int64_t B, int64_t W, int64_t page_size,
-                                                               int64_t max_q, int64_t* bytes) {
+                                                               int64_t max_q, int cache_dtype, int64_t* bytes) {
   using namespace tb::prefix;
   const char* what = "tb_shared_prefix_attention_workspace_size";
   TB_CHECK_ARG(bytes, "%s: null pointer", what);
   if (tb_status s = check_sizes(what, T, Hq, Hkv, D, G, Wp, B, W, page_size, max_q)) return s;
-  *bytes = T == 0 ? 0 : make_plan(T, Hq, Hkv, D, G, Wp, B, W, page_size, max_q).bytes;
+  *bytes = T == 0 || B == 0 || W == 0 ? 0 : make_plan(T, Hq, Hkv, D, G, Wp, B, W, page_size, max_q, cache_dtype == 3).bytes;
   return TB_OK;
 }
 
@@ -1575,7 +1806,7 @@ extern "C" tb_status tb_shared_prefix_attention(const void* q, const void* k_cac
   TB_CHECK_ARG(q_st % 8 == 0 && q_sh % 8 == 0, "%s: q's strides must be multiples of 8 elements", what);
   TB_CHECK_ARG(c_page % chunk == 0 && c_head % chunk == 0 && c_slot % chunk == 0,
                "%s: the cache's strides must be multiples of 16 bytes", what);
-  const Plan p = make_plan(T, Hq, Hkv, D, G, Wp, B, W, page_size, max_q);
+  const Plan p = make_plan(T, Hq, Hkv, D, G, Wp, B, W, page_size, max_q, cache_dtype == 3);
   if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes)) {
     tb::set_error("%s: needs a workspace of %lld bytes, got %lld", what, (long long)p.bytes,
                   (long long)(workspace ? workspace_bytes : 0));
@@ -1606,6 +1837,8 @@ extern "C" tb_status tb_shared_prefix_attention(const void* q, const void* k_cac
   a.lse = lse;
   a.part_o = (float*)workspace;
   a.part_ml = (float2*)((char*)workspace + (int64_t)(p.S1 + p.S2) * T * Hq * D * 4);
+  a.n_tile = (int*)((char*)workspace + (int64_t)(p.S1 + p.S2) * T * Hq * (D * 4 + 8));
+  a.n_own = a.n_tile + T * Hq;
   a.T = (int)T;
   a.Hq = (int)Hq;
   a.Hkv = (int)Hkv;
@@ -1618,13 +1851,13 @@ extern "C" tb_status tb_shared_prefix_attention(const void* q, const void* k_cac
   a.page_shift = __builtin_ctzll((unsigned long long)page_size);
   a.S1 = p.S1;
   a.S2 = p.S2;
-  a.direct = !p.combine;
+  a.streams = (int)(p.stream_blocks * WAVES);
+  a.stream_least = p.stream_least;
   a.scale_log2 = scale == 0.0 ? 1.0f : (float)((scale < 0.0 ? -scale : scale) * 1.44269504088896340736);
   a.flip = scale < 0.0 ? 0x80008000u : 0u;
   a.keep = scale == 0.0 ? 0u : ~0u;
   a.joint = p.joint;
   a.rounds = p.rounds;
-  a.spread = p.spread;
   a.tile_fill = p.tile_fill;
   a.by_grp = Divisor((uint32_t)a.grp);
   a.by_heads = Divisor((uint32_t)Hkv);

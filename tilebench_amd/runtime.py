@@ -71,7 +71,7 @@ SIGNATURES: dict[str, list] = {
     "tb_rotary_axes": [_c_p] * 7 + [_c_i64] * 10 + [_c_int] * 3 + [_c_p],
     "tb_rope_kv_append": [_c_p] * 12 + [_c_i64] * 20 + [_c_int] * 3 + [_c_p],
     "tb_shared_prefix_attention": [_c_p] * 13 + [_c_i64] * 19 + [ctypes.c_double, _c_int, _c_int, _c_p, _c_i64, _c_p],
-    "tb_shared_prefix_attention_workspace_size": [_c_i64] * 10 + [ctypes.POINTER(_c_i64)],
+    "tb_shared_prefix_attention_workspace_size": [_c_i64] * 10 + [_c_int, ctypes.POINTER(_c_i64)],
     "tb_gemm_tile": [_c_int, _c_i64, _c_i64, _c_i64, _c_i64, ctypes.POINTER(GemmTile)],
     "tb_l2_flush": [_c_p, _c_i64, _c_u32, _c_p],
     "tb_probe_copy": [_c_p, _c_p, _c_i64, _c_p],
