@@ -685,7 +685,7 @@ __device__ __forceinline__ void finish(uint32_t args, uint32_t outs, uint32_t st
   const bool marked = lds_read<int>(any) != 0;
   const int64_t all = (int64_t)a.T * a.Hq;
   typedef typename W::Y::el el;
-#pragma unroll 2
+#pragma unroll 4
   for (int i = threadIdx.x; i < rows * (D / 4); i += THREADS) {
     const int r = i / (D / 4), c = i % (D / 4);
     f32x4 x = lds_read<f32x4>(out_at<D>(outs, r, c));
@@ -1507,7 +1507,7 @@ __device__ __forceinline__ void row_tile(const Args& a, char* smem, int index, u
       [&](int r) { return lds_read<int>(info + 4 * r) >= 0 && (lds_read<int>(info + 4 * r) & BIG); });
 }
 
-// Tile blocks first, then streams.
+// Tiles first: they take longer (64 decodes behind 8192 tokens: 30.6 us, the other way round 35.6).
 template <int DT, bool E8, int D, int RW>
 __global__ void __launch_bounds__(THREADS, 2) attend(Args a) {
   extern __shared__ __align__(16) char smem[];
@@ -1521,43 +1521,48 @@ __global__ void __launch_bounds__(THREADS, 2) attend(Args a) {
 
 // ------------------------------------------------------------------ combine
 
-// The slots of a row: the first n_tile of the tiles', the first n_own of the streams'; n-th of both: slot_of(n).
+// The slots of a row: the first n_tile of the tiles' S1, the first n_own of the streams' S2 after them.  (Maxima and
+// sums of all slots are read along with the counts, one round of loads less; those of unused slots mean nothing.)
 struct Slots {
   int tile, own;
   __device__ __forceinline__ Slots(const Args& a, int64_t id, int first, int end) {
     const int t = (int)(id / a.Hq);
+    const int n_tile = a.S1 > 0 ? a.n_tile[id] : 0, n_own = a.n_own[id];
     const bool inside = t >= first && t < end;  // else a row of no sequence
-    tile = inside && a.S1 > 0 ? min(a.n_tile[id], a.S1) : 0;
-    own = inside && tile >= 0 ? clamp_int(a.n_own[id], 0, a.S2) : 0;
+    tile = inside ? min(n_tile, a.S1) : 0;
+    own = inside ? clamp_int(n_own, 0, a.S2) : 0;
   }
-  __device__ __forceinline__ int count() const { return tile + own; }
-  __device__ __forceinline__ int slot_of(const Args& a, int n) const { return n < tile ? n : a.S1 + n - tile; }
+  __device__ __forceinline__ bool has(const Args& a, int slot) const {
+    return slot < a.S1 ? slot < tile : slot < a.S1 + own;
+  }
 };
 
-// One wavefront a row: lane n reads the maximum and sum of the row's slots n and n + 64, then all lanes add the slots'
-// outputs in order, eight of them in flight.  A wavefront looks through `run` rows for those that their tile has not
-// written already (most of a prompt's).
+// One wavefront a row: lane n reads the maximum and sum of slots n and n + 64, then all lanes add the slots' outputs in
+// order, sixteen of them in flight.  A wavefront looks through `run` rows for those that their tile has not written
+// already (most of a prompt's); its rows lie far apart, since the others lie together.
 template <int DT, int D>
 __global__ void __launch_bounds__(THREADS) combine(Args a, int run) {
   typedef typename Ty<DT>::el el;
-  constexpr int PER = D / 64, AT_ONCE = 8;
+  constexpr int PER = D / 64, AT_ONCE = 16;
   struct alignas(4 * PER) Part { float x[PER]; };
   struct alignas(2 * PER) Out { el x[PER]; };
-  const int lane = threadIdx.x & 63;
-  const int64_t rows = (int64_t)a.T * a.Hq, id0 = ((int64_t)blockIdx.x * WAVES + (threadIdx.x >> 6)) * run;
-  if (id0 >= rows) return;
+  const int lane = threadIdx.x & 63, n = a.S1 + a.S2;
+  const int64_t rows = (int64_t)a.T * a.Hq, all = (int64_t)gridDim.x * WAVES;
+  const int64_t id0 = (int64_t)blockIdx.x * WAVES + (threadIdx.x >> 6);
   const int first = query_start(a, 0), end = query_start(a, a.B);
-  bool open = lane < run && id0 + lane < rows;
-  if (open && run > 1) open = Slots(a, id0 + lane, first, end).tile >= 0;
+  bool open = lane < run && id0 + lane * all < rows;
+  if (open && run > 1) open = Slots(a, id0 + lane * all, first, end).tile >= 0;
   for (unsigned long long rest = __ballot(open); rest; rest &= rest - 1) {
-    const int64_t id = id0 + __builtin_ctzll(rest);
-    const Slots slots(a, id, first, end);
-    if (slots.tile < 0) continue;
-    const int n = __builtin_amdgcn_readfirstlane(slots.count());
+    const int64_t id = id0 + __builtin_ctzll(rest) * all;
     float2 ml[2] = {float2{NEG_INF, 0.0f}, float2{NEG_INF, 0.0f}};
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-      if (lane + 64 * i < n) ml[i] = a.part_ml[slots.slot_of(a, lane + 64 * i) * rows + id];
+      if (lane + 64 * i < n) ml[i] = a.part_ml[(lane + 64 * i) * rows + id];
+    const Slots slots(a, id, first, end);
+    if (slots.tile < 0) continue;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (!slots.has(a, lane + 64 * i)) ml[i] = float2{NEG_INF, 0.0f};
     float top = fmaxf(ml[0].x, ml[1].x);
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
@@ -1581,7 +1586,7 @@ __global__ void __launch_bounds__(THREADS) combine(Args a, int run) {
           const int s = live ? __builtin_ctzll(live) : 0;
           w[k] = live ? __shfl(weight[i], s) : 0.0f;
           p[k] = Part{};
-          if (live) p[k] = *(const Part*)(a.part_o + (slots.slot_of(a, s + 64 * i) * rows + id) * D + lane * PER);
+          if (live) p[k] = *(const Part*)(a.part_o + ((s + 64 * i) * rows + id) * D + lane * PER);
           live &= live - 1;
         }
 #pragma unroll
@@ -1606,15 +1611,17 @@ __global__ void __launch_bounds__(THREADS) combine_many(Args a) {
   constexpr int PER = D / 32, HALVES = 2 * WAVES;
   struct alignas(4 * PER) Part { float x[PER]; };
   __shared__ float joined[HALVES][D];
-  const int lane = threadIdx.x & 63, half = (int)threadIdx.x >> 5, at = lane & 31;
+  const int lane = threadIdx.x & 63, half = (int)threadIdx.x >> 5, at = lane & 31, n = a.S1 + a.S2;
   const int64_t rows = (int64_t)a.T * a.Hq, id = blockIdx.x;
-  const Slots slots(a, id, query_start(a, 0), query_start(a, a.B));
-  if (slots.tile < 0) return;  // written by its tile
-  const int n = slots.count();
   float2 ml[2] = {float2{NEG_INF, 0.0f}, float2{NEG_INF, 0.0f}};
 #pragma unroll
   for (int i = 0; i < 2; ++i)
-    if (lane + 64 * i < n) ml[i] = a.part_ml[slots.slot_of(a, lane + 64 * i) * rows + id];
+    if (lane + 64 * i < n) ml[i] = a.part_ml[(lane + 64 * i) * rows + id];
+  const Slots slots(a, id, query_start(a, 0), query_start(a, a.B));
+  if (slots.tile < 0) return;  // written by its tile
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (!slots.has(a, lane + 64 * i)) ml[i] = float2{NEG_INF, 0.0f};
   float top = fmaxf(ml[0].x, ml[1].x);
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
@@ -1634,8 +1641,7 @@ __global__ void __launch_bounds__(THREADS) combine_many(Args a) {
     const float l0 = __shfl(ml[0].y, s & 63), l1 = __shfl(ml[1].y, s & 63);
     const float w = s < 64 ? w0 : w1, l = s < 64 ? l0 : l1;
     Part p{};
-    if (s < n && !(l == 0.0f))  // an empty slot's output is not there
-      p = *(const Part*)(a.part_o + (slots.slot_of(a, s) * rows + id) * D + at * PER);
+    if (s < n && !(l == 0.0f)) p = *(const Part*)(a.part_o + (s * rows + id) * D + at * PER);  // an empty one is not there
 #pragma unroll
     for (int k = 0; k < PER; ++k) x[k] += w * p.x[k];
   }
@@ -1693,9 +1699,10 @@ inline Plan make_plan(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t G, 
     if (groups == 1 && !p.rounds) p.S1 = (int)between(p.tile_fill / between(units, 1, FILL), 1, p.S1);
     p.tile_blocks = (rows / tile + groups) * Hkv + FILL;
   }
-  // streams of at least four steps, of so many that a sequence falls to at most 63 of them
+  // A sequence falls to at most S2 - 1 full streams and one more; S2 up to 64, as far as 512 MB of partial results go.
   const int64_t tok = (e8 || D == 64) ? 64 : 32, most = ceil_div(W * page, tok);
-  p.stream_least = (int)between(ceil_div(most, MAX_SPLIT - 2), 4, 1 << 30);
+  const int64_t slots = between((512 << 20) / (T * Hq * (D * 4 + 8)), 4, MAX_SPLIT);
+  p.stream_least = (int)ceil_div(most, slots - 1);
   p.S2 = (int)(ceil_div(most, p.stream_least) + 1);
   p.stream_blocks = between(ceil_div(B * Hkv * most, WAVES * p.stream_least), 1, p.S1 > 0 && !p.rounds ? FILL / 2 : FILL);
   p.bytes = (int64_t)(p.S1 + p.S2) * T * Hq * (D * 4 + 8) + 2 * T * Hq * 4;
@@ -1712,7 +1719,7 @@ tb_status launch(Args& a, const Plan& p, hipStream_t stream, const char* what) {
                      a);
   if (tb_status s = launch_status(what)) return s;
   const int64_t rows = (int64_t)a.T * a.Hq, run = a.big && rows >= 32768 ? 16 : 1;
-  if (a.S1 + a.S2 > 16 && rows <= 16384)  // 69 slots: 8.0 us by wavefronts, 5.0 by blocks
+  if (a.S1 > 24 && rows <= 16384)  // 69 slots: 8.0 us by wavefronts, 5.0 by blocks
     hipLaunchKernelGGL((combine_many<DT, D>), dim3((unsigned)rows), dim3(THREADS), 0, stream, a);
   else
     hipLaunchKernelGGL((combine<DT, D>), dim3((unsigned)ceil_div(rows, WAVES * run)), dim3(THREADS), 0, stream, a, (int)run);
