@@ -85,8 +85,8 @@ struct Args {
   const int* cu_q;          // [B + 1]
   void* out;
   float* lse;
-  float* part_o;  // [slots][T * Hq][D]
-  float2* part_ml;  // [slots][T * Hq]: maximum (log2) and sum
+  float* part_o;    // [T * Hq][S1 + S2 slots][D]: a row's partial outputs lie together
+  float2* part_ml;  // [T * Hq][S1 + S2]: maximum (log2) and sum
   int* n_tile;      // [T * Hq]: slots 0 .. that the row's tiles used, -1 where its result is final
   int* n_own;       // [T * Hq]: slots S1 .. that its own tokens used
   int T, Hq, Hkv, grp, G, Wp, B, W;
@@ -683,7 +683,7 @@ __device__ __forceinline__ void finish(uint32_t args, uint32_t outs, uint32_t st
                                        int rows, int q0, int first, int h, int split, int splits, Big big) {
   const Args a = saved_args(args);
   const bool marked = lds_read<int>(any) != 0;
-  const int64_t all = (int64_t)a.T * a.Hq;
+  const int slots = a.S1 + a.S2;
   typedef typename W::Y::el el;
 #pragma unroll 4
   for (int i = threadIdx.x; i < rows * (D / 4); i += THREADS) {
@@ -713,10 +713,10 @@ __device__ __forceinline__ void finish(uint32_t args, uint32_t outs, uint32_t st
     if (final)
       store4((el*)a.out + id * D + c * 4, x * inverse(ml[1]));
     else if (!(ml[1] == 0.0f))
-      *(f32x4*)(a.part_o + (split * all + id) * D + c * 4) = x;
+      *(f32x4*)(a.part_o + (id * slots + split) * D + c * 4) = x;
     if (c == 0) {
       if (final) a.lse[id] = natural_lse(ml[0], ml[1]);
-      if (TILES && !final) a.part_ml[split * all + id] = float2{ml[0], ml[1]};
+      if (TILES && !final) a.part_ml[id * slots + split] = float2{ml[0], ml[1]};
       if (TILES && split == 0) {
         a.n_tile[id] = final ? -1 : splits;
         if (own_here) a.n_own[id] = 0;
@@ -1113,11 +1113,10 @@ __device__ __forceinline__ void stream_rows(const Args& a, char* smem, int index
       // this unit's results
       const Args b = saved_args(lds_addr(smem) + L::ARGS);
       const float l = W::over_groups_sum(w.l);
-      const int64_t all = (int64_t)b.T * b.Hq;
       const bool marked = lds_read<int>(any) != 0;
       const int g = lane / SH, rows = u.n_q * b.grp;
       if (row < rows && rows <= FEW) {
-        const int64_t id = (int64_t)(u.q0 + qi) * b.Hq + u.h * b.grp + head, slot = (b.S1 + u.slot) * all + id;
+        const int64_t id = (int64_t)(u.q0 + qi) * b.Hq + u.h * b.grp + head, slot = id * (b.S1 + b.S2) + b.S1 + u.slot;
         if (!(l == 0.0f)) {
 #pragma unroll
           for (int d = 0; d < W::DT_N; ++d) {
@@ -1367,11 +1366,15 @@ __device__ __forceinline__ void row_tile(const Args& a, char* smem, int index, u
     return false;
   };
   // e4m3 codes pass through registers: rows lane / LANES + i * (64 / LANES), 16 codes a lane, and one scale a lane (of
-  // the keys of the wavefront's tokens, then of their values).
+  // the keys of the wavefront's tokens, then of their values).  Two sets, for even and odd steps: a step's loads have
+  // two steps' time.
   constexpr int LANES = D / 16;
-  u32x4 codes[2][E8 ? NI : 1];
-  float scale = 0.0f;
-  auto fetch = [&](int n) __attribute__((always_inline)) {
+  struct Codes {
+    u32x4 x[2][E8 ? NI : 1];
+    float scale;
+  };
+  Codes codes[2];
+  auto fetch = [&](int n, Codes& c) __attribute__((always_inline)) {
     const int t0 = n * TOK + wave * MINE;  // the wavefront's first token
     win.cover(src, min(t0, src.len - 1) >> a.page_shift, min(t0 + MINE - 1, src.len - 1) >> a.page_shift, a.n_pages);
     if (!E8) {
@@ -1389,13 +1392,13 @@ __device__ __forceinline__ void row_tile(const Args& a, char* smem, int index, u
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       const int64_t off = offset(lane / LANES + i * (64 / LANES), a.c_page, a.c_slot) + (lane % LANES) * 16;
-      codes[0][i] = *(const u32x4*)(kp + off);
-      codes[1][i] = *(const u32x4*)(vp + off);
+      c.x[0][i] = *(const u32x4*)(kp + off);
+      c.x[1][i] = *(const u32x4*)(vp + off);
     }
     const int64_t off = offset(lane % MINE, a.s_page, a.s_slot) + h * a.s_head;
-    scale = ((lane / MINE) & 1 ? a.vs : a.ks)[off];
+    c.scale = ((lane / MINE) & 1 ? a.vs : a.ks)[off];
   };
-  auto place = [&](int n) __attribute__((always_inline)) {
+  auto place = [&](int n, const Codes& c) __attribute__((always_inline)) {
     if (!E8) return;
     const uint32_t stage = base + (n & 1) * L::STAGE;
 #pragma unroll
@@ -1409,17 +1412,20 @@ __device__ __forceinline__ void row_tile(const Args& a, char* smem, int index, u
         for (int half = 0; half < 2; ++half) {
           u32x4 x;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] = W::Y::up8(codes[kv][i][half * 2 + e / 2], e & 1);
+          for (int e = 0; e < 4; ++e) x[e] = W::Y::up8(c.x[kv][i][half * 2 + e / 2], e & 1);
           *(__attribute__((address_space(3))) u32x4*)(uintptr_t)(row + ((((lane % LANES) * 2 + half) ^ swizzle) << 4)) = x;
         }
       }
     }
     if (lane < 2 * MINE)
       *(__attribute__((address_space(3))) float*)(uintptr_t)(
-          scale_at(stage + 2 * L::TILE_BYTES, wave * MINE + lane % MINE) + (lane / MINE) * 128) = scale;
+          scale_at(stage + 2 * L::TILE_BYTES, wave * MINE + lane % MINE) + (lane / MINE) * 128) = c.scale;
   };
   bool have = next_run(a);
-  if (have) fetch(n0);
+  if (have) {
+    fetch(n0, codes[0]);
+    if (E8 && n0 + 1 < n1) fetch(n0 + 1, codes[1]);
+  }
 
   // What the rows see, worked out while the first tokens are on their way.
   int mine = -1, prefix_limit = 0, own_limit = 0;  // sequence from the group's first
@@ -1445,7 +1451,7 @@ __device__ __forceinline__ void row_tile(const Args& a, char* smem, int index, u
     p[2 * L::ROWS] = own_limit;
     if (wr == 0 && lane == 0) *(int*)(smem + L::ANY) = 0;
   }
-  if (have) place(n0);
+  if (have) place(n0, codes[0]);
   block_barrier();
 
   while (have) {
@@ -1465,13 +1471,15 @@ __device__ __forceinline__ void row_tile(const Args& a, char* smem, int index, u
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) seen_by_all = min(seen_by_all, __shfl_xor(seen_by_all, d));
     seen_by_all = __builtin_amdgcn_readfirstlane(seen_by_all);
-    for (int n = n0; n < n1; ++n) {
+    // one step; `now` held the step's codes, `other` those of the next
+    auto step = [&](int n, Codes& now, Codes& other) __attribute__((always_inline)) {
       const uint32_t stage = base + (n & 1) * L::STAGE;
-      wait_vm<0>();
+      if (!E8) wait_vm<0>();
       if ((n + 1) * TOK > seen_by_all)  // each wavefront looks at the tokens it has fetched
         W::template set_apart<MINE>(stage + L::TILE_BYTES, wave * MINE, n * TOK, L::ROWS, marks, any, limit_of);
       block_barrier();  // the step's tokens are there, the other stage is free
-      if (n + 1 < n1) fetch(n + 1);
+      if (!E8 && n + 1 < n1) fetch(n + 1, other);
+      if (E8 && n + 2 < n1) fetch(n + 2, now);
 #pragma unroll
       for (int c = 0; c < SHARE / STEP; ++c) {
         const int tok0 = wt * SHARE + c * STEP, t0 = n * TOK + tok0;
@@ -1484,14 +1492,19 @@ __device__ __forceinline__ void row_tile(const Args& a, char* smem, int index, u
         w.template weights<STEP>(s, t0, limit, full, a.scale_log2, stage + 2 * L::TILE_BYTES, tok0, p);
         w.template values<STEP>(kb + L::TILE_BYTES, p);
       }
-      if (n + 1 < n1) place(n + 1);
+      if (n + 1 < n1) place(n + 1, other);
+    };
+    for (int n = n0; n < n1; n += E8 ? 2 : 1) {
+      step(n, codes[0], codes[1]);
+      if (E8 && n + 1 < n1) step(n + 1, codes[1], codes[0]);
     }
     if (todo > 0) {
       have = next_run(saved_args(base + L::ARGS));
       if (have) {
         block_barrier();  // both stages may still be read
-        fetch(n0);
-        place(n0);
+        fetch(n0, codes[0]);
+        if (E8 && n0 + 1 < n1) fetch(n0 + 1, codes[1]);
+        place(n0, codes[0]);
       }
     } else {
       have = false;
@@ -1557,7 +1570,7 @@ __global__ void __launch_bounds__(THREADS) combine(Args a, int run) {
     float2 ml[2] = {float2{NEG_INF, 0.0f}, float2{NEG_INF, 0.0f}};
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-      if (lane + 64 * i < n) ml[i] = a.part_ml[(lane + 64 * i) * rows + id];
+      if (lane + 64 * i < n) ml[i] = a.part_ml[id * n + lane + 64 * i];
     const Slots slots(a, id, first, end);
     if (slots.tile < 0) continue;
 #pragma unroll
@@ -1586,7 +1599,7 @@ __global__ void __launch_bounds__(THREADS) combine(Args a, int run) {
           const int s = live ? __builtin_ctzll(live) : 0;
           w[k] = live ? __shfl(weight[i], s) : 0.0f;
           p[k] = Part{};
-          if (live) p[k] = *(const Part*)(a.part_o + ((s + 64 * i) * rows + id) * D + lane * PER);
+          if (live) p[k] = *(const Part*)(a.part_o + (id * n + s + 64 * i) * D + lane * PER);
           live &= live - 1;
         }
 #pragma unroll
@@ -1616,7 +1629,7 @@ __global__ void __launch_bounds__(THREADS) combine_many(Args a) {
   float2 ml[2] = {float2{NEG_INF, 0.0f}, float2{NEG_INF, 0.0f}};
 #pragma unroll
   for (int i = 0; i < 2; ++i)
-    if (lane + 64 * i < n) ml[i] = a.part_ml[(lane + 64 * i) * rows + id];
+    if (lane + 64 * i < n) ml[i] = a.part_ml[id * n + lane + 64 * i];
   const Slots slots(a, id, query_start(a, 0), query_start(a, a.B));
   if (slots.tile < 0) return;  // written by its tile
 #pragma unroll
@@ -1641,7 +1654,7 @@ __global__ void __launch_bounds__(THREADS) combine_many(Args a) {
     const float l0 = __shfl(ml[0].y, s & 63), l1 = __shfl(ml[1].y, s & 63);
     const float w = s < 64 ? w0 : w1, l = s < 64 ? l0 : l1;
     Part p{};
-    if (s < n && !(l == 0.0f)) p = *(const Part*)(a.part_o + (s * rows + id) * D + at * PER);  // an empty one is not there
+    if (s < n && !(l == 0.0f)) p = *(const Part*)(a.part_o + (id * n + s) * D + at * PER);  // an empty one is not there
 #pragma unroll
     for (int k = 0; k < PER; ++k) x[k] += w * p.x[k];
   }
@@ -1664,7 +1677,7 @@ struct Plan {
   int row_waves = 2;                                            // tiles of 64 or 128 rows
   int tile_fill = FILL;
   int S1 = 0, S2 = 0, stream_least = 0;
-  bool joint = false, rounds = false;
+  bool joint = false, rounds = false, many = false;  // many: slots a row
   int64_t bytes = 0;
 };
 
@@ -1698,6 +1711,7 @@ inline Plan make_plan(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t G, 
     p.S1 = (int)between(cuts, 1, p.rounds ? between(room, 1, 8) : MAX_SPLIT);
     if (groups == 1 && !p.rounds) p.S1 = (int)between(p.tile_fill / between(units, 1, FILL), 1, p.S1);
     p.tile_blocks = (rows / tile + groups) * Hkv + FILL;
+    p.many = p.tile_fill / units > 24 && T * Hq <= 16384;
   }
   // A sequence falls to at most S2 - 1 full streams and one more; S2 up to 64, as far as 512 MB of partial results go.
   const int64_t tok = (e8 || D == 64) ? 64 : 32, most = ceil_div(W * page, tok);
@@ -1719,7 +1733,7 @@ tb_status launch(Args& a, const Plan& p, hipStream_t stream, const char* what) {
                      a);
   if (tb_status s = launch_status(what)) return s;
   const int64_t rows = (int64_t)a.T * a.Hq, run = a.big && rows >= 32768 ? 16 : 1;
-  if (a.S1 > 24 && rows <= 16384)  // 69 slots: 8.0 us by wavefronts, 5.0 by blocks
+  if (p.many)  // 69 slots: 8.0 us by wavefronts, 5.0 by blocks
     hipLaunchKernelGGL((combine_many<DT, D>), dim3((unsigned)rows), dim3(THREADS), 0, stream, a);
   else
     hipLaunchKernelGGL((combine<DT, D>), dim3((unsigned)ceil_div(rows, WAVES * run)), dim3(THREADS), 0, stream, a, (int)run);
