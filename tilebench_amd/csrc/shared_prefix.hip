@@ -243,7 +243,7 @@ struct Window {
   __device__ __forceinline__ void cover(const Tokens& s, int lo, int hi, int n_pages) {
     if (lo >= first && hi - 64 < first) return;
     first = lo;
-    int id = s.table[min(lo + (int)(threadIdx.x & 63), s.width - 1)];
+    int id = ((const __attribute__((address_space(1))) int*)s.table)[min(lo + (int)(threadIdx.x & 63), s.width - 1)];
     id = min(max(id, 0), n_pages - 1);
     asm volatile("" : "+v"(id));  // the wait for the load belongs here, not at the uses in the loop
     ids = id;
@@ -387,14 +387,15 @@ struct Wave {
     }
   }
 
-  // Scores of the tokens that a row does not see: -inf.  left: tokens up to the row's limit, from the lane group's first.
+  // Scores (weights) of the tokens that a row does not see: `instead`.  left: tokens up to the row's limit, from the lane
+  // group's first.
   template <int TOK>
-  static __device__ __forceinline__ void hide(acc_t (&s)[TOK / SH], int left) {
+  static __device__ __forceinline__ void hide(acc_t (&s)[TOK / SH], int left, float instead) {
     __builtin_amdgcn_sched_barrier(0);  // comparisons hoisted over the products would take all scalar registers
 #pragma unroll
     for (int t = 0; t < TOK / SH; ++t) {
 #pragma unroll
-      for (int r = 0; r < REGS; ++r) s[t][r] = t * SH + token_of(r, 0) < left ? s[t][r] : NEG_INF;
+      for (int r = 0; r < REGS; ++r) s[t][r] = t * SH + token_of(r, 0) < left ? s[t][r] : instead;
       __builtin_amdgcn_sched_barrier(0);
     }
   }
@@ -405,22 +406,22 @@ struct Wave {
   __device__ __forceinline__ void weights(acc_t (&s)[TOK / SH], int t0, int limit, bool full, float scale,
                                           uint32_t sbase, int tok0, v8 (&p)[TOK / KS]) {
     const int g = (threadIdx.x & 63) / SH;
+    if (SC) {
+#pragma unroll
+      for (int t = 0; t < TOK / SH; ++t)
+#pragma unroll
+        for (int r = 0; r < REGS; r += 4) {
+          const f32x4 k = lds_read<f32x4>(scale_at(sbase, tok0 + t * SH + token_of(r, g)));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[t][r + i] *= k[i];
+        }
+    }
+    if (!full) hide<TOK>(s, limit - t0 - 4 * g, NEG_INF);
     float top = NEG_INF;
-    if (!full) hide<TOK>(s, limit - t0 - 4 * g);
 #pragma unroll
     for (int t = 0; t < TOK / SH; ++t)
 #pragma unroll
-      for (int r = 0; r < REGS; r += 4) {
-        const int tok = t * SH + token_of(r, g);
-        if (SC) {
-          const f32x4 k = lds_read<f32x4>(scale_at(sbase, tok0 + tok));
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[t][r + i] *= full || s[t][r + i] > NEG_INF ? k[i] : 1.0f;
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) top = fmaxf(top, s[t][r + i]);
-        if (SC && r % 8 == 4) __builtin_amdgcn_sched_barrier(0);  // all scales at once would spill
-      }
+      for (int r = 0; r < REGS; ++r) top = fmaxf(top, s[t][r]);
     top = over_groups_max(top) * scale;
     if (__any(top > m + (LIFT + SLACK))) {
       const float ref = fmaxf(m, top - LIFT);
@@ -444,11 +445,11 @@ struct Wave {
         for (int i = 0; i < 4; ++i) {
           const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r + i], scale, -use));
           sum += w;
-          s[t][r + i] = !SC ? w : full || w > 0.0f ? w * v[i] : 0.0f;
+          s[t][r + i] = SC ? w * v[i] : w;
         }
-        if (SC && r % 8 == 4) __builtin_amdgcn_sched_barrier(0);
       }
     l += sum;
+    if (SC && !full) hide<TOK>(s, limit - t0 - 4 * g, 0.0f);  // whatever their scales are
 #pragma unroll
     for (int k = 0; k < TOK / KS; ++k)
 #pragma unroll
@@ -1296,7 +1297,8 @@ __device__ __forceinline__ void row_tile(const Args& a, char* smem, int index, u
   constexpr int NI = MINE * D * ESIZE / 1024;  // in copies of 1 KiB
   constexpr int SHARE = TOK * RW / WAVES;      // tokens of a step that a wavefront attends to
   constexpr int BIG = 1 << 30;                 // on a row's sequence number: it has more than 16 rows
-  constexpr int STEP = SHARE > 64 ? 64 : SHARE;
+  constexpr int MOST = E8 ? 32 : 64;           // in steps of so many (with scales 64 would spill)
+  constexpr int STEP = SHARE > MOST ? MOST : SHARE;
   static_assert(NI >= 1, "a wavefront fetches whole copies");
   typedef Copier<RB, NI> Copy;
   typedef Wave<DT, false, D, SH, E8> W;
