@@ -11,15 +11,26 @@
 // Angles.  A 32-bit product loses 2^-24 of the angle: 4e-3 rad at position
 // 65536, more than an fp16 ulp of the result.  The product and its reduction
 // to [-1/2, 1/2] turns are done in 64 bits, sine and cosine of the reduced angle
-// in 32 (1 ulp).  They depend on (token, pair) only, so a block computes them
-// once per token into LDS and all heads read them there: 64 per token instead of
-// 64 per head and token.
+// in 32 (1 ulp).  They depend on (token, pair) only: a wavefront computes its
+// token's once into LDS and its lanes read them there for 8 rows of 128.
 //
 // Layout of the work.  A head is D / (2 VEC) items of 2 VEC elements, one item a
-// lane; LP = the next power of two lanes hold a head, so that the absolute
-// maximum of an 8-bit cache row is a shuffle reduction and the row is read
-// once.  VEC = 8 makes 16-byte accesses; VEC = 4 and 1 serve heads, rotations
-// or strides that are not multiples of 16 (all widths give the same bits).
+// lane, two accesses of 16 bytes (VEC = 8; 4 for fp32).  A wavefront takes 64
+// items of one token and the four of a block follow each other in memory; no
+// barrier, no loop.  Where a row's maximum is needed (8-bit caches), a power of
+// two of lanes holds it, so the row is read once and the maximum is a shuffle.
+// VEC = 4 and 1 serve heads, rotations or strides that are not multiples of 16
+// bytes (all widths give the same bits).
+//
+// What bounds it: bytes in flight.  A wavefront lives for its chain of loads, a
+// microsecond or more each, so axes, frequencies, positions, slots and rows are all asked
+// for before the first of them is waited for: 20001 tokens of 32 + 8 fp16 heads
+// of 128 take 74 us (5.5 TB/s), and 80 us (5.1 TB/s) with the positions' loads
+// behind the axes'.  A 410 MB copy takes 64 us.  Wavefronts with 2, 3 and 4 times the
+// items take 80, 95 and 124 us (before that change); four tokens to a block and
+// a loop over their heads 83 us; 8-byte accesses 96 us.  4800 tokens of 16 + 16
+// bf16 heads of 80 take 11.9 us (4.1 TB/s), 7001 tokens into a bf16 cache 31.4
+// us (5.5 TB/s), 4096 into an 8-bit cache 18.8 us (4.9 TB/s), one token 3.4 us.
 //
 // 8-bit cache rows: s = absmax / 448 over the fp32 values (rotated, never
 // rounded to 16 bits before), code = e4m3(x / s), both IEEE; a row of zeros
@@ -29,7 +40,7 @@
 namespace tb {
 namespace rotary {
 
-constexpr int THREADS = 256, MAX_TOKENS = 4, MAX_D = 512;
+constexpr int THREADS = 256, WAVES = 4, MAX_D = 512;
 
 enum { F32 = 0, F16 = 1, BF16 = 2 };
 enum { DENSE = 0, CACHE = 1, CACHE_E4M3 = 2 };
@@ -50,9 +61,9 @@ struct Elem<F16> {
 };
 template <>
 struct Elem<BF16> {
-  typedef uint16_t type;
-  static __device__ __forceinline__ float up(uint16_t x) { return __builtin_bit_cast(float, (uint32_t)x << 16); }
-  static __device__ __forceinline__ uint16_t down(float x) { return (uint16_t)bf16_bits(x); }
+  typedef __bf16 type;
+  static __device__ __forceinline__ float up(__bf16 x) { return (float)x; }
+  static __device__ __forceinline__ __bf16 down(float x) { return (__bf16)x; }
 };
 
 // One of q, k, v: `heads` rows a token, at element strides st (token) and sh (head).
@@ -76,7 +87,10 @@ struct Args {
   int page_shift;
   int64_t T;
   int D, P, A;  // P = R / 2 pairs
-  int lp_shift, items, tokens;
+  int items, lanes;    // items of a head, lanes that hold it
+  Divisor by_lanes, by_portions;
+  int rows, portions;  // heads of a token; wavefronts that share them
+  int64_t t0, end;     // tokens of the launch
   int interleaved, inverse;
 };
 
@@ -94,176 +108,207 @@ __device__ __forceinline__ float2 cos_sin(int pos, float freq, bool inverse) {
   return float2{c, inverse ? -s : s};
 }
 
-template <int DT, int VEC, int MODE>
+// x / s rounded as the division is, for s in [2^-60, 2^60]: the product with s's rounded reciprocal, corrected once by
+// the exact remainder (3 operations instead of the division's 10).
+__device__ __forceinline__ float quotient(float x, float s, float inv) {
+  const float q = x * inv;
+  return __builtin_fmaf(__builtin_fmaf(-q, s, x), inv, q);
+}
+
+// e4m3 codes of N (1 or a multiple of 4) values.
+template <int N>
+__device__ __forceinline__ void codes(const float* x, uint8_t* c) {
+  if (N == 1) {
+    c[0] = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[0], 0.0f, 0, false);
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < N; e += 4) {
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(x[e], x[e + (N > 1)], 0, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(x[e + 2 * (N > 1)], x[e + 3 * (N > 1)], w, true);
+    __builtin_memcpy(c + e, &w, 4);
+  }
+}
+
+template <int DT, int VEC, int MODE, bool INTER>
 __global__ void __launch_bounds__(THREADS) rotate_heads(Args a) {
   typedef Elem<DT> E;
   typedef typename E::type T;
   typedef Chunk<T, VEC> C;
   constexpr int PASSES = VEC == 1 ? MAX_D / 128 : 1;  // items of a lane
-  __shared__ float2 trig[MAX_TOKENS * MAX_D / 2];
+  __shared__ float2 all_trig[WAVES][MAX_D / 2];
 
-  const int tid = threadIdx.x;
-  const int64_t t0 = (int64_t)blockIdx.x * a.tokens;
-  const int here = (int)min((int64_t)a.tokens, a.T - t0);  // tokens of this block
-  const int rows = a.src[0].heads + a.src[1].heads + a.src[2].heads;
-  const int lp = 1 << a.lp_shift, lane = tid & (lp - 1), per_pass = THREADS >> a.lp_shift;
-  const int total = here * rows, stride = per_pass * (int)gridDim.y;
-  const int rot_items = a.P / VEC;
-
-  C x1[PASSES], x2[PASSES];
-  auto offset1 = [&](int j) __attribute__((always_inline)) {
-    return j < rot_items && !a.interleaved ? j * VEC : 2 * j * VEC;
-  };
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const uint32_t portion = blockIdx.x * WAVES + wave, token = (uint32_t)a.by_portions.divide((int)portion);
+  const int64_t t = a.t0 + token;
+  if (t >= a.end) return;  // no barrier follows
+  float2* const trig = all_trig[wave];
+  const int n = (int)(portion - token * (uint32_t)a.portions) * 64 + lane;
+  const int row = a.by_lanes.divide(n), item = n - row * a.lanes;
+  const bool is_k = row >= a.src[0].heads, is_v = MODE != DENSE && row >= a.src[0].heads + a.src[1].heads;
+  const int head = row - (is_k ? a.src[0].heads : 0) - (is_v ? a.src[1].heads : 0);
+  const bool in = row < a.rows;
+  auto offset1 = [&](int j) __attribute__((always_inline)) { return j * VEC < a.P && !INTER ? j * VEC : 2 * j * VEC; };
   auto offset2 = [&](int j) __attribute__((always_inline)) {
-    return j < rot_items && !a.interleaved ? a.P + j * VEC : (2 * j + 1) * VEC;
+    return j * VEC < a.P && !INTER ? a.P + j * VEC : (2 * j + 1) * VEC;
   };
-  // head `row` of the token tile: its section and head within it
-  auto locate = [&](int row, int& sec, int& head, int& tok) __attribute__((always_inline)) {
-    tok = row / rows;
-    head = row - tok * rows;
-    sec = 0;
-    if (head >= a.src[0].heads) {
-      head -= a.src[0].heads;
-      sec = 1;
-      if (head >= a.src[1].heads) {
-        head -= a.src[1].heads;
-        sec = 2;
-      }
-    }
-  };
-  auto load = [&](int row) __attribute__((always_inline)) {
-    int sec, head, tok;
-    locate(row, sec, head, tok);
-    const Source& s = a.src[sec];
-    const T* p = (const T*)s.p + (t0 + tok) * s.st + head * s.sh;
+
+  // What the angles are made of is asked for first, then the row: it is on its way while they are computed.  No load
+  // waits for another (each takes a microsecond in a busy memory system).
+  const int places = a.axes && a.A > 1 ? min(lane, a.A - 1) : 0;
+  const int axis = a.axes ? a.axes[min(lane, a.P - 1)] : 0;
+  const float freq = a.inv_freq[min(lane, a.P - 1)];
+  const int place = a.positions[places * a.T + t];  // lane i: on axis i
+  const int64_t slot = MODE == DENSE ? 0 : a.slots[t];
+  C x1[PASSES], x2[PASSES];
+  if (in) {
+    const T* p = is_v   ? (const T*)a.src[2].p + t * a.src[2].st
+                 : is_k ? (const T*)a.src[1].p + t * a.src[1].st
+                        : (const T*)a.src[0].p + t * a.src[0].st;
+    p += head * (is_v ? a.src[2].sh : is_k ? a.src[1].sh : a.src[0].sh);
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
-      const int j = lane + i * lp;
+      const int j = item + i * 64;
       if (j < a.items) {
         x1[i] = *(const C*)(p + offset1(j));
         x2[i] = *(const C*)(p + offset2(j));
       }
     }
-  };
-
-  // the first rows are on their way while the angles are computed
-  int row = (int)blockIdx.y * per_pass + (tid >> a.lp_shift);
-  if (row < total) load(row);
-  for (int i = tid; i < here * a.P; i += THREADS) {
-    const int tok = i / a.P, pair = i - tok * a.P;
-    const int ax = a.axes ? min(max(a.axes[pair], 0), a.A - 1) : 0;
-    trig[i] = cos_sin(a.positions[ax * a.T + t0 + tok], a.inv_freq[pair], a.inverse);
   }
-  __syncthreads();
+  for (int i = lane;; i += 64) {
+    const bool mine = i < a.P, more = i >= 64;
+    const int ax = more && mine && a.axes ? a.axes[i] : axis;
+    const int pos = __shfl(place, min(max(ax, 0), a.A - 1));
+    if (mine) trig[i] = cos_sin(pos, more ? a.inv_freq[i] : freq, a.inverse);
+    if (i - lane + 64 >= a.P) break;
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 
-  for (; row < total; row += stride) {
-    int sec, head, tok;
-    locate(row, sec, head, tok);
-    float y1[PASSES][VEC], y2[PASSES][VEC];
+  float y1[PASSES][VEC], y2[PASSES][VEC];
 #pragma unroll
-    for (int i = 0; i < PASSES; ++i) {
-      const int j = lane + i * lp;
+  for (int i = 0; i < PASSES; ++i) {
+    const int j = item + i * 64;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      y1[i][e] = MODE != CACHE_E4M3 || j < a.items ? E::up(x1[i].e[e]) : 0.0f;  // nothing in the row's maximum
+      y2[i][e] = MODE != CACHE_E4M3 || j < a.items ? E::up(x2[i].e[e]) : 0.0f;
+    }
+    if (in && !is_v && j * VEC < a.P) {
+      const float2* cs = trig + j * VEC;
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        y1[i][e] = j < a.items ? E::up(x1[i].e[e]) : 0.0f;
-        y2[i][e] = j < a.items ? E::up(x2[i].e[e]) : 0.0f;
-      }
-      if (sec < 2 && j < rot_items) {
-        const float2* cs = trig + tok * a.P + j * VEC;
-        if (VEC > 1 && a.interleaved) {
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            float* y = 2 * e < VEC ? &y1[i][(2 * e) % VEC] : &y2[i][(2 * e) % VEC];
-            const float p = y[0], q = y[1];
-            y[0] = p * cs[e].x - q * cs[e].y;
-            y[1] = q * cs[e].x + p * cs[e].y;
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            const float p = y1[i][e], q = y2[i][e];
-            y1[i][e] = p * cs[e].x - q * cs[e].y;
-            y2[i][e] = q * cs[e].x + p * cs[e].y;
-          }
-        }
+        // pairs (x1[e], x2[e]), or neighbours within the 2 VEC elements
+        float& u = INTER && VEC > 1 ? (2 * e < VEC ? y1[i][(2 * e) % VEC] : y2[i][(2 * e) % VEC]) : y1[i][e];
+        float& v = INTER && VEC > 1 ? (2 * e < VEC ? y1[i][(2 * e + 1) % VEC] : y2[i][(2 * e + 1) % VEC]) : y2[i][e];
+        const float p = u, q = v;
+        u = p * cs[e].x - q * cs[e].y;
+        v = q * cs[e].x + p * cs[e].y;
       }
     }
-    const int64_t t = t0 + tok;
-    // the next row's loads go out before this row's stores
-    const int next = row + stride;
-    if (next < total) load(next);
-
-    int64_t at;
-    if (MODE == DENSE || sec == 0) {
-      at = (t * a.src[sec].heads + head) * a.D;
-    } else {
-      const int64_t slot = a.slots[t];
-      if (slot < 0 || slot >= a.n_slots) continue;  // a padded token: nothing is written
-      const int64_t page = slot >> a.page_shift, in = slot & ((1 << a.page_shift) - 1);
-      at = page * a.cp + head * a.ch + in * a.cs;
-      if (MODE == CACHE_E4M3) {
-        // the largest magnitude as bits: NaN above inf above every number
-        uint32_t m = 0;
+  }
+  int64_t at = (t * (is_k ? a.src[1].heads : a.src[0].heads) + head) * a.D;
+  bool kept = in;
+  if (MODE != DENSE && is_k) {
+    kept = in && slot >= 0 && slot < a.n_slots;  // a padded token: nothing is written
+    const int64_t page = slot >> a.page_shift, within = slot & ((1 << a.page_shift) - 1);
+    at = page * a.cp + head * a.ch + within * a.cs;
+    if (MODE == CACHE_E4M3) {
+      // the largest magnitude as bits: NaN above inf above every number
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < PASSES; ++i)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          m = max(m, __builtin_bit_cast(uint32_t, y1[i][e]) & 0x7FFFFFFFu);
+          m = max(m, __builtin_bit_cast(uint32_t, y2[i][e]) & 0x7FFFFFFFu);
+        }
+      for (int d = a.lanes >> 1; d > 0; d >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d));
+      const float s = __builtin_bit_cast(float, m) / 448.0f;
+      if (kept && item == 0) (is_v ? a.scale[1] : a.scale[0])[page * a.sp + head * a.sh + within * a.ss] = s;
+      if (s >= 0x1p-60f && s <= 0x1p60f) {
+        const float inv = 1.0f / s;
 #pragma unroll
         for (int i = 0; i < PASSES; ++i)
 #pragma unroll
           for (int e = 0; e < VEC; ++e) {
-            m = max(m, __builtin_bit_cast(uint32_t, y1[i][e]) & 0x7FFFFFFFu);
-            m = max(m, __builtin_bit_cast(uint32_t, y2[i][e]) & 0x7FFFFFFFu);
+            y1[i][e] = quotient(y1[i][e], s, inv);
+            y2[i][e] = quotient(y2[i][e], s, inv);
           }
-        for (int d = lp >> 1; d > 0; d >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d));
-        const float s = __builtin_bit_cast(float, m) / 448.0f;
-        if (lane == 0) a.scale[sec - 1][page * a.sp + head * a.sh + in * a.ss] = s;
-        uint8_t* dst = (uint8_t*)a.out[sec] + at;
+      } else {
 #pragma unroll
-        for (int i = 0; i < PASSES; ++i) {
-          const int j = lane + i * lp;
-          if (j >= a.items) continue;
-          Chunk<uint8_t, VEC> c1, c2;
+        for (int i = 0; i < PASSES; ++i)
 #pragma unroll
           for (int e = 0; e < VEC; ++e) {
-            c1.e[e] = m == 0 ? 0 : (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(y1[i][e] / s, 0.0f, 0, false);
-            c2.e[e] = m == 0 ? 0 : (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(y2[i][e] / s, 0.0f, 0, false);
+            y1[i][e] = m == 0 ? 0.0f : y1[i][e] / s;
+            y2[i][e] = m == 0 ? 0.0f : y2[i][e] / s;
           }
-          *(Chunk<uint8_t, VEC>*)(dst + offset1(j)) = c1;
-          *(Chunk<uint8_t, VEC>*)(dst + offset2(j)) = c2;
-        }
-        continue;
       }
-    }
-    T* dst = (T*)a.out[sec] + at;
+      uint8_t* dst = (uint8_t*)(is_v ? a.out[2] : a.out[1]) + at;
 #pragma unroll
-    for (int i = 0; i < PASSES; ++i) {
-      const int j = lane + i * lp;
-      if (j >= a.items) continue;
-      C c1, c2;
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        c1.e[e] = E::down(y1[i][e]);
-        c2.e[e] = E::down(y2[i][e]);
+      for (int i = 0; i < PASSES; ++i) {
+        const int j = item + i * 64;
+        if (!kept || j >= a.items) continue;
+        Chunk<uint8_t, VEC> c1, c2;
+        codes<VEC>(y1[i], c1.e);
+        codes<VEC>(y2[i], c2.e);
+        *(Chunk<uint8_t, VEC>*)(dst + offset1(j)) = c1;
+        *(Chunk<uint8_t, VEC>*)(dst + offset2(j)) = c2;
       }
-      *(C*)(dst + offset1(j)) = c1;
-      *(C*)(dst + offset2(j)) = c2;
+      return;
     }
+  }
+  T* dst = (T*)(is_v ? a.out[2] : is_k ? a.out[1] : a.out[0]) + at;
+#pragma unroll
+  for (int i = 0; i < PASSES; ++i) {
+    const int j = item + i * 64;
+    if (!kept || j >= a.items) continue;
+    C c1, c2;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      c1.e[e] = E::down(y1[i][e]);
+      c2.e[e] = E::down(y2[i][e]);
+    }
+    *(C*)(dst + offset1(j)) = c1;
+    *(C*)(dst + offset2(j)) = c2;
   }
 }
 
 template <int DT, int VEC, int MODE>
-tb_status launch(const Args& a, dim3 grid, hipStream_t stream, const char* what) {
-  hipLaunchKernelGGL((rotate_heads<DT, VEC, MODE>), grid, dim3(THREADS), 0, stream, a);
-  return launch_status(what);
+tb_status launch(Args& a, hipStream_t stream, const char* what) {
+  a.items = a.D / (2 * VEC);
+  a.lanes = a.items;
+  if (MODE == CACHE_E4M3 || VEC == 1)  // a power of two: the row's maximum is taken over its lanes
+    for (a.lanes = 1; a.lanes < a.items && a.lanes < 64;) a.lanes *= 2;
+  a.by_lanes = Divisor((uint32_t)a.lanes);
+  a.rows = a.src[0].heads + a.src[1].heads + a.src[2].heads;
+  a.portions = (a.rows * a.lanes + 63) / 64;
+  a.by_portions = Divisor((uint32_t)a.portions);
+  const int64_t most = (1 << 25) / a.portions;  // tokens of a launch: it holds 2^32 threads
+  for (a.t0 = 0; a.t0 < a.T; a.t0 += most) {
+    const int64_t tokens = a.T - a.t0 < most ? a.T - a.t0 : most;
+    a.end = a.t0 + tokens;
+    const dim3 grid((unsigned)((tokens * a.portions + WAVES - 1) / WAVES));
+    if (a.interleaved)
+      hipLaunchKernelGGL((rotate_heads<DT, VEC, MODE, true>), grid, dim3(THREADS), 0, stream, a);
+    else
+      hipLaunchKernelGGL((rotate_heads<DT, VEC, MODE, false>), grid, dim3(THREADS), 0, stream, a);
+    if (tb_status s = launch_status(what)) return s;
+  }
+  return TB_OK;
 }
 
 template <int DT, int MODE>
-tb_status launch_vec(int vec, const Args& a, dim3 grid, hipStream_t stream, const char* what) {
-  if (vec == 8) return launch<DT, 8, MODE>(a, grid, stream, what);
-  if (vec == 4) return launch<DT, 4, MODE>(a, grid, stream, what);
-  return launch<DT, 1, MODE>(a, grid, stream, what);
+tb_status launch_vec(int vec, Args& a, hipStream_t stream, const char* what) {
+  if constexpr (DT != F32)
+    if (vec == 8) return launch<DT, 8, MODE>(a, stream, what);
+  if (vec == 4) return launch<DT, 4, MODE>(a, stream, what);
+  return launch<DT, 1, MODE>(a, stream, what);
 }
 
 // The widest access that every head, rotation, stride and pointer allows.
 struct Width {
-  int vec = 8;
+  int vec;
+  explicit Width(int64_t elem) : vec(elem == 4 ? 4 : 8) {}
   void lengths(int64_t P, int64_t D) {
     while (vec > 1 && (P % vec || (D - 2 * P) % (2 * vec))) vec = vec == 8 ? 4 : 1;
   }
@@ -275,25 +320,6 @@ struct Width {
     }
   }
 };
-
-// Fills the launch geometry.  Blocks of one pass over their rows for up to 2048
-// of them (a decode batch: as many loads as possible at once), beyond that
-// blocks of four tokens, whose threads make several passes and share the angles.
-inline dim3 geometry(Args& a, int vec) {
-  a.items = a.D / (2 * vec);
-  int lp_shift = 0;
-  while ((1 << lp_shift) < a.items && lp_shift < 6) ++lp_shift;
-  a.lp_shift = lp_shift;
-  const int64_t rows = a.src[0].heads + a.src[1].heads + a.src[2].heads;
-  const int64_t per_pass = THREADS >> lp_shift;
-  const int64_t split = (rows + per_pass - 1) / per_pass;
-  if (a.T * split <= 2048) {
-    a.tokens = 1;
-    return dim3((unsigned)a.T, (unsigned)split);
-  }
-  a.tokens = MAX_TOKENS;
-  return dim3((unsigned)((a.T + MAX_TOKENS - 1) / MAX_TOKENS), 1);
-}
 
 inline tb_status check_rotation(const char* what, int64_t T, int64_t Hq, int64_t Hk, int64_t D, int64_t R, int64_t A) {
   TB_CHECK_ARG(T >= 0 && T < (1ll << 31), "%s: bad number of tokens %lld", what, (long long)T);
@@ -336,7 +362,7 @@ extern "C" tb_status tb_rotary_axes(const void* q, void* q_out, const void* k, v
   a.interleaved = interleaved != 0;
   a.inverse = inverse != 0;
   const int64_t elem = dtype == F32 ? 4 : 2;
-  Width w;
+  Width w(elem);
   w.lengths(a.P, D);
   w.tensor(q, elem, q_st, q_sh, 0);
   w.tensor(q_out, elem, D, 0, 0);
@@ -344,10 +370,9 @@ extern "C" tb_status tb_rotary_axes(const void* q, void* q_out, const void* k, v
     w.tensor(k, elem, k_st, k_sh, 0);
     w.tensor(k_out, elem, D, 0, 0);
   }
-  const dim3 grid = geometry(a, w.vec);
-  if (dtype == F32) return launch_vec<F32, DENSE>(w.vec, a, grid, stream, what);
-  if (dtype == F16) return launch_vec<F16, DENSE>(w.vec, a, grid, stream, what);
-  return launch_vec<BF16, DENSE>(w.vec, a, grid, stream, what);
+  if (dtype == F32) return launch_vec<F32, DENSE>(w.vec, a, stream, what);
+  if (dtype == F16) return launch_vec<F16, DENSE>(w.vec, a, stream, what);
+  return launch_vec<BF16, DENSE>(w.vec, a, stream, what);
 }
 
 extern "C" tb_status tb_rope_kv_append(const void* q, const void* k, const void* v, void* q_out,
@@ -401,7 +426,7 @@ extern "C" tb_status tb_rope_kv_append(const void* q, const void* k, const void*
   a.A = (int)A;
   a.interleaved = interleaved != 0;
   const int64_t c_elem = cache_dtype == 3 ? 1 : 2;
-  Width w;
+  Width w(2);
   w.lengths(a.P, D);
   w.tensor(q, 2, q_st, q_sh, 0);
   w.tensor(k, 2, k_st, k_sh, 0);
@@ -409,10 +434,9 @@ extern "C" tb_status tb_rope_kv_append(const void* q, const void* k, const void*
   w.tensor(q_out, 2, D, 0, 0);
   w.tensor(k_cache, c_elem, c_page, c_head, c_slot);
   w.tensor(v_cache, c_elem, c_page, c_head, c_slot);
-  const dim3 grid = geometry(a, w.vec);
   if (cache_dtype == 3)
-    return dtype == F16 ? launch_vec<F16, CACHE_E4M3>(w.vec, a, grid, stream, what)
-                        : launch_vec<BF16, CACHE_E4M3>(w.vec, a, grid, stream, what);
-  return dtype == F16 ? launch_vec<F16, CACHE>(w.vec, a, grid, stream, what)
-                      : launch_vec<BF16, CACHE>(w.vec, a, grid, stream, what);
+    return dtype == F16 ? launch_vec<F16, CACHE_E4M3>(w.vec, a, stream, what)
+                        : launch_vec<BF16, CACHE_E4M3>(w.vec, a, stream, what);
+  return dtype == F16 ? launch_vec<F16, CACHE>(w.vec, a, stream, what)
+                      : launch_vec<BF16, CACHE>(w.vec, a, stream, what);
 }

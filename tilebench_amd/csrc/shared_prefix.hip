@@ -56,18 +56,6 @@ constexpr int FILL = 512;    // blocks that fill the device: two on each of 256 
 constexpr int MAX_SPLIT = 64;
 constexpr float NEG_INF = -__builtin_inff();
 
-// Division of n < 2^31 by a divisor that the host knows: n / d = (umulhi(n, mul) + n) >> shift.
-struct Divisor {
-  uint32_t d = 1, mul = 0, shift = 0;
-  Divisor() = default;
-  explicit Divisor(uint32_t by) : d(by) {
-    while ((1ull << shift) < by) ++shift;
-    mul = (uint32_t)((((1ull << shift) - by) << 32) / by + 1);
-  }
-  __device__ __forceinline__ int divide(int n) const { return (int)((__umulhi((uint32_t)n, mul) + (uint32_t)n) >> shift); }
-  __device__ __forceinline__ int rest(int n, int quotient) const { return n - quotient * (int)d; }
-};
-
 struct Args {
   const void* q;
   int64_t q_st, q_sh;
@@ -1882,8 +1870,8 @@ extern "C" tb_status tb_shared_prefix_attention(const void* q, const void* k_cac
   a.joint = p.joint;
   a.rounds = p.rounds;
   a.tile_fill = p.tile_fill;
-  a.by_grp = Divisor((uint32_t)a.grp);
-  a.by_heads = Divisor((uint32_t)Hkv);
+  a.by_grp = tb::Divisor((uint32_t)a.grp);
+  a.by_heads = tb::Divisor((uint32_t)Hkv);
   a.near = c_slot >= 0 && c_slot < (1 << 23);
   a.big = max_q * a.grp > FEW;
   a.tile_blocks = (int)p.tile_blocks;

@@ -112,4 +112,16 @@ __device__ __forceinline__ uint32_t bf16_bits(float f) {
   return (b + 0x7FFFu + ((b >> 16) & 1u)) >> 16;
 }
 
+// Division of n < 2^31 by a divisor that the host knows: n / d = (umulhi(n, mul) + n) >> shift.
+struct Divisor {
+  uint32_t d = 1, mul = 0, shift = 0;
+  Divisor() = default;
+  explicit Divisor(uint32_t by) : d(by) {
+    while ((1ull << shift) < by) ++shift;
+    mul = (uint32_t)((((1ull << shift) - by) << 32) / by + 1);
+  }
+  __device__ __forceinline__ int divide(int n) const { return (int)((__umulhi((uint32_t)n, mul) + (uint32_t)n) >> shift); }
+  __device__ __forceinline__ int rest(int n, int quotient) const { return n - quotient * (int)d; }
+};
+
 }  // namespace tb
