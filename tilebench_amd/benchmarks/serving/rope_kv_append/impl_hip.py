@@ -29,13 +29,13 @@ def check(q, k, v, positions, inv_freq, axes, slots, k_cache, v_cache, k_scale=N
     if k is None or v is None:
         raise ValueError(f"{op}: k and v are required")
     sizes = paged.check_rotation(op, q, k, positions, inv_freq, axes)
-    if q.dtype == torch.float32:
+    if q.dtype is torch.float32:
         raise TypeError(f"{op}: q, k and v must be float16 or bfloat16")
     if v.shape != k.shape:
         raise ValueError(f"{op}: k and v must have one shape")
-    if v.dtype != k.dtype or slots.dtype != torch.int32:
+    if v.dtype is not k.dtype or slots.dtype is not torch.int32:
         raise TypeError(f"{op}: v must have k's type and slots be int32")
-    if tuple(slots.shape) != (sizes[0],):
+    if slots.shape != q.shape[:1]:
         raise ValueError(f"{op}: slots must be one slot per token")
     return sizes + paged.check_cache(op, q.dtype, sizes[2], sizes[3], k_cache, v_cache, k_scale, v_scale)
 
@@ -47,7 +47,7 @@ def run(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tens
     rt.require_device(q, k, v, positions, inv_freq, axes, slots, k_cache, v_cache, k_scale, v_scale)
     T, Hq, Hkv, D, R, A, pages, page = check(q, k, v, positions, inv_freq, axes, slots, k_cache, v_cache, k_scale,
                                              v_scale)
-    q_out = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device)
+    q_out = paged.dense(q)
     q, k, v = paged.rows(q), paged.rows(k), paged.rows(v)
     positions, inv_freq, slots = positions.contiguous(), inv_freq.contiguous(), slots.contiguous()
     axes = None if axes is None else axes.contiguous()

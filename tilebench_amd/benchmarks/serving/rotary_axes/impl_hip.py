@@ -23,18 +23,19 @@ def run(q: torch.Tensor, k, positions: torch.Tensor, inv_freq: torch.Tensor, axe
     global _last_config
     rt.require_device(q, k, positions, inv_freq, axes)
     T, Hq, Hk, D, R, A = paged.check_rotation("rotary_axes", q, k, positions, inv_freq, axes)
-    q_out = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device)
+    q_out = paged.dense(q)
     k_out = None
     kst = ksh = 0
     q = paged.rows(q)
     if k is not None:
         k = paged.rows(k)
-        k_out = torch.empty((T, Hk, D), dtype=q.dtype, device=q.device)
-        kst, ksh = k.stride(0), k.stride(1)
+        k_out = paged.dense(k)
+        kst, ksh, _ = k.stride()
+    qst, qsh, _ = q.stride()
     positions, inv_freq = positions.contiguous(), inv_freq.contiguous()
     axes = None if axes is None else axes.contiguous()
     rt.call("tb_rotary_axes", q.data_ptr(), q_out.data_ptr(), rt.ptr(k), rt.ptr(k_out), positions.data_ptr(),
-            inv_freq.data_ptr(), rt.ptr(axes), T, Hq, Hk, D, R, A, q.stride(0), q.stride(1), kst, ksh,
+            inv_freq.data_ptr(), rt.ptr(axes), T, Hq, Hk, D, R, A, qst, qsh, kst, ksh,
             paged.DTYPES[q.dtype], interleaved, inverse, rt.stream_handle(q.device))
     _last_config = {"kernel": "rotate_heads", "block": 256}
     return (q_out, k_out)

@@ -19,6 +19,7 @@ Lengths, offsets and page ids stay on the device and are clamped there.  No
 counters, no state: the workspace is allocated per call.
 """
 import ctypes
+import functools
 
 import torch
 
@@ -30,39 +31,51 @@ rt.load_library()
 _last_config = None
 
 
+@functools.lru_cache(maxsize=1024)
+def workspace_bytes(*sizes) -> int:
+    """Bytes of workspace of a call of these sizes (tb_shared_prefix_attention_workspace_size's, in its order)."""
+    need = ctypes.c_int64(0)
+    rt.call("tb_shared_prefix_attention_workspace_size", *sizes, ctypes.byref(need))
+    return need.value
+
+
 def check(q, k_cache, v_cache, prefix_pages, prefix_lens, group_offsets, pages, lens, cu_q, max_q, scale=None,
           k_scale=None, v_scale=None):
     """The sizes of a call; raises TypeError or ValueError for what run refuses (no GPU needed)."""
     op = "shared_prefix_attention"
-    if q.dim() != 3:
+    shape = q.shape
+    if len(shape) != 3:
         raise ValueError(f"{op}: q must be [tokens, heads, head_dim]")
-    if q.dtype not in (torch.float16, torch.bfloat16):
+    if q.dtype is not torch.float16 and q.dtype is not torch.bfloat16:
         raise TypeError(f"{op}: q must be float16 or bfloat16")
-    T, Hq, D = q.shape
+    T, Hq, D = shape
     Hkv = k_cache.shape[1] if k_cache.dim() == 4 else 0
     n_pages, page = paged.check_cache(op, q.dtype, Hkv, D, k_cache, v_cache, k_scale, v_scale)
     if D not in (64, 128) or Hkv < 1 or Hq < 1 or Hq % Hkv:
         raise ValueError(f"{op}: need a head dimension of 64 or 128 and query heads that share the key/value heads "
                          f"(got {Hq} and {Hkv} heads of {D})")
-    size = k_cache.element_size()
-    if any(s * size % 16 for s in k_cache.stride()[:3]) or k_cache.data_ptr() % 16 or v_cache.data_ptr() % 16:
+    s_page, s_head, s_slot, _ = k_cache.stride()
+    if (s_page | s_head | s_slot) * k_cache.element_size() % 16 or (k_cache.data_ptr() | v_cache.data_ptr()) % 16:
         raise ValueError(f"{op}: the caches' rows must be 16-byte aligned")
-    tables = (prefix_pages, prefix_lens, group_offsets)
-    if any(t is None for t in tables) and any(t is not None for t in tables):
-        raise ValueError(f"{op}: prefix_pages, prefix_lens and group_offsets come together")
-    if any(t is not None and t.dtype != torch.int32 for t in (*tables, pages, lens, cu_q)):
+    if pages.dtype is not torch.int32 or lens.dtype is not torch.int32 or cu_q.dtype is not torch.int32:
         raise TypeError(f"{op}: page tables, lengths and offsets must be int32")
-    if pages.dim() != 2 or lens.dim() != 1 or lens.shape[0] != pages.shape[0] or cu_q.dim() != 1 \
-            or cu_q.shape[0] != pages.shape[0] + 1:
+    table = pages.shape
+    if len(table) != 2 or lens.shape != table[:1] or cu_q.dim() != 1 or cu_q.shape[0] != table[0] + 1:
         raise ValueError(f"{op}: pages must be [sequences, pages], lens [sequences], cu_q [sequences + 1]")
-    B, W = pages.shape
+    B, W = table
     G = Wp = 0
-    if prefix_pages is not None:
-        if prefix_pages.dim() != 2 or prefix_lens.dim() != 1 or group_offsets.dim() != 1 \
-                or prefix_lens.shape[0] != prefix_pages.shape[0] or group_offsets.shape[0] != prefix_pages.shape[0] + 1:
+    if prefix_pages is not None and prefix_lens is not None and group_offsets is not None:
+        if prefix_pages.dtype is not torch.int32 or prefix_lens.dtype is not torch.int32 \
+                or group_offsets.dtype is not torch.int32:
+            raise TypeError(f"{op}: page tables, lengths and offsets must be int32")
+        table = prefix_pages.shape
+        if len(table) != 2 or prefix_lens.shape != table[:1] or group_offsets.dim() != 1 \
+                or group_offsets.shape[0] != table[0] + 1:
             raise ValueError(f"{op}: prefix_pages must be [groups, pages], prefix_lens [groups], group_offsets "
                              "[groups + 1]")
-        G, Wp = prefix_pages.shape
+        G, Wp = table
+    elif prefix_pages is not None or prefix_lens is not None or group_offsets is not None:
+        raise ValueError(f"{op}: prefix_pages, prefix_lens and group_offsets come together")
     if (G == 0) != (Wp == 0) or (T > 0 and (B < 1 or W < 1)):
         raise ValueError(f"{op}: empty page tables")
     if max_q < 0:
@@ -79,28 +92,29 @@ def run(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, prefix_pa
     T, Hq, Hkv, D, G, Wp, B, W, n_pages, page = check(q, k_cache, v_cache, prefix_pages, prefix_lens, group_offsets,
                                                       pages, lens, cu_q, max_q, scale, k_scale, v_scale)
     q = paged.rows(q)
-    if q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
+    q_st, q_sh, _ = q.stride()
+    if q_st % 8 or q_sh % 8 or q.data_ptr() % 16:
         q = q.contiguous() if not q.is_contiguous() else q.clone()
+        q_st, q_sh, _ = q.stride()
     pages, lens, cu_q = pages.contiguous(), lens.contiguous(), cu_q.contiguous()
     if G:
         prefix_pages, prefix_lens = prefix_pages.contiguous(), prefix_lens.contiguous()
         group_offsets = group_offsets.contiguous()
     else:
         prefix_pages = prefix_lens = group_offsets = None
-    out = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device)
-    lse = torch.empty((T, Hq), dtype=torch.float32, device=q.device)
-    need = ctypes.c_int64(0)
-    rt.call("tb_shared_prefix_attention_workspace_size", T, Hq, Hkv, D, G, Wp, B, W, page, max_q,
-            paged.DTYPES[k_cache.dtype], ctypes.byref(need))
-    ws = torch.empty(need.value, dtype=torch.uint8, device=q.device) if need.value else None
+    out = paged.dense(q)
+    lse = q.new_empty((T, Hq), dtype=torch.float32)
+    cache_dtype = paged.DTYPES[k_cache.dtype]
+    need = workspace_bytes(T, Hq, Hkv, D, G, Wp, B, W, page, max_q, cache_dtype)
+    ws = q.new_empty(need, dtype=torch.uint8) if need else None
     cs = k_cache.stride()
     ss = (0, 0, 0) if k_scale is None else k_scale.stride()
     rt.call("tb_shared_prefix_attention", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), rt.ptr(k_scale),
             rt.ptr(v_scale), rt.ptr(prefix_pages), rt.ptr(prefix_lens), rt.ptr(group_offsets), pages.data_ptr(),
             lens.data_ptr(), cu_q.data_ptr(), out.data_ptr(), lse.data_ptr(), T, Hq, Hkv, D, G, Wp, B, W, max_q,
-            n_pages, page, q.stride(0), q.stride(1), cs[0], cs[1], cs[2], *ss, D ** -0.5 if scale is None else scale,
-            paged.DTYPES[q.dtype], paged.DTYPES[k_cache.dtype], rt.ptr(ws), need.value, rt.stream_handle(q.device))
-    _last_config = {"kernels": ["attend", "combine"] if need.value else ["attend_each"], "workspace_bytes": need.value}
+            n_pages, page, q_st, q_sh, cs[0], cs[1], cs[2], *ss, D ** -0.5 if scale is None else scale,
+            paged.DTYPES[q.dtype], cache_dtype, rt.ptr(ws), need, rt.stream_handle(q.device))
+    _last_config = {"kernels": ["attend", "combine"] if need else ["attend_each"], "workspace_bytes": need}
     return (out, lse)
 
 
