@@ -42,7 +42,8 @@ def reference(x):
 def check(got, x, ref=None):
     """Results against fp64.  A weight is rounded to the type (u, half a step) and so is the output; scores are sums
     of D products in fp32 (D + 8 roundings of sum |q k|), exp2 and the sum over n tokens add n + 16 more;
-    fp16 weights below the normals add 2^-33 of the largest each, with e4m3 values 2^-29 of a code (448 at most)."""
+    fp16 weights (with e4m3 values: weight times scale) below the normals add 2^-25 each where the largest is at least
+    2^8, so 2^-33 of the largest value a token."""
     q, kc = x[0], x[1]
     out, lse = got[0].detach().cpu().double(), got[1].detach().cpu().double()
     want, want_lse, mean = ref if ref is not None else reference(x)
@@ -57,7 +58,8 @@ def check(got, x, ref=None):
     e = 2.0 ** -24 * ((D + 8) * qk * (x[10] or D ** -0.5) + n + 16)
     small = 0.0
     if q.dtype == torch.float16:
-        small = n * 2.0 ** -29 * 448 if len(x) > 11 else n * 2.0 ** -33 * float(x[2].float().nan_to_num(0, 0, 0).abs().max())
+        v = x[2].float() * x[12][..., None] if len(x) > 11 else x[2].float()
+        small = n * 2.0 ** -33 * float(v.nan_to_num(0, 0, 0).abs().max())
     bound = 1.01 * (u * (want.abs() + mean) + 2 * e * mean) + small + 2.0 ** -25
     finite = want.isfinite()
     assert torch.equal(out.isnan(), want.isnan()), "NaN in other places"

@@ -209,6 +209,40 @@ def test_append_special_rows(gpu):
                 assert (i, t, h) in bad or b[t, h].isfinite().all()
 
 
+def test_codes_are_rounded_as_by_division(gpu):
+    """Rows of every magnitude: scale absmax / 448, codes x / scale, both rounded once; v is stored as it is."""
+    _say("append codes")
+    x = list(T.generate_rope_kv_append_inputs(221, 1, 4, 4, 128, 16, "e4m3", dtype=torch.bfloat16, seed=3, device="cpu"))
+    v = x[2].float() * 2.0 ** torch.arange(-120, 101).float()[:, None, None]
+    x[2] = v.to(torch.bfloat16)
+    out = _append(x, gpu)
+    v, slots = x[2].float(), x[6].long()
+    s = v.abs().amax(dim=-1) / 448.0
+    code = (v / s[..., None]).to(torch.float8_e4m3fn)
+    at = (slots // 16, slice(None), slots % 16)
+    assert torch.equal(out[4].cpu()[at], s)
+    assert torch.equal(out[2].cpu().view(torch.uint8)[at], code.view(torch.uint8))
+
+
+def test_more_tokens_than_a_launch_has_wavefronts(gpu):
+    """The tokens past 2^25 come in a second launch."""
+    _say("rotary of 2^25 tokens")
+    from tilebench_amd.benchmarks.serving.rotary_axes import impl_hip
+
+    n = (1 << 25) + 5
+    q = torch.randn(n, 1, 2, device=gpu, dtype=torch.float16)
+    pos = torch.arange(n, device=gpu, dtype=torch.int32)
+    f = torch.tensor([0.37])
+    out, _ = impl_hip.run(q, None, pos, f.to(gpu))
+    torch.cuda.synchronize()
+    for a in (0, n // 2, (1 << 25) - 7):
+        part = slice(a, a + 12)
+        _close(out[part], definition(q[part].cpu(), pos[part].cpu()[None], f, None, False), q[part], torch.float16)
+    # a rotation keeps lengths: two roundings to fp16 (2^-11 of each channel) and the angle's 2^-20
+    a, b = q.double().norm(dim=-1), out.double().norm(dim=-1)
+    assert bool(((a - b).abs() <= 2.0 ** -10 * a + 2.0 ** -20).all())
+
+
 def test_append_past_4_gib_of_cache(gpu):
     """Offsets of more than 32 bits: rows at the end of a pool of 5 GiB a side."""
     _say("append 64-bit offsets")

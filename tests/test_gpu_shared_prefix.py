@@ -104,6 +104,21 @@ def test_splits_of_long_prefixes_and_scales(gpu):
             check(got, x)
 
 
+# value scales from those of values around 1e-4 to those of values around 1e4, alone and mixed within a sequence
+@pytest.mark.parametrize("low, high", [(-14, -14), (-7, -7), (12, 12), (-14, 12)])
+@pytest.mark.parametrize("kw", [
+    dict(n_q=[1, 2], lens=[200, 70], prefix=[500]), dict(n_q=[1, 2], lens=[900, 70], prefix=[1100], D=128),
+    dict(n_q=ONES, lens=[300] * 40, prefix=[900], D=128), dict(n_q=[90, 3], lens=[800, 20], prefix=[30])],
+    ids=["joint", "few", "tile", "chunk"])
+def test_value_scales_of_any_size(gpu, kw, low, high):
+    for dtype in (F16, BF16):
+        _say("value scales", kw, low, high, dtype)
+        x = make(**kw, cache="e4m3", dtype=dtype, seed=low + 20)
+        g = torch.Generator().manual_seed(high)
+        x[12] *= 2.0 ** torch.randint(low, high + 1, x[12].shape, generator=g)
+        check(_run(x, gpu), x)
+
+
 @pytest.mark.parametrize("kw", [
     dict(n_q=[1, 1], lens=[20, 70], prefix=[40]), dict(n_q=[1, 2], lens=[20, 70], prefix=[1100]), dict(n_q=ONES, lens=[20] * 40, prefix=[90], D=128),
     dict(n_q=[70, 3], lens=[80, 20], prefix=[30], D=128), dict(n_q=[4, 2, 1], lens=[40, 3, 9])],
@@ -212,6 +227,28 @@ def test_past_4_gib_of_cache(gpu):
     got = impl_hip.run(*y)
     torch.cuda.synchronize()
     check(got, x)
+
+
+def test_more_rows_than_a_launch_has_wavefronts(gpu):
+    """17 million rows: the combining wavefronts take several each."""
+    _say("attention of 17 million rows")
+    from tilebench_amd.benchmarks.serving.shared_prefix_attention import impl_hip
+
+    B, Hq = 270001, 64
+    x = make([1] * 50, [1 + i % 3 for i in range(50)], prefix=[40], Hq=Hq, Hkv=8, page=16, seed=17)
+    y = _to(x, gpu)
+    rows = torch.arange(B, device=gpu) % 50
+    q = torch.randn(B, Hq, 64, device=gpu, dtype=F16)
+    y[0], y[5], y[6], y[7] = q, torch.tensor([0, B], device=gpu).int(), y[6][rows], y[7][rows]
+    y[8] = torch.arange(B + 1, device=gpu).int()
+    out, lse = impl_hip.run(*y)
+    torch.cuda.synchronize()
+    for at in (0, 131000, B - 50):
+        at = at // 50 * 50
+        z = list(x)
+        z[0] = q[at:at + 50].cpu()
+        check((out[at:at + 50], lse[at:at + 50]), z)
+    assert bool((lse[:, :] != 0).all()) and bool(out.isfinite().all())
 
 
 def test_replays_streams_and_overlapping_calls(gpu):

@@ -101,19 +101,20 @@ def test_entry_point_checks_before_touching_a_device():
         pytest.skip("libtbhip.so is not built")
     lib, fake = rt.load_library(), 1 << 40
     base = dict(q=fake, kc=fake, ks=None, pp=fake, cu=fake, T=8, Hq=8, Hkv=2, D=64, G=1, Wp=90, B=2, W=4, max_q=4, N=16,
-                P=16, q_st=512, c_slot=64, dtype=1, cache=1, ws=None, wb=0)
+                P=16, q_st=512, c_slot=64, scale=0.125, dtype=1, cache=1, ws=None, wb=0)
 
     def attend(**kw):
         a = {**base, **kw}
         return lib.tb_shared_prefix_attention(
             a["q"], a["kc"], fake, a["ks"], a["ks"], a["pp"], fake, fake, fake, fake, a["cu"], fake, fake, a["T"],
             a["Hq"], a["Hkv"], a["D"], a["G"], a["Wp"], a["B"], a["W"], a["max_q"], a["N"], a["P"], a["q_st"], 64, 2048,
-            1024, a["c_slot"], 0, 0, 0, 0.125, a["dtype"], a["cache"], a["ws"], a["wb"], None)
+            1024, a["c_slot"], 0, 0, 0, a["scale"], a["dtype"], a["cache"], a["ws"], a["wb"], None)
 
     for kw in (dict(T=-1), dict(Hq=7), dict(Hkv=0), dict(D=96), dict(P=12), dict(P=8192), dict(G=0), dict(Wp=0),
                dict(B=0), dict(W=0), dict(dtype=0), dict(cache=2), dict(cache=3), dict(ks=fake), dict(N=0),
                dict(N=1 << 30), dict(q=None), dict(pp=None), dict(cu=None), dict(q_st=510), dict(c_slot=60),
-               dict(T=1 << 30), dict(W=1 << 28), dict(max_q=-1)):
+               dict(T=1 << 30), dict(W=1 << 28), dict(max_q=-1), dict(T=1 << 61), dict(max_q=1 << 61), dict(B=1 << 61),
+               dict(scale=float("nan")), dict(scale=float("-inf")), dict(scale=1e39)):
         assert attend(**kw) == rt.TB_E_INVALID, kw
         assert "tb_shared_prefix_attention" in lib.tb_last_error().decode()
     assert attend(q=fake + 8) == rt.TB_E_ALIGN and attend(kc=fake + 8) == rt.TB_E_ALIGN

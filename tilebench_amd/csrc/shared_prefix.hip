@@ -14,10 +14,10 @@
 //   streams the own tokens of the sequences of up to 16 rows, laid end to end and
 //           shared out evenly to the wavefronts
 //   combine joins the partial results of a row (one slot per split) by their maxima
-// Short calls are done by a block for each sequence and head (attend_each).
-// so a prefix is read once per tile however many sequences share it.
+// so a prefix is read once per tile however many sequences share it.  Short calls
+// are done by a block for each sequence and head (attend_each).
 //
-// One wavefront's step over TOK tokens in LDS (attend_tile):
+// One wavefront's step over TOK tokens in LDS:
 //   S^T = K Q^T    K rows from LDS, Q in registers; a lane holds one row's scores
 //   P^T            exp2 of the scores against the running maximum, in registers; the
 //                  tokens a lane holds are in the order of the next product's operand
@@ -288,10 +288,9 @@ struct Wave {
   static constexpr int REGS = SH * SH / 64; // accumulator registers of a tile
 
   // log2 of the largest weight when m is set, and how far weights may grow past it before m is set again.  fp16:
-  // weights down to 2^-32 (e4m3: 2^-28) of the largest are kept; with e4m3 values their scales are multiplied in, which leaves
-  // room for scales up to 2^10 (a row of fp16 values has at most 146).
-  static constexpr float LIFT = DT == BF16 ? 0.0f : SC ? 4.0f : 8.0f;
-  static constexpr float SLACK = DT == BF16 || !SC ? 6.0f : 2.0f;
+  // weights down to 2^-32 of the largest are kept.  With scales the operand is weight * scale of the value, so in fp16
+  // it is that product's bound, the largest scale times the largest weight, which m keeps in range.
+  static constexpr float LIFT = DT == BF16 ? 0.0f : 8.0f, SLACK = 6.0f;
 
   v8 q[STEPS];
   acc_t o[DT_N];
@@ -411,6 +410,25 @@ struct Wave {
 #pragma unroll
       for (int r = 0; r < REGS; ++r) top = fmaxf(top, s[t][r]);
     top = over_groups_max(top) * scale;
+    if (SC && DT == F16) {
+      acc_t v[TOK / SH];
+#pragma unroll
+      for (int t = 0; t < TOK / SH; ++t)
+#pragma unroll
+        for (int r = 0; r < REGS; r += 4) {
+          const f32x4 x = lds_read<f32x4>(scale_at(sbase, tok0 + t * SH + token_of(r, g)) + 128);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[t][r + i] = x[i];
+        }
+      if (!full) hide<TOK>(v, limit - t0 - 4 * g, 0.0f);
+      float most = 0.0f;
+#pragma unroll
+      for (int t = 0; t < TOK / SH; ++t)
+#pragma unroll
+        for (int r = 0; r < REGS; ++r) most = fmaxf(most, fabsf(v[t][r]));
+      most = fminf(fmaxf(over_groups_max(most), 0x1p-60f), 0x1p60f);  // the sums of weights / scale stay finite
+      top += __builtin_amdgcn_logf(most);
+    }
     if (__any(top > m + (LIFT + SLACK))) {
       const float ref = fmaxf(m, top - LIFT);
       const float alpha = __builtin_amdgcn_exp2f(m - (ref == NEG_INF ? 0.0f : ref));
@@ -846,11 +864,11 @@ __device__ __forceinline__ void attend_few(const Args& a, char* smem, const FewT
                                   [](int) { return true; });
 }
 
-// Outputs of queries t0 .. t1 - 1 that attend to nothing.
+// Outputs of queries t0 .. t1 - 1 that attend to nothing, every step-th one.
 template <int DT, int D>
-__device__ __forceinline__ void empty_rows(const Args& a, int h, int t0, int t1) {
-  for (int t = t0; t < t1; ++t) {
-    const int64_t id = (int64_t)t * a.Hq + h * a.grp;
+__device__ __forceinline__ void empty_rows(const Args& a, int h, int t0, int t1, int step) {
+  for (int64_t t = t0; t < t1; t += step) {
+    const int64_t id = t * a.Hq + h * a.grp;
     for (int i = threadIdx.x; i < a.grp * D; i += THREADS) ((typename Ty<DT>::el*)a.out)[id * D + i] = 0;
     for (int i = threadIdx.x; i < a.grp; i += THREADS) a.lse[id + i] = NEG_INF;
   }
@@ -864,11 +882,10 @@ __global__ void __launch_bounds__(THREADS, 2) attend_each(Args a) {
   const int b = a.by_heads.divide((int)blockIdx.x);
   FewTask f;
   f.h = a.by_heads.rest((int)blockIdx.x, b);
-  if (b == 0) {  // rows of no sequence
-    const int first = query_start(a, 0);
-    empty_rows<DT, D>(a, f.h, 0, first);
-    empty_rows<DT, D>(a, f.h, max(query_start(a, a.B), first), a.T);
-  }
+  // rows of no sequence, dealt out to the blocks
+  const int first = query_start(a, 0), end = max(query_start(a, a.B), first);
+  if (b < first) empty_rows<DT, D>(a, f.h, b, first, a.B);
+  if (b < a.T - end) empty_rows<DT, D>(a, f.h, end + b, a.T, a.B);
   const Seq s = sequence(a, b);
   f.q0 = s.q0;
   f.n_q = s.n_q;
@@ -885,7 +902,7 @@ __global__ void __launch_bounds__(THREADS, 2) attend_each(Args a) {
     f.prefix = Tokens{a.prefix_pages + (int64_t)lo * a.Wp, a.Wp, prefix_length(a, lo)};
   }
   if (f.rows > FEW)  // more queries than max_q announced: nothing was planned for them
-    empty_rows<DT, D>(a, f.h, f.q0, f.q0 + s.n_q);
+    empty_rows<DT, D>(a, f.h, f.q0, f.q0 + s.n_q, 1);
   else if (f.rows > 0)
     attend_few<DT, E8, D>(a, smem, f, arg_word);
 }
@@ -953,6 +970,7 @@ __device__ __forceinline__ void stream_rows(const Args& a, char* smem, int index
     const int want = mine * per;
     int seen = 0;
     for (;; x0 += 64) {
+      if (x0 >= a.B) return;  // not with lengths that stay as they are during the call
       if (a.B > 64) count(x0 + lane);
       int incl = steps * a.Hkv;
 #pragma unroll
@@ -1000,6 +1018,10 @@ __device__ __forceinline__ void stream_rows(const Args& a, char* smem, int index
         at = 0;
         x0 += 64;
         count(x0 + lane);
+        if (x0 >= a.B) {  // not with lengths that stay as they are during the call
+          left = 0;
+          return;
+        }
       }
       const unsigned long long some = __ballot(steps > 0) >> at;
       if (some) {
@@ -1722,7 +1744,8 @@ tb_status launch(Args& a, const Plan& p, hipStream_t stream, const char* what) {
   hipLaunchKernelGGL((attend<DT, E8, D, RW>), dim3((unsigned)(p.tile_blocks + p.stream_blocks)), dim3(THREADS), lds, stream,
                      a);
   if (tb_status s = launch_status(what)) return s;
-  const int64_t rows = (int64_t)a.T * a.Hq, run = a.big && rows >= 32768 ? 16 : 1;
+  const int64_t rows = (int64_t)a.T * a.Hq, most = WAVES << 22;  // a launch holds 2^32 threads
+  const int64_t run = rows > most ? 64 : a.big && rows >= 32768 ? 16 : 1;
   if (p.many)  // 69 slots: 8.0 us by wavefronts, 5.0 by blocks
     hipLaunchKernelGGL((combine_many<DT, D>), dim3((unsigned)rows), dim3(THREADS), 0, stream, a);
   else
@@ -1762,8 +1785,8 @@ tb_status check_sizes(const char* what, int64_t T, int64_t Hq, int64_t Hkv, int6
   TB_CHECK_ARG((Wp == 0) == (G == 0), "%s: %lld groups with page tables of %lld", what, (long long)G, (long long)Wp);
   const int64_t most = (1ll << 31) - 1;
   // row, token and block numbers are 32-bit in the kernels
-  TB_CHECK_ARG(T * Hq <= most && B * Hkv <= most / MAX_SPLIT / 4 && G * Hkv <= most / MAX_SPLIT / 4 && W <= most / 2 / page_size &&
-                   Wp <= most / 2 / page_size && max_q * Hq <= most,
+  TB_CHECK_ARG(T <= most && Hq <= most && B <= most && G <= most && max_q <= most && T * Hq <= most && B * Hkv <= most / MAX_SPLIT / 4 && G * Hkv <= most / MAX_SPLIT / 4 && W <= most / 4 / page_size &&
+                   Wp <= most / 4 / page_size && max_q * Hq <= most,
                "%s: sizes past 2^31", what);
   TB_CHECK_ARG(B == 0 || W == 0 || Hkv * B <= (1ll << 30) / ceil_div(W * page_size, 32), "%s: sizes past 2^31", what);
   return TB_OK;
@@ -1802,7 +1825,7 @@ extern "C" tb_status tb_shared_prefix_attention(const void* q, const void* k_cac
                cache_dtype, dtype);
   TB_CHECK_ARG((cache_dtype == 3) == (k_scale != nullptr) && (cache_dtype == 3) == (v_scale != nullptr),
                "%s: scales belong to e4m3 caches, and only to them", what);
-  TB_CHECK_ARG(scale - scale == 0.0, "%s: the scale must be finite", what);
+  TB_CHECK_ARG(fabs(scale) < 1e38, "%s: the scale must be finite (in 32 bits)", what);
   TB_CHECK_ARG(n_pages >= 1 && n_pages <= ((1ll << 31) - 1) / page_size, "%s: bad number of pages %lld", what,
                (long long)n_pages);
   if (T == 0) return TB_OK;
