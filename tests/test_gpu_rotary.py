@@ -210,17 +210,17 @@ def test_append_special_rows(gpu):
 
 
 def test_codes_are_rounded_as_by_division(gpu):
-    """Rows of every magnitude: scale absmax / 448, codes x / scale, both rounded once; v is stored as it is."""
+    """Rows of every magnitude: the scale absmax / 448 and the codes x * 448 / absmax, each rounded from 64 bits."""
     _say("append codes")
     x = list(T.generate_rope_kv_append_inputs(221, 1, 4, 4, 128, 16, "e4m3", dtype=torch.bfloat16, seed=3, device="cpu"))
     v = x[2].float() * 2.0 ** torch.arange(-120, 101).float()[:, None, None]
     x[2] = v.to(torch.bfloat16)
     out = _append(x, gpu)
     v, slots = x[2].float(), x[6].long()
-    s = v.abs().amax(dim=-1) / 448.0
-    code = (v / s[..., None]).to(torch.float8_e4m3fn)
+    s = v.double().abs().amax(dim=-1) / 448.0
+    code = (v / s[..., None]).float().to(torch.float8_e4m3fn)
     at = (slots // 16, slice(None), slots % 16)
-    assert torch.equal(out[4].cpu()[at], s)
+    assert torch.equal(out[4].cpu()[at], s.float())
     assert torch.equal(out[2].cpu().view(torch.uint8)[at], code.view(torch.uint8))
 
 

@@ -9,9 +9,9 @@
 // negated angle, so the gradient is the same kernel with the sine negated.
 //
 // Angles.  A 32-bit product loses 2^-24 of the angle: 4e-3 rad at position
-// 65536, more than an fp16 ulp of the result.  The product and its reduction
-// to [-1/2, 1/2] turns are done in 64 bits, sine and cosine of the reduced angle
-// in 32 (1 ulp).  They depend on (token, pair) only: a wavefront computes its
+// 65536, more than an fp16 ulp of the result.  The product, its reduction and sine
+// and cosine are done in 64 bits, which cost what 32 bits do here, and rounded to
+// 32.  They depend on (token, pair) only: a wavefront computes its
 // token's once into LDS and its lanes read them there for 8 rows of 128.
 //
 // Layout of the work.  A head is D / (2 VEC) items of 2 VEC elements, one item a
@@ -33,8 +33,9 @@
 // us (5.5 TB/s), 4096 into an 8-bit cache 18.8 us (4.9 TB/s), one token 3.4 us.
 //
 // 8-bit cache rows: s = absmax / 448 over the fp32 values (rotated, never
-// rounded to 16 bits before), code = e4m3(x / s), both IEEE; a row of zeros
-// stores s = 0 and codes 0; a row with inf or NaN reads back as NaN.
+// rounded to 16 bits before), code = e4m3(x / s) with s before it is rounded to 32
+// bits to be stored; a row of zeros stores s = 0 and codes 0; a row with inf or
+// NaN reads back as NaN.
 #include "tb_common.h"
 
 namespace tb {
@@ -99,20 +100,33 @@ struct alignas(VEC * sizeof(E) < 16 ? VEC * sizeof(E) : 16) Chunk {
   E e[VEC];
 };
 
-// cos and sin of position * frequency: the turns and their nearest whole number in 64 bits.
+// cos and sin of position * frequency, in 64 bits: the nearest whole turn and quarter turn are taken off, which is
+// exact, and the Taylor series are summed over the rest, |angle| <= pi / 4 (x^13 / 13! < 2^-37 is left out).
 __device__ __forceinline__ float2 cos_sin(int pos, float freq, bool inverse) {
-  const double turns = (double)pos * (double)freq * 0.15915494309189533577;
-  const float x = (float)(2.0 * (turns - __builtin_rint(turns)));
-  float s, c;
-  sincospif(x, &s, &c);
-  return float2{c, inverse ? -s : s};
+  double turns = (double)pos * (double)freq * 0.15915494309189533577;
+  turns -= __builtin_rint(turns);
+  const double quarter = __builtin_rint(4.0 * turns);
+  const double x = __builtin_fma(4.0, turns, -quarter) * 1.57079632679489661923, z = x * x;
+  double s = -1.0 / 39916800.0, c = -1.0 / 3628800.0;
+  s = __builtin_fma(s, z, 1.0 / 362880.0);
+  c = __builtin_fma(c, z, 1.0 / 40320.0);
+  s = __builtin_fma(s, z, -1.0 / 5040.0);
+  c = __builtin_fma(c, z, -1.0 / 720.0);
+  s = __builtin_fma(s, z, 1.0 / 120.0);
+  c = __builtin_fma(c, z, 1.0 / 24.0);
+  s = __builtin_fma(s, z, -1.0 / 6.0);
+  c = __builtin_fma(c, z, -0.5);
+  const float sine = (float)__builtin_fma(s * z, x, x), cosine = (float)__builtin_fma(c, z, 1.0);
+  const int n = (int)quarter;
+  const float u = n & 1 ? sine : cosine, v = n & 1 ? cosine : sine;
+  return float2{(n + 1) & 2 ? -u : u, ((n & 2) != 0) != inverse ? -v : v};
 }
 
-// x / s rounded as the division is, for s in [2^-60, 2^60]: the product with s's rounded reciprocal, corrected once by
-// the exact remainder (3 operations instead of the division's 10).
-__device__ __forceinline__ float quotient(float x, float s, float inv) {
+// x / (s + rest) rounded to 32 bits, for s in [2^-60, 2^60] with the rounded reciprocal inv: the product with that,
+// corrected once by the exact remainder (4 operations; a division takes 10).
+__device__ __forceinline__ float quotient(float x, float s, float rest, float inv) {
   const float q = x * inv;
-  return __builtin_fmaf(__builtin_fmaf(-q, s, x), inv, q);
+  return __builtin_fmaf(__builtin_fmaf(-q, rest, __builtin_fmaf(-q, s, x)), inv, q);
 }
 
 // e4m3 codes of N (1 or a multiple of 4) values.
@@ -226,21 +240,22 @@ __global__ void __launch_bounds__(THREADS) rotate_heads(Args a) {
       const float s = __builtin_bit_cast(float, m) / 448.0f;
       if (kept && item == 0) (is_v ? a.scale[1] : a.scale[0])[page * a.sp + head * a.sh + within * a.ss] = s;
       if (s >= 0x1p-60f && s <= 0x1p60f) {
-        const float inv = 1.0f / s;
+        const float rest = __builtin_fmaf(-448.0f, s, __builtin_bit_cast(float, m)) / 448.0f, inv = 1.0f / s;
 #pragma unroll
         for (int i = 0; i < PASSES; ++i)
 #pragma unroll
           for (int e = 0; e < VEC; ++e) {
-            y1[i][e] = quotient(y1[i][e], s, inv);
-            y2[i][e] = quotient(y2[i][e], s, inv);
+            y1[i][e] = quotient(y1[i][e], s, rest, inv);
+            y2[i][e] = quotient(y2[i][e], s, rest, inv);
           }
-      } else {
+      } else {  // out of that range: zeros, infinities, NaN and what is near them
+        const double d = (double)__builtin_bit_cast(float, m) / 448.0;
 #pragma unroll
         for (int i = 0; i < PASSES; ++i)
 #pragma unroll
           for (int e = 0; e < VEC; ++e) {
-            y1[i][e] = m == 0 ? 0.0f : y1[i][e] / s;
-            y2[i][e] = m == 0 ? 0.0f : y2[i][e] / s;
+            y1[i][e] = m == 0 ? 0.0f : (float)((double)y1[i][e] / d);
+            y2[i][e] = m == 0 ? 0.0f : (float)((double)y2[i][e] / d);
           }
       }
       uint8_t* dst = (uint8_t*)(is_v ? a.out[2] : a.out[1]) + at;
