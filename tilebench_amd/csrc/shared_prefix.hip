@@ -1709,6 +1709,7 @@ inline Plan make_plan(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t G, 
     p.each_blocks = B * Hkv;
     return p;
   }
+  int64_t tiles = 0;  // blocks of them that run at once
   if (Wp > 0 || big) {
     // a group's rows padded to tiles, those of 64 counted 5 / 4 (they read each token twice as often)
     const int64_t each = ceil_div(rows, groups);
@@ -1716,13 +1717,16 @@ inline Plan make_plan(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t G, 
     const int64_t tile = 32 * p.row_waves, units = ceil_div(rows, tile) * Hkv;
     const int64_t tokens = (Wp + (big ? W : 0)) * page, cuts = ceil_div(tokens, 256);
     p.rounds = units >= FILL;
-    // where there is much else to read, tiles leave every CU's second place to it
-    p.tile_fill = !big && B * W > groups * Wp ? FILL / 2 : FILL;
+    // Where there is more to read of own tokens than of prefixes by all tiles, tiles leave every CU's second place to
+    // the streams (64 decodes of up to 1024 own tokens behind 32768: 76 us, else 81); where less, they take both places
+    // (96 sequences of up to 1400 own tokens in four groups of up to 15689: 124 us, else 139).
+    p.tile_fill = !big && B * W * Hkv >= units * Wp ? FILL / 2 : FILL;
     // partial results of up to 512 MB where only a last round of tiles is split
     const int64_t room = (512 << 20) / (T * Hq * (D * 4 + 8));
     p.S1 = (int)between(cuts, 1, p.rounds ? between(room, 1, 8) : MAX_SPLIT);
     if (groups == 1 && !p.rounds) p.S1 = (int)between(p.tile_fill / between(units, 1, FILL), 1, p.S1);
     p.tile_blocks = (rows / tile + groups) * Hkv + FILL;
+    tiles = p.rounds ? FILL : between(units * p.S1, 1, p.tile_fill);
     p.many = p.tile_fill / units > 24 && T * Hq <= 16384;
   }
   // A sequence falls to at most S2 - 1 full streams and one more; S2 up to 64, as far as 512 MB of partial results go.
@@ -1730,7 +1734,11 @@ inline Plan make_plan(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t G, 
   const int64_t slots = between((512 << 20) / (T * Hq * (D * 4 + 8)), 4, MAX_SPLIT);
   p.stream_least = (int)ceil_div(most, slots - 1);
   p.S2 = (int)(ceil_div(most, p.stream_least) + 1);
-  p.stream_blocks = between(ceil_div(B * Hkv * most, WAVES * p.stream_least), 1, p.S1 > 0 && !p.rounds ? FILL / 2 : FILL);
+  // Streams fill the device after tiles that do so (those four groups: 118 us, with half as many 124), or beside few
+  // tiles most of it (64 decodes of 1024 to 4096 own tokens behind 1000: 130 us, with FILL / 2 152); beside as many
+  // tiles as they are, all run at once (64 decodes of up to 1024 behind 8192: 41 us, with FILL 44).
+  const int64_t fill = tiles > FILL / 2 || tiles == 0 ? FILL : tiles <= FILL / 4 ? FILL * 3 / 4 : FILL / 2;
+  p.stream_blocks = between(ceil_div(B * Hkv * most, WAVES * p.stream_least), 1, fill);
   p.bytes = (int64_t)(p.S1 + p.S2) * T * Hq * (D * 4 + 8) + 2 * T * Hq * 4;
   return p;
 }
