@@ -30,12 +30,13 @@
 // items take 80, 95 and 124 us (before that change); four tokens to a block and
 // a loop over their heads 83 us; 8-byte accesses 96 us.  4800 tokens of 16 + 16
 // bf16 heads of 80 take 11.9 us (4.1 TB/s), 7001 tokens into a bf16 cache 31.4
-// us (5.5 TB/s), 4096 into an 8-bit cache 18.8 us (4.9 TB/s), one token 3.4 us.
+// us (5.5 TB/s), 4096 into an 8-bit cache 21.3 us (4.3 TB/s), one token 3.5 us.
 //
-// 8-bit cache rows: s = absmax / 448 over the fp32 values (rotated, never
-// rounded to 16 bits before), code = e4m3(x / s) with s before it is rounded to 32
-// bits to be stored; a row of zeros stores s = 0 and codes 0; a row with inf or
-// NaN reads back as NaN.
+// 8-bit cache rows: s = absmax / 448 and code = e4m3(x / s), rotated, compared and
+// divided in 64 bits, the scale rounded to 32 bits and the quotient to 32 and then
+// to 8: in 32 bits a few quotients in a million fall on the other side of a
+// border between codes (4096 tokens: 19.0 us, in 64 bits 21.3).  A row of zeros
+// stores s = 0 and codes 0; a row with inf or NaN reads back as NaN.
 #include "tb_common.h"
 
 namespace tb {
@@ -58,7 +59,10 @@ template <>
 struct Elem<F16> {
   typedef _Float16 type;
   static __device__ __forceinline__ float up(_Float16 x) { return (float)x; }
-  static __device__ __forceinline__ _Float16 down(float x) { return (_Float16)x; }
+  static __device__ __forceinline__ _Float16 down(float x) {
+    asm("" : "+v"(x));  // or single values would be rounded once, within the product (v_fma_mixlo_f16), and wide ones twice
+    return (_Float16)x;
+  }
 };
 template <>
 struct Elem<BF16> {
@@ -102,7 +106,7 @@ struct alignas(VEC * sizeof(E) < 16 ? VEC * sizeof(E) : 16) Chunk {
 
 // cos and sin of position * frequency, in 64 bits: the nearest whole turn and quarter turn are taken off, which is
 // exact, and the Taylor series are summed over the rest, |angle| <= pi / 4 (x^13 / 13! < 2^-37 is left out).
-__device__ __forceinline__ float2 cos_sin(int pos, float freq, bool inverse) {
+__device__ __forceinline__ double2 cos_sin(int pos, float freq, bool inverse) {
   double turns = (double)pos * (double)freq * 0.15915494309189533577;
   turns -= __builtin_rint(turns);
   const double quarter = __builtin_rint(4.0 * turns);
@@ -116,31 +120,40 @@ __device__ __forceinline__ float2 cos_sin(int pos, float freq, bool inverse) {
   c = __builtin_fma(c, z, 1.0 / 24.0);
   s = __builtin_fma(s, z, -1.0 / 6.0);
   c = __builtin_fma(c, z, -0.5);
-  const float sine = (float)__builtin_fma(s * z, x, x), cosine = (float)__builtin_fma(c, z, 1.0);
+  const double sine = __builtin_fma(s * z, x, x), cosine = __builtin_fma(c, z, 1.0);
   const int n = (int)quarter;
-  const float u = n & 1 ? sine : cosine, v = n & 1 ? cosine : sine;
-  return float2{(n + 1) & 2 ? -u : u, ((n & 2) != 0) != inverse ? -v : v};
+  const double u = n & 1 ? sine : cosine, v = n & 1 ? cosine : sine;
+  return double2{(n + 1) & 2 ? -u : u, ((n & 2) != 0) != inverse ? -v : v};
 }
 
-// x / (s + rest) rounded to 32 bits, for s in [2^-60, 2^60] with the rounded reciprocal inv: the product with that,
-// corrected once by the exact remainder (4 operations; a division takes 10).
-__device__ __forceinline__ float quotient(float x, float s, float rest, float inv) {
-  const float q = x * inv;
-  return __builtin_fmaf(__builtin_fmaf(-q, rest, __builtin_fmaf(-q, s, x)), inv, q);
+__device__ __forceinline__ uint32_t upper(double x) {
+  return (uint32_t)(__builtin_bit_cast(uint64_t, x) >> 32) & 0x7FFFFFFFu;
 }
 
-// e4m3 codes of N (1 or a multiple of 4) values.
+// e4m3 codes of N (1 or a multiple of 4) values x * inv.
 template <int N>
-__device__ __forceinline__ void codes(const float* x, uint8_t* c) {
-  if (N == 1) {
-    c[0] = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[0], 0.0f, 0, false);
-    return;
-  }
+__device__ __forceinline__ void codes(const double* x, double inv, uint8_t* c) {
+  float y[N < 4 ? 4 : N] = {};
+#pragma unroll
+  for (int e = 0; e < N; ++e) y[e] = (float)(x[e] * inv);
 #pragma unroll
   for (int e = 0; e < N; e += 4) {
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(x[e], x[e + (N > 1)], 0, false);
-    w = __builtin_amdgcn_cvt_pk_fp8_f32(x[e + 2 * (N > 1)], x[e + 3 * (N > 1)], w, true);
-    __builtin_memcpy(c + e, &w, 4);
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[e], y[e + 1], 0, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(y[e + 2], y[e + 3], w, true);
+    __builtin_memcpy(c + e, &w, N < 4 ? N : 4);
+  }
+}
+
+// The pairs of an item, (x1[e], x2[e]) or neighbours within its 2 N elements, by the angles of its N pairs.
+template <int N, bool INTER, typename F, typename CosSin>
+__device__ __forceinline__ void rotate(F (&x1)[N], F (&x2)[N], const CosSin* cs) {
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    F& u = INTER && N > 1 ? (2 * e < N ? x1[(2 * e) % N] : x2[(2 * e) % N]) : x1[e];
+    F& v = INTER && N > 1 ? (2 * e < N ? x1[(2 * e + 1) % N] : x2[(2 * e + 1) % N]) : x2[e];
+    const F p = u, q = v;
+    u = fma(p, cs[e].x, -(q * cs[e].y));  // written out, so that all widths round alike
+    v = fma(q, cs[e].x, p * cs[e].y);
   }
 }
 
@@ -150,13 +163,15 @@ __global__ void __launch_bounds__(THREADS) rotate_heads(Args a) {
   typedef typename E::type T;
   typedef Chunk<T, VEC> C;
   constexpr int PASSES = VEC == 1 ? MAX_D / 128 : 1;  // items of a lane
-  __shared__ float2 all_trig[WAVES][MAX_D / 2];
+  // cosines and sines of the block's wavefronts; 8-bit caches have them in 64 bits too
+  extern __shared__ __align__(16) char smem[];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const uint32_t portion = blockIdx.x * WAVES + wave, token = (uint32_t)a.by_portions.divide((int)portion);
   const int64_t t = a.t0 + token;
   if (t >= a.end) return;  // no barrier follows
-  float2* const trig = all_trig[wave];
+  float2* const trig = (float2*)smem + wave * a.P;
+  double2* const fine = (double2*)(smem + WAVES * a.P * sizeof(float2)) + wave * a.P;
   const int n = (int)(portion - token * (uint32_t)a.portions) * 64 + lane;
   const int row = a.by_lanes.divide(n), item = n - row * a.lanes;
   const bool is_k = row >= a.src[0].heads, is_v = MODE != DENSE && row >= a.src[0].heads + a.src[1].heads;
@@ -193,95 +208,78 @@ __global__ void __launch_bounds__(THREADS) rotate_heads(Args a) {
     const bool mine = i < a.P, more = i >= 64;
     const int ax = more && mine && a.axes ? a.axes[i] : axis;
     const int pos = __shfl(place, min(max(ax, 0), a.A - 1));
-    if (mine) trig[i] = cos_sin(pos, more ? a.inv_freq[i] : freq, a.inverse);
+    if (mine) {
+      const double2 cs = cos_sin(pos, more ? a.inv_freq[i] : freq, a.inverse);
+      trig[i] = float2{(float)cs.x, (float)cs.y};
+      if (MODE == CACHE_E4M3) fine[i] = cs;
+    }
     if (i - lane + 64 >= a.P) break;
   }
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 
-  float y1[PASSES][VEC], y2[PASSES][VEC];
+  // where a row of the caches goes (a padded token: nowhere)
+  const bool kept = in && (MODE == DENSE || !is_k || (slot >= 0 && slot < a.n_slots));
+  const int64_t page = slot >> a.page_shift, within = slot & ((1 << a.page_shift) - 1);
+  if (MODE == CACHE_E4M3 && is_k) {
+    double y1[PASSES][VEC], y2[PASSES][VEC], most = 0.0;
+    uint32_t top = 0;  // the largest magnitude's upper half: NaN above inf above every number
 #pragma unroll
-  for (int i = 0; i < PASSES; ++i) {
-    const int j = item + i * 64;
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      y1[i][e] = MODE != CACHE_E4M3 || j < a.items ? E::up(x1[i].e[e]) : 0.0f;  // nothing in the row's maximum
-      y2[i][e] = MODE != CACHE_E4M3 || j < a.items ? E::up(x2[i].e[e]) : 0.0f;
-    }
-    if (in && !is_v && j * VEC < a.P) {
-      const float2* cs = trig + j * VEC;
+    for (int i = 0; i < PASSES; ++i) {
+      const int j = item + i * 64;
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        // pairs (x1[e], x2[e]), or neighbours within the 2 VEC elements
-        float& u = INTER && VEC > 1 ? (2 * e < VEC ? y1[i][(2 * e) % VEC] : y2[i][(2 * e) % VEC]) : y1[i][e];
-        float& v = INTER && VEC > 1 ? (2 * e < VEC ? y1[i][(2 * e + 1) % VEC] : y2[i][(2 * e + 1) % VEC]) : y2[i][e];
-        const float p = u, q = v;
-        u = p * cs[e].x - q * cs[e].y;
-        v = q * cs[e].x + p * cs[e].y;
+        y1[i][e] = j < a.items ? E::up(x1[i].e[e]) : 0.0f;
+        y2[i][e] = j < a.items ? E::up(x2[i].e[e]) : 0.0f;
+      }
+      if (!is_v && j * VEC < a.P) rotate<VEC, INTER>(y1[i], y2[i], fine + j * VEC);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        most = fmax(most, fmax(fabs(y1[i][e]), fabs(y2[i][e])));
+        top = max(top, max(upper(y1[i][e]), upper(y2[i][e])));
       }
     }
-  }
-  int64_t at = (t * (is_k ? a.src[1].heads : a.src[0].heads) + head) * a.D;
-  bool kept = in;
-  if (MODE != DENSE && is_k) {
-    kept = in && slot >= 0 && slot < a.n_slots;  // a padded token: nothing is written
-    const int64_t page = slot >> a.page_shift, within = slot & ((1 << a.page_shift) - 1);
-    at = page * a.cp + head * a.ch + within * a.cs;
-    if (MODE == CACHE_E4M3) {
-      // the largest magnitude as bits: NaN above inf above every number
-      uint32_t m = 0;
-#pragma unroll
-      for (int i = 0; i < PASSES; ++i)
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          m = max(m, __builtin_bit_cast(uint32_t, y1[i][e]) & 0x7FFFFFFFu);
-          m = max(m, __builtin_bit_cast(uint32_t, y2[i][e]) & 0x7FFFFFFFu);
-        }
-      for (int d = a.lanes >> 1; d > 0; d >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d));
-      const float s = __builtin_bit_cast(float, m) / 448.0f;
-      if (kept && item == 0) (is_v ? a.scale[1] : a.scale[0])[page * a.sp + head * a.sh + within * a.ss] = s;
-      if (s >= 0x1p-60f && s <= 0x1p60f) {
-        const float rest = __builtin_fmaf(-448.0f, s, __builtin_bit_cast(float, m)) / 448.0f, inv = 1.0f / s;
-#pragma unroll
-        for (int i = 0; i < PASSES; ++i)
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            y1[i][e] = quotient(y1[i][e], s, rest, inv);
-            y2[i][e] = quotient(y2[i][e], s, rest, inv);
-          }
-      } else {  // out of that range: zeros, infinities, NaN and what is near them
-        const double d = (double)__builtin_bit_cast(float, m) / 448.0;
-#pragma unroll
-        for (int i = 0; i < PASSES; ++i)
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            y1[i][e] = m == 0 ? 0.0f : (float)((double)y1[i][e] / d);
-            y2[i][e] = m == 0 ? 0.0f : (float)((double)y2[i][e] / d);
-          }
-      }
-      uint8_t* dst = (uint8_t*)(is_v ? a.out[2] : a.out[1]) + at;
-#pragma unroll
-      for (int i = 0; i < PASSES; ++i) {
-        const int j = item + i * 64;
-        if (!kept || j >= a.items) continue;
-        Chunk<uint8_t, VEC> c1, c2;
-        codes<VEC>(y1[i], c1.e);
-        codes<VEC>(y2[i], c2.e);
-        *(Chunk<uint8_t, VEC>*)(dst + offset1(j)) = c1;
-        *(Chunk<uint8_t, VEC>*)(dst + offset2(j)) = c2;
-      }
-      return;
+    for (int d = a.lanes >> 1; d > 0; d >>= 1) {
+      most = fmax(most, __shfl_xor(most, d));
+      top = max(top, (uint32_t)__shfl_xor((int)top, d));
     }
+    if (!kept) return;
+    if (top >= 0x7FF00000u) most = top > 0x7FF00000u ? __builtin_nan("") : __builtin_inf();
+    const double inv = most == 0.0 ? 0.0 : 448.0 / most;
+    if (item == 0)
+      (is_v ? a.scale[1] : a.scale[0])[page * a.sp + head * a.sh + within * a.ss] = (float)(most * (1.0 / 448.0));
+    uint8_t* dst = (uint8_t*)(is_v ? a.out[2] : a.out[1]) + page * a.cp + head * a.ch + within * a.cs;
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+      const int j = item + i * 64;
+      if (j >= a.items) continue;
+      Chunk<uint8_t, VEC> c1, c2;
+      codes<VEC>(y1[i], inv, c1.e);
+      codes<VEC>(y2[i], inv, c2.e);
+      *(Chunk<uint8_t, VEC>*)(dst + offset1(j)) = c1;
+      *(Chunk<uint8_t, VEC>*)(dst + offset2(j)) = c2;
+    }
+    return;
   }
+  if (!kept) return;
+  const int64_t at = MODE != DENSE && is_k ? page * a.cp + head * a.ch + within * a.cs
+                                           : (t * (is_k ? a.src[1].heads : a.src[0].heads) + head) * a.D;
   T* dst = (T*)(is_v ? a.out[2] : is_k ? a.out[1] : a.out[0]) + at;
 #pragma unroll
   for (int i = 0; i < PASSES; ++i) {
     const int j = item + i * 64;
-    if (!kept || j >= a.items) continue;
+    if (j >= a.items) continue;
+    float y1[VEC], y2[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      y1[e] = E::up(x1[i].e[e]);
+      y2[e] = E::up(x2[i].e[e]);
+    }
+    if (!is_v && j * VEC < a.P) rotate<VEC, INTER>(y1, y2, trig + j * VEC);
     C c1, c2;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
-      c1.e[e] = E::down(y1[i][e]);
-      c2.e[e] = E::down(y2[i][e]);
+      c1.e[e] = E::down(y1[e]);
+      c2.e[e] = E::down(y2[e]);
     }
     *(C*)(dst + offset1(j)) = c1;
     *(C*)(dst + offset2(j)) = c2;
@@ -298,15 +296,16 @@ tb_status launch(Args& a, hipStream_t stream, const char* what) {
   a.rows = a.src[0].heads + a.src[1].heads + a.src[2].heads;
   a.portions = (a.rows * a.lanes + 63) / 64;
   a.by_portions = Divisor((uint32_t)a.portions);
+  const size_t lds = WAVES * a.P * (sizeof(float2) + (MODE == CACHE_E4M3 ? sizeof(double2) : 0));
   const int64_t most = (1 << 25) / a.portions;  // tokens of a launch: it holds 2^32 threads
   for (a.t0 = 0; a.t0 < a.T; a.t0 += most) {
     const int64_t tokens = a.T - a.t0 < most ? a.T - a.t0 : most;
     a.end = a.t0 + tokens;
     const dim3 grid((unsigned)((tokens * a.portions + WAVES - 1) / WAVES));
     if (a.interleaved)
-      hipLaunchKernelGGL((rotate_heads<DT, VEC, MODE, true>), grid, dim3(THREADS), 0, stream, a);
+      hipLaunchKernelGGL((rotate_heads<DT, VEC, MODE, true>), grid, dim3(THREADS), lds, stream, a);
     else
-      hipLaunchKernelGGL((rotate_heads<DT, VEC, MODE, false>), grid, dim3(THREADS), 0, stream, a);
+      hipLaunchKernelGGL((rotate_heads<DT, VEC, MODE, false>), grid, dim3(THREADS), lds, stream, a);
     if (tb_status s = launch_status(what)) return s;
   }
   return TB_OK;
