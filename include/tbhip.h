@@ -455,8 +455,8 @@ tb_status tb_rotary_axes(const void* q, void* q_out, const void* k, void* k_out,
  *   [0, pages * page_size) write nothing; a slot named twice in one call holds
  *   an unspecified mix of both tokens.  q' goes to q_out, dense [T, Hq, D].
  *   dtype 1 = fp16, 2 = bf16; cache_dtype the same, or 3: e4m3 codes of
- *   x / s with s = absmax / 448 over the fp32 row (rotated, not rounded
- *   before), s in k_scale / v_scale fp32 [pages, Hkv, page_size] at strides
+ *   x / s with s = absmax / 448 over the row (rotated, in fp64), s rounded to
+ *   fp32 in k_scale / v_scale fp32 [pages, Hkv, page_size] at strides
  *   s_page, s_head, s_slot.  A zero row has s = 0 and zero codes; a row with
  *   inf or NaN reads back as NaN.
  * Requires page_size a power of two up to 4096, pages * page_size < 2^31, and
@@ -473,7 +473,8 @@ tb_status tb_rope_kv_append(const void* q, const void* k, const void* v, void* q
 
 /*
  * Paged attention of a batch whose sequences share prefixes by groups; a
- * prefix is read once for all rows of its group (128 at a time).
+ * prefix is read once for 64 or 128 rows of its group at a time (the query
+ * heads of a key/value head times the queries), own tokens once.
  *   q [T, Hq, D] (dtype 1 = fp16, 2 = bf16) at strides q_st, q_sh: the queries of
  *   sequence b are rows cu_q[b] .. cu_q[b + 1] - 1 (cu_q int32 [B + 1], at most
  *   max_q of a sequence).  Sequence b's tokens are the prefix of its group, then
@@ -488,13 +489,19 @@ tb_status tb_rope_kv_append(const void* q, const void* k, const void* v, void* q
  *   out [T, Hq, D] dense = softmax(scale * q k) v, lse fp32 [T, Hq] the natural
  *   logarithm of the sum.  Rows that see no token, and rows of no sequence, give
  *   0 and -inf.  Sums are fp32; the weights are rounded to `dtype` before the
- *   product with the values.
+ *   product with the values (with e4m3 caches, cache_dtype 3, after they are
+ *   multiplied by the values' scales, which may be of any size).  Tokens that a
+ *   row does not see leave no trace in it, whatever they hold.
  * Lengths, offsets and page ids are read on the device and clamped to the
  * tables and the pool, so malformed ones never address memory outside them.
  * Needs the workspace reported by tb_shared_prefix_attention_workspace_size
  * (16-byte aligned, no clearing, not shared by calls that overlap).
+ * A sequence with more than max_q queries gets results without its own tokens,
+ * or empty ones.  The same call gives the same bits each time.
  * Requires D 64 or 128, Hq a multiple of Hkv, page_size a power of two up to
- * 4096, 16-byte aligned q, caches and out, cache strides in multiples of 16
+ * 4096, a scale below 1e38 in magnitude (it may be 0 or negative), T * Hq and
+ * max_q * Hq below 2^31, B * Hkv and G * Hkv at most 2^23, tables of at most 2^29
+ * tokens a row, n_pages * page_size < 2^31, 16-byte aligned q, caches and out, cache strides in multiples of 16
  * bytes, q strides in multiples of 8.  No counterpart in the reference's
  * quantised operators.
  */
@@ -508,7 +515,8 @@ tb_status tb_shared_prefix_attention(const void* q, const void* k_cache, const v
                                      double scale, int dtype, int cache_dtype, void* workspace,
                                      int64_t workspace_bytes, hipStream_t stream);
 
-/* Workspace bytes tb_shared_prefix_attention needs for these sizes (0 if none). */
+/* Workspace bytes tb_shared_prefix_attention needs for these sizes (0 if none);
+ * cache_dtype as there. */
 tb_status tb_shared_prefix_attention_workspace_size(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t G,
                                                     int64_t Wp, int64_t B, int64_t W, int64_t page_size,
                                                     int64_t max_q, int cache_dtype, int64_t* bytes);

@@ -12,8 +12,8 @@ the caches (tilebench_amd.paged says how these are laid out; head dimension 64 o
 Group g holds the sequences group_offsets[g] .. group_offsets[g + 1] - 1 (int32
 [G + 1], from 0 to B); its prefix is prefix_lens[g] tokens (int32 [G]) on the pages
 prefix_pages[g] (int32 [G, Wp]).  Without prefixes the three are None.  scale
-defaults to D ** -0.5.  Rows that see no token, and rows of no sequence, give 0
-and -inf.
+defaults to D ** -0.5.  float8_e4m3fn caches come with k_scale and v_scale.  Rows
+that see no token, and rows of no sequence, give 0 and -inf.
 
 Lengths, offsets and page ids stay on the device and are clamped there.  No
 counters, no state: the workspace is allocated per call.
