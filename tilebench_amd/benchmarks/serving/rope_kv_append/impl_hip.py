@@ -57,7 +57,7 @@ def run(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tens
             inv_freq.data_ptr(), rt.ptr(axes), slots.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
             rt.ptr(k_scale), rt.ptr(v_scale), T, Hq, Hkv, D, R, A, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], pages,
             page, cs[0], cs[1], cs[2], *ss, paged.DTYPES[q.dtype], paged.DTYPES[k_cache.dtype], interleaved,
-            rt.stream_handle(q.device))
+            rt.stream_handle(q.get_device()))
     _last_config = {"kernel": "rotate_heads", "block": 256}
     return (q_out, k_cache, v_cache) if k_scale is None else (q_out, k_cache, v_cache, k_scale, v_scale)
 

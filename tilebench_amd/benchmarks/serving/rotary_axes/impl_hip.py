@@ -36,7 +36,7 @@ def run(q: torch.Tensor, k, positions: torch.Tensor, inv_freq: torch.Tensor, axe
     axes = None if axes is None else axes.contiguous()
     rt.call("tb_rotary_axes", q.data_ptr(), q_out.data_ptr(), rt.ptr(k), rt.ptr(k_out), positions.data_ptr(),
             inv_freq.data_ptr(), rt.ptr(axes), T, Hq, Hk, D, R, A, qst, qsh, kst, ksh,
-            paged.DTYPES[q.dtype], interleaved, inverse, rt.stream_handle(q.device))
+            paged.DTYPES[q.dtype], interleaved, inverse, rt.stream_handle(q.get_device()))
     _last_config = {"kernel": "rotate_heads", "block": 256}
     return (q_out, k_out)
 

@@ -113,7 +113,7 @@ def run(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, prefix_pa
             rt.ptr(v_scale), rt.ptr(prefix_pages), rt.ptr(prefix_lens), rt.ptr(group_offsets), pages.data_ptr(),
             lens.data_ptr(), cu_q.data_ptr(), out.data_ptr(), lse.data_ptr(), T, Hq, Hkv, D, G, Wp, B, W, max_q,
             n_pages, page, q_st, q_sh, cs[0], cs[1], cs[2], *ss, D ** -0.5 if scale is None else scale,
-            paged.DTYPES[q.dtype], cache_dtype, rt.ptr(ws), need, rt.stream_handle(q.device))
+            paged.DTYPES[q.dtype], cache_dtype, rt.ptr(ws), need, rt.stream_handle(q.get_device()))
     _last_config = {"kernels": ["attend", "combine"] if need else ["attend_each"], "workspace_bytes": need}
     return (out, lse)
 

@@ -146,30 +146,35 @@ def require_device(*tensors) -> None:
             raise HipBackendUnavailable(f"libtbhip.so is built for gfx950, the device is {arch!r}")
         _device_checked = True
     if tensors:
-        here = torch.cuda.current_device()
-        for i, t in enumerate(tensors):
+        here, tensor = torch._C._cuda_getDevice(), torch.Tensor
+        for t in tensors:
             # get_device() is the GPU's index, or -1 off the GPU; one call per
             # tensor (0.05 us) instead of building its torch.device (0.25 us)
-            if isinstance(t, torch.Tensor) and t.get_device() != here:
+            if isinstance(t, tensor) and t.get_device() != here:
+                i = next(i for i, x in enumerate(tensors) if x is t)
                 raise ValueError(f"hip backend: input {i} is on {t.device}, the kernels run on cuda:{here}")
 
 
 def stream_handle(device=None) -> int:
     """Raw hipStream_t of torch's current stream on `device` (whatever
-    torch.cuda.current_stream takes).  For the device of a GPU tensor it is asked
+    torch.cuda.current_stream takes).  For the device of a GPU tensor, or its number, it is asked
     for directly: torch.cuda.current_stream() builds a Stream object around it,
     1.9 of the 9.6 us a small call took on the host (0.2 us this way)."""
     import torch
 
-    if isinstance(device, torch.device) and device.type == "cuda" and device.index is not None:
-        return torch._C._cuda_getCurrentRawStream(device.index)
+    if type(device) is int:
+        return torch._C._cuda_getCurrentRawStream(device)
+    index = device.index if isinstance(device, torch.device) else None
+    if index is not None and device.type == "cuda":
+        return torch._C._cuda_getCurrentRawStream(index)
     return torch.cuda.current_stream(device).cuda_stream
 
 
 def call(name: str, *args) -> None:
     """Call an entry point with (already converted) arguments and check it."""
-    lib = load_library()
-    check(getattr(lib, name)(*args), name)
+    status = getattr(_lib or load_library(), name)(*args)
+    if status != TB_OK:
+        check(status, name)
 
 
 def ptr(t) -> int:
