@@ -30,13 +30,14 @@
 // items take 80, 95 and 124 us (before that change); four tokens to a block and
 // a loop over their heads 83 us; 8-byte accesses 96 us.  4800 tokens of 16 + 16
 // bf16 heads of 80 take 11.9 us (4.1 TB/s), 7001 tokens into a bf16 cache 31.4
-// us (5.5 TB/s), 4096 into an 8-bit cache 21.3 us (4.3 TB/s), one token 3.5 us.
+// us (5.5 TB/s), 4096 into an 8-bit cache 20.5 us (4.5 TB/s), one token 3.5 us.
 //
-// 8-bit cache rows: s = absmax / 448 and code = e4m3(x / s), rotated, compared and
-// divided in 64 bits, the scale rounded to 32 bits and the quotient to 32 and then
-// to 8: in 32 bits a few quotients in a million fall on the other side of a
-// border between codes (4096 tokens: 19.0 us, in 64 bits 21.3).  A row of zeros
-// stores s = 0 and codes 0; a row with inf or NaN reads back as NaN.
+// 8-bit cache rows: s = absmax / 448 and code = e4m3(x / s), as in 64 bits: the
+// scale is rounded to 32 bits, the quotient to 32 and then to 8.  Keys are rotated,
+// compared and divided in 64 bits; with 32 a few quotients in a million fall on the
+// other side of a border between codes (4096 tokens: 19.0 us, so 20.5, values in
+// 64 bits too 21.3).  A row of zeros stores s = 0 and codes 0; a row with inf or
+// NaN reads back as NaN.
 #include "tb_common.h"
 
 namespace tb {
@@ -130,12 +131,26 @@ __device__ __forceinline__ uint32_t upper(double x) {
   return (uint32_t)(__builtin_bit_cast(uint64_t, x) >> 32) & 0x7FFFFFFFu;
 }
 
-// e4m3 codes of N (1 or a multiple of 4) values x * inv.
-template <int N>
-__device__ __forceinline__ void codes(const double* x, double inv, uint8_t* c) {
+// x / (s + rest) rounded to 32 bits, for s in [2^-60, 2^60] with the rounded reciprocal inv: the product with that,
+// corrected once by the exact remainder.
+struct Reciprocal {
+  float s, rest, inv;
+  __device__ __forceinline__ float operator()(float x) const {
+    const float q = x * inv;
+    return fmaf(fmaf(-q, rest, fmaf(-q, s, x)), inv, q);
+  }
+};
+struct Reciprocal64 {
+  double inv;
+  __device__ __forceinline__ float operator()(double x) const { return (float)(x * inv); }
+};
+
+// e4m3 codes of N (1 or a multiple of 4) quotients.
+template <int N, typename F, typename Quotient>
+__device__ __forceinline__ void codes(const F* x, Quotient quotient, uint8_t* c) {
   float y[N < 4 ? 4 : N] = {};
 #pragma unroll
-  for (int e = 0; e < N; ++e) y[e] = (float)(x[e] * inv);
+  for (int e = 0; e < N; ++e) y[e] = quotient(x[e]);
 #pragma unroll
   for (int e = 0; e < N; e += 4) {
     int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[e], y[e + 1], 0, false);
@@ -220,6 +235,43 @@ __global__ void __launch_bounds__(THREADS) rotate_heads(Args a) {
   // where a row of the caches goes (a padded token: nowhere)
   const bool kept = in && (MODE == DENSE || !is_k || (slot >= 0 && slot < a.n_slots));
   const int64_t page = slot >> a.page_shift, within = slot & ((1 << a.page_shift) - 1);
+  if (MODE == CACHE_E4M3 && is_v) {  // values are not rotated: 32 bits hold them
+    float y1[PASSES][VEC], y2[PASSES][VEC];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        y1[i][e] = item + i * 64 < a.items ? E::up(x1[i].e[e]) : 0.0f;
+        y2[i][e] = item + i * 64 < a.items ? E::up(x2[i].e[e]) : 0.0f;
+        top = max(top, __builtin_bit_cast(uint32_t, y1[i][e]) & 0x7FFFFFFFu);
+        top = max(top, __builtin_bit_cast(uint32_t, y2[i][e]) & 0x7FFFFFFFu);
+      }
+    for (int d = a.lanes >> 1; d > 0; d >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
+    if (!kept) return;
+    const float most = __builtin_bit_cast(float, top), s = most / 448.0f;
+    const Reciprocal by{s, fmaf(-448.0f, s, most) / 448.0f, 1.0f / s};
+    const bool normal = s >= 0x1p-60f && s <= 0x1p60f;
+    const double inv = most == 0.0f ? 0.0 : 448.0 / (double)most;
+    if (item == 0) a.scale[1][page * a.sp + head * a.sh + within * a.ss] = s;
+    uint8_t* dst = (uint8_t*)a.out[2] + page * a.cp + head * a.ch + within * a.cs;
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+      const int j = item + i * 64;
+      if (j >= a.items) continue;
+      Chunk<uint8_t, VEC> c1, c2;
+      if (normal) {
+        codes<VEC>(y1[i], by, c1.e);
+        codes<VEC>(y2[i], by, c2.e);
+      } else {
+        codes<VEC>(y1[i], Reciprocal64{inv}, c1.e);
+        codes<VEC>(y2[i], Reciprocal64{inv}, c2.e);
+      }
+      *(Chunk<uint8_t, VEC>*)(dst + offset1(j)) = c1;
+      *(Chunk<uint8_t, VEC>*)(dst + offset2(j)) = c2;
+    }
+    return;
+  }
   if (MODE == CACHE_E4M3 && is_k) {
     double y1[PASSES][VEC], y2[PASSES][VEC], most = 0.0;
     uint32_t top = 0;  // the largest magnitude's upper half: NaN above inf above every number
@@ -231,7 +283,7 @@ __global__ void __launch_bounds__(THREADS) rotate_heads(Args a) {
         y1[i][e] = j < a.items ? E::up(x1[i].e[e]) : 0.0f;
         y2[i][e] = j < a.items ? E::up(x2[i].e[e]) : 0.0f;
       }
-      if (!is_v && j * VEC < a.P) rotate<VEC, INTER>(y1[i], y2[i], fine + j * VEC);
+      if (j * VEC < a.P) rotate<VEC, INTER>(y1[i], y2[i], fine + j * VEC);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
         most = fmax(most, fmax(fabs(y1[i][e]), fabs(y2[i][e])));
@@ -245,16 +297,15 @@ __global__ void __launch_bounds__(THREADS) rotate_heads(Args a) {
     if (!kept) return;
     if (top >= 0x7FF00000u) most = top > 0x7FF00000u ? __builtin_nan("") : __builtin_inf();
     const double inv = most == 0.0 ? 0.0 : 448.0 / most;
-    if (item == 0)
-      (is_v ? a.scale[1] : a.scale[0])[page * a.sp + head * a.sh + within * a.ss] = (float)(most * (1.0 / 448.0));
-    uint8_t* dst = (uint8_t*)(is_v ? a.out[2] : a.out[1]) + page * a.cp + head * a.ch + within * a.cs;
+    if (item == 0) a.scale[0][page * a.sp + head * a.sh + within * a.ss] = (float)(most * (1.0 / 448.0));
+    uint8_t* dst = (uint8_t*)a.out[1] + page * a.cp + head * a.ch + within * a.cs;
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
       const int j = item + i * 64;
       if (j >= a.items) continue;
       Chunk<uint8_t, VEC> c1, c2;
-      codes<VEC>(y1[i], inv, c1.e);
-      codes<VEC>(y2[i], inv, c2.e);
+      codes<VEC>(y1[i], Reciprocal64{inv}, c1.e);
+      codes<VEC>(y2[i], Reciprocal64{inv}, c2.e);
       *(Chunk<uint8_t, VEC>*)(dst + offset1(j)) = c1;
       *(Chunk<uint8_t, VEC>*)(dst + offset2(j)) = c2;
     }
