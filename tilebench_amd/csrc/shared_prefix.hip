@@ -192,25 +192,28 @@ __device__ __forceinline__ V lds_read(uint32_t addr) {
   return *(const __attribute__((address_space(3))) V*)(uintptr_t)addr;
 }
 
-// 16 (or 4) bytes a lane from global memory to LDS at lds + 16 (4) * lane.
+// 16 (or 4) bytes a lane from global memory to LDS at lds + 16 (4) * lane.  One wait state lies between a scalar write of
+// m0 and such a load, which would else find the m0 before it: the compiler keeps none within inline asm.
 __device__ __forceinline__ void dma16(uint32_t lds, const char* p) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
                :
                : "s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(p)
                : "memory", "m0");
 }
-// the same from a uniform address plus a 32-bit offset of each lane
+// the same from a uniform address plus a 32-bit offset of each lane.  The address is copied by a scalar instruction,
+// which is that wait state too: it may come from a vector one (readfirstlane), and five would lie between that and a load.
 __device__ __forceinline__ void dma16(uint32_t lds, const char* p, uint32_t off) {
   const uint64_t u = (uint64_t)(uintptr_t)p;
   const uint64_t base = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)u) |
                         (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(u >> 32)) << 32;
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2"
-               :
+  uint64_t at;
+  asm volatile("s_mov_b32 m0, %1\n\ts_mov_b64 %0, %3\n\tglobal_load_lds_dwordx4 %2, %0"
+               : "=&s"(at)
                : "s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(off), "s"(base)
                : "memory", "m0");
 }
 __device__ __forceinline__ void dma4(uint32_t lds, const char* p) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
                :
                : "s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(p)
                : "memory", "m0");
