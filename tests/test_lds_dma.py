@@ -82,16 +82,29 @@ def test_the_reader_sees_both_kinds():
     assert not offences([fresh[0], "s_add_u32 s3, s3, s5", fresh[2]])[1]
 
 
-@pytest.mark.parametrize("part", ["prefix"])
-def test_loads_to_lds_keep_their_distances(part, tmp_path):
+@pytest.fixture(scope="module")
+def kernels(tmp_path_factory):
+    """{kernel: (loads to LDS, [what is too close])} of the built library."""
     if not rt.LIB_PATH.exists() or not all(shutil.which(LLVM / t) for t in ("llvm-objcopy", "llvm-objdump")):
         pytest.skip("no built library or no LLVM tools")
-    loads, bad = 0, []
-    for path in code_objects(rt.LIB_PATH, tmp_path):
+    out = {}
+    for path in code_objects(rt.LIB_PATH, tmp_path_factory.mktemp("code")):
         text = subprocess.run([LLVM / "llvm-objdump", "-d", "--no-show-raw-insn", path], check=True, capture_output=True,
                               text=True).stdout
         for name, body in re.findall(r"^[0-9a-f]+ <(\S+)>:\n(.*?)(?=\n\n|\Z)", text, re.M | re.S):
-            if part in name:
-                n, b = offences(body.splitlines())
-                loads, bad = loads + n, bad + [f"{name}: {x}" for x in b]
-    assert loads > 0 and not bad, (len(bad), bad[:5])
+            if "_lds_" in body or " lds" in body:
+                out[name] = offences(body.splitlines())
+    return out
+
+
+@pytest.mark.parametrize("part", ["prefix", "fp8", "w4a16", "ntg"])
+def test_loads_to_lds_keep_their_distances(part, kernels):
+    some = {name: x for name, x in kernels.items() if part in name}
+    assert sum(loads for loads, _ in some.values()) > 0
+    bad = [f"{name}: {x}" for name, (_, b) in some.items() for x in b]
+    assert not bad, (len(bad), bad[:5])
+
+
+def test_every_kernel_with_such_loads_is_looked_at(kernels):
+    assert not [k for k, (loads, _) in kernels.items()
+                if loads and not any(part in k for part in ("prefix", "fp8", "w4a16", "ntg"))]

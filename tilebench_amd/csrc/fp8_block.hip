@@ -40,7 +40,6 @@
 namespace tb {
 namespace fp8blk {
 
-typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x2v __attribute__((ext_vector_type(2)));
@@ -79,24 +78,6 @@ __device__ __forceinline__ i32x4 make_rsrc4(const void* p, uint32_t bytes) {
   r[2] = __builtin_amdgcn_readfirstlane((int)bytes);
   r[3] = (int)RSRC_DW3;
   return r;
-}
-
-// DMAs into LDS at m0 (wave-uniform base; lane l lands at +16 l or +4 l), as
-// inline asm so that the compiler does not tie barriers to their completion;
-// the kernel waits for them (vmcnt) before the barrier that publishes them.
-__device__ __forceinline__ void dma16(uint32_t lds_addr, uint32_t voff, const i32x4& rsrc, uint32_t soff) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
-               :
-               : "s"(__builtin_amdgcn_readfirstlane((int)lds_addr)), "v"(voff), "s"(rsrc),
-                 "s"(__builtin_amdgcn_readfirstlane((int)soff))
-               : "memory", "m0");
-}
-__device__ __forceinline__ void dma4(uint32_t lds_addr, uint32_t voff, const i32x4& rsrc, uint32_t soff) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, %3 offen lds"
-               :
-               : "s"(__builtin_amdgcn_readfirstlane((int)lds_addr)), "v"(voff), "s"(rsrc),
-                 "s"(__builtin_amdgcn_readfirstlane((int)soff))
-               : "memory", "m0");
 }
 
 // Tiles in groups of 8 tile rows, column-major inside a group; with the tile

@@ -38,7 +38,6 @@ namespace tb {
 namespace fp8gemm {
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
-typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x2v __attribute__((ext_vector_type(2)));
 
@@ -84,27 +83,6 @@ __device__ __forceinline__ i32x4 make_rsrc4(const void* p, uint32_t bytes) {
   r[2] = __builtin_amdgcn_readfirstlane((int)bytes);
   r[3] = (int)RSRC_DW3;
   return r;
-}
-
-// One 16-byte-per-lane DMA into LDS at m0 (wave-uniform base, lane l -> +16 l).
-// Issued as inline asm so that the compiler does not tie the next barrier to
-// its completion; the kernel waits for it explicitly (vmcnt) before the
-// barrier that publishes the stage.
-__device__ __forceinline__ void dma16(uint32_t lds_addr, uint32_t voff, const i32x4& rsrc, uint32_t soff) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
-               :
-               : "s"(__builtin_amdgcn_readfirstlane((int)lds_addr)), "v"(voff), "s"(rsrc),
-                 "s"(__builtin_amdgcn_readfirstlane((int)soff))
-               : "memory", "m0");
-}
-
-// One 4-byte-per-lane DMA into LDS at m0 (lane l -> +4 l).
-__device__ __forceinline__ void dma4(uint32_t lds_addr, uint32_t voff, const i32x4& rsrc, uint32_t soff) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, %3 offen lds"
-               :
-               : "s"(__builtin_amdgcn_readfirstlane((int)lds_addr)), "v"(voff), "s"(rsrc),
-                 "s"(__builtin_amdgcn_readfirstlane((int)soff))
-               : "memory", "m0");
 }
 
 __global__ void __launch_bounds__(THREADS, 1)

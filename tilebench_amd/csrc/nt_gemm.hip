@@ -45,7 +45,6 @@
 namespace tb {
 namespace ntg {
 
-typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -69,17 +68,6 @@ __device__ __forceinline__ i32x4 make_rsrc4(const void* p, uint32_t bytes) {
   r[2] = __builtin_amdgcn_readfirstlane((int)bytes);
   r[3] = (int)RSRC_DW3;
   return r;
-}
-
-// One 16-byte-per-lane DMA into LDS (wave-uniform base, lane l -> +16 l), as
-// inline asm so the compiler does not tie barriers to its completion; the
-// kernel waits for it explicitly (vmcnt) before the barrier that publishes it.
-__device__ __forceinline__ void dma16(uint32_t lds_addr, uint32_t voff, const i32x4& rsrc, uint32_t soff) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
-               :
-               : "s"(__builtin_amdgcn_readfirstlane((int)lds_addr)), "v"(voff), "s"(rsrc),
-                 "s"(__builtin_amdgcn_readfirstlane((int)soff))
-               : "memory", "m0");
 }
 
 template <int BM, int BN>
@@ -921,7 +909,7 @@ extern "C" tb_status tb_matmul_int8(const int8_t* a, const uint8_t* b, int32_t* 
       return st;
     const int64_t n4 = M * N / 4;
     hipLaunchKernelGGL(reduce_planes_i32, dim3((unsigned)((n4 + 255) / 256)), dim3(256), 0, stream,
-                       reinterpret_cast<const i32x4*>(planes), reinterpret_cast<i32x4*>(out), n4, splits);
+                       reinterpret_cast<const tb::i32x4*>(planes), reinterpret_cast<tb::i32x4*>(out), n4, splits);
     return tb::launch_status("tb_matmul_int8(reduce)");
   }
   return launch_any<KIND_I8, OUT_I32>(reinterpret_cast<const uint8_t*>(a), reinterpret_cast<const uint8_t*>(bt), out, M,

@@ -11,7 +11,6 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 typedef __amdgpu_buffer_rsrc_t rsrc_t;
-typedef int i32x4 __attribute__((ext_vector_type(4)));
 constexpr uint32_t RSRC_DW3 = 0x00020000u;
 constexpr uint32_t OOB = 0x80000000u;
 __device__ __forceinline__ rsrc_t make_rsrc(const void* p, uint32_t bytes) {
@@ -118,20 +117,6 @@ __device__ __forceinline__ bool grouped_tile(const int* __restrict__ offsets, in
 
 typedef int v2i __attribute__((ext_vector_type(2)));
 
-__device__ __forceinline__ void dma16(uint32_t lds_addr, uint32_t voff, const i32x4& rsrc, uint32_t soff) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
-               :
-               : "s"(__builtin_amdgcn_readfirstlane((int)lds_addr)), "v"(voff), "s"(rsrc),
-                 "s"(__builtin_amdgcn_readfirstlane((int)soff))
-               : "memory", "m0");
-}
-__device__ __forceinline__ void dma4(uint32_t lds_addr, uint32_t voff, const i32x4& rsrc, uint32_t soff) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, %3 offen lds"
-               :
-               : "s"(__builtin_amdgcn_readfirstlane((int)lds_addr)), "v"(voff), "s"(rsrc),
-                 "s"(__builtin_amdgcn_readfirstlane((int)soff))
-               : "memory", "m0");
-}
 __device__ __forceinline__ i32x4 rsrc4(const void* p, uint32_t bytes) {
   const uint64_t base = (uint64_t)(uintptr_t)p;
   i32x4 r;
