@@ -210,6 +210,22 @@ def test_layouts_give_the_same_bits(gpu, cache):
     assert torch.equal(again[0], want[0]) and torch.equal(again[1], want[1])
 
 
+@pytest.mark.parametrize("T,Hq,Hkv", [(1, 8, 2), (1, 1, 1), (3, 1, 1)])
+def test_one_token_of_an_odd_projection(gpu, T, Hq, Hkv):
+    """Dimensions of size 1 keep odd strides in PyTorch's copies."""
+    _say("attention odd strides", T, Hq, Hkv)
+    from tilebench_amd.benchmarks.serving.shared_prefix_attention import impl_hip
+
+    x = _to(make([1] * T, [9] * T, prefix=[30], Hq=Hq, Hkv=Hkv, seed=12), gpu)
+    want = impl_hip.run(*x)
+    for shift, gap in ((0, 3), (3, 0), (3, 5)):
+        wide = torch.zeros(T + 1, Hq * 64 + shift + gap, dtype=F16, device=gpu)
+        q = wide[:, shift:shift + Hq * 64].view(T + 1, Hq, 64)[1:]
+        q.copy_(x[0])
+        got = impl_hip.run(q, *x[1:])
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 def test_past_4_gib_of_cache(gpu):
     """Pages at the end of a 6 GiB pool."""
     _say("attention 64-bit offsets")

@@ -7,6 +7,7 @@ import pytest
 import torch
 
 from tests.shared_prefix_cases import make, reference
+from tilebench_amd import paged
 from tilebench_amd import runtime as rt
 
 
@@ -131,3 +132,18 @@ def test_entry_point_checks_before_touching_a_device():
     # short prefixes: every sequence reads its own
     assert size(8, 8, 2, 64, 1, 4, 2, 4, 16, 4, 1, ctypes.byref(need)) == rt.TB_OK and need.value == 0
     assert size(8, 8, 2, 64, 1, 4, 2, 4, 16, 4, 1, None) == rt.TB_E_INVALID
+
+
+@pytest.mark.parametrize("tokens,heads", [(1, 8), (1, 1), (3, 1), (3, 8)])
+@pytest.mark.parametrize("shift,gap", [(0, 3), (3, 0), (8, 8), (3, 5)])
+def test_queries_of_any_layout_are_taken(tokens, heads, shift, gap):
+    """Slices of a wider projection, one token or one head of it among them, whose row stride PyTorch keeps in copies."""
+    wide = torch.randn(tokens + 1, heads * 64 + shift + gap, generator=torch.Generator().manual_seed(1)).half()
+    x = wide[:, shift:shift + heads * 64].view(tokens + 1, heads, 64)[1:]
+    y = paged.aligned_rows(x, 8)
+    assert torch.equal(y, x) and y.data_ptr() % 16 == 0 and y.stride(-1) == 1
+    assert all(s % 8 == 0 for s in y.stride()[:-1])
+    fine = x.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in x.stride()[:-1])
+    assert (y.data_ptr() == x.data_ptr()) == fine                           # copied only where it has to be
+    last = torch.empty(tokens, 64, heads).half().transpose(1, 2)            # the last dimension strided
+    assert paged.aligned_rows(last, 8).stride(-1) == 1

@@ -91,11 +91,8 @@ def run(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, prefix_pa
                       v_scale)
     T, Hq, Hkv, D, G, Wp, B, W, n_pages, page = check(q, k_cache, v_cache, prefix_pages, prefix_lens, group_offsets,
                                                       pages, lens, cu_q, max_q, scale, k_scale, v_scale)
-    q = paged.rows(q)
+    q = paged.aligned_rows(q, 8)
     q_st, q_sh, _ = q.stride()
-    if q_st % 8 or q_sh % 8 or q.data_ptr() % 16:
-        q = q.contiguous() if not q.is_contiguous() else q.clone()
-        q_st, q_sh, _ = q.stride()
     pages, lens, cu_q = pages.contiguous(), lens.contiguous(), cu_q.contiguous()
     if G:
         prefix_pages, prefix_lens = prefix_pages.contiguous(), prefix_lens.contiguous()

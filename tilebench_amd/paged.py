@@ -85,6 +85,15 @@ def rows(x):
     return x if x.stride(-1) == 1 else x.contiguous()
 
 
+def aligned_rows(x, step):
+    """x with its last dimension contiguous, rows that start on 16 bytes and strides in multiples of `step` elements."""
+    x = rows(x)
+    if any(s % step for s in x.stride()[:-1]) or x.data_ptr() % 16:
+        # dimensions of size 1 keep any stride in clone() and contiguous()
+        x = x.new_empty(x.shape).copy_(x)
+    return x
+
+
 def dense(x):
     """An empty dense tensor of x's shape, type and device."""
     return torch.empty_like(x, memory_format=torch.contiguous_format)
