@@ -516,7 +516,10 @@ tb_status tb_shared_prefix_attention(const void* q, const void* k_cache, const v
                                      int64_t workspace_bytes, hipStream_t stream);
 
 /* Workspace bytes tb_shared_prefix_attention needs for these sizes (0 if none);
- * cache_dtype as there. */
+ * cache_dtype as there.  At most 72 MiB and 16 bytes for each of the T * Hq rows,
+ * and 640 MiB, or five results (4 D + 8 bytes) if that is more, for the rows of
+ * sequences with up to 16 queries times Hq / Hkv (all rows if no sequence may have
+ * more, 16 B * Hkv at most otherwise). */
 tb_status tb_shared_prefix_attention_workspace_size(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t G,
                                                     int64_t Wp, int64_t B, int64_t W, int64_t page_size,
                                                     int64_t max_q, int cache_dtype, int64_t* bytes);

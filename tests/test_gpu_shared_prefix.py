@@ -80,6 +80,43 @@ def test_attention_matches_the_formula(gpu, name, dtype, cache):
     check(_run(x, gpu), x)
 
 
+# Calls whose partial results would take more than 512 MiB with slots for every row: only rows that need some have them.
+COMPACT = {
+    # rounds of whole tiles and a split last one; sequences of up to 16 rows among longer ones
+    "prompts": dict(n_q=[200] * 36 + [1, 2, 0, 1, 17, 3], lens=[200 + i for i in range(36)] + [50, 2, 9, 300, 40, 3],
+                    prefix=[300], Hq=64, Hkv=8, pad=3),
+    "prompts_groups": dict(n_q=[200] * 36 + [1, 2, 0, 1, 17, 3], lens=[200 + i for i in range(36)] + [50, 2, 9, 300, 40, 3],
+                           prefix=[300, 0, 120], bounds=[0, 10, 25, 42], Hq=64, Hkv=8, pad=3),
+    "prompts_alone": dict(n_q=[1, 2, 0, 1, 17, 3] + [200] * 36, lens=[50, 2, 9, 300, 40, 3] + [200 + i for i in range(36)],
+                          Hq=64, Hkv=8, pad=3),
+    "mixed": dict(n_q=[3 + 30 * (i % 40 == 0) for i in range(1430)], lens=[40 + i % 200 for i in range(1430)], prefix=[700],
+                  Hq=64, Hkv=8),
+    "decodes": dict(n_q=[1] * 1200, lens=[1 + i % 90 for i in range(1200)], prefix=[2100], Hq=64, Hkv=8, spare=400),
+    # fewer tiles, shared out by their steps: some are split and some are not
+    "tenants": dict(n_q=[2] * 150, lens=[2 + i % 90 for i in range(150)],
+                    prefix=[(17 * i) % 300 + 3000 * (i % 50 == 7) for i in range(150)], bounds=list(range(151)), Hq=32,
+                    Hkv=8, D=128, spare=1024),
+    "tenants_drafts": dict(n_q=[1 + 10 * (i % 2) for i in range(150)], lens=[11 + i % 90 for i in range(150)],
+                           prefix=[(17 * i) % 300 + 3000 * (i % 50 == 7) for i in range(150)], bounds=list(range(151)),
+                           Hq=32, Hkv=8, D=128, spare=1024),
+    "five_tenants": dict(n_q=[1] * 300, lens=[1 + i % 90 for i in range(300)], prefix=[900, 0, 3000, 20, 700],
+                         bounds=[0, 60, 100, 180, 181, 300], Hq=32, Hkv=8, D=128, spare=1024),
+    "one_tenant": dict(n_q=[1] * 500, lens=[1 + i % 90 for i in range(500)], prefix=[900], Hq=32, Hkv=8, D=128, spare=246),
+}
+
+
+@pytest.mark.parametrize("name,dtype,cache", [(name, F16, "same") for name in COMPACT] +
+                         [(name, BF16, "e4m3") for name in ("prompts", "tenants_drafts")])
+def test_slots_only_for_rows_that_need_them(gpu, name, dtype, cache):
+    _say("attention compact", name, dtype, cache)
+    kw = dict(COMPACT[name], dtype=dtype, cache=cache, seed=len(name))
+    x = make(**kw)
+    got = _run(x, gpu)
+    check(got, make(**dict(kw, spare=0)))  # the same call with tables as wide as they need to be
+    again = _run(x, gpu)
+    assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
+
+
 def test_splits_of_long_prefixes_and_scales(gpu):
     for seed, (scale, kw) in enumerate([
             (None, dict(n_q=[1] * 3, lens=[9, 700, 33], prefix=[20000], Hq=16, Hkv=2, D=128, page=64)),

@@ -147,3 +147,36 @@ def test_queries_of_any_layout_are_taken(tokens, heads, shift, gap):
     assert (y.data_ptr() == x.data_ptr()) == fine                           # copied only where it has to be
     last = torch.empty(tokens, 64, heads).half().transpose(1, 2)            # the last dimension strided
     assert paged.aligned_rows(last, 8).stride(-1) == 1
+
+
+MIB = 1 << 20
+
+
+@pytest.mark.parametrize("kw", [
+    dict(T=16384, Hq=64, Hkv=8, W=256, B=1, max_q=16384),                        # one long prompt
+    dict(T=131072, Hq=64, Hkv=8, W=2048, B=1, max_q=131072),
+    dict(T=8192, Hq=64, Hkv=8, W=64, B=16, max_q=512, G=1, Wp=94),               # prompts behind a cached one
+    dict(T=32768, Hq=64, Hkv=8, W=64, B=64, max_q=512, G=4, Wp=94),
+    dict(T=4385, Hq=32, Hkv=8, W=15, B=16, max_q=500, G=1, Wp=94),
+    dict(T=40000, Hq=32, Hkv=8, W=64, B=10000, max_q=4000, G=1, Wp=94),          # one prompt among many decodes
+    dict(T=300, Hq=32, Hkv=8, W=64, B=300, max_q=1, G=300, Wp=2048),             # a group for each sequence
+    dict(T=10000, Hq=32, Hkv=8, W=2048, B=10000, max_q=1, G=10000, Wp=2048),
+    dict(T=4096, Hq=64, Hkv=8, W=2048, B=4096, max_q=1, G=1, Wp=128),
+    dict(T=270001, Hq=64, Hkv=8, D=64, W=1, B=270001, max_q=1, G=1, Wp=3, page=16),
+])
+@pytest.mark.parametrize("cache", [1, 3])
+def test_workspaces_are_bounded(kw, cache):
+    """Results of what tiles split, five of every row that streams may work on or 640 MiB of them, 16 bytes a row."""
+    if not rt.LIB_PATH.exists():
+        pytest.skip("libtbhip.so is not built")
+    c = {**dict(D=128, G=0, Wp=0, page=64), **kw}
+    need = ctypes.c_int64(-1)
+    size = rt.load_library().tb_shared_prefix_attention_workspace_size
+    args = [c[k] for k in ("T", "Hq", "Hkv", "D", "G", "Wp", "B", "W", "page", "max_q")]
+    assert size(*args, cache, ctypes.byref(need)) == rt.TB_OK
+    rows, each = c["T"] * c["Hq"], c["D"] * 4 + 8
+    prompts = c["max_q"] * c["Hq"] // c["Hkv"] > 16   # then streams take sequences of up to 16 rows a key/value head
+    few = min(rows, c["B"] * c["Hkv"] * 16) if prompts else rows
+    assert 0 <= need.value <= max(5 * few * each, 640 * MIB) + 72 * MIB + 16 * rows, need.value / MIB
+    if few <= 16384:
+        assert need.value <= 512 * MIB

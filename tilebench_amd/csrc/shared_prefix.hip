@@ -65,6 +65,7 @@ constexpr int THREADS = 256, WAVES = 4;
 constexpr int FEW = 16;      // rows of a sequence that the token-splitting blocks take
 constexpr int FILL = 512;    // blocks that fill the device: two on each of 256 CUs
 constexpr int MAX_SPLIT = 64;
+constexpr int64_t PARTIALS = 512 << 20;  // bytes of partial results from which only rows that need them have some
 constexpr float NEG_INF = -__builtin_inff();
 
 struct Args {
@@ -84,10 +85,15 @@ struct Args {
   const int* cu_q;          // [B + 1]
   void* out;
   float* lse;
-  float* part_o;    // [T * Hq][S1 + S2 slots][D]: a row's partial outputs lie together
-  float2* part_ml;  // [T * Hq][S1 + S2]: maximum (log2) and sum
-  int* n_tile;      // [T * Hq]: slots 0 .. that the row's tiles used, -1 where its result is final
-  int* n_own;       // [T * Hq]: slots S1 .. that its own tokens used
+  float* part_o;    // [slots][D]: partial outputs, those of a row together (see Slots)
+  float2* part_ml;  // [slots]: maximum (log2) and sum
+  int* n_tile;      // [T * Hq]: slots that the row's tiles used, -1 where its result is final
+  int* n_own;       // [T * Hq]: slots that its own tokens used
+  int* tile_at;     // [T * Hq], compact: the first of the tiles' slots, -1 for the one beside the own tokens'
+  int* own_at;      // [T * Hq], compact: which of own_rows the row is
+  int compact, tile_slots, own_rows;
+  int direct_rows;  // own_rows are the rows of the call, else FEW for each sequence and key/value head
+  int own_first, own_stride;  // slots: own row n has its from own_first + n * own_stride on
   int T, Hq, Hkv, grp, G, Wp, B, W;
   Divisor by_grp, by_heads;  // grp, Hkv
   int n_pages, page_shift;
@@ -698,13 +704,20 @@ __device__ __forceinline__ void stash(const W& w, uint32_t outs, uint32_t stats,
     }
   if (g == 0) *(__attribute__((address_space(3))) f32x2*)(uintptr_t)(stats + part_row * 8) = f32x2{w.m, l};
 }
-// rows: how many; q0: query of row `first`.  big(r): its result is complete if the unit was not split.
+// Rows that sequence b's of key/value head h follow among own_rows, where these are FEW for each.
+__device__ __forceinline__ int64_t own_rows_before(const Args& a, int b, int h) { return ((int64_t)b * a.Hkv + h) * FEW; }
+// The first slot of own row `n`: S2 for its streams and, compact, one for a tile that was not split.
+__device__ __forceinline__ int64_t own_slot(const Args& a, int64_t n) { return a.own_first + n * a.own_stride; }
+
+// rows: how many; q0: query of row `first`.  own_row: the rows' places among own_rows, any + 4: the splits of the split
+// units before this one (both compact).  big(r): its result is complete if the unit was not split.
 template <typename W, int D, int ROWS, int PARTS, bool TILES, typename Big>
 __device__ __forceinline__ void finish(uint32_t args, uint32_t outs, uint32_t stats, uint32_t marks, uint32_t any,
-                                       int rows, int q0, int first, int h, int split, int splits, Big big) {
+                                       int rows, int q0, int first, int h, int split, int splits, uint32_t own_row,
+                                       Big big) {
   const Args a = saved_args(args);
   const bool marked = lds_read<int>(any) != 0;
-  const int slots = a.S1 + a.S2;
+  const int slots = a.S1 + a.S2, before = TILES ? lds_read<int>(any + 4) : 0;
   typedef typename W::Y::el el;
 #pragma unroll 4
   for (int i = threadIdx.x; i < rows * (D / 4); i += THREADS) {
@@ -731,15 +744,20 @@ __device__ __forceinline__ void finish(uint32_t args, uint32_t outs, uint32_t st
     const int qi = a.by_grp.divide(first + r);
     const int64_t id = (int64_t)(q0 + qi) * a.Hq + h * a.grp + a.by_grp.rest(first + r, qi);
     const bool own_here = !TILES || big(r), final = own_here && splits == 1;
+    int64_t slot = id * slots + split;
+    if (TILES && a.compact)
+      slot = splits > 1 ? before * ROWS + r * splits + split
+                        : own_slot(a, a.direct_rows ? id : lds_read<int>(own_row + 4 * r)) + a.S2;
     if (final)
       store4((el*)a.out + id * D + c * 4, x * inverse(ml[1]));
     else if (!(ml[1] == 0.0f))
-      *(f32x4*)(a.part_o + (id * slots + split) * D + c * 4) = x;
+      *(f32x4*)(a.part_o + slot * D + c * 4) = x;
     if (c == 0) {
       if (final) a.lse[id] = natural_lse(ml[0], ml[1]);
-      if (TILES && !final) a.part_ml[id * slots + split] = float2{ml[0], ml[1]};
+      if (TILES && !final) a.part_ml[slot] = float2{ml[0], ml[1]};
       if (TILES && split == 0) {
         a.n_tile[id] = final ? -1 : splits;
+        if (a.compact) a.tile_at[id] = splits > 1 ? before * ROWS + r * splits : -1;
         if (own_here) a.n_own[id] = 0;
       }
     }
@@ -874,7 +892,7 @@ __device__ __forceinline__ void attend_few(const Args& a, char* smem, const FewT
   const uint32_t outs = lds_addr(smem), stats = outs + L::STATS;
   stash<W, D>(w, outs, stats, wave * FEW + row);
   block_barrier();
-  finish<W, D, FEW, WAVES, false>(outs + L::ARGS, outs, stats, marks, outs + L::ANY, f.rows, f.q0, 0, h, 0, 1,
+  finish<W, D, FEW, WAVES, false>(outs + L::ARGS, outs, stats, marks, outs + L::ANY, f.rows, f.q0, 0, h, 0, 1, 0,
                                   [](int) { return true; });
 }
 
@@ -1085,6 +1103,11 @@ __device__ __forceinline__ void stream_rows(const Args& a, char* smem, int index
     w.init((const el*)a.q + (u.q0 + qi) * a.q_st + (u.h * a.grp + head) * a.q_sh, valid, a.flip, a.keep);
   };
 
+  // the unit's sequence, which only its results need
+  auto note = [&]() __attribute__((always_inline)) {
+    if (lane == 0) *(__attribute__((address_space(3))) int*)(uintptr_t)(any + 4) = x0 + at;
+  };
+  note();
   UnitOf u = unit_here(a);
   W w;
   queries(w, u);
@@ -1141,7 +1164,9 @@ __device__ __forceinline__ void stream_rows(const Args& a, char* smem, int index
       const bool marked = lds_read<int>(any) != 0;
       const int g = lane / SH, rows = u.n_q * b.grp;
       if (row < rows && rows <= FEW) {
-        const int64_t id = (int64_t)(u.q0 + qi) * b.Hq + u.h * b.grp + head, slot = id * (b.S1 + b.S2) + b.S1 + u.slot;
+        const int64_t id = (int64_t)(u.q0 + qi) * b.Hq + u.h * b.grp + head;
+        const int64_t own_row = b.direct_rows ? id : own_rows_before(b, lds_read<int>(any + 4), u.h) + row;
+        const int64_t slot = own_slot(b, own_row) + u.slot;
         if (!(l == 0.0f)) {
 #pragma unroll
           for (int d = 0; d < W::DT_N; ++d) {
@@ -1154,6 +1179,7 @@ __device__ __forceinline__ void stream_rows(const Args& a, char* smem, int index
         if (g == 0) {
           b.part_ml[slot] = float2{w.m, l};
           if (ends) b.n_own[id] = u.slot + 1;
+          if (ends && b.compact) b.own_at[id] = (int)own_row;
         }
       }
       if (rows > FEW)  // more queries than max_q announced: nothing was planned for them
@@ -1164,6 +1190,7 @@ __device__ __forceinline__ void stream_rows(const Args& a, char* smem, int index
       if (!more) return;
       if (marked) clear_marks();
       u = v;
+      note();
       w = next;
       set_limits();
     }
@@ -1184,7 +1211,7 @@ struct TileLayout {
   static constexpr int TILE_BYTES = TOK * RB;
   static constexpr int STAGE = 2 * TILE_BYTES + (E8 ? 2 * TOK * 4 : 0);
   static constexpr int MARKS = 2 * STAGE;
-  static constexpr int ROW_INFO = MARKS + ROWS * 64, STATS = ROW_INFO + ROWS * 12, ANY = STATS + WAVES * 32 * 8;
+  static constexpr int ROW_INFO = MARKS + ROWS * 64, STATS = ROW_INFO + ROWS * 16, ANY = STATS + WAVES * 32 * 8;
   static constexpr int ARGS = ANY + 16, LDS = ARGS + sizeof(Args);
   static_assert(MARKS >= WAVES * 32 * D * 4, "the outputs reuse the stages");
 };
@@ -1193,12 +1220,13 @@ struct TileLayout {
 // `units` units of `steps` steps (set by count(entry), an entry a lane, 64 at a time); a unit is cut into splits of
 // about the same number of steps, `fill` blocks in all at most (units beside: an entry's last split may be short), of
 // `least` steps at least and `most` splits at most.
+// before: if asked for (`number`), the splits of the units before this one that are split too.
 struct Unit {
-  int entry, lane, at, split, splits;
+  int entry, lane, at, split, splits, before;
 };
 template <typename Count>
-__device__ __forceinline__ bool share_out(int entries, int index, int fill, int least, int most, Unit& u, int& total,
-                                          Count count) {
+__device__ __forceinline__ bool share_out(int entries, int index, int fill, int least, int most, bool number,
+                                          Unit& u, int& total, Count count) {
   const int lane = threadIdx.x & 63;
   int units = 0, steps = 0;
   total = 0;
@@ -1220,7 +1248,7 @@ __device__ __forceinline__ bool share_out(int entries, int index, int fill, int 
   // steps of a split: sum of units * ceil(steps / share) <= sum of units * (steps / share + 1) <= fill
   const int room = max(fill - total, fill / 4);
   const float share = fmaxf(as_float(__builtin_amdgcn_readfirstlane(as_uint(all))) / (float)room, (float)least);
-  int seen = 0;
+  int seen = 0, split_before = 0;
   for (int x0 = 0; x0 < entries; x0 += 64) {
     if (entries > 64) count(x0 + lane, units, steps);
     int cuts = (int)ceilf((float)steps / share);
@@ -1236,6 +1264,15 @@ __device__ __forceinline__ bool share_out(int entries, int index, int fill, int 
       }
     }
     const int here = __builtin_amdgcn_readlane(incl, entries > 1 ? 63 : 0);
+    int split_incl = cuts > 1 ? n : 0;
+    const int split_n = split_incl;
+    if (number && entries > 1) {
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(split_incl, d);
+        if (lane >= d) split_incl += o;
+      }
+    }
     if (index < seen + here) {
       u.lane = entries > 1 ? __builtin_ctzll(__ballot(seen + incl > index)) : 0;
       const int at = index - seen - __builtin_amdgcn_readlane(incl - n, u.lane);
@@ -1244,9 +1281,11 @@ __device__ __forceinline__ bool share_out(int entries, int index, int fill, int 
       u.splits = __builtin_amdgcn_readlane(cuts, u.lane);
       u.split = (int)((uint32_t)at / (uint32_t)of);
       u.at = at - u.split * of;
+      u.before = split_before + __builtin_amdgcn_readlane(split_incl - split_n, u.lane) + u.at * u.splits;
       return true;
     }
     seen += here;
+    split_before += __builtin_amdgcn_readlane(split_incl, 63);
   }
   return false;
 }
@@ -1258,7 +1297,7 @@ __device__ __forceinline__ bool share_out(int entries, int index, int fill, int 
 // run on one XCD, whose L2 then holds the keys and values that they share.
 struct TileUnit {
   Group gr;
-  int g, tile, h, split, splits;
+  int g, tile, h, split, splits, before;
 };
 template <int ROWS, int TOK>
 __device__ __forceinline__ bool find_tile(const Args& a, int index, TileUnit& t) {
@@ -1271,7 +1310,7 @@ __device__ __forceinline__ bool find_tile(const Args& a, int index, TileUnit& t)
     steps = (gr.len + (a.big ? a.W << a.page_shift : 0) + TOK - 1) / TOK;  // own tokens: the most there may be
   };
   Unit u;
-  int total, split = 0, splits = 0;
+  int total, split = 0, splits = 0, before = 0;
   if (a.rounds) {
     // units in order, uncut: of the count of units, which of them this block takes
     if (a.G == 1) {
@@ -1296,10 +1335,14 @@ __device__ __forceinline__ bool find_tile(const Args& a, int index, TileUnit& t)
       index -= whole;
       if (index >= tail * splits) return false;
       split = index / tail;
-      index = whole + index - split * tail;
+      index -= split * tail;
+      before = index * splits;
+      index += whole;
     }
   }
-  if (!share_out(a.G, index, a.tile_fill, 256 / TOK, a.rounds ? 1 : a.S1, u, total, count)) return false;
+  if (!share_out(a.G, index, a.tile_fill, 256 / TOK, a.rounds ? 1 : a.S1, a.compact && !a.rounds, u, total, count))
+    return false;
+  t.before = a.rounds ? before : u.before;
   t.split = a.rounds ? split : u.split;
   t.splits = a.rounds ? splits : u.splits;
   t.g = u.entry;
@@ -1454,7 +1497,7 @@ __device__ __forceinline__ void row_tile(const Args& a, char* smem, int index, u
   }
 
   // What the rows see, worked out while the first tokens are on their way.
-  int mine = -1, prefix_limit = 0, own_limit = 0;  // sequence from the group's first
+  int mine = -1, prefix_limit = 0, own_limit = 0, own_row = 0;  // sequence from the group's first
   bool big = false;
   {
     const int i = table.find(a, t);
@@ -1465,17 +1508,22 @@ __device__ __forceinline__ void row_tile(const Args& a, char* smem, int index, u
       prefix_limit = clamp_int(gr.len + end, 0, gr.len);
       own_limit = clamp_int(end, 0, s.own);
       big = s.n_q * a.grp > FEW;
+      if (a.compact && !big) own_row = (int)own_rows_before(a, gr.b0 + i, h) + (t - s.q0) * a.grp + hq - h * a.grp;
     }
   }
   for (int i = threadIdx.x; i < L::ROWS * 16; i += THREADS) *(uint32_t*)(smem + L::MARKS + 4 * i) = 0;
   if (threadIdx.x < ARG_WORDS) *(uint32_t*)(smem + L::ARGS + 4 * threadIdx.x) = arg_word;
-  // of every row, for the marks: sequence (-1: no row), prefix tokens and own tokens that it sees
+  // of every row, for the marks: sequence (-1: no row), prefix tokens and own tokens that it sees; its place among own_rows
   if (wt == 0 && lane < SH) {
     int* p = (int*)(smem + L::ROW_INFO) + wr * SH + lane;
     p[0] = big ? mine | BIG : mine;
     p[L::ROWS] = prefix_limit;
     p[2 * L::ROWS] = own_limit;
-    if (wr == 0 && lane == 0) *(int*)(smem + L::ANY) = 0;
+    p[3 * L::ROWS] = own_row;
+    if (wr == 0 && lane == 0) {
+      *(int*)(smem + L::ANY) = 0;
+      *(int*)(smem + L::ANY + 4) = u.before;
+    }
   }
   if (have) place(n0, codes[0]);
   block_barrier();
@@ -1543,7 +1591,7 @@ __device__ __forceinline__ void row_tile(const Args& a, char* smem, int index, u
   const int first = u.tile * L::ROWS;
   finish<W, D, L::ROWS, WAVES / RW, true>(
       base + L::ARGS, base, base + L::STATS, marks, any, min(gr.rows - first, L::ROWS), gr.q0, first, h, u.split, u.splits,
-      [&](int r) { return lds_read<int>(info + 4 * r) >= 0 && (lds_read<int>(info + 4 * r) & BIG); });
+      info + 4 * 3 * L::ROWS, [&](int r) { return lds_read<int>(info + 4 * r) >= 0 && (lds_read<int>(info + 4 * r) & BIG); });
 }
 
 // Tiles first: they take longer (64 decodes behind 8192 tokens: 30.6 us, the other way round 35.6).
@@ -1560,26 +1608,55 @@ __global__ void __launch_bounds__(THREADS, 2) attend(Args a) {
 
 // ------------------------------------------------------------------ combine
 
-// The slots of a row: the first n_tile of the tiles' S1, the first n_own of the streams' S2 after them.  (Maxima and
-// sums of all slots are read along with the counts, one round of loads less; those of unused slots mean nothing.)
+// The slots of a row: those of its tiles, as slots 0 .. tile - 1 of S1, and those of its streams, S1 .. S1 + own - 1.
+//
+// Where all of them for every row take at most 512 MB, they lie together, slot s of row `id` at id * (S1 + S2) + s, and the
+// maxima and sums of all are read along with the counts, one round of loads less (those of unused slots mean nothing).
+// Otherwise (`compact`) only rows that need slots have them: each row of a split tile as many as the tile has splits (a
+// tile of x > 1 shares is cut into fewer than 2 x, of at most FILL shares in all, so there are at most 2 * FILL such
+// splits; in a last round of tiles FILL), and each row of a sequence of up to 16 rows S2 for its streams and one for a tile
+// that was not split.  Their places are read along with the counts (combine at 4385 queries of 32 heads: 13.2 us, with
+// slots for every row 12.5, which took 1 GB).
+template <bool COMPACT>
 struct Slots {
-  int tile, own;
+  int tile = 0, own = 0, tile_at = 0, own_at = 0;
+  Slots() = default;
   __device__ __forceinline__ Slots(const Args& a, int64_t id, int first, int end) {
     const int t = (int)(id / a.Hq);
     const int n_tile = a.S1 > 0 ? a.n_tile[id] : 0, n_own = a.n_own[id];
+    if (COMPACT) {
+      tile_at = a.S1 > 0 ? a.tile_at[id] : 0;
+      own_at = a.own_at[id];
+    }
     const bool inside = t >= first && t < end;  // else a row of no sequence
     tile = inside ? min(n_tile, a.S1) : 0;
     own = inside ? clamp_int(n_own, 0, a.S2) : 0;
   }
+  // those that lane k holds
+  __device__ __forceinline__ Slots of(int k) const {
+    Slots s;
+    s.tile = __builtin_amdgcn_readlane(tile, k);
+    s.own = __builtin_amdgcn_readlane(own, k);
+    s.tile_at = __builtin_amdgcn_readlane(tile_at, k);
+    s.own_at = __builtin_amdgcn_readlane(own_at, k);
+    return s;
+  }
   __device__ __forceinline__ bool has(const Args& a, int slot) const {
     return slot < a.S1 ? slot < tile : slot < a.S1 + own;
+  }
+  // where a slot that the row has lies (offsets that the sequences do not cover are read as any others, hence the limits)
+  __device__ __forceinline__ int64_t at(const Args& a, int64_t id, int slot) const {
+    if (!COMPACT) return id * (a.S1 + a.S2) + slot;
+    const int64_t mine = own_slot(a, clamp_int(own_at, 0, a.own_rows - 1));
+    if (slot >= a.S1) return mine + slot - a.S1;
+    return tile_at < 0 ? mine + a.S2 : clamp_int(tile_at, 0, max(a.tile_slots - a.S1, 0)) + slot;
   }
 };
 
 // One wavefront a row: lane n reads the maximum and sum of slots n and n + 64, then all lanes add the slots' outputs in
 // order, sixteen of them in flight.  A wavefront looks through `run` rows for those that their tile has not written
 // already (most of a prompt's); its rows lie far apart, since the others lie together.
-template <int DT, int D>
+template <int DT, int D, bool COMPACT>
 __global__ void __launch_bounds__(THREADS) combine(Args a, int run) {
   typedef typename Ty<DT>::el el;
   constexpr int PER = D / 64, AT_ONCE = 16;
@@ -1590,15 +1667,27 @@ __global__ void __launch_bounds__(THREADS) combine(Args a, int run) {
   const int64_t id0 = (int64_t)blockIdx.x * WAVES + (threadIdx.x >> 6);
   const int first = query_start(a, 0), end = query_start(a, a.B);
   bool open = lane < run && id0 + lane * all < rows;
-  if (open && run > 1) open = Slots(a, id0 + lane * all, first, end).tile >= 0;
+  Slots<COMPACT> held;
+  if (open && (COMPACT || run > 1)) {
+    held = Slots<COMPACT>(a, id0 + lane * all, first, end);
+    open = held.tile >= 0;
+  }
   for (unsigned long long rest = __ballot(open); rest; rest &= rest - 1) {
-    const int64_t id = id0 + __builtin_ctzll(rest) * all;
+    const int k = __builtin_ctzll(rest);
+    const int64_t id = id0 + k * all;
     float2 ml[2] = {float2{NEG_INF, 0.0f}, float2{NEG_INF, 0.0f}};
+    if (!COMPACT) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      if (lane + 64 * i < n) ml[i] = a.part_ml[id * n + lane + 64 * i];
-    const Slots slots(a, id, first, end);
+      for (int i = 0; i < 2; ++i)
+        if (lane + 64 * i < n) ml[i] = a.part_ml[id * n + lane + 64 * i];
+    }
+    const Slots<COMPACT> slots = COMPACT ? held.of(k) : Slots<COMPACT>(a, id, first, end);
     if (slots.tile < 0) continue;
+    if (COMPACT) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (slots.has(a, lane + 64 * i)) ml[i] = a.part_ml[slots.at(a, id, lane + 64 * i)];
+    }
 #pragma unroll
     for (int i = 0; i < 2; ++i)
       if (!slots.has(a, lane + 64 * i)) ml[i] = float2{NEG_INF, 0.0f};
@@ -1625,7 +1714,7 @@ __global__ void __launch_bounds__(THREADS) combine(Args a, int run) {
           const int s = live ? __builtin_ctzll(live) : 0;
           w[k] = live ? __shfl(weight[i], s) : 0.0f;
           p[k] = Part{};
-          if (live) p[k] = *(const Part*)(a.part_o + (id * n + s + 64 * i) * D + lane * PER);
+          if (live) p[k] = *(const Part*)(a.part_o + slots.at(a, id, s + 64 * i) * D + lane * PER);
           live &= live - 1;
         }
 #pragma unroll
@@ -1644,7 +1733,7 @@ __global__ void __launch_bounds__(THREADS) combine(Args a, int run) {
 }
 
 // The same with a block a row, for many slots: lanes 0 .. 31 and 32 .. 63 of each wavefront read a slot's output each.
-template <int DT, int D>
+template <int DT, int D, bool COMPACT>
 __global__ void __launch_bounds__(THREADS) combine_many(Args a) {
   typedef typename Ty<DT>::el el;
   constexpr int PER = D / 32, HALVES = 2 * WAVES;
@@ -1653,11 +1742,18 @@ __global__ void __launch_bounds__(THREADS) combine_many(Args a) {
   const int lane = threadIdx.x & 63, half = (int)threadIdx.x >> 5, at = lane & 31, n = a.S1 + a.S2;
   const int64_t rows = (int64_t)a.T * a.Hq, id = blockIdx.x;
   float2 ml[2] = {float2{NEG_INF, 0.0f}, float2{NEG_INF, 0.0f}};
+  if (!COMPACT) {
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
-    if (lane + 64 * i < n) ml[i] = a.part_ml[id * n + lane + 64 * i];
-  const Slots slots(a, id, query_start(a, 0), query_start(a, a.B));
+    for (int i = 0; i < 2; ++i)
+      if (lane + 64 * i < n) ml[i] = a.part_ml[id * n + lane + 64 * i];
+  }
+  const Slots<COMPACT> slots(a, id, query_start(a, 0), query_start(a, a.B));
   if (slots.tile < 0) return;  // written by its tile
+  if (COMPACT) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (slots.has(a, lane + 64 * i)) ml[i] = a.part_ml[slots.at(a, id, lane + 64 * i)];
+  }
 #pragma unroll
   for (int i = 0; i < 2; ++i)
     if (!slots.has(a, lane + 64 * i)) ml[i] = float2{NEG_INF, 0.0f};
@@ -1680,7 +1776,7 @@ __global__ void __launch_bounds__(THREADS) combine_many(Args a) {
     const float l0 = __shfl(ml[0].y, s & 63), l1 = __shfl(ml[1].y, s & 63);
     const float w = s < 64 ? w0 : w1, l = s < 64 ? l0 : l1;
     Part p{};
-    if (s < n && !(l == 0.0f)) p = *(const Part*)(a.part_o + (id * n + s) * D + at * PER);  // an empty one is not there
+    if (s < n && !(l == 0.0f)) p = *(const Part*)(a.part_o + slots.at(a, id, s) * D + at * PER);  // an empty one is not there
 #pragma unroll
     for (int k = 0; k < PER; ++k) x[k] += w * p.x[k];
   }
@@ -1704,6 +1800,8 @@ struct Plan {
   int tile_fill = FILL;
   int S1 = 0, S2 = 0, stream_least = 0;
   bool joint = false, rounds = false, many = false;  // many: slots a row
+  bool compact = false, direct_rows = true;
+  int64_t tile_slots = 0, own_rows = 0, slots = 0;  // compact; of partial results
   int64_t bytes = 0;
 };
 
@@ -1735,25 +1833,36 @@ inline Plan make_plan(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t G, 
     // the streams (64 decodes of up to 1024 own tokens behind 32768: 76 us, else 81); where less, they take both places
     // (96 sequences of up to 1400 own tokens in four groups of up to 15689: 124 us, else 139).
     p.tile_fill = !big && B * W * Hkv >= units * Wp ? FILL / 2 : FILL;
-    // partial results of up to 512 MB where only a last round of tiles is split
-    const int64_t room = (512 << 20) / (T * Hq * (D * 4 + 8));
-    p.S1 = (int)between(cuts, 1, p.rounds ? between(room, 1, 8) : MAX_SPLIT);
+    p.S1 = (int)between(cuts, 1, p.rounds ? 8 : MAX_SPLIT);
     if (groups == 1 && !p.rounds) p.S1 = (int)between(p.tile_fill / between(units, 1, FILL), 1, p.S1);
     p.tile_blocks = (rows / tile + groups) * Hkv + FILL;
     tiles = p.rounds ? FILL : between(units * p.S1, 1, p.tile_fill);
     p.many = p.tile_fill / units > 24 && T * Hq <= 16384;
   }
-  // A sequence falls to at most S2 - 1 full streams and one more; S2 up to 64, as far as 512 MB of partial results go.
-  const int64_t tok = (e8 || D == 64) ? 64 : 32, most = ceil_div(W * page, tok);
-  const int64_t slots = between((512 << 20) / (T * Hq * (D * 4 + 8)), 4, MAX_SPLIT);
-  p.stream_least = (int)ceil_div(most, slots - 1);
-  p.S2 = (int)(ceil_div(most, p.stream_least) + 1);
+  // A sequence falls to at most S2 - 1 full streams and one more; S2 up to 64, as far as 512 MB of partial results go, but
+  // at least 4.
+  const int64_t tok = (e8 || D == 64) ? 64 : 32, most = ceil_div(W * page, tok), row_bytes = D * 4 + 8;
+  auto streams = [&](int64_t rows_of_streams) {
+    const int64_t slots = between(PARTIALS / (rows_of_streams * row_bytes), 4, MAX_SPLIT);
+    p.stream_least = (int)ceil_div(most, slots - 1);
+    p.S2 = (int)(ceil_div(most, p.stream_least) + 1);
+  };
+  streams(T * Hq);
+  p.slots = (p.S1 + p.S2) * T * Hq;
+  p.compact = p.slots * row_bytes > PARTIALS;
+  if (p.compact) {
+    p.own_rows = big ? between(B * Hkv * FEW, 1, T * Hq) : T * Hq;
+    p.direct_rows = p.own_rows == T * Hq;
+    streams(p.own_rows);
+    p.tile_slots = p.S1 > 1 ? (p.rounds ? 1 : 2) * FILL * 32 * p.row_waves : 0;
+    p.slots = p.tile_slots + p.own_rows * (p.S2 + 1);
+  }
   // Streams fill the device after tiles that do so (those four groups: 118 us, with half as many 124), or beside few
   // tiles most of it (64 decodes of 1024 to 4096 own tokens behind 1000: 130 us, with FILL / 2 152); beside as many
   // tiles as they are, all run at once (64 decodes of up to 1024 behind 8192: 41 us, with FILL 44).
   const int64_t fill = tiles > FILL / 2 || tiles == 0 ? FILL : tiles <= FILL / 4 ? FILL * 3 / 4 : FILL / 2;
   p.stream_blocks = between(ceil_div(B * Hkv * most, WAVES * p.stream_least), 1, fill);
-  p.bytes = (int64_t)(p.S1 + p.S2) * T * Hq * (D * 4 + 8) + 2 * T * Hq * 4;
+  p.bytes = p.slots * row_bytes + (p.compact ? 4 : 2) * T * Hq * 4;
   return p;
 }
 
@@ -1768,10 +1877,13 @@ tb_status launch(Args& a, const Plan& p, hipStream_t stream, const char* what) {
   if (tb_status s = launch_status(what)) return s;
   const int64_t rows = (int64_t)a.T * a.Hq, most = WAVES << 22;  // a launch holds 2^32 threads
   const int64_t run = rows > most ? 64 : a.big && rows >= 32768 ? 16 : 1;
-  if (p.many)  // 69 slots (8 queries about 131001 tokens): 119.7 us in all, by wavefronts 122.5
-    hipLaunchKernelGGL((combine_many<DT, D>), dim3((unsigned)rows), dim3(THREADS), 0, stream, a);
-  else
-    hipLaunchKernelGGL((combine<DT, D>), dim3((unsigned)ceil_div(rows, WAVES * run)), dim3(THREADS), 0, stream, a, (int)run);
+  if (p.many) {  // 69 slots (8 queries about 131001 tokens): 119.7 us in all, by wavefronts 122.5
+    const auto kernel = p.compact ? combine_many<DT, D, true> : combine_many<DT, D, false>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)rows), dim3(THREADS), 0, stream, a);
+  } else {
+    const auto kernel = p.compact ? combine<DT, D, true> : combine<DT, D, false>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)ceil_div(rows, WAVES * run)), dim3(THREADS), 0, stream, a, (int)run);
+  }
   return launch_status(what);
 }
 
@@ -1893,9 +2005,17 @@ extern "C" tb_status tb_shared_prefix_attention(const void* q, const void* k_cac
   a.out = out;
   a.lse = lse;
   a.part_o = (float*)workspace;
-  a.part_ml = (float2*)((char*)workspace + (int64_t)(p.S1 + p.S2) * T * Hq * D * 4);
-  a.n_tile = (int*)((char*)workspace + (int64_t)(p.S1 + p.S2) * T * Hq * (D * 4 + 8));
+  a.part_ml = (float2*)((char*)workspace + p.slots * D * 4);
+  a.n_tile = (int*)((char*)workspace + p.slots * (D * 4 + 8));
   a.n_own = a.n_tile + T * Hq;
+  a.tile_at = a.n_own + T * Hq;  // these two compact only
+  a.own_at = a.tile_at + T * Hq;
+  a.compact = p.compact;
+  a.direct_rows = p.direct_rows;
+  a.own_first = p.compact ? (int)p.tile_slots : p.S1;
+  a.own_stride = p.compact ? p.S2 + 1 : p.S1 + p.S2;
+  a.tile_slots = (int)p.tile_slots;
+  a.own_rows = (int)p.own_rows;
   a.T = (int)T;
   a.Hq = (int)Hq;
   a.Hkv = (int)Hkv;
