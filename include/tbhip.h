@@ -490,8 +490,10 @@ tb_status tb_rope_kv_append(const void* q, const void* k, const void* v, void* q
  *   logarithm of the sum.  Rows that see no token, and rows of no sequence, give
  *   0 and -inf.  Sums are fp32; the weights are rounded to `dtype` before the
  *   product with the values (with e4m3 caches, cache_dtype 3, after they are
- *   multiplied by the values' scales, which may be of any size).  Tokens that a
- *   row does not see leave no trace in it, whatever they hold.
+ *   multiplied by the values' scales, whose magnitudes may lie anywhere below
+ *   2^90, far apart within a row; fp16 keeps products down to 2^-32 of a row's
+ *   largest).  Tokens that a row does not see leave no trace in it, whatever they
+ *   hold.
  * Lengths, offsets and page ids are read on the device and clamped to the
  * tables and the pool, so malformed ones never address memory outside them.
  * Needs the workspace reported by tb_shared_prefix_attention_workspace_size

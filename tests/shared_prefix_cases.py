@@ -72,3 +72,39 @@ def check(got, x, ref=None):
     assert torch.equal(lse.isnan(), want_lse.isnan())
     worst = (lse - want_lse).abs()[some] - (2 * e + 2.0 ** -22 * (1 + want_lse.abs()[some]))
     assert worst.numel() == 0 or float(worst.max()) <= 0, f"lse over the bound by {float(worst.max())}"
+
+
+def far_scales(x, ratio, seed=0):
+    """Keys and values of an e4m3 cache such that every query attends to about half of the tokens (the first of every
+    prefix among them), and next to nothing to the others, whose values are `ratio` times as large."""
+    g = torch.Generator().manual_seed(seed)
+    q, kc, vc, ks, vs = x[0], x[1], x[2], x[11], x[12]
+    pages, heads, page, D = kc.shape
+    sign = torch.randint(0, 2, (D,), generator=g).float() * 2 - 1
+    x[0] = (6 * sign * (1 + 0.1 * torch.rand(q.shape, generator=g))).to(q.dtype)
+    near = torch.randint(0, 2, (pages, heads, page), generator=g).bool()
+    near[x[3][:, 0].long(), :, 0] = True
+    k = torch.where(near[..., None], 0.5, -0.5) * sign * (1 + 0.1 * torch.rand(kc.shape, generator=g))
+    ks.copy_(k.abs().amax(dim=-1) / 448.0)
+    kc.copy_((k / ks[..., None]).to(kc.dtype))
+    vs *= torch.where(near, 1.0, ratio)
+
+
+def check_far_scales(got, x):
+    """As check, but for what weights below fp16's normals lose: a product of weight and scale is off by 2^-25 where the
+    largest is at least 2^8, so by 2^-33 of the largest, which is at most the sum of all; an e4m3 code is at most 448."""
+    q, kc, vc = x[0], x[1], x[2]
+    want, lse, mean = reference(x)
+    y = list(x)
+    y[2] = torch.full_like(vc.float(), 448.0).to(vc.dtype)
+    largest = impl_torch.run(*y, dtype=torch.float64)[0]
+    half = q.dtype == torch.float16
+    n, D = (x[6].shape[1] + x[3].shape[1]) * kc.shape[2], q.shape[2]
+    k = kc.float() * x[11][..., None]
+    qk = float(q.float().norm(dim=-1).max()) * float(k.norm(dim=-1).max())
+    e = 2.0 ** -24 * ((D + 8) * qk * D ** -0.5 + n + 16)
+    u = 2.0 ** -11 if half else 2.0 ** -8
+    bound = 1.01 * (u * (want.abs() + mean) + 2 * e * mean) + (n * 2.0 ** -33 * largest if half else 0) + 2.0 ** -25
+    over = ((got[0].cpu().double() - want).abs() - bound).max()
+    assert float(over) <= 0, f"over the bound by {float(over)}, values up to {float(want.abs().max())}"
+    assert float(((got[1].cpu().double() - lse).abs() - 2 * e - 2.0 ** -22 * (1 + lse.abs())).max()) <= 0

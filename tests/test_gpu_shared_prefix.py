@@ -3,7 +3,7 @@ the CPU (bounds: shared_prefix_cases.check)."""
 import pytest
 import torch
 
-from tests.shared_prefix_cases import check, make, reference
+from tests.shared_prefix_cases import check, check_far_scales, far_scales, make, reference
 from tilebench_amd.data import tensors as T
 
 pytestmark = pytest.mark.gpu
@@ -154,6 +154,20 @@ def test_value_scales_of_any_size(gpu, kw, low, high):
         g = torch.Generator().manual_seed(high)
         x[12] *= 2.0 ** torch.randint(low, high + 1, x[12].shape, generator=g)
         check(_run(x, gpu), x)
+
+
+@pytest.mark.parametrize("ratio", [2.0 ** 30, 2.0 ** 50, 2.0 ** -50, 0.0])
+@pytest.mark.parametrize("kw", [
+    dict(n_q=[1, 2], lens=[200, 70], prefix=[500]), dict(n_q=[1, 2], lens=[900, 70], prefix=[1100], D=128),
+    dict(n_q=ONES, lens=[300] * 40, prefix=[900], D=128), dict(n_q=[90, 3], lens=[800, 20], prefix=[30])],
+    ids=["joint", "few", "tile", "chunk"])
+def test_values_beside_others_of_no_weight(gpu, kw, ratio):
+    """Tokens of next to no weight whose values are far larger or smaller than those that count, or zero."""
+    for dtype in (F16, BF16):
+        _say("far scales", kw, ratio, dtype)
+        x = make(**kw, cache="e4m3", dtype=dtype, seed=31)
+        far_scales(x, ratio)
+        check_far_scales(_run(x, gpu), x)
 
 
 @pytest.mark.parametrize("kw", [

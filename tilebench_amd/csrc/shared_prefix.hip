@@ -308,9 +308,14 @@ struct Wave {
   static constexpr int REGS = SH * SH / 64; // accumulator registers of a tile
 
   // log2 of the largest weight when m is set, and how far weights may grow past it before m is set again.  fp16:
-  // weights down to 2^-32 of the largest are kept.  With scales the operand is weight * scale of the value, so in fp16
-  // it is that product's bound, the largest scale times the largest weight, which m keeps in range.
+  // weights down to 2^-32 of the largest are kept.
   static constexpr float LIFT = DT == BF16 ? 0.0f : 8.0f, SLACK = 6.0f;
+  // fp16 operands that are weight * scale of the value: the same holds for these products, the largest of which m follows.
+  // (A bound made of the largest weight and the largest scale would not do: beside a token of no weight whose scale is
+  // 2^30 times as large, products that count fell out of fp16's range.)  Weights reach 2^REACH; scales that have nothing
+  // to give even so, below 2^-45, have nothing to give to an fp16 output either.  bf16 has fp32's range.
+  static constexpr bool RANGED = SC && DT == F16;
+  static constexpr float REACH = 32.0f;
 
   v8 q[STEPS];
   acc_t o[DT_N];
@@ -430,27 +435,9 @@ struct Wave {
 #pragma unroll
       for (int r = 0; r < REGS; ++r) top = fmaxf(top, s[t][r]);
     top = over_groups_max(top) * scale;
-    if (SC && DT == F16) {
-      acc_t v[TOK / SH];
-#pragma unroll
-      for (int t = 0; t < TOK / SH; ++t)
-#pragma unroll
-        for (int r = 0; r < REGS; r += 4) {
-          const f32x4 x = lds_read<f32x4>(scale_at(sbase, tok0 + t * SH + token_of(r, g)) + 128);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) v[t][r + i] = x[i];
-        }
-      if (!full) hide<TOK>(v, limit - t0 - 4 * g, 0.0f);
-      float most = 0.0f;
-#pragma unroll
-      for (int t = 0; t < TOK / SH; ++t)
-#pragma unroll
-        for (int r = 0; r < REGS; ++r) most = fmaxf(most, fabsf(v[t][r]));
-      most = fminf(fmaxf(over_groups_max(most), 0x1p-60f), 0x1p60f);  // the sums of weights / scale stay finite
-      top += __builtin_amdgcn_logf(most);
-    }
-    if (__any(top > m + (LIFT + SLACK))) {
-      const float ref = fmaxf(m, top - LIFT);
+    constexpr float lift = RANGED ? REACH : LIFT, slack = RANGED ? 0.0f : SLACK;
+    if (__any(top > m + (lift + slack))) {
+      const float ref = fmaxf(m, top - lift);
       const float alpha = __builtin_amdgcn_exp2f(m - (ref == NEG_INF ? 0.0f : ref));
       m = ref;
       l *= alpha;
@@ -474,8 +461,32 @@ struct Wave {
           s[t][r + i] = SC ? w * v[i] : w;
         }
       }
-    l += sum;
     if (SC && !full) hide<TOK>(s, limit - t0 - 4 * g, 0.0f);  // whatever their scales are
+    if (RANGED) {
+      float most = 0.0f;
+#pragma unroll
+      for (int t = 0; t < TOK / SH; ++t)
+#pragma unroll
+        for (int r = 0; r < REGS; ++r) most = fmaxf(most, fabsf(s[t][r]));
+      most = over_groups_max(most);
+      constexpr float room = 1 << (int)(LIFT + SLACK);
+      if (__any(most > room)) {
+        const float ref = most > room ? m + (__builtin_amdgcn_logf(fminf(most, 0x1p100f)) - LIFT) : m;
+        const float alpha = __builtin_amdgcn_exp2f(m - (ref == NEG_INF ? 0.0f : ref));
+        m = ref;
+        l *= alpha;
+        sum *= alpha;
+#pragma unroll
+        for (int t = 0; t < TOK / SH; ++t)
+#pragma unroll
+          for (int r = 0; r < REGS; ++r) s[t][r] *= alpha;
+#pragma unroll
+        for (int d = 0; d < DT_N; ++d)
+#pragma unroll
+          for (int r = 0; r < REGS; ++r) o[d][r] *= alpha;
+      }
+    }
+    l += sum;
 #pragma unroll
     for (int k = 0; k < TOK / KS; ++k)
 #pragma unroll
