@@ -455,8 +455,8 @@ tb_status tb_rotary_axes(const void* q, void* q_out, const void* k, void* k_out,
  *   [0, pages * page_size) write nothing; a slot named twice in one call holds
  *   an unspecified mix of both tokens.  q' goes to q_out, dense [T, Hq, D].
  *   dtype 1 = fp16, 2 = bf16; cache_dtype the same, or 3: e4m3 codes of
- *   x / s with s = absmax / 448 over the row (rotated, in fp64), s rounded to
- *   fp32 in k_scale / v_scale fp32 [pages, Hkv, page_size] at strides
+ *   x / s with s = absmax / 448 over the row, as they are in fp64 (keys after a
+ *   rotation to 2^-36), s rounded to fp32 in k_scale / v_scale fp32 [pages, Hkv, page_size] at strides
  *   s_page, s_head, s_slot.  A zero row has s = 0 and zero codes; a row with
  *   inf or NaN reads back as NaN.
  * Requires page_size a power of two up to 4096, pages * page_size < 2^31, and

@@ -224,6 +224,25 @@ def test_codes_are_rounded_as_by_division(gpu):
     assert torch.equal(out[2].cpu().view(torch.uint8)[at], code.view(torch.uint8))
 
 
+def test_keys_are_quantised_as_in_64_bits(gpu):
+    """Rotated keys' scales and codes are those of the definition in 64 bits, but for scales next to a border.
+
+    Sine and cosine are off by at most 2^-36.5 (their series 2^-37 and 2^-41, the angle of up to 2^15.2 rad by 2^-37.8), a key by
+    that times |a| + |b|, at most 2^0.5 times the row's largest: 2^-36 of the scale, half as much again for safety."""
+    _say("append keys in 64 bits")
+    x = T.generate_rope_kv_append_inputs(8192, 1, 8, 8, 128, 64, "e4m3", dtype=torch.bfloat16, seed=5, device="cpu")
+    out = _append(x, gpu)
+    rows, slots = definition(x[1], *x[3:6], False), x[6].long()
+    at = (slots // 64, slice(None), slots % 64)
+    want = np.abs(rows).max(axis=-1) / 448.0
+    step = np.spacing(want.astype(np.float32)).astype(np.float64)
+    away = np.abs(want / step - np.floor(want / step) - 0.5) * step > 1.5 * 2.0 ** -36 * want
+    scales = out[3].cpu()[at].numpy()
+    assert away.mean() > 0.99 and (scales == want.astype(np.float32))[away].all()
+    codes = torch.from_numpy((rows / want[..., None]).astype(np.float32)).to(torch.float8_e4m3fn)
+    assert torch.equal(out[1].cpu()[at].float(), codes.float())
+
+
 def test_more_tokens_than_a_launch_has_wavefronts(gpu):
     """The tokens past 2^25 come in a second launch."""
     _say("rotary of 2^25 tokens")

@@ -9,7 +9,7 @@ two tokens of one call holds an unspecified mix of both; the others are not
 affected.
 
 float8_e4m3fn caches take fp32 k_scale and v_scale and store each row of a head
-as codes of x / s with s = absmax / 448 (rotated and divided in 64 bits; a zero row
+as codes of x / s with s = absmax / 448, the codes and scales of 64-bit arithmetic (a zero row
 stores s = 0 and zero codes, a row with inf or NaN reads back as NaN); run then
 returns (q', k_cache, v_cache, k_scale, v_scale).
 """

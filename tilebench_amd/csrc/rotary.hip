@@ -33,11 +33,12 @@
 // us (5.5 TB/s), 4096 into an 8-bit cache 20.5 us (4.5 TB/s), one token 3.5 us.
 //
 // 8-bit cache rows: s = absmax / 448 and code = e4m3(x / s), as in 64 bits: the
-// scale is rounded to 32 bits, the quotient to 32 and then to 8.  Keys are rotated,
-// compared and divided in 64 bits; with 32 a few quotients in a million fall on the
-// other side of a border between codes (4096 tokens: 19.0 us, so 20.5, values in
-// 64 bits too 21.3).  A row of zeros stores s = 0 and codes 0; a row with inf or
-// NaN reads back as NaN.
+// scale is rounded to 32 bits, the quotient to 32 and then to 8.  Keys are rotated
+// (by sines and cosines of 2^-36), compared and divided in 64 bits; with 32 a few
+// quotients in a million fall on the other side of a border between codes (4096
+// tokens: 19.0 us, so 20.5, values in 64 bits too 21.3).  Values are divided in 32
+// bits, the quotient corrected by the exact remainder.  A row of zeros stores s = 0
+// and codes 0; a row with inf or NaN reads back as NaN.
 #include "tb_common.h"
 
 namespace tb {
@@ -106,13 +107,15 @@ struct alignas(VEC * sizeof(E) < 16 ? VEC * sizeof(E) : 16) Chunk {
 };
 
 // cos and sin of position * frequency, in 64 bits: the nearest whole turn and quarter turn are taken off, which is
-// exact, and the Taylor series are summed over the rest, |angle| <= pi / 4 (x^13 / 13! < 2^-37 is left out).
+// exact, and the Taylor series are summed over the rest, |angle| <= pi / 4 (x^13 / 13! < 2^-37 and x^14 / 14! < 2^-41 are
+// left out).
 __device__ __forceinline__ double2 cos_sin(int pos, float freq, bool inverse) {
   double turns = (double)pos * (double)freq * 0.15915494309189533577;
   turns -= __builtin_rint(turns);
   const double quarter = __builtin_rint(4.0 * turns);
   const double x = __builtin_fma(4.0, turns, -quarter) * 1.57079632679489661923, z = x * x;
-  double s = -1.0 / 39916800.0, c = -1.0 / 3628800.0;
+  double s = -1.0 / 39916800.0, c = 1.0 / 479001600.0;
+  c = __builtin_fma(c, z, -1.0 / 3628800.0);
   s = __builtin_fma(s, z, 1.0 / 362880.0);
   c = __builtin_fma(c, z, 1.0 / 40320.0);
   s = __builtin_fma(s, z, -1.0 / 5040.0);
