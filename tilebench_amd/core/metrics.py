@@ -91,6 +91,8 @@ def _eval_expr(expr, ctx: dict) -> float | None:
 def eval_ctx(params: dict, dtype_str: str, problem_size: int | None = None) -> dict:
     ctx = {"n": int(params.get("n", problem_size or 1)), "dtype_size": dtype_size(dtype_str)}
     ctx.update({k: v for k, v in params.items() if isinstance(v, (int, float))})
+    if "cache" in params:  # bytes of an element of a key/value cache, and of a row's scale
+        ctx["cache_size"], ctx["scale_size"] = (1, 4) if params["cache"] == "e4m3" else (ctx["dtype_size"], 0)
     return ctx
 
 
