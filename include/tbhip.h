@@ -502,9 +502,10 @@ tb_status tb_rope_kv_append(const void* q, const void* k, const void* v, void* q
  * or empty ones.  The same call gives the same bits each time.
  * Requires D 64 or 128, Hq a multiple of Hkv, page_size a power of two up to
  * 4096, a scale below 1e38 in magnitude (it may be 0 or negative), T * Hq and
- * max_q * Hq below 2^31, B * Hkv and G * Hkv at most 2^23, tables of at most 2^29
- * tokens a row, n_pages * page_size < 2^31, 16-byte aligned q, caches and out, cache strides in multiples of 16
- * bytes, q strides in multiples of 8.  No counterpart in the reference's
+ * max_q * Hq below 2^31, B * Hkv and G * Hkv below 2^23, tables of fewer than 2^29
+ * tokens a row, B * Hkv * ceil(W * page_size / 32) at most 2^30, n_pages *
+ * page_size < 2^31, 16-byte aligned q, caches and out, cache strides in multiples
+ * of 16 bytes, q strides in multiples of 8.  No counterpart in the reference's
  * quantised operators.
  */
 tb_status tb_shared_prefix_attention(const void* q, const void* k_cache, const void* v_cache, const float* k_scale,

@@ -180,3 +180,25 @@ def test_workspaces_are_bounded(kw, cache):
     assert 0 <= need.value <= max(5 * few * each, 640 * MIB) + 72 * MIB + 16 * rows, need.value / MIB
     if few <= 16384:
         assert need.value <= 512 * MIB
+
+
+def test_limits_of_sizes_are_the_documented_ones():
+    """The largest sizes that the header allows are taken, one more is refused by name."""
+    if not rt.LIB_PATH.exists():
+        pytest.skip("libtbhip.so is not built")
+    lib, need = rt.load_library(), ctypes.c_int64(-1)
+
+    def size(T=8, Hq=8, Hkv=8, G=1, Wp=1, B=1, W=1, page=64, max_q=1):
+        return lib.tb_shared_prefix_attention_workspace_size(T, Hq, Hkv, 64, G, Wp, B, W, page, max_q, 1,
+                                                             ctypes.byref(need))
+
+    table = 2 ** 29 // 64
+    for fits, over in ((dict(T=2 ** 28 - 1), dict(T=2 ** 28)), (dict(max_q=2 ** 28 - 1), dict(max_q=2 ** 28)),
+                       (dict(B=2 ** 20 - 1), dict(B=2 ** 20)), (dict(G=2 ** 20 - 1), dict(G=2 ** 20)),
+                       (dict(Wp=table - 1), dict(Wp=table)), (dict(W=table - 1, Hkv=1, Hq=1), dict(W=table, Hkv=1, Hq=1))):
+        assert size(**fits) == rt.TB_OK, fits
+        assert size(**over) == rt.TB_E_INVALID and "2^31" in lib.tb_last_error().decode(), over
+    # sequences, key/value heads and steps of 32 tokens: 2^30 at most
+    assert size(B=2 ** 16, W=2 ** 10) == rt.TB_OK
+    assert size(B=2 ** 16, W=2 ** 10 + 1) == rt.TB_E_INVALID
+    assert "65536 sequences" in lib.tb_last_error().decode() and "2^30" in lib.tb_last_error().decode()

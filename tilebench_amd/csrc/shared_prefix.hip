@@ -1934,7 +1934,9 @@ tb_status check_sizes(const char* what, int64_t T, int64_t Hq, int64_t Hkv, int6
                    max_q * Hq <= most && B * Hkv <= most / MAX_SPLIT / 4 && G * Hkv <= most / MAX_SPLIT / 4 &&
                    W <= most / 4 / page_size && Wp <= most / 4 / page_size,
                "%s: sizes past 2^31", what);
-  TB_CHECK_ARG(B == 0 || W == 0 || Hkv * B <= (1ll << 30) / ceil_div(W * page_size, 32), "%s: sizes past 2^31", what);
+  TB_CHECK_ARG(B == 0 || W == 0 || Hkv * B <= (1ll << 30) / ceil_div(W * page_size, 32),
+               "%s: %lld sequences times %lld key/value heads times tables of %lld tokens in steps of 32 exceed 2^30", what,
+               (long long)B, (long long)Hkv, (long long)(W * page_size));
   return TB_OK;
 }
 
