@@ -496,6 +496,8 @@ tb_status tb_rope_kv_append(const void* q, const void* k, const void* v, void* q
  *   hold.
  * Lengths, offsets and page ids are read on the device and clamped to the
  * tables and the pool, so malformed ones never address memory outside them.
+ * Offsets that do not ascend leave the rows of their sequences and groups with
+ * contents that are not specified, and other memory alone.
  * Needs the workspace reported by tb_shared_prefix_attention_workspace_size
  * (16-byte aligned, no clearing, not shared by calls that overlap).
  * A sequence with more than max_q queries gets results without its own tokens,

@@ -224,6 +224,45 @@ def test_malformed_lengths_and_ids_stay_inside(gpu):
     _run(y, gpu)
 
 
+@pytest.mark.parametrize("kw", [
+    dict(n_q=[1, 2, 40], lens=[30, 9, 60], prefix=[33, 20], bounds=[0, 1, 3]),                           # tiles
+    dict(n_q=[1, 2, 1, 1], lens=[30, 9, 60, 4], prefix=[33, 20], bounds=[0, 1, 4]),                      # a block each
+    dict(n_q=[1, 2, 1, 1], lens=[30, 9, 900, 4], prefix=[1500, 20], bounds=[0, 1, 4], D=128),            # streams
+    dict(n_q=[1, 1, 1, 1] * 40, lens=[30, 9, 60, 4] * 40, prefix=[1100] * 80, bounds=[2 * i for i in range(81)]),
+    COMPACT["tenants_drafts"]], ids=["tiles", "each", "streams", "groups", "compact"])
+def test_offsets_out_of_order_leave_other_memory_alone(gpu, kw):
+    """cu_q and group_offsets that do not ascend: their rows hold anything, but nothing around the buffers changes."""
+    import ctypes
+
+    from tilebench_amd import runtime as rt
+
+    _say("attention offsets out of order", len(kw["n_q"]))
+    x = make(**kw, seed=7)
+    y = _to(x, gpu)
+    T, Hq, D = x[0].shape
+    (pages, Hkv, page, _), (G, Wp), (B, W) = x[1].shape, x[3].shape, x[6].shape
+    need = ctypes.c_int64(0)
+    rt.call("tb_shared_prefix_attention_workspace_size", T, Hq, Hkv, D, G, Wp, B, W, page, x[9], 1, ctypes.byref(need))
+    guard = 1 << 16
+    buffers = [torch.full((n + 2 * guard,), 0xA5, dtype=torch.uint8, device=gpu)
+               for n in (T * Hq * D * 2, T * Hq * 4, need.value)]
+    g = torch.Generator().manual_seed(1)
+    backwards = lambda t: t.flip(0).contiguous()                                     # noqa: E731
+    wild = lambda t: torch.randint(-9, T + 90, t.shape, generator=g).int()           # noqa: E731
+    for cu, go in ((backwards(x[8]), x[5]), (x[8], backwards(x[5])), (wild(x[8]), x[5]), (x[8], wild(x[5])),
+                   (wild(x[8]), wild(x[5])), (x[8], torch.full_like(x[5], 0)),
+                   (x[8], torch.tensor([0, B] * len(x[5])).int()[:len(x[5])])):
+        cu, go = cu.to(gpu), go.to(gpu)
+        out, lse, ws = (b.data_ptr() + guard for b in buffers)
+        rt.call("tb_shared_prefix_attention", y[0].data_ptr(), y[1].data_ptr(), y[2].data_ptr(), None, None,
+                y[3].data_ptr(), y[4].data_ptr(), go.data_ptr(), y[6].data_ptr(), y[7].data_ptr(), cu.data_ptr(), out,
+                lse, T, Hq, Hkv, D, G, Wp, B, W, x[9], pages, page, Hq * D, D, Hkv * page * D, page * D, D, 0, 0, 0,
+                D ** -0.5, 1, 1, ws if need.value else None, need.value, rt.stream_handle(y[0].get_device()))
+        torch.cuda.synchronize()
+        for b in buffers:
+            assert bool((b[:guard] == 0xA5).all()) and bool((b[-guard:] == 0xA5).all())
+
+
 def test_more_queries_than_announced_are_empty_or_right(gpu):
     _say("attention max_q too small")
     x = make([60, 1], [60, 9], Hq=4, Hkv=2, seed=8)

@@ -1293,7 +1293,8 @@ __device__ __forceinline__ bool share_out(int entries, int index, int fill, int 
       u.split = (int)((uint32_t)at / (uint32_t)of);
       u.at = at - u.split * of;
       u.before = split_before + __builtin_amdgcn_readlane(split_incl - split_n, u.lane) + u.at * u.splits;
-      return true;
+      // Groups that overlap can hold more units than 32 bits count.
+      return (uint32_t)u.split < (uint32_t)u.splits && (!number || (uint32_t)u.before <= (uint32_t)(2 * FILL - u.splits));
     }
     seen += here;
     split_before += __builtin_amdgcn_readlane(split_incl, 63);
