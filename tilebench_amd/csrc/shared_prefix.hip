@@ -185,8 +185,7 @@ template <int RB, int SH, bool E8>
 __device__ __forceinline__ constexpr int swizzle_v(int t) {
   if (!E8 && SH == 16) return RB == 256 ? (t & 7) << 1 : ((t >> 1) & 3) << 1;
   if (!E8) return RB == 256 ? (t & 3) << 2 : ((t >> 1) & 1) << 2;
-  if (SH == 16) return RB == 128 ? ((t >> 1) & 3) | ((t >> 4) & 1) << 2 : ((t >> 2) & 1) | ((t >> 4) & 1) << 1;
-  return RB == 128 ? (((t >> 1) & 1) | ((t >> 3) & 1) << 1) << 1 : ((t >> 3) & 1) << 1;
+  return RB == 128 ? ((t >> 1) & 3) | ((t >> 4) & 1) << 2 : ((t >> 2) & 1) | ((t >> 4) & 1) << 1;
 }
 
 typedef __attribute__((address_space(3))) char lds_char;
@@ -297,6 +296,7 @@ __device__ __forceinline__ float as_float(uint32_t x) { return __builtin_bit_cas
 // E8: the tiles hold e4m3 codes (else 16-bit values); SC: keys and values have scales.
 template <int DT, bool E8, int D, int SH, bool SC = E8>
 struct Wave {
+  static_assert(SH == 16 || !E8, "tiles of 32 rows hold 16-bit values");
   typedef Ty<DT> Y;
   typedef typename Y::v8 v8;
   typedef typename std::conditional<SH == 16, f32x4, f32x16>::type acc_t;
@@ -501,11 +501,11 @@ struct Wave {
     __device__ __forceinline__ explicit Values(uint32_t vbase) {
       const int lane = threadIdx.x & 63, i = lane & 15;
       const int gx = lane / SH;                          // the group's four tokens
-      const int sub = SH == 32 ? (lane >> 4) & 1 : 0;    // 16 of a tile's 32 channels
+      const int sub = SH == 32 ? (lane >> 4) & 1 : 0;    // 16 of a 16-bit tile's 32 channels
       if (E8) {
         const int r = i >> 1, tok = gx * 4 + (r & 3) + (r >> 2) * (KS / 2);
         at = vbase + tok * RB + (i & 1) * 8;
-        x = (uint32_t)(sub ^ swizzle_v<RB, SH, E8>(tok)) << 4;
+        x = (uint32_t)swizzle_v<RB, SH, E8>(tok) << 4;
       } else {
         const int r = i >> 2, b = i & 3, tok = gx * 4 + r;
         at = vbase + tok * RB + (b & 1) * 8;
@@ -514,7 +514,7 @@ struct Wave {
     }
     __device__ __forceinline__ v8 read(int d, int k) const {
       if (E8) {
-        const uint32_t p = at + (x ^ (uint32_t)(d * (SH / 16) * 16)) + k * KS * RB;
+        const uint32_t p = at + (x ^ (uint32_t)(d * 16)) + k * KS * RB;
         const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2*)(uintptr_t)p);
         u32x4 u;
         u[0] = Y::up8((uint32_t)w[0], false);
