@@ -117,6 +117,35 @@ def test_slots_only_for_rows_that_need_them(gpu, name, dtype, cache):
     assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
 
 
+@pytest.mark.parametrize("name", ["prompts", "five_tenants"])
+def test_replays_with_slots_only_where_needed(gpu, name):
+    """Two captured calls, replayed in turn with other contents, eager calls between them."""
+    _say("attention compact graphs", name)
+    from tilebench_amd.benchmarks.serving.shared_prefix_attention import impl_hip
+
+    xs = [_to(make(**COMPACT[name], seed=80 + i), gpu) for i in range(2)]
+    impl_hip.run(*xs[0])
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for x in xs:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(impl_hip.run(*x))
+    for seed in range(3):
+        new = [_to(make(**COMPACT[name], seed=90 + 2 * seed + i), gpu) for i in range(2)]
+        for x, y in zip(xs, new):
+            y[7] = torch.clamp(y[7] - seed, min=0)     # other lengths, the same tables
+            for a, b in zip(x, y):
+                if isinstance(a, torch.Tensor):
+                    a.copy_(b)
+        want = [impl_hip.run(*y) for y in new]
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(outs, want):
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
 def test_splits_of_long_prefixes_and_scales(gpu):
     for seed, (scale, kw) in enumerate([
             (None, dict(n_q=[1] * 3, lens=[9, 700, 33], prefix=[20000], Hq=16, Hkv=2, D=128, page=64)),
