@@ -493,7 +493,10 @@ tb_status tb_rope_kv_append(const void* q, const void* k, const void* v, void* q
  *   multiplied by the values' scales, whose magnitudes may lie anywhere below
  *   2^90, far apart within a row; fp16 keeps products down to 2^-32 of a row's
  *   largest).  Tokens that a row does not see leave no trace in it, whatever they
- *   hold.
+ *   hold; an infinity among the values that it does see makes its result that
+ *   infinity, or NaN where the weight may be too small for `dtype` to hold.
+ *   Work is shared out by the tables' widths, since lengths are read on the
+ *   device: tables much wider than the longest row need cost speed.
  * Lengths, offsets and page ids are read on the device and clamped to the
  * tables and the pool, so malformed ones never address memory outside them.
  * Offsets that do not ascend leave the rows of their sequences and groups with

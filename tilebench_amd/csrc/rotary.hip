@@ -28,15 +28,15 @@
 // of 128 take 74 us (5.5 TB/s), and 80 us (5.1 TB/s) with the positions' loads
 // behind the axes'.  A 410 MB copy takes 64 us.  Wavefronts with 2, 3 and 4 times the
 // items take 80, 95 and 124 us (before that change); four tokens to a block and
-// a loop over their heads 83 us; 8-byte accesses 96 us.  4800 tokens of 16 + 16
-// bf16 heads of 80 take 11.9 us (4.1 TB/s), 7001 tokens into a bf16 cache 31.4
-// us (5.5 TB/s), 4096 into an 8-bit cache 20.5 us (4.5 TB/s), one token 3.5 us.
+// a loop over their heads 83 us; 8-byte accesses 96 us.  Replayed from a graph, 4800
+// tokens of 16 + 16 bf16 heads of 80 take 11.2 us (4.4 TB/s), 7001 tokens into a bf16
+// cache 30.3 us (5.7 TB/s), 4096 into an 8-bit cache 21.0 us (4.4 TB/s), one token 3.0 us.
 //
 // 8-bit cache rows: s = absmax / 448 and code = e4m3(x / s), as in 64 bits: the
 // scale is rounded to 32 bits, the quotient to 32 and then to 8.  Keys are rotated
 // (by sines and cosines of 2^-36), compared and divided in 64 bits; with 32 a few
 // quotients in a million fall on the other side of a border between codes (4096
-// tokens: 19.0 us, so 20.5, values in 64 bits too 21.3).  Values are divided in 32
+// tokens on one card: 19.0 us, so 20.5, values in 64 bits too 21.3).  Values are divided in 32
 // bits, the quotient corrected by the exact remainder.  A row of zeros stores s = 0
 // and codes 0; a row with inf or NaN reads back as NaN.
 #include "tb_common.h"

@@ -30,14 +30,14 @@
 // the way to LDS); the keys' scales multiply the scores, the values' scales the
 // weights.
 //
-// What bounds it, and what it takes (kernel, us):
-//   prompts behind 6000 tokens (bf16, 32 heads)   514   matrix cores 45 % busy at 2.0 GHz, the
-//              exponentials take as long again; 932 TFLOP/s of a call (matrix products 1377)
-//   8 queries about 131001 tokens (64 heads)      106   memory, 5.3 TB/s
+// What bounds it, and what it takes (kernel, us, in a kernel trace):
+//   prompts behind 6000 tokens (bf16, 32 heads)   538   matrix cores 44 % busy at 1.9 GHz, vector work
+//              47 %: the exponentials take as long again; 910 TFLOP/s of a call (matrix products 1325)
+//   8 queries about 131001 tokens (64 heads)      108   memory, 5.2 TB/s
 //   64 decodes behind 8192, up to 1024 own         31   half of it the first loads and the last
 //              results of blocks that live for 20 us
-//   96 x 1-2 queries, four e4m3 prefixes           90   vector work: 19 instructions a product
-// and 6 to 12 for the combine.  Why tiles of 64 or 128 rows, streams and shares are as they are is said
+//   96 x 1-2 queries, four e4m3 prefixes           91   vector work: 19 instructions a product
+// and 6 to 13 for the combine.  Why tiles of 64 or 128 rows, streams and shares are as they are is said
 // at each; the first kernel, with a launch for each kind of work, took 772, 171, 83 and 169 in all.
 //
 // Values that a row does not attend to never reach it: masked scores are selected
@@ -1889,7 +1889,7 @@ tb_status launch(Args& a, const Plan& p, hipStream_t stream, const char* what) {
   if (tb_status s = launch_status(what)) return s;
   const int64_t rows = (int64_t)a.T * a.Hq, most = WAVES << 22;  // a launch holds 2^32 threads
   const int64_t run = rows > most ? 64 : a.big && rows >= 32768 ? 16 : 1;
-  if (p.many) {  // 69 slots (8 queries about 131001 tokens): 119.7 us in all, by wavefronts 122.5
+  if (p.many) {  // 65 to 108 slots (8 queries about 131001 tokens): 116.6 us in all, by wavefronts 118.7
     const auto kernel = p.compact ? combine_many<DT, D, true> : combine_many<DT, D, false>;
     hipLaunchKernelGGL(kernel, dim3((unsigned)rows), dim3(THREADS), 0, stream, a);
   } else {
