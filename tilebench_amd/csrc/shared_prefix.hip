@@ -31,9 +31,9 @@
 // weights.
 //
 // What bounds it, and what it takes (kernel, us, in a kernel trace):
-//   prompts behind 6000 tokens (bf16, 32 heads)   538   matrix cores 44 % busy at 1.9 GHz, vector work
+//   prompts behind 6000 tokens (bf16, 32 heads)   525   matrix cores 44 % busy at 1.9 GHz, vector work
 //              47 %: the exponentials take as long again; 910 TFLOP/s of a call (matrix products 1325)
-//   8 queries about 131001 tokens (64 heads)      108   memory, 5.2 TB/s
+//   8 queries about 131001 tokens (64 heads)      107   memory, 5.2 TB/s
 //   64 decodes behind 8192, up to 1024 own         31   half of it the first loads and the last
 //              results of blocks that live for 20 us
 //   96 x 1-2 queries, four e4m3 prefixes           91   vector work: 19 instructions a product
@@ -1744,8 +1744,8 @@ __global__ void __launch_bounds__(THREADS) combine(Args a, int run) {
   }
 }
 
-// The same with a block a row, for many slots: lanes 0 .. 31 and 32 .. 63 of each wavefront read a slot's output each.
-template <int DT, int D, bool COMPACT>
+// The same with a block a row, for many slots (of few rows: they lie together): lanes 0 .. 31 and 32 .. 63 of each wavefront read a slot's output each.
+template <int DT, int D>
 __global__ void __launch_bounds__(THREADS) combine_many(Args a) {
   typedef typename Ty<DT>::el el;
   constexpr int PER = D / 32, HALVES = 2 * WAVES;
@@ -1754,18 +1754,11 @@ __global__ void __launch_bounds__(THREADS) combine_many(Args a) {
   const int lane = threadIdx.x & 63, half = (int)threadIdx.x >> 5, at = lane & 31, n = a.S1 + a.S2;
   const int64_t rows = (int64_t)a.T * a.Hq, id = blockIdx.x;
   float2 ml[2] = {float2{NEG_INF, 0.0f}, float2{NEG_INF, 0.0f}};
-  if (!COMPACT) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      if (lane + 64 * i < n) ml[i] = a.part_ml[id * n + lane + 64 * i];
-  }
-  const Slots<COMPACT> slots(a, id, query_start(a, 0), query_start(a, a.B));
+  for (int i = 0; i < 2; ++i)
+    if (lane + 64 * i < n) ml[i] = a.part_ml[id * n + lane + 64 * i];
+  const Slots<false> slots(a, id, query_start(a, 0), query_start(a, a.B));
   if (slots.tile < 0) return;  // written by its tile
-  if (COMPACT) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-      if (slots.has(a, lane + 64 * i)) ml[i] = a.part_ml[slots.at(a, id, lane + 64 * i)];
-  }
 #pragma unroll
   for (int i = 0; i < 2; ++i)
     if (!slots.has(a, lane + 64 * i)) ml[i] = float2{NEG_INF, 0.0f};
@@ -1788,7 +1781,7 @@ __global__ void __launch_bounds__(THREADS) combine_many(Args a) {
     const float l0 = __shfl(ml[0].y, s & 63), l1 = __shfl(ml[1].y, s & 63);
     const float w = s < 64 ? w0 : w1, l = s < 64 ? l0 : l1;
     Part p{};
-    if (s < n && !(l == 0.0f)) p = *(const Part*)(a.part_o + slots.at(a, id, s) * D + at * PER);  // an empty one is not there
+    if (s < n && !(l == 0.0f)) p = *(const Part*)(a.part_o + (id * n + s) * D + at * PER);  // an empty one is not there
 #pragma unroll
     for (int k = 0; k < PER; ++k) x[k] += w * p.x[k];
   }
@@ -1849,7 +1842,7 @@ inline Plan make_plan(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t G, 
     if (groups == 1 && !p.rounds) p.S1 = (int)between(p.tile_fill / between(units, 1, FILL), 1, p.S1);
     p.tile_blocks = (rows / tile + groups) * Hkv + FILL;
     tiles = p.rounds ? FILL : between(units * p.S1, 1, p.tile_fill);
-    p.many = p.tile_fill / units > 24 && T * Hq <= 16384;
+    p.many = p.tile_fill / units > 24 && T * Hq <= 16384;  // at most 21 units of 128 rows: never compact
   }
   // A sequence falls to at most S2 - 1 full streams and one more; S2 up to 64, as far as 512 MB of partial results go, but
   // at least 4.
@@ -1890,8 +1883,7 @@ tb_status launch(Args& a, const Plan& p, hipStream_t stream, const char* what) {
   const int64_t rows = (int64_t)a.T * a.Hq, most = WAVES << 22;  // a launch holds 2^32 threads
   const int64_t run = rows > most ? 64 : a.big && rows >= 32768 ? 16 : 1;
   if (p.many) {  // 65 to 108 slots (8 queries about 131001 tokens): 116.6 us in all, by wavefronts 118.7
-    const auto kernel = p.compact ? combine_many<DT, D, true> : combine_many<DT, D, false>;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)rows), dim3(THREADS), 0, stream, a);
+    hipLaunchKernelGGL((combine_many<DT, D>), dim3((unsigned)rows), dim3(THREADS), 0, stream, a);
   } else {
     const auto kernel = p.compact ? combine<DT, D, true> : combine<DT, D, false>;
     hipLaunchKernelGGL(kernel, dim3((unsigned)ceil_div(rows, WAVES * run)), dim3(THREADS), 0, stream, a, (int)run);
