@@ -189,6 +189,29 @@ def test_append_into_pools_of_other_orders(gpu, cache):
             assert torch.equal(u8(a), u8(b))
 
 
+@pytest.mark.parametrize("cache", ["same", "e4m3"])
+def test_keys_and_values_of_one_head_in_different_orders(gpu, cache):
+    """With one head [pages, page, 1, D] and [pages, 1, page, D] are one order, whatever the strides say."""
+    _say("append one head", cache)
+    from tilebench_amd.benchmarks.serving.rope_kv_append import impl_hip as append
+    from tilebench_amd.benchmarks.serving.shared_prefix_attention import impl_hip as attend
+
+    y = [v.to(gpu) for v in T.generate_rope_kv_append_inputs(40, 1, 8, 1, 64, 16, cache, seed=9, device="cpu")]
+    pools = [y[7].clone(), y[8].clone(), *(s.clone() for s in y[9:])]
+    for i in range(1, len(pools), 2):
+        x = pools[i].view(torch.uint8) if pools[i].element_size() == 1 else pools[i]
+        other = x.new_empty(x.transpose(1, 2).shape).transpose(1, 2)
+        pools[i] = other.copy_(x).view(pools[i].dtype)
+        assert pools[i].stride() != pools[i - 1].stride()
+    want, got = append.run(*y), append.run(*y[:7], *pools)
+    tables = [torch.tensor(t, dtype=torch.int32, device=gpu) for t in ([[0, 1, 2]], [40], [0, 40])]
+    a, b = (attend.run(x[0], *x[1:3], None, None, None, *tables, 40, None, *x[3:]) for x in (want, got))
+    torch.cuda.synchronize()
+    for u, v in zip((*want, *a), (*got, *b)):
+        u, v = (t.view(torch.uint8) if t.element_size() == 1 else t for t in (u, v))
+        assert torch.equal(u, v)
+
+
 def test_append_special_rows(gpu):
     """Zero rows (s = 0, codes 0), rows with inf and NaN (read back as NaN), next to ordinary heads."""
     _say("append special rows")

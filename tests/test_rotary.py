@@ -201,3 +201,22 @@ def test_entry_points_check_before_touching_a_device():
                dict(cache=2), dict(cache=3), dict(scale=fake)):
         assert append(**kw) == rt.TB_E_INVALID, kw
         assert "tb_rope_kv_append" in lib.tb_last_error().decode()
+
+
+def test_caches_of_one_head_or_page_in_either_order():
+    """Strides of dimensions of size 1 say nothing: [pages, page, 1, D] pools beside [pages, 1, page, D] ones."""
+    for pages, heads, page in ((4, 1, 8), (1, 2, 8), (1, 1, 1), (4, 2, 1)):
+        k = torch.zeros(pages, heads, page, 16).half()
+        v = torch.zeros(pages, page, heads, 16).half().permute(0, 2, 1, 3)
+        if heads > 1 and page > 1:
+            v = torch.zeros(pages + 1, 3, heads, page, 16).half()[1:, 1]      # one page of a wider pool
+        assert pages > 1 and page == 1 or v.stride() != k.stride() or k.numel() == 16
+        assert paged.check_cache("op", torch.float16, heads, 16, k, v, None, None) == (pages, page)
+        c = k.to(torch.float8_e4m3fn)
+        scales = torch.zeros(pages, heads, page), torch.zeros(pages, page, heads).transpose(1, 2)
+        if heads > 1 and page > 1:
+            scales = scales[0], torch.zeros(pages + 1, 3, heads, page)[1:, 1]
+        assert paged.check_cache("op", torch.float16, heads, 16, c, c, *scales) == (pages, page)
+    one = torch.zeros(4, 1, 1, 16).half().expand(4, 1, 8, 16)                 # but no dimension may be expanded
+    with pytest.raises(ValueError, match="expanded"):
+        paged.check_cache("op", torch.float16, 1, 16, one, one, None, None)

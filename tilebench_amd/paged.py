@@ -49,10 +49,16 @@ def check_rotation(op, q, k, positions, inv_freq, axes):
     return T, Hq, 0 if k is None else kshape[1], D, 2 * pairs, A
 
 
+def _strides(x):
+    """Strides but for dimensions of size 1, where they do not matter."""
+    return [s for s, n in zip(x.stride(), x.shape) if n > 1]
+
+
 def check_cache(op, dtype, heads, head_dim, k_cache, v_cache, k_scale, v_scale):
     """(pages, page_size) of a cache that holds `heads` heads of `head_dim` for inputs of `dtype`."""
     shape, strides, kind = k_cache.shape, k_cache.stride(), k_cache.dtype
-    if len(shape) != 4 or v_cache.shape != shape or v_cache.stride() != strides:
+    if len(shape) != 4 or v_cache.shape != shape or (v_cache.stride() != strides
+                                                     and _strides(v_cache) != _strides(k_cache)):
         raise ValueError(f"{op}: k_cache and v_cache must be [pages, heads, page_size, head_dim] of one shape and "
                          "memory order")
     pages, h, page, d = shape
@@ -62,7 +68,7 @@ def check_cache(op, dtype, heads, head_dim, k_cache, v_cache, k_scale, v_scale):
         raise ValueError(f"{op}: the page size must be a power of two up to {MAX_PAGE} (got {page})")
     if pages < 1 or pages * page >= 1 << 31:
         raise ValueError(f"{op}: a cache holds 1 to 2^31 - 1 slots (got {pages} pages of {page})")
-    if strides[3] != 1 or 0 in strides:
+    if strides[3] != 1 or (0 in strides and 0 in _strides(k_cache)):
         raise ValueError(f"{op}: the cache's last dimension must be contiguous and no dimension expanded")
     if v_cache.dtype is not kind or (kind is not dtype and kind is not torch.float8_e4m3fn):
         raise TypeError(f"{op}: the caches must be {dtype} like the inputs, or float8_e4m3fn")
@@ -72,7 +78,9 @@ def check_cache(op, dtype, heads, head_dim, k_cache, v_cache, k_scale, v_scale):
         if k_scale.dtype is not torch.float32 or v_scale.dtype is not torch.float32:
             raise TypeError(f"{op}: scales must be float32")
         order = k_scale.stride()
-        if k_scale.shape != shape[:3] or v_scale.shape != shape[:3] or v_scale.stride() != order or 0 in order:
+        if k_scale.shape != shape[:3] or v_scale.shape != shape[:3] \
+                or (v_scale.stride() != order and _strides(v_scale) != _strides(k_scale)) \
+                or (0 in order and 0 in _strides(k_scale)):
             raise ValueError(f"{op}: scales must be [pages, heads, page_size] of one memory order, no dimension "
                              "expanded")
     elif k_scale is not None or v_scale is not None:
