@@ -228,6 +228,9 @@ tb_status tb_moe_w4a16_down(const uint16_t* act, const int32_t* sorted_ids, cons
                             hipStream_t stream);
 tb_status tb_moe_combine(const uint16_t* y, const int32_t* topk_ids, uint16_t* out, int64_t tokens, int64_t topk,
                          int64_t experts, int64_t H, hipStream_t stream);
+/* tb_moe_combine of bf16 rows (the layers of other weight formats). */
+tb_status tb_moe_combine_bf16(const uint16_t* y, const int32_t* topk_ids, uint16_t* out, int64_t tokens, int64_t topk,
+                              int64_t experts, int64_t H, hipStream_t stream);
 tb_status tb_fused_moe_w4a16_workspace_size(int64_t tokens, int64_t topk, int64_t experts, int64_t H, int64_t I,
                                             int64_t* bytes);
 tb_status tb_fused_moe_w4a16(const uint16_t* X, const float* logits, const uint8_t* W13, const uint16_t* S13,
@@ -351,7 +354,8 @@ tb_status tb_matmul_workspace_size(int dtype, int64_t M, int64_t N, int64_t K, i
  *   TB_OP_W4A16_GROUPED    R                N      E
  *   TB_OP_MOE_GATE_UP      tokens * topk    2 I    E
  *   TB_OP_MOE_DOWN         tokens * topk    H      E
- *   TB_OP_FP8_SCALED, _FP8_BLOCK, _MATMUL_F32, _F16, _FP8, _INT8: ignored
+ *   TB_OP_FP8_SCALED, _FP8_BLOCK, _MATMUL_F32, _F16, _FP8, _INT8, _MXFP4: ignored
+ *   TB_OP_MXFP4_GROUPED    R                N      E
  * Replaces: the get_last_config() of the reference's tuned operators
  * (matmul_fp32_fp16_fp8/impl_triton.py:124), which reports the configuration
  * that ran.
@@ -366,7 +370,9 @@ enum {
   TB_OP_MATMUL_F32 = 6,
   TB_OP_MATMUL_F16 = 7,
   TB_OP_MATMUL_FP8 = 8,
-  TB_OP_MATMUL_INT8 = 9
+  TB_OP_MATMUL_INT8 = 9,
+  TB_OP_MXFP4 = 16,
+  TB_OP_MXFP4_GROUPED = 17
 };
 typedef struct {
   const char* kernel;
@@ -531,6 +537,84 @@ tb_status tb_shared_prefix_attention(const void* q, const void* k_cache, const v
 tb_status tb_shared_prefix_attention_workspace_size(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t G,
                                                     int64_t Wp, int64_t B, int64_t W, int64_t page_size,
                                                     int64_t max_q, int cache_dtype, int64_t* bytes);
+
+/*
+ * Routing to experts.  Per row of logits [T, E] (dtype 0 = fp32, 1 = fp16, 2 =
+ * bf16; `row` elements between rows):
+ *   s = 1 / (1 + exp(-x)), or with softmax != 0 exp(x - max) / sum;
+ *   c = s + bias (fp32 [E], or null: c = s);
+ *   the E experts are `groups` groups of consecutive ones; a group's score is
+ *   the sum of its group_top (1 or 2) largest c, and the experts of the
+ *   top_groups best groups can be chosen (equal scores: lowest group first);
+ *   ids int32 [T, k]: the k largest c, descending (equal: lowest expert first);
+ *   weights fp32 [T, k]: scale * s of these, over their sum if renormalize.
+ * Computed in fp64 and rounded once.  NaN ranks above every number; a softmax
+ * row of -inf alone has scores 0, and weights that sum to 0 are 0.
+ * Requires E <= 1024, E % groups == 0, groups <= 64, k <= 32 and k <=
+ * top_groups * E / groups, E / groups >= group_top.
+ * Beside tb_moe_topk_gating (softmax of the chosen logits alone), which replaces
+ * moe_topk_gating/impl_triton.py:58 run(logits, M, E, k).
+ */
+tb_status tb_moe_expert_routing(const void* logits, const float* bias, float* weights, int32_t* ids, int64_t T,
+                                int64_t E, int64_t k, int64_t groups, int64_t top_groups, int64_t group_top,
+                                int64_t row, int softmax, int renormalize, double scale, int dtype,
+                                hipStream_t stream);
+
+/*
+ * Microscaled 4-bit floating point (MXFP4).  A matrix [rows, K] is
+ *   codes  uint8 [rows, K / 2], dense: e2m1 (bit 3 the sign; 0, 0.5, 1, 1.5, 2,
+ *          3, 4, 6), channel 2 j in the low and 2 j + 1 in the high four bits;
+ *   scales uint8 [rows, K / 32], scale_row bytes between rows: 2^(scale - 127)
+ *          for 32 channels, 255 is NaN.
+ *
+ * tb_mxfp4_quant: x [M, K] (dtype 0 = fp32, 1 = fp16, 2 = bf16; x_row elements
+ *   between rows) to codes and scales.  A block's scale is 2^(floor(log2(largest
+ *   magnitude)) - 2), held to 2^-127 .. 2^127; codes are x / scale rounded to
+ *   nearest even, beyond 6 to 6.  A zero block has scale 0, a block with inf or
+ *   NaN has scale 255 and codes 0.
+ *   gated: x is [M, 2 K], gate then up, and the values are silu(gate) * up =
+ *   gate / (1 + exp(-gate)) * up; scales and codes are those of its fp64 value.
+ *   Requires K % 32 == 0, x and its rows 16-byte aligned, codes 4-byte aligned.
+ * tb_mxfp4_dequant: y [M, K] of `dtype` = code * scale, rounded once.  Requires
+ *   K % 32 == 0, codes 4-byte and y 16-byte aligned.
+ * Nearest in the reference: quantize_global/impl_triton.py:31 run(x) and
+ *   weight_dequant/impl_triton.py:43 run(X, S, M, N, TILE_SIZE).
+ */
+tb_status tb_mxfp4_quant(const void* x, uint8_t* codes, uint8_t* scales, int64_t M, int64_t K, int64_t x_row,
+                         int64_t scale_row, int gated, int dtype, hipStream_t stream);
+tb_status tb_mxfp4_dequant(const uint8_t* codes, const uint8_t* scales, void* y, int64_t M, int64_t K,
+                           int64_t scale_row, int dtype, hipStream_t stream);
+
+/*
+ * Products of MXFP4 matrices on the scaled 4-bit matrix cores, fp32
+ * accumulation, one rounding to dtype (1 = fp16, 2 = bf16).  Results are
+ * reproducible bit for bit; a row's last bit may depend on the number of rows
+ * (calls of few rows add four parts of K in order).  A scale of 255 makes the
+ * results that it takes part in NaN.
+ *
+ * tb_mxfp4_gemm: Y [M, N] = a [M, K] w [N, K]^T.
+ * tb_moe_mxfp4_grouped_gemm: product rows m = offsets[e] .. offsets[e + 1] - 1
+ *   (int32 [experts + 1], ascending) use w[e] of w [experts, N, K] (codes dense,
+ *   sw_expert bytes between experts' scales).  Product row m is
+ *     row m of a, or with gather (int32 [R]) row gather[m] / topk (a negative one or
+ *     one past a_rows: a row of zeros);
+ *     written to row m of Y [R, N], or with scatter (int32 [R]) to row scatter[m]
+ *     (outside 0 .. R - 1: not written; one that is named twice holds either),
+ *     there times weights[row of Y] (fp32 [R], null: 1) before the rounding.
+ *   tb_moe_align's sorted ids are such gather rows of tokens and scatter rows of
+ *   pairs.  Rows of Y that no product row goes to are left as they were.
+ *   Offsets are held to 0 .. R.
+ * Requires K % 32 == 0, a and w 16-byte aligned, rows of scales (sa_row, sw_row,
+ * sw_expert) on 4 bytes; experts <= 4096; gathered a below 2 GiB.
+ * Nearest in the reference: matmul_fp32_fp16_fp8/impl_triton.py:124 run(a, b).
+ */
+tb_status tb_mxfp4_gemm(const uint8_t* a, const uint8_t* sa, const uint8_t* w, const uint8_t* sw, void* y, int64_t M,
+                        int64_t N, int64_t K, int64_t sa_row, int64_t sw_row, int dtype, hipStream_t stream);
+tb_status tb_moe_mxfp4_grouped_gemm(const uint8_t* a, const uint8_t* sa, const uint8_t* w, const uint8_t* sw,
+                                    const int32_t* offsets, const int32_t* gather, const int32_t* scatter,
+                                    const float* weights, void* y, int64_t R, int64_t a_rows, int64_t experts,
+                                    int64_t N, int64_t K, int64_t topk, int64_t sa_row, int64_t sw_row,
+                                    int64_t sw_expert, int dtype, hipStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -123,13 +123,13 @@ __global__ void __launch_bounds__(ALIGN_THREADS)
   }
 }
 
-// out[t, c .. c+7] = fp16(sum_j fp32(y[t * topk + j, c .. c+7])), slots with an
+// out[t, c .. c+7] = T(sum_j fp32(y[t * topk + j, c .. c+7])), T fp16 or bf16, slots with an
 // expert id outside [0, experts) skipped.  One 16-byte granule per thread.
 // All of a token's ids are loaded first, then all its rows (an unrouted slot
 // through an out-of-range offset, reading zeros without memory traffic, and
 // skipped in the sum so that results do not depend on it): one round trip
 // per thread instead of one per slot.
-template <int KMAX>
+template <int KMAX, bool BF16>
 __global__ void __launch_bounds__(256)
     moe_combine_kernel(const u32x4* __restrict__ y, const int* __restrict__ ids, u32x4* __restrict__ out,
                        int64_t tokens, int topk, int experts, int64_t g_per_row) {
@@ -155,14 +155,21 @@ __global__ void __launch_bounds__(256)
     if (!(j < topk && (unsigned)id[j] < (unsigned)experts)) continue;  // slot order, unrouted slots skipped
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const f16x2 h = as_h2(v[j][q]);
-      s[2 * q] += (float)h[0];
-      s[2 * q + 1] += (float)h[1];
+      if constexpr (BF16) {
+        s[2 * q] += __builtin_bit_cast(float, v[j][q] << 16);
+        s[2 * q + 1] += __builtin_bit_cast(float, v[j][q] & 0xFFFF0000u);
+      } else {
+        const f16x2 h = as_h2(v[j][q]);
+        s[2 * q] += (float)h[0];
+        s[2 * q + 1] += (float)h[1];
+      }
     }
   }
   u32x4 o;
 #pragma unroll
-  for (int q = 0; q < 4; ++q) o[q] = as_u32(f16x2{(_Float16)s[2 * q], (_Float16)s[2 * q + 1]});
+  for (int q = 0; q < 4; ++q)
+    o[q] = BF16 ? bf16_bits(s[2 * q]) | bf16_bits(s[2 * q + 1]) << 16
+                : as_u32(f16x2{(_Float16)s[2 * q], (_Float16)s[2 * q + 1]});
   out[g] = o;
 }
 
@@ -216,30 +223,43 @@ extern "C" tb_status tb_moe_align(const int32_t* topk_ids, int64_t pairs, int64_
   return tb::launch_status("tb_moe_align");
 }
 
-extern "C" tb_status tb_moe_combine(const uint16_t* y, const int32_t* topk_ids, uint16_t* out, int64_t tokens,
-                                    int64_t topk, int64_t experts, int64_t H, hipStream_t stream) {
+namespace {
+template <bool BF16>
+tb_status combine(const char* fn, const uint16_t* y, const int32_t* topk_ids, uint16_t* out, int64_t tokens, int64_t topk,
+                  int64_t experts, int64_t H, hipStream_t stream) {
   using namespace tb::moe;
-  TB_CHECK_ARG(y && topk_ids && out, "tb_moe_combine: null pointer");
-  TB_CHECK_ARG(tokens > 0 && topk > 0 && experts > 0 && H > 0, "tb_moe_combine: sizes must be positive");
-  TB_CHECK_ARG(H % 8 == 0, "tb_moe_combine: H must be a multiple of 8 (got %lld)", (long long)H);
-  TB_CHECK_ARG(tokens * topk < (1ll << 31), "tb_moe_combine: tokens * topk must be < 2^31");
-  TB_CHECK_ARG(topk <= 32, "tb_moe_combine: topk must be at most 32 (got %lld)", (long long)topk);
-  TB_CHECK_ARG(topk * H * 2 < (1ll << 31), "tb_moe_combine: a token's topk rows must be < 2 GiB");
+  TB_CHECK_ARG(y && topk_ids && out, "%s: null pointer", fn);
+  TB_CHECK_ARG(tokens > 0 && topk > 0 && experts > 0 && H > 0, "%s: sizes must be positive", fn);
+  TB_CHECK_ARG(H % 8 == 0, "%s: H must be a multiple of 8 (got %lld)", fn, (long long)H);
+  TB_CHECK_ARG(tokens * topk < (1ll << 31), "%s: tokens * topk must be < 2^31", fn);
+  TB_CHECK_ARG(topk <= 32, "%s: topk must be at most 32 (got %lld)", fn, (long long)topk);
+  TB_CHECK_ARG(topk * H * 2 < (1ll << 31), "%s: a token's topk rows must be < 2 GiB", fn);
   TB_CHECK_ALIGN(y, 16, "y");
   TB_CHECK_ALIGN(out, 16, "out");
   TB_CHECK_ALIGN(topk_ids, 4, "topk_ids");
   const int64_t g_per_row = H / 8, granules = tokens * g_per_row;
   const int64_t blocks = (granules + 255) / 256;
-  TB_CHECK_ARG(blocks < (1ll << 31), "tb_moe_combine: problem too large");
+  TB_CHECK_ARG(blocks < (1ll << 31), "%s: problem too large", fn);
   auto* yv = reinterpret_cast<const tb::u32x4*>(y);
   auto* ov = reinterpret_cast<tb::u32x4*>(out);
   if (topk <= 8)
-    hipLaunchKernelGGL(moe_combine_kernel<8>, dim3((unsigned)blocks), dim3(256), 0, stream, yv, topk_ids, ov, tokens,
+    hipLaunchKernelGGL((moe_combine_kernel<8, BF16>), dim3((unsigned)blocks), dim3(256), 0, stream, yv, topk_ids, ov, tokens,
                        (int)topk, (int)experts, g_per_row);
   else
-    hipLaunchKernelGGL(moe_combine_kernel<32>, dim3((unsigned)blocks), dim3(256), 0, stream, yv, topk_ids, ov, tokens,
+    hipLaunchKernelGGL((moe_combine_kernel<32, BF16>), dim3((unsigned)blocks), dim3(256), 0, stream, yv, topk_ids, ov, tokens,
                        (int)topk, (int)experts, g_per_row);
-  return tb::launch_status("tb_moe_combine");
+  return tb::launch_status(fn);
+}
+}  // namespace
+
+extern "C" tb_status tb_moe_combine(const uint16_t* y, const int32_t* topk_ids, uint16_t* out, int64_t tokens,
+                                    int64_t topk, int64_t experts, int64_t H, hipStream_t stream) {
+  return combine<false>("tb_moe_combine", y, topk_ids, out, tokens, topk, experts, H, stream);
+}
+
+extern "C" tb_status tb_moe_combine_bf16(const uint16_t* y, const int32_t* topk_ids, uint16_t* out, int64_t tokens,
+                                         int64_t topk, int64_t experts, int64_t H, hipStream_t stream) {
+  return combine<true>("tb_moe_combine_bf16", y, topk_ids, out, tokens, topk, experts, H, stream);
 }
 
 extern "C" tb_status tb_fused_moe_w4a16_workspace_size(int64_t tokens, int64_t topk, int64_t experts, int64_t H,

@@ -165,6 +165,18 @@ inline NtTile pick_nt_tile(int64_t M, int64_t N, int64_t Kb) {
   return best;
 }
 
+enum MxTile { MX_256 = 0, MX_32x32, MX_64x64, MX_128x128 };
+
+// The tile of an MXFP4 product of M rows, dense (experts = 0) or over `experts` experts.
+inline MxTile pick_mx_tile(int64_t M, int64_t N, int64_t K, int64_t experts) {
+  const int64_t each = experts ? M / std::min(M, experts) : M;
+  if (each <= 32) return MX_32x32;
+  const int64_t rows = experts ? each : M, times = experts ? std::min(M, experts) : 1;
+  auto tiles = [&](int64_t t) { return times * ((rows + t - 1) / t) * ((N + t - 1) / t); };
+  if (tiles(256) >= 192) return MX_256;
+  return tiles(128) >= 192 ? MX_128x128 : MX_64x64;
+}
+
 constexpr int DEC_WAVES = 8, DEC_UNIT = 32, DEC_MAX_SPLITS = 16;
 struct DecodePlan {
   int cols;       // columns of a slab, 128 or 256

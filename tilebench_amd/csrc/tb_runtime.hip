@@ -264,11 +264,14 @@ tb_status tb_probe_copy(const void* src, void* dst, int64_t bytes, hipStream_t s
 
 tb_status tb_gemm_tile(int op, int64_t M, int64_t N, int64_t K, int64_t experts, tb_tile* tile) {
   TB_CHECK_ARG(tile != nullptr, "tb_gemm_tile: null output");
-  TB_CHECK_ARG(op >= TB_OP_W4A16 && op <= TB_OP_MATMUL_INT8, "tb_gemm_tile: unknown operator %d", op);
-  const bool expert_op = op >= TB_OP_W4A16_GROUPED && op <= TB_OP_MOE_DOWN;
+  TB_CHECK_ARG((op >= TB_OP_W4A16 && op <= TB_OP_MATMUL_INT8) || op == TB_OP_MXFP4 || op == TB_OP_MXFP4_GROUPED,
+               "tb_gemm_tile: unknown operator %d", op);
+  const bool expert_op = (op >= TB_OP_W4A16_GROUPED && op <= TB_OP_MOE_DOWN) || op == TB_OP_MXFP4_GROUPED;
   TB_CHECK_ARG(M > 0 && N > 0 && K > 0 && (experts > 0 || !expert_op), "tb_gemm_tile: sizes must be positive");
   if (op == TB_OP_W4A16)
     tb::describe_w4a16(M, N, K, tile);
+  else if (op == TB_OP_MXFP4 || op == TB_OP_MXFP4_GROUPED)
+    tb::describe_mxfp4(M, N, K, expert_op ? experts : 0, tile);
   else if (expert_op)
     tb::describe_experts(op, M, N, experts, tile);
   else if (op == TB_OP_FP8_SCALED)

@@ -410,6 +410,60 @@ def generate_shared_prefix_attention_inputs(B, prefix, own, Hq=32, Hkv=8, D=128,
             *pools[2:])
 
 
+# ----------------------------------------------------------------------------- MXFP4 expert layers
+
+
+def mxfp4_matrix(x, device=DEFAULT_DEVICE):
+    """Codes and scales of x [.., K] by the torch reference, rows of scales padded as the quantiser leaves them."""
+    from tilebench_amd.benchmarks.experts.mxfp4_quant import impl_torch as quant_ref
+    from tilebench_amd.experts import empty_scales
+
+    codes, scales = quant_ref.run(x)
+    return codes.to(device), empty_scales(x.shape[:-1], x.shape[-1], device).copy_(scales)
+
+
+def generate_moe_expert_routing_inputs(T, E=256, k=8, groups=8, top_groups=4, group_top=2, score="sigmoid",
+                                       dtype=torch.float32, seed=0, device=DEFAULT_DEVICE):
+    g = _gen(seed)
+    logits = (torch.randn(T, E, generator=g) * 1.5).to(dtype)
+    bias = torch.randn(E, generator=g) * 0.05
+    return logits.to(device), int(k), bias.to(device), int(groups), int(top_groups), int(group_top), score
+
+
+def generate_mxfp4_quant_inputs(M, K, gated=False, dtype=torch.float16, seed=0, device=DEFAULT_DEVICE):
+    x = fp8_activations(M, K * (2 if gated else 1), seed=seed).to(dtype)
+    return x.to(device), bool(gated)
+
+
+def generate_mxfp4_dequant_inputs(M, K, dtype=torch.bfloat16, seed=0, device=DEFAULT_DEVICE):
+    return (*mxfp4_matrix(torch.randn(M, K, generator=_gen(seed)) * 0.02, device), dtype)
+
+
+def generate_mxfp4_gemm_inputs(M, N, K, dtype=torch.bfloat16, seed=0, device=DEFAULT_DEVICE):
+    g = _gen(seed)
+    return (*mxfp4_matrix(torch.randn(M, K, generator=g), device),
+            *mxfp4_matrix(torch.randn(N, K, generator=g) * 0.02, device), dtype)
+
+
+def generate_moe_mxfp4_grouped_gemm_inputs(tokens, topk=8, experts=64, K=4096, N=2816, zipf_s=1.1, dtype=torch.bfloat16,
+                                           seed=0, device=DEFAULT_DEVICE):
+    """Tokens, the experts' weights, and the pairs of a Zipf routing sorted by expert (gathered rows)."""
+    g = _gen(seed)
+    flat = zipf_routing(tokens, topk, experts, zipf_s, seed).reshape(-1)
+    offsets = torch.zeros(experts + 1, dtype=torch.int64)
+    offsets[1:] = torch.cumsum(torch.bincount(flat, minlength=experts), 0)
+    pairs = torch.sort(flat, stable=True).indices
+    a = mxfp4_matrix(torch.randn(tokens, K, generator=g), device)
+    parts = [mxfp4_matrix(torch.randn(N, K, generator=g) * 0.02, device) for _ in range(experts)]
+    from tilebench_amd.experts import empty_scales
+
+    scales = empty_scales((experts, N), K, device)
+    for e, (_, s) in enumerate(parts):
+        scales[e].copy_(s)
+    return (*a, torch.stack([c for c, _ in parts]), scales, offsets.int().to(device), pairs.int().to(device), int(topk),
+            None, None, dtype)
+
+
 GENERATORS = {
     "int4_dequant": generate_int4_dequant_inputs,
     "w4a16_gemm": generate_w4a16_gemm_inputs,
@@ -428,6 +482,11 @@ GENERATORS = {
     "rotary_axes": generate_rotary_axes_inputs,
     "rope_kv_append": generate_rope_kv_append_inputs,
     "shared_prefix_attention": generate_shared_prefix_attention_inputs,
+    "moe_expert_routing": generate_moe_expert_routing_inputs,
+    "mxfp4_quant": generate_mxfp4_quant_inputs,
+    "mxfp4_dequant": generate_mxfp4_dequant_inputs,
+    "mxfp4_gemm": generate_mxfp4_gemm_inputs,
+    "moe_mxfp4_grouped_gemm": generate_moe_mxfp4_grouped_gemm_inputs,
 }
 
 
@@ -443,9 +502,9 @@ def infer_problem_size(operator_name, params):
     if operator_name == "int4_dequant":
         return p.get("K", 1) * p.get("N", 1)
     if operator_name in ("w4a16_gemm", "fp8_scaled_gemm", "fp8_block_scaled_gemm", "matmul_int8",
-                         "matmul_fp32_fp16_fp8"):
+                         "matmul_fp32_fp16_fp8", "mxfp4_gemm"):
         return 2 * p.get("M", 1) * p.get("N", 1) * p.get("K", 1)
-    if operator_name in ("fp8_act_quant", "fp8_act_quant_blocks"):
+    if operator_name in ("fp8_act_quant", "fp8_act_quant_blocks", "mxfp4_quant", "mxfp4_dequant"):
         return p.get("M", 1) * p.get("K", 1)
     if operator_name == "moe_topk_gating":
         return p.get("M", 1) * p.get("E", 1)
@@ -453,7 +512,9 @@ def infer_problem_size(operator_name, params):
         return p.get("M", 1) * p.get("N", p.get("M", 1))
     if operator_name == "dequantize_rowwise":
         return p.get("rows", 1) * p.get("cols", 1)
-    if operator_name == "moe_w4a16_grouped_gemm":
+    if operator_name == "moe_expert_routing":
+        return p.get("T", 1) * p.get("E", 256)
+    if operator_name in ("moe_w4a16_grouped_gemm", "moe_mxfp4_grouped_gemm"):
         return 2 * p.get("tokens", 1) * p.get("topk", 1) * p.get("K", 1) * p.get("N", 1)
     if operator_name == "fused_moe_w4a16":
         return 6 * p.get("tokens", 1) * p.get("topk", 1) * p.get("H", 1) * p.get("I", 1)

@@ -14,14 +14,18 @@ BENCHMARK_ROOT = PACKAGE_ROOT / "benchmarks"
 OPERATOR_ROOT = BENCHMARK_ROOT / "operators"
 #: operators of the attention path, which read and write a key/value cache that the caller keeps
 SERVING_ROOT = BENCHMARK_ROOT / "serving"
+#: operators of expert layers with MXFP4 weights: routing, quantisation, products
+EXPERTS_ROOT = BENCHMARK_ROOT / "experts"
 PEAK_PERFORMANCE_ROOT = DATA_ROOT / "peak_performance"
 REPO_ROOT = Path(os.environ.get("TILEBENCH_REPO_ROOT") or PACKAGE_ROOT.parent).resolve()
 RESULTS_ROOT = REPO_ROOT / "results"
 
 
 def operator_dir(operator_name: str) -> Path:
-    serving = SERVING_ROOT / operator_name
-    return serving if serving.is_dir() else OPERATOR_ROOT / operator_name
+    for root in (SERVING_ROOT, EXPERTS_ROOT):
+        if (root / operator_name).is_dir():
+            return root / operator_name
+    return OPERATOR_ROOT / operator_name
 
 
 def operator_package(operator_name: str) -> str:
@@ -42,3 +46,7 @@ def list_operators() -> list[str]:
 
 def list_serving_operators() -> list[str]:
     return sorted(p.parent.name for p in SERVING_ROOT.glob("*/config.yaml"))
+
+
+def list_expert_operators() -> list[str]:
+    return sorted(p.parent.name for p in EXPERTS_ROOT.glob("*/config.yaml"))

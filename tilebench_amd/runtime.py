@@ -40,6 +40,7 @@ class GemmTile(ctypes.Structure):
 #: tb_gemm_tile's operators
 (OP_W4A16, OP_W4A16_GROUPED, OP_MOE_GATE_UP, OP_MOE_DOWN, OP_FP8_SCALED, OP_FP8_BLOCK, OP_MATMUL_F32, OP_MATMUL_F16,
  OP_MATMUL_FP8, OP_MATMUL_INT8) = range(10)
+OP_MXFP4, OP_MXFP4_GROUPED = 16, 17
 
 #: symbol -> argtypes (every entry point returns an int status).
 SIGNATURES: dict[str, list] = {
@@ -56,6 +57,7 @@ SIGNATURES: dict[str, list] = {
     "tb_moe_w4a16_gate_up": [_c_p] * 7 + [_c_i64] * 6 + [_c_p],
     "tb_moe_w4a16_down": [_c_p] * 8 + [_c_i64] * 5 + [_c_p],
     "tb_moe_combine": [_c_p, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_p],
+    "tb_moe_combine_bf16": [_c_p, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_p],
     "tb_fused_moe_w4a16_workspace_size": [_c_i64] * 5 + [ctypes.POINTER(_c_i64)],
     "tb_fused_moe_w4a16": [_c_p] * 9 + [_c_i64] * 7 + [_c_p, _c_i64, _c_p],
     "tb_fp8_scaled_gemm": [_c_p, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_p],
@@ -72,6 +74,11 @@ SIGNATURES: dict[str, list] = {
     "tb_rope_kv_append": [_c_p] * 12 + [_c_i64] * 20 + [_c_int] * 3 + [_c_p],
     "tb_shared_prefix_attention": [_c_p] * 13 + [_c_i64] * 19 + [ctypes.c_double, _c_int, _c_int, _c_p, _c_i64, _c_p],
     "tb_shared_prefix_attention_workspace_size": [_c_i64] * 10 + [_c_int, ctypes.POINTER(_c_i64)],
+    "tb_moe_expert_routing": [_c_p] * 4 + [_c_i64] * 7 + [_c_int] * 2 + [ctypes.c_double, _c_int, _c_p],
+    "tb_mxfp4_quant": [_c_p] * 3 + [_c_i64] * 4 + [_c_int] * 2 + [_c_p],
+    "tb_mxfp4_dequant": [_c_p] * 3 + [_c_i64] * 3 + [_c_int, _c_p],
+    "tb_mxfp4_gemm": [_c_p] * 5 + [_c_i64] * 5 + [_c_int, _c_p],
+    "tb_moe_mxfp4_grouped_gemm": [_c_p] * 9 + [_c_i64] * 9 + [_c_int, _c_p],
     "tb_gemm_tile": [_c_int, _c_i64, _c_i64, _c_i64, _c_i64, ctypes.POINTER(GemmTile)],
     "tb_l2_flush": [_c_p, _c_i64, _c_u32, _c_p],
     "tb_probe_copy": [_c_p, _c_p, _c_i64, _c_p],
