@@ -366,7 +366,9 @@ def check_route(logits, k, bias=None, scale=1.0, renormalize=True, **kw):
 @pytest.mark.parametrize("T_,E,k,groups,top_groups,group_top", [
     (1, 256, 8, 8, 4, 2), (67, 256, 8, 8, 4, 2), (130, 60, 4, 1, 1, 1), (33, 384, 7, 16, 11, 1), (20, 1024, 32, 64, 3, 2),
     (9, 1, 1, 1, 1, 1), (11, 7, 7, 1, 1, 1), (50, 64, 6, 4, 1, 2), (40, 160, 6, 8, 3, 1), (21, 500, 3, 5, 2, 2),
-    (70, 128, 2, 2, 2, 2), (300, 8, 2, 1, 1, 1)])
+    (70, 128, 2, 2, 2, 2), (300, 8, 2, 1, 1, 1), (19, 1024, 8, 8, 4, 2), (23, 512, 8, 1, 1, 1), (10, 768, 8, 16, 5, 2),
+    (13, 700, 5, 7, 3, 1), (37, 12, 3, 2, 1, 2), (31, 90, 8, 5, 2, 2), (31, 90, 5, 3, 2, 1), (15, 90, 8, 15, 7, 2),
+    (9, 128, 8, 64, 9, 2), (258, 250, 8, 1, 1, 1)])
 def test_routing(gpu, T_, E, k, groups, top_groups, group_top, score, dtype):
     say("routing", T_, E, k, groups, score, dtype)
     g = gen(E + k)
