@@ -180,9 +180,10 @@ def test_product(gpu, M, N, K, dtype):
     check_gemm(*matrix(M, K, M), *matrix(N, K, N + 1), dtype, K)
 
 
-@pytest.mark.parametrize("M,N,K,tile", [(1700, 1900, 96, 128), (3500, 3600, 96, 256), (3500, 3592, 1056, 256),
-                                        (3333, 3601, 256, 256)])
-def test_product_on_large_tiles(gpu, M, N, K, tile):
+@pytest.mark.parametrize("M,N,K,tile", [
+    (700, 700, 544, 32), (1700, 1900, 96, 64), (200, 2112, 7168, 64), (260, 4097, 4128, 64), (3500, 3600, 96, 128),
+    (1801, 8193, 1056, 128), (4001, 4001, 1056, 128), (2500, 6000, 2080, 256), (4001, 4004, 2080, 256), (2500, 6001, 2112, 256)])
+def test_product_on_every_tile(gpu, M, N, K, tile):
     say("gemm", M, N, K)
     assert rt.gemm_tile(rt.OP_MXFP4, M, N, K)["BM"] == tile
     check_gemm(*matrix(M, K, 1), *matrix(N, K, 2), torch.bfloat16, K)
@@ -293,12 +294,16 @@ def test_grouped_product(gpu, counts, N, K, dtype):
     assert torch.equal(check_grouped(a, sa, w, sw, offsets, dtype, K, scatter=scatter)[scatter.long()], plain)
 
 
-@pytest.mark.parametrize("rows,N,K,tile", [(330, 900, 96, 128), (1400, 1300, 96, 256), (1400, 1304, 1408, 256)])
-def test_grouped_product_on_large_tiles(gpu, rows, N, K, tile):
+@pytest.mark.parametrize("rows,N,K,tile", [
+    (20, 600, 288, (32, 32)), (330, 900, 96, (32, 128)), (50, 640, 1408, (32, 128)), (700, 600, 160, (32, 128)),
+    (6, 2815, 4128, (64, 64)), (1400, 1300, 96, (128, 128)), (600, 1200, 544, (128, 128)), (1400, 1304, 1408, (256, 256)),
+    (2000, 2001, 1056, (256, 256))])
+def test_grouped_product_on_every_tile(gpu, rows, N, K, tile):
     say("grouped", rows, N, K)
-    counts = [rows, rows // 3, 0, rows * 2, rows - 1, 300, 257, rows + 5]
+    counts = [rows, rows // 3, 0, rows * 2, rows - 1, 300, 257, rows + 5] if rows > 6 else [rows, 3, 0, 65, 1, 20, 4, 1]
     R, E = sum(counts), len(counts)
-    assert rt.gemm_tile(rt.OP_MXFP4_GROUPED, R, N, K, E)["BM"] == tile
+    picked = rt.gemm_tile(rt.OP_MXFP4_GROUPED, R, N, K, E)
+    assert (picked["BM"], picked["BN"]) == tile
     a, sa = matrix(R, K, 3)
     w, sw = experts_of(E, N, K, 4)
     offsets = torch.tensor([0, *torch.tensor(counts).cumsum(0).tolist()], dtype=torch.int32, device="cuda")

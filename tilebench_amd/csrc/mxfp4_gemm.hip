@@ -45,7 +45,7 @@ struct Args {
   int sa_row, sw_row;                     // bytes between rows of scales
   int tiles_m, tiles_n;                   // grouped: tiles_m is the upper bound
   int bf16, vec;                          // output type; rows of Y start on 16 bytes
-  Divisor by_topk;
+  Divisor by_topk, by_tiles_n, by_band;   // of tiles_n and of 8 tiles_n
 };
 
 // A tile: expert, first row, rows, first column.
@@ -59,55 +59,79 @@ __device__ __forceinline__ int xcd_run(int b, int n) {
   return x * q + min(x, rem) + (b >> 3);
 }
 
-// The tile'th row tile of TM rows over all experts; every wavefront for itself, 64 experts at a time.
-__device__ __forceinline__ bool find_rows(const Args& p, int tile, int tm, Place& at) {
-  const int lane = threadIdx.x & 63;
-  int before = 0;
-  for (int b = 0; b < p.E; b += 64) {
-    const int i = b + lane;
-    const int lo = i < p.E ? min(max(p.offsets[i], 0), p.M) : 0;
-    const int hi = i < p.E ? min(max(p.offsets[i + 1], 0), p.M) : 0;
-    const int own = hi > lo ? (hi - lo + tm - 1) / tm : 0;
-    int upto = own;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int o = __shfl_up(upto, d);
-      if (lane >= d) upto += o;
-    }
-    const uint64_t past = __ballot(tile < before + upto);
-    if (past) {
-      const int src = __builtin_ctzll(past);
-      const int begin = __builtin_amdgcn_readlane(lo, src), end = __builtin_amdgcn_readlane(hi, src);
-      const int first = before + __builtin_amdgcn_readlane(upto - own, src);
-      at.e = b + src;
-      at.m0 = begin + (tile - first) * tm;
-      at.rows = min(tm, end - at.m0);
-      return true;
-    }
-    before += __builtin_amdgcn_readlane(upto, 63);
-  }
-  return false;
+// v plus those of the lanes before (DPP: by 1, 2, 4 and 8 within rows of 16, then the rows' last lanes go on).
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, true);
+  return v;
 }
 
-// The tile of this block.  Dense: runs of blocks walk 8 row tiles, then the next
-// columns, so that a run's operands stay in its XCD's L2.  Grouped: an expert's
-// column tiles follow each other.
-template <bool GROUPED>
-__device__ __forceinline__ bool place(const Args& p, int tm, int tn, Place& at) {
-  const int idx = xcd_run(blockIdx.x, gridDim.x);
+// A run of row tiles: expert, its rows, the tiles before it and its own.
+struct Run {
+  int e, begin, end, before, tiles;
+};
+
+// Rows lo .. hi - 1 of lane's expert of the 64 from b on, and their tiles.
+__device__ __forceinline__ int tiles_of(const Args& p, int b, int shift, int& lo, int& hi) {
+  const int i = b + (threadIdx.x & 63);
+  lo = i < p.E ? min(max(p.offsets[i], 0), p.M) : 0;
+  hi = i < p.E ? min(max(p.offsets[i + 1], 0), p.M) : 0;
+  return hi > lo ? ((hi - lo - 1) >> shift) + 1 : 0;
+}
+
+// The tile of this block.  Runs of consecutive tiles go to one XCD and walk 8 row tiles (of an expert), then the next
+// columns, so that a run's operands stay in its L2.  Grouped: every wavefront counts the tiles of all experts, 64 at a
+// time, since runs have to share out the tiles there are, not the grid, which is an upper bound (64 experts of 512 rows,
+// N = 2816, K = 4096: 264 us, with runs of the grid, where the last XCDs find nothing, 396).
+template <bool GROUPED, int TM, int TN>
+__device__ __forceinline__ bool place(const Args& p, Place& at) {
+  int idx;
+  Run run{0, 0, p.M, 0, p.tiles_m};
   if constexpr (GROUPED) {
-    const int tile = idx / p.tiles_n;
-    at.n0 = (idx - tile * p.tiles_n) * tn;
-    return find_rows(p, tile, tm, at);
+    constexpr int SHIFT = TM == 32 ? 5 : TM == 64 ? 6 : TM == 128 ? 7 : 8;
+    static_assert(TM == 1 << SHIFT, "rows of a tile");
+    int lo, hi, total = 0, own = 0, upto = 0;
+    for (int b = 0; b < p.E; b += 64) {
+      own = tiles_of(p, b, SHIFT, lo, hi);
+      upto = wave_scan(own);
+      total = min(total + __builtin_amdgcn_readlane(upto, 63), p.tiles_m);  // more only if segments overlap
+    }
+    if ((int)blockIdx.x >= total * p.tiles_n) return false;
+    idx = xcd_run(blockIdx.x, total * p.tiles_n);
+    const int tile = p.by_tiles_n.divide(idx);
+    int before = 0;
+    uint64_t past = 0;
+    for (int b = 0; b < p.E; b += 64) {
+      if (p.E > 64) {
+        own = tiles_of(p, b, SHIFT, lo, hi);
+        upto = wave_scan(own);
+      }
+      past = __ballot(tile < before + upto);
+      run.e = b;
+      if (past) break;
+      before += __builtin_amdgcn_readlane(upto, 63);
+    }
+    const int src = __builtin_ctzll(past | 1ull << 63);
+    run.e += src;
+    run.begin = __builtin_amdgcn_readlane(lo, src);
+    run.end = __builtin_amdgcn_readlane(hi, src);
+    run.tiles = __builtin_amdgcn_readlane(own, src);
+    run.before = before + __builtin_amdgcn_readlane(upto, src) - run.tiles;
+    idx -= run.before * p.tiles_n;
   } else {
-    const int per = 8 * p.tiles_n, band = idx / per, in = idx - band * per;
-    const int rows = min(p.tiles_m - band * 8, 8);
-    at.e = 0;
-    at.m0 = (band * 8 + in % rows) * tm;
-    at.rows = min(tm, p.M - at.m0);
-    at.n0 = in / rows * tn;
-    return true;
+    idx = xcd_run(blockIdx.x, gridDim.x);
   }
+  const int band = p.by_band.divide(idx), in = idx - band * 8 * p.tiles_n;
+  const int rows = min(run.tiles - band * 8, 8), col = rows == 8 ? in >> 3 : in / rows;
+  at.e = run.e;
+  at.m0 = run.begin + (band * 8 + in - col * rows) * TM;
+  at.rows = min(TM, run.end - at.m0);
+  at.n0 = col * TN;
+  return true;
 }
 
 // Row of A of product row m (-1: none).
@@ -214,7 +238,7 @@ template <int KS, int D, bool GROUPED>
 __global__ void __launch_bounds__(64 * KS, KS / 4) mx_skinny(Args p) {
   __shared__ __attribute__((aligned(16))) float part[KS][32 * SK_ROW];
   Place at;
-  if (!place<GROUPED>(p, 32, SK_N, at)) return;
+  if (!place<GROUPED, 32, SK_N>(p, at)) return;
   const int t = threadIdx.x, lane = t & 63, r = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int K2 = p.K / 2, nk = (K2 + STEP - 1) / STEP;
@@ -308,32 +332,31 @@ __global__ void __launch_bounds__(64 * KS, KS / 4) mx_skinny(Args p) {
 
 // ------------------------------------------------------------------ tiles
 // One 64 FI x 64 FJ tile per block: four wavefronts, 2 x 2, of FI x FJ fragments of
-// 32 x 32.  Both operands and their scales stream HBM -> LDS by DMA, ST stages of one step.
-// Codes lie in rows of 128 bytes, 16-byte chunk c of row i at slot c ^ ((i ^ (i >> 3)) & 7), so that
-// writes and fragment reads are free of conflicts; scales in rows of 8 bytes.  A step is
-// four substeps of one MFMA per fragment pair.  While a substep's MFMAs run, the next
-// one's fragments are read (one ds_read_b128 each); the barrier sits before the last substep, when every
-// wavefront has read the stage: it then takes the DMAs of the step ST later.
-template <int FI_, int FJ_, int ST_>
+// 32 x 32.  Both operands and their scales stream HBM -> LDS by DMA.  Codes: ST stages of one step, rows of
+// 128 bytes, 16-byte chunk c of row i at slot c ^ ((i ^ (i >> 3)) & 7), so that writes and fragment reads are free of conflicts
+// (rows of 64 bytes and twice the stages: 1.3 to 1.4 times slower, a DMA then takes 16 lines for its KiB instead of 8).
+// Scales: two buffers of CS steps, 8 CS bytes of a row at once, since a load of a row's 8 bytes takes a whole line's time
+// and, from HBM, a whole line.  A step is four substeps of one MFMA per fragment pair.  While a substep's MFMAs run, the
+// next one's fragments are read (one ds_read_b128 each); the barrier sits before the last substep, when every wavefront
+// has read the stage: it then takes the DMAs of the step ST later.
+template <int FI_, int FJ_, int ST_, int CS_, int WM_ = 2>
 struct Tile {
-  static constexpr int FI = FI_, FJ = FJ_, ST = ST_;
-  static constexpr int TM = 64 * FI, TN = 64 * FJ;
+  static constexpr int FI = FI_, FJ = FJ_, ST = ST_, CS = CS_, WM = WM_;
+  static constexpr int TM = 32 * FI * WM, TN = 32 * FJ * (4 / WM);
   static constexpr int A_ST = TM * STEP, STAGE = (TM + TN) * STEP;     // A rows, then W rows
-  static constexpr int SC = (TM + TN) * STEP_BLOCKS, SC_OFF = ST * STAGE;
-  static constexpr int PAD_OFF = SC_OFF + ST * SC;                     // scale DMAs of wavefronts that have none land here
-  static constexpr int LDS_BYTES = PAD_OFF + 256;
-  static constexpr int C_STRIDE = TN + 8;  // 16-bit elements of a staged output row
-  static_assert(LDS_BYTES <= 160 * 1024 && TM * C_STRIDE * 2 <= LDS_BYTES, "LDS budget");
+  static constexpr int SROW = CS * STEP_BLOCKS, SC = (TM + TN) * SROW, SC_OFF = ST * STAGE;
+  static constexpr int NS = SC / 1024, DS = (NS + 3) / 4;              // scale DMAs of a buffer, of a wavefront
+  static constexpr int PAD_OFF = SC_OFF + 2 * SC;                      // those of wavefronts that have none land here
+  static constexpr int LDS_BYTES = PAD_OFF + (NS % 4 ? 1024 : 0);
+  static_assert(LDS_BYTES <= 160 * 1024 && SC % 1024 == 0 && TM * SROW % 1024 == 0, "LDS layout");
 };
 
-template <int FI, int FJ, int ST, bool GROUPED>
-__global__ void __launch_bounds__(256, 1) mx_tile(Args p) {
-  typedef Tile<FI, FJ, ST> C;
-  extern __shared__ __attribute__((aligned(128))) uint8_t lds[];
-  Place at;
-  if (!place<GROUPED>(p, C::TM, C::TN, at)) return;
+// The tile at `at` by WM x (4 / WM) wavefronts of FI x FJ fragments: 2 x 2 of them cover it, 1 x 4 its first half of rows.
+template <class C, int FI, int FJ, int WM, bool GROUPED>
+__device__ __forceinline__ void tile_product(const Args& p, const Place& at, uint8_t* lds) {
+  constexpr int ST = C::ST, CS = C::CS;
   const int t = threadIdx.x, lane = t & 63, r = lane & 31, h = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(t >> 6), wm = wave >> 1, wn = wave & 1;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6), wm = WM == 2 ? wave >> 1 : 0, wn = WM == 2 ? wave & 1 : wave;
   const int K2 = p.K / 2, nk = (K2 + STEP - 1) / STEP;
   const Operands o = operands<GROUPED>(p, at, C::TN);
   const i32x4 ra = rsrc4(o.a, o.a_bytes), rw = rsrc4(o.w, o.w_bytes);
@@ -345,12 +368,12 @@ __global__ void __launch_bounds__(256, 1) mx_tile(Args p) {
     return v;
   };
 
-  // A wavefront's DMAs of a step: 8 A rows each (lane L: row + L / 8, slot L % 8), 8 W rows each, then scales, 32 rows
-  // each (lane L: row + L / 2, scales 4 (L % 2) .. + 3).
-  constexpr int DA = 2 * FI, DW = 2 * FJ, NS = (C::TM + C::TN) / 32, DS = (NS + 3) / 4, PER = DA + DW + DS;
-  uint32_t off[PER];
+  // A wavefront's DMAs: of a step 8 A rows each (lane L: row + L / 8, slot L % 8), then 8 W rows each; of a scale
+  // buffer 16 bytes a lane, SROW / 16 lanes a row.
+  constexpr int DA = C::TM / 32, DW = C::TN / 32, PER = DA + DW, DS = C::DS, SL = C::SROW / 16;
+  uint32_t off[PER], soff[DS];
 #pragma unroll
-  for (int d = 0; d < DA + DW; ++d) {
+  for (int d = 0; d < PER; ++d) {
     const int row = 8 * (d < DA ? DA * wave + d : DW * wave + d - DA) + (lane >> 3);
     const uint32_t c = (uint32_t)((lane & 7) ^ ((row ^ (row >> 3)) & 7)) * 16u;
     const int at_row = d < DA ? buffer_row<GROUPED>(p, at, row) : at.n0 + row < p.N ? row : -1;
@@ -358,23 +381,24 @@ __global__ void __launch_bounds__(256, 1) mx_tile(Args p) {
   }
 #pragma unroll
   for (int d = 0; d < DS; ++d) {
-    const int q = wave + 4 * d, row = 32 * q + (lane >> 1), wrow = row - C::TM;
-    const int at_row = q >= NS ? -1 : row < C::TM ? buffer_row<GROUPED>(p, at, row) : at.n0 + wrow < p.N ? wrow : -1;
-    off[DA + DW + d] =
-        at_row >= 0 ? (uint32_t)at_row * (uint32_t)(row < C::TM ? p.sa_row : p.sw_row) + 4u * (lane & 1) : BUF_OOB;
+    const int q = wave + 4 * d, row = 64 / SL * q + lane / SL, wrow = row - C::TM;
+    const int at_row = q >= C::NS ? -1 : row < C::TM ? buffer_row<GROUPED>(p, at, row) : at.n0 + wrow < p.N ? wrow : -1;
+    soff[d] = at_row >= 0 ? (uint32_t)at_row * (uint32_t)(row < C::TM ? p.sa_row : p.sw_row) + 16u * (lane % SL) : BUF_OOB;
   }
+  // past the last step: empty buffers (zeros, no traffic)
   auto issue_one = [&](int k, int st, int d) __attribute__((always_inline)) {
-    const bool live = k < nk;  // past the last step: empty buffers (zeros, no traffic)
-    const uint32_t dst = lds0 + (uint32_t)(st * C::STAGE), soff = (uint32_t)(live ? k : 0) * STEP;
-    if (d < DA) {
-      dma16(dst + (uint32_t)(8 * (DA * wave + d) * STEP), off[d], live_rsrc(live, ra), soff);
-    } else if (d < DA + DW) {
-      dma16(dst + (uint32_t)(C::A_ST + 8 * (DW * wave + d - DA) * STEP), off[d], live_rsrc(live, rw), soff);
-    } else {
-      const int q = wave + 4 * (d - DA - DW);
-      dma4(lds0 + (uint32_t)(q < NS ? C::SC_OFF + st * C::SC + q * 256 : C::PAD_OFF), off[d],
-           live_rsrc(live, q * 32 < C::TM ? rsa : rsw), (uint32_t)(live ? k : 0) * STEP_BLOCKS);
-    }
+    const bool live = k < nk;
+    const uint32_t dst = lds0 + (uint32_t)(st * C::STAGE), from = (uint32_t)(live ? k : 0) * STEP;
+    if (d < DA)
+      dma16(dst + (uint32_t)((DA * wave + d) * 1024), off[d], live_rsrc(live, ra), from);
+    else
+      dma16(dst + (uint32_t)(C::A_ST + (DW * wave + d - DA) * 1024), off[d], live_rsrc(live, rw), from);
+  };
+  auto issue_scales = [&](int buffer, int d) __attribute__((always_inline)) {  // of the steps from CS * buffer on
+    const bool live = buffer * CS < nk;
+    const int q = wave + 4 * d;
+    dma16(lds0 + (uint32_t)(q < C::NS ? C::SC_OFF + (buffer & 1) * C::SC + q * 1024 : C::PAD_OFF), soff[d],
+          live_rsrc(live, q * (64 / SL) < C::TM ? rsa : rsw), (uint32_t)(live ? buffer : 0) * C::SROW);
   };
 
   // fragment f (f < FI: A rows 32 (FI wm + f) .., then W rows 32 (FJ wn + f - FI) ..) of substep s: chunk 2 s + h of
@@ -386,7 +410,7 @@ __global__ void __launch_bounds__(256, 1) mx_tile(Args p) {
   for (int f = 0; f < NFR; ++f) {
     const int row = 32 * (f < FI ? FI * wm + f : FJ * wn + f - FI) + r;
     base[f] = lds0 + (uint32_t)((f < FI ? 0 : C::A_ST) + row * STEP + ((h ^ ((row ^ (row >> 3)) & 7)) << 4));
-    sbase[f] = lds0 + (uint32_t)(C::SC_OFF + ((f < FI ? 0 : C::TM) + row) * STEP_BLOCKS);
+    sbase[f] = lds0 + (uint32_t)(C::SC_OFF + ((f < FI ? 0 : C::TM) + row) * C::SROW);
   }
   struct Frag {
     i32x4 v[NFR];
@@ -396,11 +420,14 @@ __global__ void __launch_bounds__(256, 1) mx_tile(Args p) {
     fr.v[f] = *(lds_i4*)((lds_u8*)(uintptr_t)(base[f] ^ (uint32_t)(s << 5)) + st * C::STAGE);
   };
   const uint32_t tail = tail_mask(p.K, h);
-  uint32_t sc[NFR], sc_next[NFR];
-  auto read_scale = [&](int k, int st, int f) __attribute__((always_inline)) {
+  // the scales read beside a step's last substep are picked apart when the next one starts: there the wait for them is
+  // the fragments' too
+  u32x2 raw[NFR];
+  uint32_t sc[NFR];
+  auto read_scale = [&](int k, int f) __attribute__((always_inline)) {
     typedef __attribute__((address_space(3))) const u32x2 lds_u2;
-    const u32x2 v = *(lds_u2*)((lds_u8*)(uintptr_t)sbase[f] + st * C::SC);
-    sc_next[f] = pick_scales(v, h) & (k == nk - 1 ? tail : ~0u);
+    const uint32_t at_step = (uint32_t)(((k / CS) & 1) * C::SC + k % CS * STEP_BLOCKS);
+    raw[f] = *(lds_u2*)((lds_u8*)(uintptr_t)(sbase[f] + at_step));
   };
 
   f32x16 acc[FI][FJ];
@@ -409,7 +436,10 @@ __global__ void __launch_bounds__(256, 1) mx_tile(Args p) {
 #pragma unroll
     for (int j = 0; j < FJ; ++j) acc[i][j] = f32x16{};
 
-  constexpr int VM0 = PER * (ST - 1), VM1 = PER * (ST - 2);
+  // Codes of step k + 1 have landed when those of the ST - 2 steps behind are all that is outstanding; scales among them
+  // only make the wait longer.
+  constexpr int NOW = PER / 2;  // DMAs of a step that go out beside the last substep; the others beside the next one's first
+  constexpr int VM0 = PER * (ST - 2) + NOW, VM1 = PER * (ST - 2);
   static_assert(VM0 < 64, "vmcnt range");
   constexpr int WAIT_PRO = (VM0 & 15) | ((VM0 >> 4) << 14) | (7 << 4) | (15 << 8);
   constexpr int WAIT_STEP = (VM1 & 15) | ((VM1 >> 4) << 14) | (7 << 4) | (0 << 8);
@@ -419,120 +449,157 @@ __global__ void __launch_bounds__(256, 1) mx_tile(Args p) {
     asm volatile("" ::: "memory");
   };
 #pragma unroll
+  for (int d = 0; d < DS; ++d) issue_scales(0, d);
+#pragma unroll
   for (int st = 0; st < ST; ++st)
 #pragma unroll
-    for (int d = 0; d < PER; ++d) issue_one(st, st, d);
+    for (int d = 0; d < (st < ST - 1 ? PER : NOW); ++d) issue_one(st, st, d);
+  // Thread i holds the tile's row i: where it goes, and its factor.  The loads come after the DMAs (the wait for the first
+  // is theirs too), the factor arrives during the steps.
+  int yrow = -1;
+  float factor = 1.f;
+  if constexpr (GROUPED) {
+    if (t < C::TM) yrow = row_of_y<GROUPED>(p, at, t);
+    if (p.weights && yrow >= 0) factor = p.weights[yrow];
+  }
   __builtin_amdgcn_s_waitcnt(WAIT_PRO);
   barrier();
   Frag f0, f1;
 #pragma unroll
   for (int f = 0; f < NFR; ++f) {
     read_one(f0, 0, 0, f);
-    read_scale(0, 0, f);
+    read_scale(0, f);
   }
 
   constexpr int NQ = FI * FJ;  // MFMAs of a substep
-  // one substep on `cur`; work(q) goes out beside its q-th MFMA
-  auto substep = [&](auto s, const Frag& cur, auto work) __attribute__((always_inline)) {
+  // Substep s of step k on stage st; beside its q-th MFMA go out the reads of the next substep's fragments, and DMAs
+  auto substep = [&](auto sub, int k, int st, const Frag& cur, Frag& other) __attribute__((always_inline)) {
+    constexpr int S = decltype(sub)::value;
+    const int next = (st + 1) % ST;
 #pragma unroll
     for (int q = 0; q < NQ; ++q) {
       const int i = q / FJ, j = q % FJ;
-      acc[i][j] = mfma<decltype(s)::value>(cur.v[FI + j], cur.v[i], acc[i][j], sc[FI + j], sc[i]);
-      work(q);
+      acc[i][j] = mfma<S>(cur.v[FI + j], cur.v[i], acc[i][j], sc[FI + j], sc[i]);
+#pragma unroll
+      for (int f = 0; f < NFR; ++f)
+        if (f * NQ / NFR == q) {
+          if constexpr (S < 3) {
+            read_one(other, st, S + 1, f);
+          } else {
+            read_one(other, next, 0, f);
+            read_scale(k + 1, f);
+          }
+        }
+      if constexpr (S == 3) {
+#pragma unroll
+        for (int d = 0; d < NOW; ++d)
+          if (d * NQ / NOW == q) issue_one(k + ST, st, d);
+      }
+      if constexpr (S == 0) {
+#pragma unroll
+        for (int d = NOW; d < PER; ++d)
+          if ((d - NOW) * NQ / (PER - NOW) == q) issue_one(k + ST - 1, (st + ST - 1) % ST, d);
+      }
       __builtin_amdgcn_sched_barrier(0);
     }
   };
   auto step = [&](int k, int st) __attribute__((always_inline)) {
 #pragma unroll
-    for (int f = 0; f < NFR; ++f) sc[f] = sc_next[f];
-    auto reads = [&](Frag& fr, int from, int s) __attribute__((always_inline)) {
-      return [&fr, from, s, &read_one](int q) __attribute__((always_inline)) {
-#pragma unroll
-        for (int f = 0; f < NFR; ++f)
-          if (f * NQ / NFR == q) read_one(fr, from, s, f);
-      };
-    };
-    substep(std::integral_constant<int, 0>{}, f0, reads(f1, st, 1));
-    substep(std::integral_constant<int, 1>{}, f1, reads(f0, st, 2));
-    substep(std::integral_constant<int, 2>{}, f0, reads(f1, st, 3));
-    // step k + 1 landed, and every wavefront has read this stage
+    for (int f = 0; f < NFR; ++f) sc[f] = pick_scales(raw[f], h) & (k == nk - 1 ? tail : ~0u);
+    substep(std::integral_constant<int, 0>{}, k, st, f0, f1);
+    substep(std::integral_constant<int, 1>{}, k, st, f1, f0);
+    substep(std::integral_constant<int, 2>{}, k, st, f0, f1);
+    // step k + 1 landed, and every wavefront has read this stage, and the scales of the steps before
     __builtin_amdgcn_s_waitcnt(WAIT_STEP);
     barrier();
-    const int next = (st + 1) % ST;
-    substep(std::integral_constant<int, 3>{}, f1, [&](int q) __attribute__((always_inline)) {
+    if (k % CS == 0) {
 #pragma unroll
-      for (int f = 0; f < NFR; ++f)
-        if (f * NQ / NFR == q) {
-          read_one(f0, next, 0, f);
-          read_scale(k + 1, next, f);
-        }
-#pragma unroll
-      for (int d = 0; d < PER; ++d)
-        if (d * NQ / PER == q) issue_one(k + ST, st, d);
-    });
+      for (int d = 0; d < DS; ++d) issue_scales(k / CS + 1, d);
+    }
+    substep(std::integral_constant<int, 3>{}, k, st, f1, f0);
   };
   for (int k = 0; k < nk; k += ST) {
 #pragma unroll
     for (int st = 0; st < ST; ++st)
       if (k + st < nk) step(k + st, st);
   }
-  __builtin_amdgcn_s_waitcnt(0);
-  __syncthreads();
+  // grouped: the rows of Y and their factors, where the first stage was
+  int* const map = reinterpret_cast<int*>(lds);
+  float* const factors = reinterpret_cast<float*>(lds + C::TM * 4);
+  __builtin_amdgcn_s_waitcnt(0);  // the DMAs issued past the end
+  if constexpr (GROUPED) {
+    __syncthreads();
+    if (t < C::TM) {
+      map[t] = yrow;
+      factors[t] = factor;
+    }
+    __syncthreads();
+  }
 
-  // element 4 g + e of fragment (i, j): row 32 (FI wm + i) + r, column 32 (FJ wn + j) + 8 g + 4 h + e; staged in LDS
-  // so that the stores write whole runs of a row
-  uint16_t* const ct = reinterpret_cast<uint16_t*>(lds);
+  // element 4 g + e of fragment (i, j): row 32 (FI wm + i) + r, column 32 (FJ wn + j) + 8 g + 4 h + e.  The halves of the
+  // wavefront swap groups g and g + 1, after which a lane holds eight consecutive columns: 32 bytes of a row a store.
 #pragma unroll
   for (int i = 0; i < FI; ++i) {
     const int row = 32 * (FI * wm + i) + r;
-    float s = 1.f;
-    if constexpr (GROUPED)
-      if (p.weights) {
-        const int yrow = row_of_y<GROUPED>(p, at, row);
-        s = yrow >= 0 ? p.weights[yrow] : 0.f;
-      }
+    const float s = GROUPED ? factors[row] : 1.f;
+    const int to = GROUPED ? map[row] : row < at.rows ? at.m0 + row : -1;
+    uint16_t* const y = p.y + (int64_t)to * p.N + at.n0;
 #pragma unroll
     for (int j = 0; j < FJ; ++j)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int col = 32 * (FJ * wn + j) + 8 * g + 4 * h;
-        float v[4];
+      for (int g = 0; g < 4; g += 2) {
+        uint32_t v[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = GROUPED ? acc[i][j][4 * g + e] * s : acc[i][j][4 * g + e];
-        u32x2 out;
-        out[0] = pack2(v[0], v[1], p.bf16);
-        out[1] = pack2(v[2], v[3], p.bf16);
-        *reinterpret_cast<u32x2*>(ct + row * C::C_STRIDE + col) = out;
+        for (int e = 0; e < 4; ++e) {
+          const float a0 = acc[i][j][4 * g + 2 * e], a1 = acc[i][j][4 * g + 2 * e + 1];
+          v[e] = GROUPED ? pack2(a0 * s, a1 * s, p.bf16) : pack2(a0, a1, p.bf16);
+        }
+        typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+        const u2 lo = __builtin_amdgcn_permlane32_swap(v[0], v[2], false, false);
+        const u2 hi = __builtin_amdgcn_permlane32_swap(v[1], v[3], false, false);
+        const int col = 32 * (FJ * wn + j) + 8 * (g + h), n = at.n0 + col;
+        if (to < 0 || n >= p.N) continue;
+        const u32x4 out = {lo[0], hi[0], lo[1], hi[1]};
+        if (p.vec) {
+          *reinterpret_cast<u32x4*>(y + col) = out;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (n + e < p.N) y[col + e] = (uint16_t)(out[e / 2] >> (16 * (e & 1)));
+        }
       }
-  }
-  __syncthreads();
-  for (int q = t; q < C::TM * (C::TN / 8); q += 256) {
-    const int row = q / (C::TN / 8), ch = q % (C::TN / 8) * 8, n = at.n0 + ch;
-    const int yrow = row_of_y<GROUPED>(p, at, row);
-    if (yrow < 0 || n >= p.N) continue;
-    const u32x4 v = *reinterpret_cast<const u32x4*>(ct + row * C::C_STRIDE + ch);
-    uint16_t* const y = p.y + (int64_t)yrow * p.N + n;
-    if (p.vec) {
-      *reinterpret_cast<u32x4*>(y) = v;
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (n + e < p.N) y[e] = (uint16_t)(v[e / 2] >> (16 * (e & 1)));
-    }
   }
 }
 
-constexpr int SKINNY_KS = 4, SKINNY_D = 2;
+template <int FI, int FJ, int ST, int CS, int WM, bool GROUPED>
+__global__ void __launch_bounds__(256, 1) mx_tile(Args p) {
+  typedef Tile<FI, FJ, ST, CS, WM> C;
+  extern __shared__ __attribute__((aligned(128))) uint8_t lds[];
+  Place at;
+  if (!place<GROUPED, C::TM, C::TN>(p, at)) return;
+  if constexpr (GROUPED && FI == 4) {
+    if (at.rows <= C::TM / 2) {
+      tile_product<C, FI, FJ / 2, 1, GROUPED>(p, at, lds);
+      return;
+    }
+  }
+  tile_product<C, FI, FJ, WM, GROUPED>(p, at, lds);
+}
+
+constexpr int SKINNY_KS = 4, SKINNY_D = 1;  // 8 wavefronts or two steps ahead: 2 to 10 % slower
 
 // Row tiles of TM rows: exact for a dense product, an upper bound for a grouped one.
 inline int64_t row_tiles(int64_t M, int64_t tm, int64_t E) { return E ? M / tm + (E < M ? E : M) : (M + tm - 1) / tm; }
 
-template <class F>
+// f(shape) of a tile in LDS: launch and describe take the same one.
+template <bool GROUPED, class F>
 tb_status with_tile(plan::MxTile tile, const F& f) {
+  if constexpr (GROUPED)
+    if (tile == plan::MX_32x128) return f(Tile<1, 1, 3, 4, 1>{});
   switch (tile) {
-    case plan::MX_64x64: return f(Tile<1, 1, 3>{});
-    case plan::MX_128x128: return f(Tile<2, 2, 2>{});
-    default: return f(Tile<4, 4, 2>{});
+    case plan::MX_64x64: return f(Tile<1, 1, 4, 8>{});
+    case plan::MX_128x128: return f(Tile<2, 2, 2, 2>{});
+    default: return f(Tile<4, 4, 2, 2>{});
   }
 }
 
@@ -542,6 +609,8 @@ tb_status launch_kernel(const char* fn, K kernel, int tm, int tn, int threads, s
   TB_CHECK_ARG(tiles_m * tiles_n < (1ll << 23), "%s: problem too large", fn);
   p.tiles_m = (int)tiles_m;
   p.tiles_n = (int)tiles_n;
+  p.by_tiles_n = tb::Divisor((uint32_t)tiles_n);
+  p.by_band = tb::Divisor((uint32_t)tiles_n * 8);
   if (lds)
     if (tb_status st = tb::reserve_lds(reinterpret_cast<const void*>(kernel), lds, fn)) return st;
   hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles_m * tiles_n)), dim3(threads), lds, stream, p);
@@ -553,9 +622,9 @@ tb_status launch(const char* fn, Args& p, hipStream_t stream) {
   const plan::MxTile tile = plan::pick_mx_tile(p.M, p.N, p.K, GROUPED ? p.E : 0);
   if (tile == plan::MX_32x32)
     return launch_kernel<GROUPED>(fn, &mx_skinny<SKINNY_KS, SKINNY_D, GROUPED>, 32, SK_N, 64 * SKINNY_KS, 0, p, stream);
-  return with_tile(tile, [&](auto shape) {
+  return with_tile<GROUPED>(tile, [&](auto shape) {
     typedef decltype(shape) C;
-    return launch_kernel<GROUPED>(fn, &mx_tile<C::FI, C::FJ, C::ST, GROUPED>, C::TM, C::TN, 256, C::LDS_BYTES, p, stream);
+    return launch_kernel<GROUPED>(fn, &mx_tile<C::FI, C::FJ, C::ST, C::CS, C::WM, GROUPED>, C::TM, C::TN, 256, C::LDS_BYTES, p, stream);
   });
 }
 
@@ -596,14 +665,17 @@ void fill(Args& p, int64_t M, int64_t N, int64_t K, int64_t sa_row, int64_t sw_r
 void tb::describe_mxfp4(int64_t M, int64_t N, int64_t K, int64_t experts, tb_tile* out) {
   using namespace tb::ntg::mx;
   const plan::MxTile tile = plan::pick_mx_tile(M, N, K, experts);
+  auto f = [&](auto shape) {
+    typedef decltype(shape) C;
+    *out = tb_tile{"mx_tile", C::TM, C::TN, 4, 1, 1};
+    return TB_OK;
+  };
   if (tile == plan::MX_32x32)
     *out = tb_tile{"mx_skinny", 32, SK_N, SKINNY_KS, SKINNY_KS, 1};
+  else if (experts)
+    with_tile<true>(tile, f);
   else
-    with_tile(tile, [&](auto shape) {
-      typedef decltype(shape) C;
-      *out = tb_tile{"mx_tile", C::TM, C::TN, 4, 1, 1};
-      return TB_OK;
-    });
+    with_tile<false>(tile, f);
 }
 
 extern "C" tb_status tb_mxfp4_gemm(const uint8_t* a, const uint8_t* sa, const uint8_t* w, const uint8_t* sw, void* y,

@@ -165,16 +165,50 @@ inline NtTile pick_nt_tile(int64_t M, int64_t N, int64_t Kb) {
   return best;
 }
 
-enum MxTile { MX_256 = 0, MX_32x32, MX_64x64, MX_128x128 };
+enum MxTile { MX_256 = 0, MX_32x32, MX_32x128, MX_64x64, MX_128x128 };
 
-// The tile of an MXFP4 product of M rows, dense (experts = 0) or over `experts` experts.
+// The tile of an MXFP4 product of M rows, dense (experts = 0) or over `experts` experts, by estimated time in us: a start,
+// the K steps of 256 channels times what a step of all tiles takes (or reading the weights, if that takes longer), and a
+// share of the weights' MB.  Least-squares fits over 374 sizes (1 - 8192 rows, N 128 - 28672, K 512 - 8192; 8 - 256
+// experts with 1 - 16384 rows between them; cold weights, each tile forced in turn), within a fifth; the picks take 1.2 %
+// (dense) and 2.3 % (experts) more than the best tile.  Measured, us: 1 x 4096 x 4096 5.8 (32 x 32; 64 x 64 7.4), 16 x
+// 11008 x 4096 8.9 (64 x 64; 32 x 32 11.4), 512 x 11008 x 4096 29 (128 x 128; 64 x 64 42, 256 x 256 37), 8192 x 8192 x
+// 8192 265 (256 x 256; 128 x 128 333); 64 experts, top 8, N 2816, K 4096: 32 tokens 70 (32 x 128; 64 x 64 75, 32 x 32
+// 86), 512 tokens 106 (256 x 256; 32 x 128 128), 4096 tokens 270 (256 x 256; 128 x 128 335).
+struct MxCost {
+  double start, first, slope, second, round, fill, mb_per_us, us_per_mb;
+  double operator()(double tiles, double steps, double mb) const {
+    const double x = tiles / 256;
+    const double step = x <= 1 ? first + slope * x : second + round * (std::ceil(x) - 2) + fill * (x - std::ceil(x) + 1);
+    return start + std::max(steps * step, mb / mb_per_us) + us_per_mb * mb;
+  }
+};
+
 inline MxTile pick_mx_tile(int64_t M, int64_t N, int64_t K, int64_t experts) {
-  const int64_t each = experts ? M / std::min(M, experts) : M;
-  if (each <= 32) return MX_32x32;
-  const int64_t rows = experts ? each : M, times = experts ? std::min(M, experts) : 1;
-  auto tiles = [&](int64_t t) { return times * ((rows + t - 1) / t) * ((N + t - 1) / t); };
-  if (tiles(256) >= 192) return MX_256;
-  return tiles(128) >= 192 ? MX_128x128 : MX_64x64;
+  const bool grouped = experts > 0;
+  // the host knows the rows in all: at most as many experts have some, spread evenly
+  const double active = grouped ? (double)std::min(M, experts) : 1, steps = (double)((K + 255) / 256);
+  const double mb = active * (double)N * (double)K * 0.53e-6;
+  auto tiles = [&](int64_t tm, int64_t tn) {
+    return (grouped ? expert_tile_rows((double)M, active, (double)tm) : (double)((M + tm - 1) / tm)) * (double)((N + tn - 1) / tn);
+  };
+  constexpr MxCost s64[2] = {{3.5, 0.24, 0.06, 0.46, 0.27, 0.18, 6.7, 0.043}, {6.2, 0.13, 0.10, 0.34, 0.44, 0.0, 8.9, 0.072}};
+  constexpr MxCost s128[2] = {{3.8, 0.61, 0.45, 1.18, 0.71, 0.39, 4.8, 0.052}, {7.1, 0.78, 0.19, 1.23, 1.17, 0.18, 7.3, 0.0}};
+  constexpr MxCost s256[2] = {{9.2, 1.10, 1.02, 3.39, 2.27, 0.94, 3.0, 0.024}, {9.4, 1.11, 0.80, 3.63, 3.41, 0.0, 4.6, 0.0}};
+  constexpr MxCost s32x128{4.8, 0.33, 0.08, 0.65, 0.51, 0.06, 9.0, 0.091};
+  MxTile best = MX_256;
+  double c = s256[grouped](tiles(256, 256), steps, mb);
+  auto take = [&](MxTile t, double cost) {
+    if (cost < c) best = t, c = cost;
+  };
+  take(MX_128x128, s128[grouped](tiles(128, 128), steps, mb));
+  take(MX_64x64, s64[grouped](tiles(64, 64), steps, mb));
+  if (grouped) take(MX_32x128, s32x128(tiles(32, 128), steps, mb));
+  // blocks of 32 x 32 share CUs: their loads add up
+  const double x = tiles(32, 32) / 256, full = std::min(1.0, (double)M / active / 32);
+  take(MX_32x32, grouped ? 4.4 + std::max(steps * (0.20 * std::max(1.0, x) + 0.02 * std::max(0.0, x - 0.95) * (1 + 0.24 * full * 32)), mb / 5.0) + 0.042 * mb
+                         : 2.4 + std::max(steps * 0.223 * std::max(1.0, x), mb / 4.4) + 0.053 * mb);
+  return best;
 }
 
 constexpr int DEC_WAVES = 8, DEC_UNIT = 32, DEC_MAX_SPLITS = 16;
