@@ -51,8 +51,8 @@ def run(logits: torch.Tensor, k: int, bias=None, groups: int = 1, top_groups: in
     global _last_config
     rt.require_device(logits, bias)
     T, E = check(logits, k, bias, groups, top_groups, group_top, score)
-    weights = torch.empty((T, k), dtype=torch.float32, device=logits.device)
-    ids = torch.empty((T, k), dtype=torch.int32, device=logits.device)
+    weights = logits.new_empty((T, k), dtype=torch.float32)
+    ids = logits.new_empty((T, k), dtype=torch.int32)
     if T:
         if E > 1 and logits.stride(1) != 1:
             logits = logits.contiguous()

@@ -35,9 +35,9 @@ def check(a, sa, w, sw, offsets, gather=None, topk=1, scatter=None, weights=None
         raise ValueError(f"{op}: a has {K} channels, w {2 * w.shape[2]}")
     experts.check_output(op, dtype)
     E, N = w.shape[:2]
-    for name, t in (("offsets", offsets), ("gather", gather), ("scatter", scatter)):
-        if t is not None and t.dtype is not torch.int32:
-            raise TypeError(f"{op}: {name} must be int32")
+    if offsets.dtype is not torch.int32 or (gather is not None and gather.dtype is not torch.int32) \
+            or (scatter is not None and scatter.dtype is not torch.int32):
+        raise TypeError(f"{op}: offsets, gather and scatter must be int32")
     if not 1 <= E <= 4096 or offsets.shape != (E + 1,):
         raise ValueError(f"{op}: need 1 to 4096 experts and offsets [experts + 1] (got {E} and {list(offsets.shape)})")
     if gather is not None and gather.dim() != 1:
@@ -69,13 +69,15 @@ def run(a: torch.Tensor, sa: torch.Tensor, w: torch.Tensor, sw: torch.Tensor, of
     global _last_call
     rt.require_device(a, sa, w, sw, offsets, gather, scatter, weights, out)
     R, N, K, E = check(a, sa, w, sw, offsets, gather, topk, scatter, weights, dtype, out)
-    Y = torch.empty((R, N), dtype=dtype, device=a.device) if out is None else out
-    if not Y.numel():
+    Y = a.new_empty((R, N), dtype=dtype) if out is None else out
+    if not (R and N):
         return Y
     a, w, offsets = experts.code_rows(a), experts.code_rows(w), offsets.contiguous()
     sa, sa_row, _ = experts.scale_rows(sa)
     sw, sw_row, sw_expert = experts.scale_rows(sw)
-    gather, scatter, weights = (None if t is None else t.contiguous() for t in (gather, scatter, weights))
+    gather = None if gather is None else gather.contiguous()
+    scatter = None if scatter is None else scatter.contiguous()
+    weights = None if weights is None else weights.contiguous()
     rt.call("tb_moe_mxfp4_grouped_gemm", a.data_ptr(), sa.data_ptr(), w.data_ptr(), sw.data_ptr(), offsets.data_ptr(),
             rt.ptr(gather), rt.ptr(scatter), rt.ptr(weights), Y.data_ptr(), R, a.shape[0], E, N, K, topk, sa_row, sw_row,
             sw_expert, experts.DTYPES[dtype], rt.stream_handle(a.get_device()))

@@ -27,7 +27,7 @@ def run(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.bf
     global _last_config
     rt.require_device(codes, scales)
     K = check(codes, scales, dtype)
-    out = torch.empty((*codes.shape[:-1], K), dtype=dtype, device=codes.device)
+    out = codes.new_empty((*codes.shape[:-1], K), dtype=dtype)
     if out.numel():
         codes = experts.code_rows(codes)
         scales = scales if scales.dim() == 2 else scales.flatten(0, -2)

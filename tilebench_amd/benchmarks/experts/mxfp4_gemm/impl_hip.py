@@ -31,8 +31,8 @@ def run(a: torch.Tensor, sa: torch.Tensor, w: torch.Tensor, sw: torch.Tensor, dt
     global _last_call
     rt.require_device(a, sa, w, sw)
     M, N, K = check(a, sa, w, sw, dtype)
-    Y = torch.empty((M, N), dtype=dtype, device=a.device)
-    if not Y.numel():
+    Y = a.new_empty((M, N), dtype=dtype)
+    if not (M and N):
         return Y
     a, w = experts.code_rows(a), experts.code_rows(w)
     sa, sa_row, _ = experts.scale_rows(sa)

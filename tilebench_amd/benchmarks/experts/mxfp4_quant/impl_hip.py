@@ -39,7 +39,7 @@ def run(x: torch.Tensor, gated: bool = False, **kwargs):
     rt.require_device(x)
     K = check(x, gated)
     lead = x.shape[:-1]
-    codes = torch.empty((*lead, K // 2), dtype=torch.uint8, device=x.device)
+    codes = x.new_empty((*lead, K // 2), dtype=torch.uint8)
     scales = experts.empty_scales(lead, K, x.device)
     if codes.numel():
         x = paged.aligned_rows(x if x.dim() == 2 else x.flatten(0, -2), 16 // x.element_size())

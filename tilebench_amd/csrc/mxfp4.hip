@@ -9,9 +9,10 @@
 // scales, and zero codes.  Scaling by a power of two is exact, so codes and scales
 // have one right value each.
 //
-// Gated: the values are silu(g) * u = g / (1 + exp(-g)) * u, decided in 64 bits:
-// the product's rounding error is far below the distance at which a code or an
-// exponent would turn, so they are those of the exact product.
+// Gated: the values are silu(g) * u = g / (1 + exp(-g)) * u, and codes and scales those of the product in
+// 64 bits.  Nearly all are settled in fp32: a value comes with a bound of its error, both ends of that range are rounded,
+// and where they agree (and the block's exponent does) that is the answer; a wavefront with a value next to a
+// border computes in 64 bits (about one in a thousand on N(0, 1) gates).  16008 x 1408 bf16: 23 us; 61 with all in 64 bits.
 //
 // Both are bound by memory.  Four lanes share a block, eight channels each: a
 // lane's 16-bit channels are one 16-byte load (a wavefront reads 1 KiB runs), its
@@ -94,6 +95,39 @@ __device__ __forceinline__ uint32_t quantise(const float (&v)[UNIT], int& byte) 
   return codes8(q);
 }
 
+// The same of products silu(g) * u in fp32, with bounds; false where these do not settle a code or the scale.
+// Relative error: 1 ulp each of exp2 and of the reciprocal, half of the sum and the two products, together 3.5 * 2^-23, and
+// the exponent's own, |t| ln 2 times the rounding of t and of log2(e), below |t| 2^-23.  Beyond |g| = 80, for tiny
+// blocks (products below the normals) and for what is not finite the bounds do not hold.
+__device__ __forceinline__ bool quantise_gated_bounded(const float (&g)[UNIT], const float (&u)[UNIT], int& byte, uint32_t& codes) {
+  float lo[UNIT], hi[UNIT];
+  uint32_t top_lo = 0, top_hi = 0;
+  float most = 0.f;
+#pragma unroll
+  for (int i = 0; i < UNIT; ++i) {
+    const float t = g[i] * 1.44269504f;
+    const float v = g[i] * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-t)) * u[i];
+    const float b = __builtin_fmaf(__builtin_fabsf(t), 0x1p-23f, 0x1p-20f);
+    most = fmaxf(most, __builtin_fabsf(g[i]));
+    lo[i] = __builtin_fmaf(-b, v, v);
+    hi[i] = __builtin_fmaf(b, v, v);
+    top_lo = max(top_lo, __builtin_bit_cast(uint32_t, lo[i]) & 0x7FFFFFFFu);
+    top_hi = max(top_hi, __builtin_bit_cast(uint32_t, hi[i]) & 0x7FFFFFFFu);
+  }
+  top_lo = max4(top_lo);
+  top_hi = max4(top_hi);
+  byte = (int)(top_hi >> 23) - 2;
+  const float inverse = power(min(max(254 - byte, 0), 254));
+#pragma unroll
+  for (int i = 0; i < UNIT; ++i) {
+    lo[i] *= inverse;
+    hi[i] *= inverse;
+  }
+  codes = codes8(hi);
+  // a block of zeros is settled by 64 bits too: 0 and what is below the normals look alike
+  return top_lo >> 23 == top_hi >> 23 && top_hi < 0x7F800000u && top_lo >= 0x0D800000u && most <= 80.f && codes == codes8(lo);
+}
+
 // The same of products silu(g) * u in 64 bits.  What goes on to the 4-bit rounding
 // is cut to fp32 with the last bit set where anything was cut off: a value next to a
 // border between codes stays on its side.
@@ -140,7 +174,7 @@ __global__ void __launch_bounds__(THREADS)
     if constexpr (GATED) {
       float u[UNIT];
       load_unit<DTYPE>(x, at + (int64_t)s.upr * UNIT, u);
-      q = quantise_gated(v, u, byte);
+      if (!__all(quantise_gated_bounded(v, u, byte, q))) q = quantise_gated(v, u, byte);
     } else {
       q = quantise(v, byte);
     }

@@ -22,16 +22,17 @@ def check_matrix(op, what, codes, scales, dims):
     """K of an MXFP4 matrix of `dims` dimensions (None: two or more)."""
     if codes.dtype is not torch.uint8 or scales.dtype is not torch.uint8:
         raise TypeError(f"{op}: {what} must be uint8 codes and scales")
-    shape = codes.shape
-    if len(shape) != dims if dims else len(shape) < 2:
-        raise ValueError(f"{op}: {what} must have {dims or 'two or more'} dimensions (got {len(shape)})")
-    K = 2 * shape[-1]
-    if K < BLOCK or K % BLOCK:
-        raise ValueError(f"{op}: {what} must hold a multiple of {BLOCK} channels a row (got {K})")
-    if scales.shape != (*shape[:-1], K // BLOCK):
-        raise ValueError(f"{op}: {what} needs one scale for {BLOCK} channels: {[*shape[:-1], K // BLOCK]}, got "
-                         f"{list(scales.shape)}")
-    return K
+    shape, blocks = codes.shape, scales.shape
+    n = len(shape)
+    if n != dims if dims else n < 2:
+        raise ValueError(f"{op}: {what} must have {dims or 'two or more'} dimensions (got {n})")
+    half = shape[-1]
+    if half % 16 or not half:
+        raise ValueError(f"{op}: {what} must hold a multiple of {BLOCK} channels a row (got {2 * half})")
+    if len(blocks) != n or 16 * blocks[-1] != half or blocks[0] != shape[0] or (n > 2 and blocks[1:-1] != shape[1:-1]):
+        raise ValueError(f"{op}: {what} needs one scale for {BLOCK} channels: {[*shape[:-1], half // 16]}, got "
+                         f"{list(blocks)}")
+    return 2 * half
 
 
 def check_output(op, dtype):
@@ -42,26 +43,30 @@ def check_output(op, dtype):
 def empty_scales(lead, K, device):
     """Unset scales [*lead, K / 32] whose rows start on 16 bytes."""
     S = K // BLOCK
-    return torch.empty((*lead, -(-S // 16) * 16), dtype=torch.uint8, device=device)[..., :S]
+    step = -(-S // 16) * 16
+    strides = [1]
+    for n in reversed(lead):
+        strides.append(step)
+        step *= n
+    return torch.empty_strided((*lead, S), strides[::-1], dtype=torch.uint8, device=device)
 
 
 def code_rows(codes):
     """codes dense and 16-byte aligned."""
-    codes = codes.contiguous()
+    if not codes.is_contiguous():
+        codes = codes.contiguous()
     return codes if codes.data_ptr() % 16 == 0 else codes.clone()
 
 
 def scale_rows(scales):
     """(scales, bytes between rows, bytes between matrices) of [rows, S] or [matrices, rows, S], rows on 4 bytes; copied
     where they lie otherwise."""
-    S = scales.shape[-1]
-    n = scales.shape[-2]
-    many = scales.shape[0] if scales.dim() == 3 else 1
-    row = scales.stride(-2) if n > 1 else -(-S // 4) * 4
-    matrix = scales.stride(0) if many > 1 else n * row
-    if scales.data_ptr() % 4 or (S > 1 and scales.stride(-1) != 1) or row % 4 or row < S or matrix % 4 \
-            or matrix < (n - 1) * row + S:
-        scales = empty_scales(scales.shape[:-1], S * BLOCK, scales.device).copy_(scales)
+    *_, n, S = shape = scales.shape
+    strides = scales.stride()
+    row = strides[-2] if n > 1 else -(-S // 4) * 4
+    matrix = strides[0] if len(shape) == 3 and shape[0] > 1 else n * row
+    if (row | matrix | scales.data_ptr()) % 4 or (strides[-1] != 1 and S > 1) or row < S or matrix < (n - 1) * row + S:
+        scales = empty_scales(shape[:-1], S * BLOCK, scales.device).copy_(scales)
         row = -(-S // 16) * 16
         matrix = n * row
     return scales, row, matrix
