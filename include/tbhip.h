@@ -599,7 +599,7 @@ tb_status tb_mxfp4_dequant(const uint8_t* codes, const uint8_t* scales, void* y,
  *     row m of a, or with gather (int32 [R]) row gather[m] / topk (a negative one or
  *     one past a_rows: a row of zeros);
  *     written to row m of Y [R, N], or with scatter (int32 [R]) to row scatter[m]
- *     (outside 0 .. R - 1: not written; one that is named twice holds either),
+ *     (outside 0 .. R - 1: not written; one that is named twice holds values of either),
  *     there times weights[row of Y] (fp32 [R], null: 1) before the rounding.
  *   tb_moe_align's sorted ids are such gather rows of tokens and scatter rows of
  *   pairs.  Rows of Y that no product row goes to are left as they were.

@@ -182,7 +182,7 @@ def test_product(gpu, M, N, K, dtype):
 
 @pytest.mark.parametrize("M,N,K,tile", [
     (700, 700, 544, 32), (1700, 1900, 96, 64), (200, 2112, 7168, 64), (260, 4097, 4128, 64), (3500, 3600, 96, 128),
-    (1801, 8193, 1056, 128), (4001, 4001, 1056, 128), (2500, 6000, 2080, 256), (4001, 4004, 2080, 256), (2500, 6001, 2112, 256)])
+    (1801, 8193, 1056, 128), (4001, 4001, 1056, 128), (4001, 8001, 992, 128), (2500, 6000, 2080, 256), (4001, 4004, 2080, 256), (2500, 6001, 2112, 256)])
 def test_product_on_every_tile(gpu, M, N, K, tile):
     say("gemm", M, N, K)
     assert rt.gemm_tile(rt.OP_MXFP4, M, N, K)["BM"] == tile
@@ -354,6 +354,75 @@ def test_a_grouped_row_is_the_dense_row(gpu):
         check_close(got, want.double(), want.double().abs(), K)
 
 
+@pytest.mark.parametrize("R,N", [(50, 72), (700, 600)])
+def test_a_row_named_twice_holds_values_of_either(gpu, R, N):
+    say("grouped twice", R, N)
+    a, sa = matrix(R, 160, 1)
+    w, sw = experts_of(3, N, 160, 2)
+    offsets = torch.tensor([0, R // 3, R // 2, R], dtype=torch.int32, device="cuda")
+    plain = impl("moe_mxfp4_grouped_gemm").run(a, sa, w, sw, offsets)
+    scatter = torch.arange(R, dtype=torch.int32, device="cuda")
+    scatter[R - 1] = 2                                    # rows 2 and R - 1 both go to 2, none to R - 1
+    out = torch.full_like(plain, 7.0)
+    impl("moe_mxfp4_grouped_gemm").run(a, sa, w, sw, offsets, scatter=scatter, out=out)
+    assert bool(((out[2] == plain[2]) | (out[2] == plain[R - 1])).all()) and bool((out[R - 1] == 7).all())
+    rest = torch.arange(R - 1, device="cuda") != 2
+    assert torch.equal(out[:-1][rest], plain[:-1][rest])
+
+
+@pytest.mark.parametrize("R", [3, 300])
+def test_thousands_of_experts(gpu, R):
+    """Every segment is looked up among all experts: the first, the last and one in between have rows."""
+    say("grouped experts", R)
+    E, N, K = 4096, 40, 64
+    w, sw = experts_of(E, N, K, 3)
+    a, sa = matrix(R, K, 4)
+    counts = torch.zeros(E, dtype=torch.int64)
+    counts[0], counts[2111], counts[E - 1] = 1, 1, R - 2
+    offsets = torch.cat((torch.zeros(1, dtype=torch.int64), counts.cumsum(0))).int().cuda()
+    check_grouped(a, sa, w, sw, offsets, torch.bfloat16, K)
+
+
+def random_bytes(lo, hi, *shape):
+    return torch.randint(lo, hi, shape, dtype=torch.uint8, device="cuda")
+
+
+@pytest.mark.parametrize("R", [3, 300])
+def test_weights_behind_4_gib(gpu, R):
+    say("grouped far weights", R)
+    E, N, K = 6, 1 << 18, 8192
+    w, sw = random_bytes(0, 256, E, N, K // 2), random_bytes(120, 130, E, N, K // 32)
+    a, sa = matrix(R, K, 1)
+    got = impl("moe_mxfp4_grouped_gemm").run(a, sa, w, sw, torch.tensor([0] * E + [R], dtype=torch.int32, device="cuda"))
+    cols = torch.tensor([0, 33, N // 2 + 1, *range(N - 300, N)], device="cuda")
+    x, v = dequant_ref.values(a, sa), dequant_ref.values(w[E - 1][cols], sw[E - 1][cols])
+    check_close(got[:, cols], x @ v.t(), x.abs() @ v.abs().t(), K)
+
+
+def test_results_behind_4_gib(gpu):
+    say("gemm far results")
+    M, N, K = 70000, 40000, 32
+    a, sa, w, sw = *matrix(M, K, 1), *matrix(N, K, 2)
+    got = impl("mxfp4_gemm").run(a, sa, w, sw)
+    for rows in (slice(0, 40), slice(M // 2, M // 2 + 40), slice(M - 300, M)):
+        x, v = dequant_ref.values(a[rows], sa[rows]), dequant_ref.values(w, sw)
+        check_close(got[rows], x @ v.t(), x.abs() @ v.abs().t(), K)
+
+
+@pytest.mark.parametrize("gated", [False, True])
+def test_quantisation_behind_4_gib(gpu, gated):
+    say("quant far rows", gated)
+    M, K = 65539, 32800
+    x = torch.randn(300, K, dtype=torch.bfloat16, device="cuda").repeat(-(-M // 300), 1)[:M]
+    codes, scales = impl("mxfp4_quant").run(x, gated=gated) if not gated else impl("mxfp4_quant").run(x[:, :32768], gated=True)
+    rows = torch.tensor([0, M // 2, M - 2, M - 1], device="cuda")
+    want = quant_ref.run((x[rows, :32768] if gated else x[rows]).cpu(), gated)
+    assert torch.equal(codes[rows].cpu(), want[0]) and torch.equal(scales[rows].cpu(), want[1])
+    if not gated:
+        back = impl("mxfp4_dequant").run(codes, scales)
+        assert torch.equal(back[rows].double(), dequant_ref.values(codes[rows], scales[rows]).bfloat16().double())
+
+
 # ----------------------------------------------------------------------------- routing
 
 
@@ -432,6 +501,24 @@ def test_routing_takes_any_strides(gpu):
         w, ids = impl("moe_expert_routing").run(layout(x.cuda()), 3, score="sigmoid")
         want = route_ref.run(layout(x), 3, score="sigmoid")
         assert torch.equal(ids.cpu(), want[1]) and w.shape == want[0].shape
+
+
+def test_routing_behind_4_gib(gpu):
+    say("routing far rows")
+    rows = (torch.randn(1000, 1024, generator=gen(3)) * 2).bfloat16()
+    logits = rows.cuda().repeat(2200, 1)
+    want = route_ref.run(rows[-50:], 8)
+    for k in (8, 9):                                       # lanes, rows
+        w, ids = impl("moe_expert_routing").run(logits, k)
+        assert torch.equal(ids[-50:, :8].cpu(), want[1]) and torch.equal(ids[-1000:], ids[:1000]) and torch.equal(w[-1000:], w[:1000])
+
+
+@pytest.mark.parametrize("E,k,groups,kernel", [
+    (60, 4, 1, "route_lanes"), (256, 8, 8, "route_lanes"), (256, 9, 8, "route_rows"), (90, 8, 9, "route_rows")])
+def test_routing_says_which_kernel_ran(gpu, E, k, groups, kernel):
+    say("routing config", E, k, groups)
+    check_route(torch.randn(5, E, generator=gen(1)), k, groups=groups, top_groups=groups)
+    assert impl("moe_expert_routing").get_last_config()["kernel"] == kernel
 
 
 # ----------------------------------------------------------------------------- together

@@ -60,7 +60,11 @@ def run(logits: torch.Tensor, k: int, bias=None, groups: int = 1, top_groups: in
         rt.call("tb_moe_expert_routing", logits.data_ptr(), rt.ptr(bias), weights.data_ptr(), ids.data_ptr(), T, E, k,
                 groups, top_groups, group_top, logits.stride(0), score == "softmax", renormalize, scale,
                 experts.DTYPES[logits.dtype], rt.stream_handle(logits.get_device()))
-    _last_config = {"kernel": "moe_routing_kernel", "lanes_per_row": 64, "block": 256}
+    lanes = 8 if E <= 64 else 16 if E <= 256 else 32 if E <= 512 else 64
+    if k <= 8 and (groups == 1 or E // groups % -(-E // lanes) == 0):
+        _last_config = {"kernel": "route_lanes", "lanes_per_row": lanes, "block": 128}
+    else:
+        _last_config = {"kernel": "route_rows", "lanes_per_row": 64, "block": 256}
     return weights, ids
 
 

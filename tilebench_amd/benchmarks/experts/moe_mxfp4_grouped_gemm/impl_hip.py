@@ -9,8 +9,8 @@ gather  int32 [R]: product row m takes row gather[m] // topk of a (negative or
         past its end: a row of zeros), so that tokens are quantised once and
         pairs' rows are gathered on the way.  None: row m, R = rows.
 scatter int32 [R]: product row m goes to row scatter[m] of Y (outside it:
-        nowhere; a row named twice holds either), times weights[that row]
-        (float32 [R]) if given, before the rounding.
+        nowhere; a row named twice holds values of either), times
+        weights[that row] (float32 [R]) if given, before the rounding.
 out     the Y [R, N] to write.  Rows that no product row goes to are left as
         they were, those of a Y made here not set.
 

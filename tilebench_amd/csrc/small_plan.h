@@ -196,12 +196,15 @@ inline MxTile pick_mx_tile(int64_t M, int64_t N, int64_t K, int64_t experts) {
   constexpr MxCost s128[2] = {{3.8, 0.61, 0.45, 1.18, 0.71, 0.39, 4.8, 0.052}, {7.1, 0.78, 0.19, 1.23, 1.17, 0.18, 7.3, 0.0}};
   constexpr MxCost s256[2] = {{9.2, 1.10, 1.02, 3.39, 2.27, 0.94, 3.0, 0.024}, {9.4, 1.11, 0.80, 3.63, 3.41, 0.0, 4.6, 0.0}};
   constexpr MxCost s32x128{4.8, 0.33, 0.08, 0.65, 0.51, 0.06, 9.0, 0.091};
-  MxTile best = MX_256;
-  double c = s256[grouped](tiles(256, 256), steps, mb);
+  MxTile best = MX_128x128;
+  double c = s128[grouped](tiles(128, 128), steps, mb);
   auto take = [&](MxTile t, double cost) {
     if (cost < c) best = t, c = cost;
   };
-  take(MX_128x128, s128[grouped](tiles(128, 128), steps, mb));
+  // Two dense 128 x 128 tiles share a CU, and one's stores overlap the other's steps: over four steps or fewer that counts
+  // for more than fewer reads (us, 128 x 128 and 256 x 256: 8192 x 8192 x 1024 62 and 68, 6000 x 4096 x 1024 26 and 33,
+  // 8192 x 8192 x 512 45 and 61; 8192 x 12288 x 1408 130 and 120).  Experts' segments end in halves of the larger tile.
+  if (grouped || steps > 4) take(MX_256, s256[grouped](tiles(256, 256), steps, mb));
   take(MX_64x64, s64[grouped](tiles(64, 64), steps, mb));
   if (grouped) take(MX_32x128, s32x128(tiles(32, 128), steps, mb));
   // blocks of 32 x 32 share CUs: their loads add up
