@@ -182,10 +182,12 @@ def test_product(gpu, M, N, K, dtype):
 
 @pytest.mark.parametrize("M,N,K,tile", [
     (700, 700, 544, 32), (1700, 1900, 96, 64), (200, 2112, 7168, 64), (260, 4097, 4128, 64), (3500, 3600, 96, 128),
-    (1801, 8193, 1056, 128), (4001, 4001, 1056, 128), (4001, 8001, 992, 128), (2500, 6000, 2080, 256), (4001, 4004, 2080, 256), (2500, 6001, 2112, 256)])
+    (1801, 8193, 1056, 128), (4001, 4001, 1056, 128), (4001, 8001, 512, 128), (2500, 6000, 2080, 256), (4001, 4004, 2080, 256), (2500, 6001, 2112, 256),
+    (2500, 6001, 4160, 256), (2600, 5504, 4128, 256)])
 def test_product_on_every_tile(gpu, M, N, K, tile):
     say("gemm", M, N, K)
-    assert rt.gemm_tile(rt.OP_MXFP4, M, N, K)["BM"] == tile
+    picked = rt.gemm_tile(rt.OP_MXFP4, M, N, K)
+    assert picked["BM"] == tile and picked["waves"] == (8 if tile == 256 and K <= 4096 else 4)
     check_gemm(*matrix(M, K, 1), *matrix(N, K, 2), torch.bfloat16, K)
 
 

@@ -331,32 +331,33 @@ __global__ void __launch_bounds__(64 * KS, KS / 4) mx_skinny(Args p) {
 }
 
 // ------------------------------------------------------------------ tiles
-// One 64 FI x 64 FJ tile per block: four wavefronts, 2 x 2, of FI x FJ fragments of
-// 32 x 32.  Both operands and their scales stream HBM -> LDS by DMA.  Codes: ST stages of one step, rows of
+// One tile per block: NW wavefronts, WM x NW / WM, of FI x FJ fragments of 32 x 32.  256 x 256 takes eight (but for long
+// K), so that one of a SIMD's two works while the other waits at a barrier, for its reads or for its stores (4096 tokens
+// through 64 experts' down: 222 us, four of 4 x 4 fragments 237).  Both operands and their scales stream HBM -> LDS by DMA.  Codes: ST stages of one step, rows of
 // 128 bytes, 16-byte chunk c of row i at slot c ^ ((i ^ (i >> 3)) & 7), so that writes and fragment reads are free of conflicts
 // (rows of 64 bytes and twice the stages: 1.3 to 1.4 times slower, a DMA then takes 16 lines for its KiB instead of 8).
 // Scales: two buffers of CS steps, 8 CS bytes of a row at once, since a load of a row's 8 bytes takes a whole line's time
 // and, from HBM, a whole line.  A step is four substeps of one MFMA per fragment pair.  While a substep's MFMAs run, the
 // next one's fragments are read (one ds_read_b128 each); the barrier sits before the last substep, when every wavefront
 // has read the stage: it then takes the DMAs of the step ST later.
-template <int FI_, int FJ_, int ST_, int CS_, int WM_ = 2>
+template <int FI_, int FJ_, int ST_, int CS_, int WM_ = 2, int NW_ = 4>
 struct Tile {
-  static constexpr int FI = FI_, FJ = FJ_, ST = ST_, CS = CS_, WM = WM_;
-  static constexpr int TM = 32 * FI * WM, TN = 32 * FJ * (4 / WM);
+  static constexpr int FI = FI_, FJ = FJ_, ST = ST_, CS = CS_, WM = WM_, NW = NW_;
+  static constexpr int TM = 32 * FI * WM, TN = 32 * FJ * (NW / WM);
   static constexpr int A_ST = TM * STEP, STAGE = (TM + TN) * STEP;     // A rows, then W rows
   static constexpr int SROW = CS * STEP_BLOCKS, SC = (TM + TN) * SROW, SC_OFF = ST * STAGE;
-  static constexpr int NS = SC / 1024, DS = (NS + 3) / 4;              // scale DMAs of a buffer, of a wavefront
+  static constexpr int NS = SC / 1024, DS = (NS + NW - 1) / NW;   // scale DMAs of a buffer, of a wavefront
   static constexpr int PAD_OFF = SC_OFF + 2 * SC;                      // those of wavefronts that have none land here
-  static constexpr int LDS_BYTES = PAD_OFF + (NS % 4 ? 1024 : 0);
+  static constexpr int LDS_BYTES = PAD_OFF + (NS % NW ? 1024 : 0);
   static_assert(LDS_BYTES <= 160 * 1024 && SC % 1024 == 0 && TM * SROW % 1024 == 0, "LDS layout");
 };
 
-// The tile at `at` by WM x (4 / WM) wavefronts of FI x FJ fragments: 2 x 2 of them cover it, 1 x 4 its first half of rows.
-template <class C, int FI, int FJ, int WM, bool GROUPED>
+// The tile at `at`, or with half of C's FI the first half of its rows.
+template <class C, int FI, bool GROUPED>
 __device__ __forceinline__ void tile_product(const Args& p, const Place& at, uint8_t* lds) {
-  constexpr int ST = C::ST, CS = C::CS;
+  constexpr int FJ = C::FJ, ST = C::ST, CS = C::CS, WN = C::NW / C::WM;
   const int t = threadIdx.x, lane = t & 63, r = lane & 31, h = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(t >> 6), wm = WM == 2 ? wave >> 1 : 0, wn = WM == 2 ? wave & 1 : wave;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6), wm = wave / WN, wn = wave % WN;
   const int K2 = p.K / 2, nk = (K2 + STEP - 1) / STEP;
   const Operands o = operands<GROUPED>(p, at, C::TN);
   const i32x4 ra = rsrc4(o.a, o.a_bytes), rw = rsrc4(o.w, o.w_bytes);
@@ -370,7 +371,7 @@ __device__ __forceinline__ void tile_product(const Args& p, const Place& at, uin
 
   // A wavefront's DMAs: of a step 8 A rows each (lane L: row + L / 8, slot L % 8), then 8 W rows each; of a scale
   // buffer 16 bytes a lane, SROW / 16 lanes a row.
-  constexpr int DA = C::TM / 32, DW = C::TN / 32, PER = DA + DW, DS = C::DS, SL = C::SROW / 16;
+  constexpr int DA = C::TM / (8 * C::NW), DW = C::TN / (8 * C::NW), PER = DA + DW, DS = C::DS, SL = C::SROW / 16;
   uint32_t off[PER], soff[DS];
 #pragma unroll
   for (int d = 0; d < PER; ++d) {
@@ -381,7 +382,7 @@ __device__ __forceinline__ void tile_product(const Args& p, const Place& at, uin
   }
 #pragma unroll
   for (int d = 0; d < DS; ++d) {
-    const int q = wave + 4 * d, row = 64 / SL * q + lane / SL, wrow = row - C::TM;
+    const int q = wave + C::NW * d, row = 64 / SL * q + lane / SL, wrow = row - C::TM;
     const int at_row = q >= C::NS ? -1 : row < C::TM ? buffer_row<GROUPED>(p, at, row) : at.n0 + wrow < p.N ? wrow : -1;
     soff[d] = at_row >= 0 ? (uint32_t)at_row * (uint32_t)(row < C::TM ? p.sa_row : p.sw_row) + 16u * (lane % SL) : BUF_OOB;
   }
@@ -396,7 +397,7 @@ __device__ __forceinline__ void tile_product(const Args& p, const Place& at, uin
   };
   auto issue_scales = [&](int buffer, int d) __attribute__((always_inline)) {  // of the steps from CS * buffer on
     const bool live = buffer * CS < nk;
-    const int q = wave + 4 * d;
+    const int q = wave + C::NW * d;
     dma16(lds0 + (uint32_t)(q < C::NS ? C::SC_OFF + (buffer & 1) * C::SC + q * 1024 : C::PAD_OFF), soff[d],
           live_rsrc(live, q * (64 / SL) < C::TM ? rsa : rsw), (uint32_t)(live ? buffer : 0) * C::SROW);
   };
@@ -438,7 +439,9 @@ __device__ __forceinline__ void tile_product(const Args& p, const Place& at, uin
 
   // Codes of step k + 1 have landed when those of the ST - 2 steps behind are all that is outstanding; scales among them
   // only make the wait longer.
-  constexpr int NOW = PER / 2;  // DMAs of a step that go out beside the last substep; the others beside the next one's first
+  // DMAs of a step that go out beside the last substep; the others beside the next one's first (8192 x 8192 x 8192 on eight
+  // wavefronts: a quarter 265 us, half 269, three quarters 278)
+  constexpr int NOW = C::NW == 8 ? PER / 4 : PER / 2;
   constexpr int VM0 = PER * (ST - 2) + NOW, VM1 = PER * (ST - 2);
   static_assert(VM0 < 64, "vmcnt range");
   constexpr int WAIT_PRO = (VM0 & 15) | ((VM0 >> 4) << 14) | (7 << 4) | (15 << 8);
@@ -571,19 +574,19 @@ __device__ __forceinline__ void tile_product(const Args& p, const Place& at, uin
   }
 }
 
-template <int FI, int FJ, int ST, int CS, int WM, bool GROUPED>
-__global__ void __launch_bounds__(256, 1) mx_tile(Args p) {
-  typedef Tile<FI, FJ, ST, CS, WM> C;
+template <int FI, int FJ, int ST, int CS, int WM, bool GROUPED, int NW>
+__global__ void __launch_bounds__(64 * NW, NW / 4) mx_tile(Args p) {
+  typedef Tile<FI, FJ, ST, CS, WM, NW> C;
   extern __shared__ __attribute__((aligned(128))) uint8_t lds[];
   Place at;
   if (!place<GROUPED, C::TM, C::TN>(p, at)) return;
   if constexpr (GROUPED && FI == 4) {
     if (at.rows <= C::TM / 2) {
-      tile_product<C, FI, FJ / 2, 1, GROUPED>(p, at, lds);
+      tile_product<C, FI / 2, GROUPED>(p, at, lds);
       return;
     }
   }
-  tile_product<C, FI, FJ, WM, GROUPED>(p, at, lds);
+  tile_product<C, FI, GROUPED>(p, at, lds);
 }
 
 constexpr int SKINNY_KS = 4, SKINNY_D = 1;  // 8 wavefronts or two steps ahead: 2 to 10 % slower
@@ -599,7 +602,10 @@ tb_status with_tile(plan::MxTile tile, const F& f) {
   switch (tile) {
     case plan::MX_64x64: return f(Tile<1, 1, 4, 8>{});
     case plan::MX_128x128: return f(Tile<2, 2, 2, 2>{});
-    default: return f(Tile<4, 4, 2, 2>{});
+    case plan::MX_256_LONG:
+      if constexpr (!GROUPED) return f(Tile<4, 4, 2, 2>{});
+      [[fallthrough]];
+    default: return f(Tile<4, 2, 2, 2, 2, 8>{});
   }
 }
 
@@ -624,7 +630,7 @@ tb_status launch(const char* fn, Args& p, hipStream_t stream) {
     return launch_kernel<GROUPED>(fn, &mx_skinny<SKINNY_KS, SKINNY_D, GROUPED>, 32, SK_N, 64 * SKINNY_KS, 0, p, stream);
   return with_tile<GROUPED>(tile, [&](auto shape) {
     typedef decltype(shape) C;
-    return launch_kernel<GROUPED>(fn, &mx_tile<C::FI, C::FJ, C::ST, C::CS, C::WM, GROUPED>, C::TM, C::TN, 256, C::LDS_BYTES, p, stream);
+    return launch_kernel<GROUPED>(fn, &mx_tile<C::FI, C::FJ, C::ST, C::CS, C::WM, GROUPED, C::NW>, C::TM, C::TN, 64 * C::NW, C::LDS_BYTES, p, stream);
   });
 }
 
@@ -667,7 +673,7 @@ void tb::describe_mxfp4(int64_t M, int64_t N, int64_t K, int64_t experts, tb_til
   const plan::MxTile tile = plan::pick_mx_tile(M, N, K, experts);
   auto f = [&](auto shape) {
     typedef decltype(shape) C;
-    *out = tb_tile{"mx_tile", C::TM, C::TN, 4, 1, 1};
+    *out = tb_tile{"mx_tile", C::TM, C::TN, C::NW, 1, 1};
     return TB_OK;
   };
   if (tile == plan::MX_32x32)

@@ -165,7 +165,7 @@ inline NtTile pick_nt_tile(int64_t M, int64_t N, int64_t Kb) {
   return best;
 }
 
-enum MxTile { MX_256 = 0, MX_32x32, MX_32x128, MX_64x64, MX_128x128 };
+enum MxTile { MX_256 = 0, MX_256_LONG, MX_32x32, MX_32x128, MX_64x64, MX_128x128 };
 
 // The tile of an MXFP4 product of M rows, dense (experts = 0) or over `experts` experts, by estimated time in us: a start,
 // the K steps of 256 channels times what a step of all tiles takes (or reading the weights, if that takes longer), and a
@@ -201,10 +201,13 @@ inline MxTile pick_mx_tile(int64_t M, int64_t N, int64_t K, int64_t experts) {
   auto take = [&](MxTile t, double cost) {
     if (cost < c) best = t, c = cost;
   };
-  // Two dense 128 x 128 tiles share a CU, and one's stores overlap the other's steps: over four steps or fewer that counts
-  // for more than fewer reads (us, 128 x 128 and 256 x 256: 8192 x 8192 x 1024 62 and 68, 6000 x 4096 x 1024 26 and 33,
-  // 8192 x 8192 x 512 45 and 61; 8192 x 12288 x 1408 130 and 120).  Experts' segments end in halves of the larger tile.
-  if (grouped || steps > 4) take(MX_256, s256[grouped](tiles(256, 256), steps, mb));
+  // Two dense 128 x 128 tiles share a CU, and one's stores overlap the other's steps: over two steps that counts for more
+  // than fewer reads (us, 128 x 128 and 256 x 256: 8192 x 8192 x 512 43 and 50, 16384 x 8192 x 512 97 and 116, 4096 x 4096 x
+  // 512 16 and 16; 8192 x 12288 x 768 74 and 69).  Experts' segments end in halves of the larger tile.
+  // 256 x 256 on eight wavefronts, or over more than 16 steps on four: their stalls beside stores and starts weigh less there
+  // than the larger fragments' fewer reads (us, eight and four, operands from HBM: 32768 x 4096 x 1408 187 and 196, 8192 x
+  // 8192 x 4096 153 and 159, 4096 x 28672 x 4096 272 and 278; 4096 x 8192 x 8192 143 and 141.5, 8192 x 8192 x 8192 275 and 269).
+  if (grouped || steps > 2) take(grouped || steps <= 16 ? MX_256 : MX_256_LONG, s256[grouped](tiles(256, 256), steps, mb));
   take(MX_64x64, s64[grouped](tiles(64, 64), steps, mb));
   if (grouped) take(MX_32x128, s32x128(tiles(32, 128), steps, mb));
   // blocks of 32 x 32 share CUs: their loads add up
