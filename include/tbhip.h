@@ -550,7 +550,7 @@ tb_status tb_shared_prefix_attention_workspace_size(int64_t T, int64_t Hq, int64
  *   weights fp32 [T, k]: scale * s of these, over their sum if renormalize.
  * Computed in fp64 and rounded once.  NaN ranks above every number; a softmax
  * row of -inf alone has scores 0, and weights that sum to 0 are 0.
- * Requires E <= 1024, E % groups == 0, groups <= 64, k <= 32 and k <=
+ * Requires T < 2^24, E <= 1024, E % groups == 0, groups <= 64, k <= 32 and k <=
  * top_groups * E / groups, E / groups >= group_top.
  * Beside tb_moe_topk_gating (softmax of the chosen logits alone), which replaces
  * moe_topk_gating/impl_triton.py:58 run(logits, M, E, k).
@@ -604,7 +604,7 @@ tb_status tb_mxfp4_dequant(const uint8_t* codes, const uint8_t* scales, void* y,
  *   tb_moe_align's sorted ids are such gather rows of tokens and scatter rows of
  *   pairs.  Rows of Y that no product row goes to are left as they were.
  *   Offsets are held to 0 .. R.
- * Requires K % 32 == 0, a and w 16-byte aligned, rows of scales (sa_row, sw_row,
+ * Requires K % 32 == 0, K <= 2^22, a and w 16-byte aligned, rows of scales (sa_row, sw_row,
  * sw_expert) on 4 bytes; experts <= 4096; gathered a below 2 GiB.
  * Nearest in the reference: matmul_fp32_fp16_fp8/impl_triton.py:124 run(a, b).
  */

@@ -372,6 +372,22 @@ def test_a_row_named_twice_holds_values_of_either(gpu, R, N):
     assert torch.equal(out[:-1][rest], plain[:-1][rest])
 
 
+@pytest.mark.parametrize("R,N,K", [(40, 64, 96), (700, 600, 160), (1500, 2048, 1056)])
+def test_results_at_odd_addresses(gpu, R, N, K):
+    say("grouped odd addresses", R, N)
+    a, sa = matrix(R, K, 1)
+    w, sw = experts_of(3, N, K, 2)
+    index = torch.stack((torch.arange(R).flip(0), torch.arange(R)), dim=1).int().cuda()[:, 0]        # a stride of 2
+    factors = torch.rand(R, 2, generator=gen(3)).cuda()[:, 1]
+    offsets = torch.tensor([0, 9, R // 2, 9, R // 2, 9, R, 9], dtype=torch.int32, device="cuda")[::2]
+    kw = dict(scatter=index, weights=factors)
+    want = impl("moe_mxfp4_grouped_gemm").run(a, sa, w, sw, offsets, **kw)
+    room = torch.full((R * N + 16,), 7.0, dtype=torch.bfloat16, device="cuda")
+    out = room[3:3 + R * N].view(R, N)
+    assert impl("moe_mxfp4_grouped_gemm").run(a, sa, w, sw, offsets, out=out, **kw) is out
+    assert torch.equal(out, want) and bool((room[:3] == 7).all()) and bool((room[3 + R * N:] == 7).all())
+
+
 @pytest.mark.parametrize("R", [3, 300])
 def test_thousands_of_experts(gpu, R):
     """Every segment is looked up among all experts: the first, the last and one in between have rows."""
@@ -566,6 +582,23 @@ def test_an_expert_layer(gpu, tokens, dtype):
     t = torch.finfo(dtype)  # k - 1 fp32 additions, one rounding
     bound = t.eps / 2 * total.sum(dim=1).abs() + k * 2.0 ** -23 * total.abs().sum(dim=1) + t.smallest_normal * t.eps
     assert bool(((out.double() - total.sum(dim=1)).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("tokens,k,H", [(1, 1, 8), (33, 8, 264), (70, 12, 1032), (5, 32, 16)])
+def test_combine(gpu, tokens, k, H, dtype):
+    """Additions in fp32 in slot order and one rounding: one right answer."""
+    say("combine", tokens, k, H, dtype)
+    g = gen(k)
+    y = (torch.randn(tokens * k, H, generator=g) * torch.exp2(torch.randint(-9, 10, (tokens * k, 1), generator=g).float())).to(dtype)
+    y[0, :6] = torch.tensor([float("inf"), float("-inf"), float("nan"), torch.finfo(dtype).max, -0.0, torch.finfo(dtype).tiny / 4])
+    ids = torch.randint(-1, 9, (tokens, k), generator=g).int()
+    ids[0, 0] = 0
+    total = torch.zeros(tokens, H)
+    for j in range(k):
+        row = y.view(tokens, k, H)[:, j].float()
+        total = torch.where(((ids[:, j] >= 0) & (ids[:, j] < 8))[:, None], total + row, total)
+    torch.testing.assert_close(experts.combine(y.cuda(), ids.cuda(), 8).cpu(), total.to(dtype), rtol=0, atol=0, equal_nan=True)
 
 
 def test_padded_tokens_are_routed_nowhere(gpu):
