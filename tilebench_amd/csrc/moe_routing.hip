@@ -28,6 +28,11 @@
 // Rows (everything else): one wavefront a row, lane l holds experts l, 64 + l, ...; choices are compared as
 // 64-bit keys in the order of their values (0: cannot be chosen), k rounds of a maximum over the wavefront.
 // A wavefront of the first kind that meets inf, NaN or large logits takes its rows this way, one after the other.
+//
+// Bound by the chain of steps (1 row to a few hundred: 6 us, the launch included) and by fp64 instructions: 16384 x 256
+// fp32 logits, sigmoid, 4 of 8 groups, k 8: 17 us with 40 % of the issue slots taken (18 MB, 3 us of HBM), and 64 one row to a
+// wavefront.  A lane has 16 experts at
+// most, two sorts of eight and a merge; more lanes a row mean more merges, of lists that are the same in all lanes by then.
 #include "tb_common.h"
 
 // a score is rounded before its bias is added, wherever it is computed

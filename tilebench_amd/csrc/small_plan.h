@@ -173,8 +173,8 @@ enum MxTile { MX_256 = 0, MX_256_LONG, MX_32x32, MX_32x128, MX_64x64, MX_128x128
 // experts with 1 - 16384 rows between them; cold weights, each tile forced in turn), within a fifth; the picks take 1.2 %
 // (dense) and 2.3 % (experts) more than the best tile.  Measured, us: 1 x 4096 x 4096 5.8 (32 x 32; 64 x 64 7.4), 16 x
 // 11008 x 4096 8.9 (64 x 64; 32 x 32 11.4), 512 x 11008 x 4096 29 (128 x 128; 64 x 64 42, 256 x 256 37), 8192 x 8192 x
-// 8192 265 (256 x 256; 128 x 128 333); 64 experts, top 8, N 2816, K 4096: 32 tokens 70 (32 x 128; 64 x 64 75, 32 x 32
-// 86), 512 tokens 106 (256 x 256; 32 x 128 128), 4096 tokens 270 (256 x 256; 128 x 128 335).
+// 8192 270 (256 x 256; 128 x 128 337); 64 experts, top 8, N 2816, K 4096: 32 tokens 70 (32 x 128; 64 x 64 75, 32 x 32
+// 86), 512 tokens 106 (256 x 256; 32 x 128 128), 4096 tokens 290 (256 x 256; 128 x 128 329).
 struct MxCost {
   double start, first, slope, second, round, fill, mb_per_us, us_per_mb;
   double operator()(double tiles, double steps, double mb) const {
