@@ -165,7 +165,7 @@ inline NtTile pick_nt_tile(int64_t M, int64_t N, int64_t Kb) {
   return best;
 }
 
-enum MxTile { MX_256 = 0, MX_256_LONG, MX_32x32, MX_32x128, MX_64x64, MX_128x128, MX_128_DEEP };
+enum MxTile { MX_256 = 0, MX_256_LONG, MX_32x32, MX_32x128, MX_64x64, MX_128x128, MX_128_DEEP, MX_256x128 };
 
 // The tile of an MXFP4 product of M rows, dense (experts = 0) or over `experts` experts, by estimated time in us: a start,
 // the K steps of 256 channels times what a step of all tiles takes (or reading the weights, if that takes longer), and a
@@ -196,6 +196,7 @@ inline MxTile pick_mx_tile(int64_t M, int64_t N, int64_t K, int64_t experts) {
   constexpr MxCost s128[2] = {{3.8, 0.61, 0.45, 1.18, 0.71, 0.39, 4.8, 0.052}, {7.1, 0.78, 0.19, 1.23, 1.17, 0.18, 7.3, 0.0}};
   constexpr MxCost s256[2] = {{9.2, 1.10, 1.02, 3.39, 2.27, 0.94, 3.0, 0.024}, {9.4, 1.11, 0.80, 3.63, 3.41, 0.0, 4.6, 0.0}};
   constexpr MxCost deep{5.0, 0.355, 0.30, 0.0, 0.0, 0.0, 6.0, 0.0};
+  constexpr MxCost s256x128{7.2, 0.55, 0.56, 0.0, 0.0, 0.0, 6.0, 0.03};
   constexpr MxCost s32x128{4.8, 0.33, 0.08, 0.65, 0.51, 0.06, 9.0, 0.091};
   MxTile best = MX_128x128;
   double c = s128[grouped](tiles(128, 128), steps, mb);
@@ -213,6 +214,9 @@ inline MxTile pick_mx_tile(int64_t M, int64_t N, int64_t K, int64_t experts) {
   // 8192 27 and 36, 1000 x 4000 x 4096 15.4 and 20.5, 1024 x 1024 x 1024 6.6 and 6.7; with two tiles a CU 73 and 47, 8192 x
   // 8192 x 512).  The host does not know how many tiles experts have.
   if (!grouped && tiles(128, 128) <= 256) take(MX_128_DEEP, deep(tiles(128, 128), steps, mb));
+  // ... 256 x 128 with a CU each: three stages (us, 256 x 128 and 128 x 128: 2048 x 4096 x 8192 45 and 51, 512 x 11008 x
+  // 4096 23.4 and 28.3, 1500 x 4096 x 2048 14.0 and 13.2)
+  if (!grouped && tiles(256, 128) <= 256) take(MX_256x128, s256x128(tiles(256, 128), steps, mb));
   take(MX_64x64, s64[grouped](tiles(64, 64), steps, mb));
   if (grouped) take(MX_32x128, s32x128(tiles(32, 128), steps, mb));
   // blocks of 32 x 32 share CUs: their loads add up
