@@ -301,7 +301,8 @@ def test_grouped_product(gpu, counts, N, K, dtype):
 @pytest.mark.parametrize("rows,N,K,tile", [
     (20, 600, 288, (32, 32)), (330, 900, 96, (32, 128)), (50, 640, 1408, (32, 128)), (700, 600, 160, (32, 128)),
     (6, 2815, 4128, (64, 64)), (1400, 1300, 96, (128, 128)), (600, 1200, 544, (128, 128)), (1400, 1304, 1408, (256, 256)),
-    (2000, 2001, 1056, (256, 256))])
+    (2000, 2001, 1056, (256, 256)), (330, 900, 1408, (128, 128)), (400, 1000, 2336, (128, 128)), (330, 1899, 4128, (256, 128)),
+    (700, 1200, 2080, (256, 128))])
 def test_grouped_product_on_every_tile(gpu, rows, N, K, tile):
     say("grouped", rows, N, K)
     counts = [rows, rows // 3, 0, rows * 2, rows - 1, 300, 257, rows + 5] if rows > 6 else [rows, 3, 0, 65, 1, 20, 4, 1]

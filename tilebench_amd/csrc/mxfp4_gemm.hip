@@ -605,12 +605,8 @@ tb_status with_tile(plan::MxTile tile, const F& f) {
   switch (tile) {
     case plan::MX_64x64: return f(Tile<1, 1, 4, 8>{});
     case plan::MX_128x128: return f(Tile<2, 2, 2, 2>{});
-    case plan::MX_256x128:
-      if constexpr (!GROUPED) return f(Tile<2, 2, 3, 2, 4, 8>{});
-      [[fallthrough]];
-    case plan::MX_128_DEEP:
-      if constexpr (!GROUPED) return f(Tile<2, 2, 4, 4>{});
-      [[fallthrough]];
+    case plan::MX_256x128: return f(Tile<2, 2, 3, 2, 4, 8>{});
+    case plan::MX_128_DEEP: return f(Tile<2, 2, 4, 4>{});
     case plan::MX_256_LONG:
       if constexpr (!GROUPED) return f(Tile<4, 4, 2, 2>{});
       [[fallthrough]];

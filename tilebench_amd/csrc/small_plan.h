@@ -195,7 +195,7 @@ inline MxTile pick_mx_tile(int64_t M, int64_t N, int64_t K, int64_t experts) {
   constexpr MxCost s64[2] = {{3.5, 0.24, 0.06, 0.46, 0.27, 0.18, 6.7, 0.043}, {6.2, 0.13, 0.10, 0.34, 0.44, 0.0, 8.9, 0.072}};
   constexpr MxCost s128[2] = {{3.8, 0.61, 0.45, 1.18, 0.71, 0.39, 4.8, 0.052}, {7.1, 0.78, 0.19, 1.23, 1.17, 0.18, 7.3, 0.0}};
   constexpr MxCost s256[2] = {{9.2, 1.10, 1.02, 3.39, 2.27, 0.94, 3.0, 0.024}, {9.4, 1.11, 0.80, 3.63, 3.41, 0.0, 4.6, 0.0}};
-  constexpr MxCost deep{5.0, 0.355, 0.30, 0.0, 0.0, 0.0, 6.0, 0.0};
+  constexpr MxCost deep[2] = {{5.0, 0.355, 0.30, 0.0, 0.0, 0.0, 6.0, 0.0}, {6.3, 0.33, 0.27, 0.0, 0.0, 0.0, 7.5, 0.06}};
   constexpr MxCost s256x128{7.2, 0.55, 0.56, 0.0, 0.0, 0.0, 6.0, 0.03};
   constexpr MxCost s32x128{4.8, 0.33, 0.08, 0.65, 0.51, 0.06, 9.0, 0.091};
   MxTile best = MX_128x128;
@@ -210,13 +210,16 @@ inline MxTile pick_mx_tile(int64_t M, int64_t N, int64_t K, int64_t experts) {
   // than the larger fragments' fewer reads (us, eight and four, operands from HBM: 32768 x 4096 x 1408 187 and 196, 8192 x
   // 8192 x 4096 153 and 159, 4096 x 28672 x 4096 272 and 278; 4096 x 8192 x 8192 143 and 141.5, 8192 x 8192 x 8192 275 and 269).
   if (grouped || steps > 2) take(grouped || steps <= 16 ? MX_256 : MX_256_LONG, s256[grouped](tiles(256, 256), steps, mb));
-  // dense 128 x 128 tiles that have a CU each: its LDS holds four stages instead of two (us, four and two: 2000 x 2000 x
-  // 8192 27 and 36, 1000 x 4000 x 4096 15.4 and 20.5, 1024 x 1024 x 1024 6.6 and 6.7; with two tiles a CU 73 and 47, 8192 x
-  // 8192 x 512).  The host does not know how many tiles experts have.
-  if (!grouped && tiles(128, 128) <= 256) take(MX_128_DEEP, deep(tiles(128, 128), steps, mb));
+  // 128 x 128 tiles that have a CU each (experts': at most that many): its LDS holds four stages instead of two (us, four and
+  // two: 2000 x 2000 x 8192 27 and 36, 1000 x 4000 x 4096 15.4 and 20.5, 1024 x 1024 x 1024 6.6 and 6.7, 8 experts of 2048
+  // rows in all, 1024 x 4096 14.8 and 16.9; with two tiles a CU 73 and 47, 8192 x 8192 x 512)
+  auto one_each = [&](int64_t tm, int64_t tn) {
+    return (grouped ? M / tm + std::min(M, experts) : (M + tm - 1) / tm) * ((N + tn - 1) / tn) <= 256;
+  };
+  if (one_each(128, 128)) take(MX_128_DEEP, deep[grouped](tiles(128, 128), steps, mb));
   // ... 256 x 128 with a CU each: three stages (us, 256 x 128 and 128 x 128: 2048 x 4096 x 8192 45 and 51, 512 x 11008 x
-  // 4096 23.4 and 28.3, 1500 x 4096 x 2048 14.0 and 13.2)
-  if (!grouped && tiles(256, 128) <= 256) take(MX_256x128, s256x128(tiles(256, 128), steps, mb));
+  // 4096 23.4 and 28.3, 2048 x 4096 x 2048 16.3 and 15.9, x 1024 12.6 and 12.2, 8 experts of 2048 rows in all, 2000 x 4096 23.5 and 27.4)
+  if (one_each(256, 128) && steps > 4) take(MX_256x128, s256x128(tiles(256, 128), steps, mb));
   take(MX_64x64, s64[grouped](tiles(64, 64), steps, mb));
   if (grouped) take(MX_32x128, s32x128(tiles(32, 128), steps, mb));
   // blocks of 32 x 32 share CUs: their loads add up
