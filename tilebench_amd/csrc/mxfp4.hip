@@ -99,13 +99,18 @@ __device__ __forceinline__ uint32_t quantise(const float (&v)[UNIT], int& byte) 
 // The same of products silu(g) * u in fp32, with bounds; false where these do not settle a code or the scale.
 // Relative error: 1 ulp each of exp2 and of the reciprocal, half of the sum and the two products, together 3.5 * 2^-23, and
 // the exponent's own, |t| ln 2 times the rounding of t and of log2(e), below |t| 2^-23.  Beyond |g| = 80, for tiny
-// blocks (products below the normals) and for what is not finite the bounds do not hold.
+// blocks (products below the normals) and for what is not finite the bounds do not hold.  Nor for gates below the normals:
+// g / 2 has few bits there, which a large u makes those of an ordinary product (halves of 16-bit types' gates are exact, and
+// of a normal gate it loses 2^-23 at most).
+template <int DTYPE>
 __device__ __forceinline__ bool quantise_gated_bounded(const float (&g)[UNIT], const float (&u)[UNIT], int& byte, uint32_t& codes) {
   float lo[UNIT], hi[UNIT];
   uint32_t top_lo = 0, top_hi = 0;
   float most = 0.f;
+  bool small = false;  // a gate below the normals, but not 0
 #pragma unroll
   for (int i = 0; i < UNIT; ++i) {
+    if constexpr (DTYPE == 0) small |= __builtin_amdgcn_classf(g[i], 0x90);
     const float t = g[i] * 1.44269504f;
     const float v = g[i] * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-t)) * u[i];
     const float b = __builtin_fmaf(__builtin_fabsf(t), 0x1p-23f, 0x1p-20f);
@@ -126,7 +131,8 @@ __device__ __forceinline__ bool quantise_gated_bounded(const float (&g)[UNIT], c
   }
   codes = codes8(hi);
   // a block of zeros is settled by 64 bits too: 0 and what is below the normals look alike
-  return top_lo >> 23 == top_hi >> 23 && top_hi < 0x7F800000u && top_lo >= 0x0D800000u && most <= 80.f && codes == codes8(lo);
+  return top_lo >> 23 == top_hi >> 23 && top_hi < 0x7F800000u && top_lo >= 0x0D800000u && most <= 80.f && !small &&
+         codes == codes8(lo);
 }
 
 // The same of products silu(g) * u in 64 bits.  What goes on to the 4-bit rounding
@@ -175,7 +181,7 @@ __global__ void __launch_bounds__(THREADS)
     if constexpr (GATED) {
       float u[UNIT];
       load_unit<DTYPE>(x, at + (int64_t)s.upr * UNIT, u);
-      if (!__all(quantise_gated_bounded(v, u, byte, q))) q = quantise_gated(v, u, byte);
+      if (!__all(quantise_gated_bounded<DTYPE>(v, u, byte, q))) q = quantise_gated(v, u, byte);
     } else {
       q = quantise(v, byte);
     }
