@@ -12,7 +12,8 @@
 // Gated: the values are silu(g) * u = g / (1 + exp(-g)) * u, and codes and scales those of the product in
 // 64 bits.  Nearly all are settled in fp32: a value comes with a bound of its error, both ends of that range are rounded,
 // and where they agree (and the block's exponent does) that is the answer; a wavefront with a value next to a
-// border computes in 64 bits (about one in a thousand on N(0, 1) gates).  16008 x 1408 bf16: 25 us; 61 with all in 64 bits.
+// border computes in 64 bits (about one in a thousand on N(0, 1) gates; zeros are settled like other values).  16008 x 1408
+// bf16, calls replayed over changing inputs: 26 us, with zeros among the values or half of the rows 25, with all in 64 bits 66.
 //
 // Both are bound by memory: 4096 x 7168 bf16 (74 MB) 14.8 us to codes, 5.0 TB/s, and 12.6 back, 5.9.  Four lanes share a block, eight channels each: a
 // lane's 16-bit channels are one 16-byte load (a wavefront reads 1 KiB runs), its
@@ -97,8 +98,8 @@ __device__ __forceinline__ uint32_t quantise(const float (&v)[UNIT], int& byte) 
 }
 
 // The same of products silu(g) * u in fp32, with bounds; false where these do not settle a code or the scale.
-// Relative error: 1 ulp each of exp2 and of the reciprocal, half of the sum and the two products, together 3.5 * 2^-23, and
-// the exponent's own, |t| ln 2 times the rounding of t and of log2(e), below |t| 2^-23.  Beyond |g| = 80, for tiny
+// Relative error: 1 ulp each of exp2 and of the reciprocal, half of the sum, the two products and the ends' own roundings,
+// together 5 * 2^-23, and the exponent's own, |t| ln 2 times the rounding of t and of log2(e), below |t| 2^-23.  Beyond |g| = 80, for tiny
 // blocks (products below the normals) and for what is not finite the bounds do not hold.  Nor for gates below the normals:
 // g / 2 has few bits there, which a large u makes those of an ordinary product (halves of 16-bit types' gates are exact, and
 // of a normal gate it loses 2^-23 at most).
@@ -115,24 +116,24 @@ __device__ __forceinline__ bool quantise_gated_bounded(const float (&g)[UNIT], c
     const float v = g[i] * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-t)) * u[i];
     const float b = __builtin_fmaf(__builtin_fabsf(t), 0x1p-23f, 0x1p-20f);
     most = fmaxf(most, __builtin_fabsf(g[i]));
-    lo[i] = __builtin_fmaf(-b, v, v);
+    lo[i] = v * (1.f - b);  // a sum v - b v would make +0 of -0
     hi[i] = __builtin_fmaf(b, v, v);
     top_lo = max(top_lo, __builtin_bit_cast(uint32_t, lo[i]) & 0x7FFFFFFFu);
     top_hi = max(top_hi, __builtin_bit_cast(uint32_t, hi[i]) & 0x7FFFFFFFu);
   }
   top_lo = max4(top_lo);
   top_hi = max4(top_hi);
-  byte = (int)(top_hi >> 23) - 2;
-  const float inverse = power(min(max(254 - byte, 0), 254));
+  byte = max((int)(top_hi >> 23) - 2, 0);
+  const float inverse = power(max(254 - byte, 0));
 #pragma unroll
   for (int i = 0; i < UNIT; ++i) {
     lo[i] *= inverse;
     hi[i] *= inverse;
   }
   codes = codes8(hi);
-  // a block of zeros is settled by 64 bits too: 0 and what is below the normals look alike
-  return top_lo >> 23 == top_hi >> 23 && top_hi < 0x7F800000u && top_lo >= 0x0D800000u && most <= 80.f && !small &&
-         codes == codes8(lo);
+  // a block of zeros is one in 64 bits too, or of products below 2^-149: scale 0 and zero codes with their signs either way
+  return (top_hi == 0 || (top_lo >> 23 == top_hi >> 23 && top_hi < 0x7F800000u && top_lo >= 0x0D800000u)) && most <= 80.f &&
+         !small && codes == codes8(lo);
 }
 
 // The same of products silu(g) * u in 64 bits.  What goes on to the 4-bit rounding
