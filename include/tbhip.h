@@ -548,8 +548,9 @@ tb_status tb_shared_prefix_attention_workspace_size(int64_t T, int64_t Hq, int64
  *   top_groups best groups can be chosen (equal scores: lowest group first);
  *   ids int32 [T, k]: the k largest c, descending (equal: lowest expert first);
  *   weights fp32 [T, k]: scale * s of these, over their sum if renormalize.
- * Computed in fp64 and rounded once.  NaN ranks above every number; a softmax
- * row of -inf alone has scores 0, and weights that sum to 0 are 0.
+ * Computed in fp64 and rounded once; a row's results depend on its own logits
+ * and the bias alone.  NaN ranks above every number; a softmax row of -inf alone
+ * has scores 0, and weights that sum to 0 are 0.
  * Requires T < 2^24, E <= 1024, E % groups == 0, groups <= 64, k <= 32 and k <=
  * top_groups * E / groups, E / groups >= group_top.
  * Beside tb_moe_topk_gating (softmax of the chosen logits alone), which replaces

@@ -27,12 +27,14 @@
 //
 // Rows (everything else): one wavefront a row, lane l holds experts l, 64 + l, ...; choices are compared as
 // 64-bit keys in the order of their values (0: cannot be chosen), k rounds of a maximum over the wavefront.
-// A wavefront of the first kind that meets inf, NaN or large logits takes its rows this way, one after the other.
+// Rows of the first kind that hold inf, NaN or large logits are taken this way by their wavefront, one after the other; the
+// rows beside them stay with the lanes, so that a row's results are its own (the ways' exponentials differ in their last bits).
 //
 // Bound by the chain of steps (1 row to a few hundred: 6 us, the launch included) and by fp64 instructions: 16384 x 256
-// fp32 logits, sigmoid, 4 of 8 groups, k 8: 17 us with 40 % of the issue slots taken (18 MB, 3 us of HBM), and 64 one row to a
+// fp32 logits, sigmoid, 4 of 8 groups, k 8: 16 us with 40 % of the issue slots taken (18 MB, 3 us of HBM), and 64 one row to a
 // wavefront.  A lane has 16 experts at
 // most, two sorts of eight and a merge; more lanes a row mean more merges, of lists that are the same in all lanes by then.
+// The second way: with k 12 69 us, with a quarter of the logits at -inf (k 8 or 12) 71 and 69, with one such row in seven 30.
 #include "tb_common.h"
 
 // a score is rounded before its bias is added, wherever it is computed
@@ -323,8 +325,9 @@ __global__ void __launch_bounds__(64 * WPB) route_lanes(Args p) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t t0 = ((int64_t)blockIdx.x * WPB + wave) * ROWS, t = t0 + lane / LPR;
   if (t0 >= p.T) return;  // no barrier: a row is one wavefront's
-  const bool live = t < p.T;
-  const int e0 = l * p.per, n = live ? min(max(p.E - e0, 0), p.per) : 0;
+  bool live = t < p.T;
+  const int e0 = l * p.per;
+  int n = live ? min(max(p.E - e0, 0), p.per) : 0;
   uint64_t* const own_lds = lds + wave * p.wave_words;
 
   float x[V], b[V];
@@ -353,9 +356,22 @@ __global__ void __launch_bounds__(64 * WPB) route_lanes(Args p) {
     odd = __builtin_fmaf(b[j], 0.f, odd);
     most = fmaxf(most, fabsf(x[j]));
   }
-  if (__any(odd != 0.f || !(most < 700.f))) {
-    for (int r = 0; r < ROWS && t0 + r < p.T; ++r) route_row<LPR * V / 64>(p, t0 + r, own_lds);
-    return;
+  if (const uint64_t odd_lanes = __ballot(odd != 0.f || !(most < 700.f))) {
+    // these rows by the whole wavefront, the others go on: a row takes the way of its own values
+    constexpr uint64_t ROW = LPR == 64 ? ~0ull : (1ull << (LPR & 63)) - 1;
+    int left = 0;
+    for (int r = 0; r < ROWS && t0 + r < p.T; ++r) {
+      if (odd_lanes >> (r * LPR) & ROW)
+        route_row<LPR * V / 64>(p, t0 + r, own_lds);
+      else
+        ++left;
+    }
+    if (left == 0) return;
+    wave_fence();  // the last of them may still be read
+    if (odd_lanes >> base & ROW) {
+      live = false;
+      n = 0;
+    }
   }
   float top = 0.f;
   double share = 1.0;
