@@ -353,6 +353,9 @@ struct Tile {
   static constexpr int PAD_OFF = SC_OFF + 2 * SC;                      // those of wavefronts that have none land here
   static constexpr int LDS_BYTES = PAD_OFF + (NS % NW ? 1024 : 0);
   static_assert(LDS_BYTES <= 160 * 1024 && SC % 1024 == 0 && TM * SROW % 1024 == 0, "LDS layout");
+  // A buffer of scales goes out after the wait of step k, k % CS == 0, and is read after that of step k + CS - 1, which leaves
+  // a stage's DMAs ST - 2 times under way: those of CS - 1 stages were issued behind the scales.
+  static_assert(CS >= 2 && CS >= ST - 1, "scales have to have landed when they are read");
 };
 
 // The tile at `at`, or with half of C's FI the first half of its rows.
@@ -441,7 +444,7 @@ __device__ __forceinline__ void tile_product(const Args& p, const Place& at, uin
     for (int j = 0; j < FJ; ++j) acc[i][j] = f32x16{};
 
   // Codes of step k + 1 have landed when those of the ST - 2 steps behind are all that is outstanding; scales among them
-  // only make the wait longer.
+  // only make the wait longer (that they have landed themselves is Tile's assertion).
   // DMAs of a step that go out beside the last substep; the others beside the next one's first (8192 x 8192 x 8192 on eight
   // wavefronts: a quarter 265 us, half 269, three quarters 278)
   constexpr int NOW = C::NW == 8 ? PER / 4 : PER / 2;
