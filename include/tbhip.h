@@ -347,7 +347,9 @@ tb_status tb_matmul_workspace_size(int dtype, int64_t M, int64_t N, int64_t K, i
  * current device (host code: nothing is launched; operands aligned to 16
  * bytes).  `kernel` is a static string.  A block computes tile_rows x tile_cols
  * of the product on `wavefronts` wavefronts; within it k_groups groups of them
- * take parts of K, and k_splits blocks share one tile's K.  Gate/up (N = 2 I): its
+ * take parts of K, and k_splits blocks share one tile's K.  `stages` is the number
+ * of K steps that LDS holds at once where a kernel has one tile with several such
+ * depths (mx_tile), 0 for the others.  Gate/up (N = 2 I): its
  * tile_cols columns of W13 are tile_cols / 2 activation columns.
  *   op                     M                N      experts
  *   TB_OP_W4A16            rows             N      ignored
@@ -376,7 +378,7 @@ enum {
 };
 typedef struct {
   const char* kernel;
-  int32_t tile_rows, tile_cols, wavefronts, k_groups, k_splits;
+  int32_t tile_rows, tile_cols, wavefronts, k_groups, k_splits, stages;
 } tb_tile;
 tb_status tb_gemm_tile(int op, int64_t M, int64_t N, int64_t K, int64_t experts, tb_tile* tile);
 

@@ -6,6 +6,7 @@ from pathlib import Path
 import pytest
 
 from tilebench_amd import build
+from tilebench_amd import runtime as rt
 
 SOURCE = Path(__file__).parent / "native" / "mx_tile_shape.hip"
 
@@ -24,3 +25,43 @@ def test_scales_land_before_they_are_read(shape, fits):
                          capture_output=True, text=True)
     assert (res.returncode == 0) == fits, res.stderr[-2000:]
     assert fits or "scales have to have landed" in res.stderr
+
+
+# ----------------------------------------------------------------------------- what ran
+
+
+def tile(op, M, N, K, experts=0):
+    """(kernel, rows, columns, wavefronts, stages) of a call's tile; no GPU needed."""
+    t = rt.gemm_tile(op, M, N, K, experts)
+    return t["kernel"], t["BM"], t["BN"], t["waves"], t.get("stages")
+
+
+def cases(test):
+    """The parameters of a test's first parametrisation."""
+    return next(m.args[1] for m in test.pytestmark if m.name == "parametrize")
+
+
+@pytest.mark.skipif(not rt.LIB_PATH.exists(), reason="libtbhip.so is not built")
+def test_a_tile_says_how_many_stages_it_holds():
+    """128 x 128 has two forms, which only the stages tell apart."""
+    assert tile(rt.OP_MXFP4, 3500, 3600, 96) == ("mx_tile", 128, 128, 4, 2)
+    assert tile(rt.OP_MXFP4, 1801, 2001, 4128) == ("mx_tile", 128, 128, 4, 4)
+    assert tile(rt.OP_MXFP4_GROUPED, 8027, 1300, 96, 8) == ("mx_tile", 128, 128, 4, 2)
+    assert tile(rt.OP_MXFP4_GROUPED, 2321, 900, 1408, 8) == ("mx_tile", 128, 128, 4, 4)
+    assert "stages" not in rt.gemm_tile(rt.OP_MXFP4, 1, 4096, 4096) and "stages" not in rt.gemm_tile(rt.OP_W4A16, 300, 512, 512)
+
+
+@pytest.mark.skipif(not rt.LIB_PATH.exists(), reason="libtbhip.so is not built")
+def test_the_gpu_tests_run_every_tile():
+    import test_gpu_experts as on_gpu
+
+    dense = {tile(rt.OP_MXFP4, M, N, K) for M, N, K, _ in cases(on_gpu.test_product_on_every_tile)}
+    both = {("mx_skinny", 32, 32, 4, None), ("mx_tile", 64, 64, 4, 4), ("mx_tile", 128, 128, 4, 2), ("mx_tile", 128, 128, 4, 4),
+            ("mx_tile", 256, 128, 8, 3), ("mx_tile", 256, 256, 8, 2)}
+    assert dense == both | {("mx_tile", 256, 256, 4, 2)}
+    grouped = set()
+    for rows, N, K, _ in cases(on_gpu.test_grouped_product_on_every_tile):
+        # its eight segments
+        R = rows + rows // 3 + 2 * rows + rows - 1 + 300 + 257 + rows + 5 if rows > 6 else rows + 3 + 65 + 1 + 20 + 4 + 1
+        grouped.add(tile(rt.OP_MXFP4_GROUPED, R, N, K, 8))
+    assert grouped == both | {("mx_tile", 32, 128, 4, 3)}

@@ -681,7 +681,7 @@ void tb::describe_mxfp4(int64_t M, int64_t N, int64_t K, int64_t experts, tb_til
   const plan::MxTile tile = plan::pick_mx_tile(M, N, K, experts);
   auto f = [&](auto shape) {
     typedef decltype(shape) C;
-    *out = tb_tile{"mx_tile", C::TM, C::TN, C::NW, 1, 1};
+    *out = tb_tile{"mx_tile", C::TM, C::TN, C::NW, 1, 1, C::ST};
     return TB_OK;
   };
   if (tile == plan::MX_32x32)

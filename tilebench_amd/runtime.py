@@ -34,7 +34,8 @@ class GemmTile(ctypes.Structure):
     """tb_tile: the kernel and tile of a GEMM call."""
 
     _fields_ = [("kernel", ctypes.c_char_p), ("tile_rows", ctypes.c_int32), ("tile_cols", ctypes.c_int32),
-                ("wavefronts", ctypes.c_int32), ("k_groups", ctypes.c_int32), ("k_splits", ctypes.c_int32)]
+                ("wavefronts", ctypes.c_int32), ("k_groups", ctypes.c_int32), ("k_splits", ctypes.c_int32),
+                ("stages", ctypes.c_int32)]
 
 
 #: tb_gemm_tile's operators
@@ -207,8 +208,9 @@ def gemm_tile(op: int, M: int, N: int, K: int, experts: int = 0) -> dict:
     asked for when a configuration is read, so a call pays nothing for it."""
     t = GemmTile()
     call("tb_gemm_tile", op, M, N, K, experts, ctypes.byref(t))
-    return {"kernel": t.kernel.decode(), "BM": t.tile_rows, "BN": t.tile_cols, "waves": t.wavefronts,
-            "k_groups": t.k_groups, "k_splits": t.k_splits}
+    cfg = {"kernel": t.kernel.decode(), "BM": t.tile_rows, "BN": t.tile_cols, "waves": t.wavefronts,
+           "k_groups": t.k_groups, "k_splits": t.k_splits}
+    return {**cfg, "stages": t.stages} if t.stages else cfg
 
 
 def workspace(nbytes: int, device, stream: int):
