@@ -562,6 +562,10 @@ tb_status tb_moe_expert_routing(const void* logits, const float* bias, float* we
                                 int64_t E, int64_t k, int64_t groups, int64_t top_groups, int64_t group_top,
                                 int64_t row, int softmax, int renormalize, double scale, int dtype,
                                 hipStream_t stream);
+/* The kernel that routes these sizes (a static string), the lanes that own a row
+ * in it and the threads of a block (host code: nothing is launched). */
+tb_status tb_moe_expert_routing_kernel(int64_t E, int64_t k, int64_t groups, const char** kernel, int32_t* lanes,
+                                       int32_t* threads);
 
 /*
  * Microscaled 4-bit floating point (MXFP4).  A matrix [rows, K] is

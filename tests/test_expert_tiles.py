@@ -1,4 +1,5 @@
 """Tiles of the MXFP4 products, on the host."""
+import ctypes
 import shutil
 import subprocess
 from pathlib import Path
@@ -65,3 +66,24 @@ def test_the_gpu_tests_run_every_tile():
         R = rows + rows // 3 + 2 * rows + rows - 1 + 300 + 257 + rows + 5 if rows > 6 else rows + 3 + 65 + 1 + 20 + 4 + 1
         grouped.add(tile(rt.OP_MXFP4_GROUPED, R, N, K, 8))
     assert grouped == both | {("mx_tile", 32, 128, 4, 3)}
+
+
+@pytest.mark.skipif(not rt.LIB_PATH.exists(), reason="libtbhip.so is not built")
+@pytest.mark.parametrize("E,k,groups,want", [
+    (60, 4, 1, ("route_lanes", 8, 128)), (256, 8, 8, ("route_lanes", 16, 128)), (500, 8, 5, ("route_rows", 64, 256)),
+    (384, 8, 8, ("route_lanes", 32, 128)), (1024, 8, 8, ("route_lanes", 64, 128)), (256, 9, 8, ("route_rows", 64, 256))])
+def test_the_library_says_which_routing_kernel_it_launches(E, k, groups, want):
+    """get_last_config() asks the rule that the launch follows."""
+    from tilebench_amd.benchmarks.experts.moe_expert_routing import impl_hip
+
+    lib = rt.load_library()
+    kernel, lanes, threads = ctypes.c_char_p(), ctypes.c_int32(), ctypes.c_int32()
+    out = tuple(map(ctypes.byref, (kernel, lanes, threads)))
+    assert lib.tb_moe_expert_routing_kernel(E, k, groups, *out) == rt.TB_OK
+    assert (kernel.value.decode(), lanes.value, threads.value) == want
+    before, impl_hip._last_call = impl_hip._last_call, (E, k, groups)
+    assert tuple(impl_hip.get_last_config().values()) == want
+    impl_hip._last_call = before
+    assert lib.tb_moe_expert_routing_kernel(E, 33, groups, *out) == rt.TB_E_INVALID
+    assert lib.tb_moe_expert_routing_kernel(7, 1, 2, *out) == rt.TB_E_INVALID
+    assert lib.tb_moe_expert_routing_kernel(E, k, groups, None, *out[1:]) == rt.TB_E_INVALID

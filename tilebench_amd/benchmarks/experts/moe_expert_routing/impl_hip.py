@@ -10,6 +10,8 @@ largest c, descending; equal ones go to the lowest expert, equal groups to the
 lowest group.  weights are s of these, divided by their sum if renormalize, times
 scale.  Computed in 64 bits and rounded once.
 """
+import ctypes
+
 import torch
 
 from tilebench_amd import experts
@@ -17,7 +19,7 @@ from tilebench_amd import runtime as rt
 
 rt.load_library()
 
-_last_config = None
+_last_call = None  # (E, k, groups)
 SCORES = ("sigmoid", "softmax")
 
 
@@ -48,7 +50,7 @@ def check(logits, k, bias=None, groups=1, top_groups=1, group_top=1, score="soft
 
 def run(logits: torch.Tensor, k: int, bias=None, groups: int = 1, top_groups: int = 1, group_top: int = 1,
         score: str = "softmax", renormalize: bool = True, scale: float = 1.0, **kwargs):
-    global _last_config
+    global _last_call
     rt.require_device(logits, bias)
     T, E = check(logits, k, bias, groups, top_groups, group_top, score)
     weights = logits.new_empty((T, k), dtype=torch.float32)
@@ -60,13 +62,13 @@ def run(logits: torch.Tensor, k: int, bias=None, groups: int = 1, top_groups: in
         rt.call("tb_moe_expert_routing", logits.data_ptr(), rt.ptr(bias), weights.data_ptr(), ids.data_ptr(), T, E, k,
                 groups, top_groups, group_top, logits.stride(0), score == "softmax", renormalize, scale,
                 experts.DTYPES[logits.dtype], rt.stream_handle(logits.get_device()))
-    lanes = 8 if E <= 64 else 16 if E <= 256 else 32 if E <= 512 else 64
-    if k <= 8 and (groups == 1 or E // groups % -(-E // lanes) == 0):
-        _last_config = {"kernel": "route_lanes", "lanes_per_row": lanes, "block": 128}
-    else:
-        _last_config = {"kernel": "route_rows", "lanes_per_row": 64, "block": 256}
+    _last_call = E, k, groups
     return weights, ids
 
 
 def get_last_config():
-    return _last_config
+    if _last_call is None:
+        return None
+    kernel, lanes, threads = ctypes.c_char_p(), ctypes.c_int32(), ctypes.c_int32()
+    rt.call("tb_moe_expert_routing_kernel", *_last_call, *map(ctypes.byref, (kernel, lanes, threads)))
+    return {"kernel": kernel.value.decode(), "lanes_per_row": lanes.value, "block": threads.value}

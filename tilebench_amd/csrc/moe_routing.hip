@@ -482,6 +482,12 @@ __global__ void __launch_bounds__(64 * WPB) route_lanes(Args p) {
 
 constexpr int LANE_WAVES = 2;
 
+// Lanes that own a row; 0: a whole wavefront does (route_rows).
+int lanes_of_row(int64_t E, int64_t k, int64_t groups) {
+  const int64_t lanes = E <= 64 ? 8 : E <= 256 ? 16 : E <= 512 ? 32 : 64, per = (E + lanes - 1) / lanes;
+  return k <= 8 && (groups == 1 || (E / groups) % per == 0) ? (int)lanes : 0;
+}
+
 template <int LPR, int V>
 tb_status launch_lanes_as(const char* fn, const Args& p, hipStream_t stream) {
   auto* const kernel = &route_lanes<LPR, V, LANE_WAVES>;
@@ -526,16 +532,15 @@ extern "C" tb_status tb_moe_expert_routing(const void* logits, const float* bias
   Args p{logits, bias, weights, ids, T, row, scale, (int)E, (int)k, (int)groups, (int)top_groups, (int)group_top,
          softmax, renormalize, dtype};
   TB_CHECK_ARG(T < (1ll << 24), "%s: problem too large", fn);
-  const int64_t lpr = E <= 64 ? 8 : E <= 256 ? 16 : E <= 512 ? 32 : 64;
-  p.per = (int)((E + lpr - 1) / lpr);
-  if (k <= 8 && (groups == 1 || (E / groups) % p.per == 0)) {
+  if (const int lpr = lanes_of_row(E, k, groups)) {
     const int size = dtype ? 2 : 4;
+    p.per = (int)((E + lpr - 1) / lpr);
     p.span = (int)(E / groups) / p.per;
     p.span_shift = groups > 1 && (p.span & (p.span - 1)) == 0;
     // loads of 16 bytes need addresses on 4, and offsets within a wavefront's rows below 2^31
     p.vec = tb::aligned(logits, 4) && row * size % 4 == 0 && p.per * size % 4 == 0 && row < (1ll << 24);
     p.wave_words = (int)(2 * E > 64 / lpr * 4 ? 2 * E : 64 / lpr * 4);  // route_row's, or the lists of eight
-    return launch_lanes(fn, p, (int)lpr, stream);
+    return launch_lanes(fn, p, lpr, stream);
   }
   const int64_t blocks = (T + WAVES - 1) / WAVES;
   const size_t lds = (size_t)WAVES * 2 * 8 * (size_t)E;
@@ -544,4 +549,17 @@ extern "C" tb_status tb_moe_expert_routing(const void* logits, const float* bias
   if (tb_status st = tb::reserve_lds(reinterpret_cast<const void*>(kernel), lds, fn)) return st;
   hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(64 * WAVES), lds, stream, p);
   return tb::launch_status(fn);
+}
+
+extern "C" tb_status tb_moe_expert_routing_kernel(int64_t E, int64_t k, int64_t groups, const char** kernel, int32_t* lanes,
+                                                  int32_t* threads) {
+  using namespace tb::routing;
+  const char* const fn = "tb_moe_expert_routing_kernel";
+  TB_CHECK_ARG(kernel && lanes && threads, "%s: null output", fn);
+  TB_CHECK_ARG(E > 0 && E <= 1024 && k > 0 && k <= 32 && groups > 0 && E % groups == 0, "%s: no routing has these sizes", fn);
+  const int n = lanes_of_row(E, k, groups);
+  *kernel = n ? "route_lanes" : "route_rows";
+  *lanes = n ? n : 64;
+  *threads = 64 * (n ? LANE_WAVES : WAVES);
+  return TB_OK;
 }

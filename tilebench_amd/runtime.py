@@ -76,6 +76,7 @@ SIGNATURES: dict[str, list] = {
     "tb_shared_prefix_attention": [_c_p] * 13 + [_c_i64] * 19 + [ctypes.c_double, _c_int, _c_int, _c_p, _c_i64, _c_p],
     "tb_shared_prefix_attention_workspace_size": [_c_i64] * 10 + [_c_int, ctypes.POINTER(_c_i64)],
     "tb_moe_expert_routing": [_c_p] * 4 + [_c_i64] * 7 + [_c_int] * 2 + [ctypes.c_double, _c_int, _c_p],
+    "tb_moe_expert_routing_kernel": [_c_i64] * 3 + [ctypes.POINTER(ctypes.c_char_p)] + [ctypes.POINTER(ctypes.c_int32)] * 2,
     "tb_mxfp4_quant": [_c_p] * 3 + [_c_i64] * 4 + [_c_int] * 2 + [_c_p],
     "tb_mxfp4_dequant": [_c_p] * 3 + [_c_i64] * 3 + [_c_int, _c_p],
     "tb_mxfp4_gemm": [_c_p] * 5 + [_c_i64] * 5 + [_c_int, _c_p],
