@@ -97,16 +97,23 @@ def align(ids, experts: int):
 
 def combine(y, ids, experts: int):
     """out [T, H]: each token's rows of y [T * k, H] added in fp32 in slot order, rounded once; ids int32 [T, k] outside
-    [0, experts) are left out."""
+    [0, experts) are left out.  A y that does not start on 16 bytes, or whose H is no multiple of 8, is copied in the
+    call."""
     if y.dtype is not torch.float16 and y.dtype is not torch.bfloat16 or ids.dtype is not torch.int32:
         raise TypeError("combine: y must be float16 or bfloat16 and ids int32")
     if y.dim() != 2 or ids.dim() != 2 or y.shape[0] != ids.numel():
         raise ValueError("combine: y must be [tokens * k, H] with ids [tokens, k]")
     rt.require_device(y, ids)
-    y, ids = y.contiguous(), ids.contiguous()
     T, k = ids.shape
+    H = y.shape[1]
+    if H % 8:
+        y = torch.nn.functional.pad(y, (0, -H % 8))
+    else:
+        y = y.contiguous()
+        y = y if y.data_ptr() % 16 == 0 else y.clone()
+    ids = ids.contiguous()
     out = torch.empty((T, y.shape[1]), dtype=y.dtype, device=y.device)
     if out.numel():
         rt.call("tb_moe_combine" if y.dtype is torch.float16 else "tb_moe_combine_bf16", y.data_ptr(), ids.data_ptr(),
                 out.data_ptr(), T, k, experts, y.shape[1], rt.stream_handle(y.get_device()))
-    return out
+    return out if out.shape[1] == H else out[:, :H].contiguous()
