@@ -1,8 +1,11 @@
-"""Expert layers on the GPU: the steps between the products."""
+"""Expert layers on the GPU: the steps between the products, and references in graphs."""
 import pytest
 import torch
 
 from tilebench_amd import experts
+from tilebench_amd.benchmarks.experts.mxfp4_dequant import impl_torch as dequant_ref
+from tilebench_amd.benchmarks.experts.mxfp4_gemm import impl_torch as gemm_ref
+from tilebench_amd.benchmarks.experts.mxfp4_quant import impl_torch as quant_ref
 
 pytestmark = pytest.mark.gpu
 
@@ -13,6 +16,10 @@ def say(*what):
 
 def gen(seed):
     return torch.Generator().manual_seed(seed)
+
+
+def matrix(rows, K, seed):
+    return [t.cuda() for t in quant_ref.run(torch.randn(rows, K, generator=gen(seed)))]
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
@@ -30,3 +37,28 @@ def test_combine_of_any_rows(gpu, tokens, k, H, skip, dtype):
         total = torch.where(((ids[:, j] >= 0) & (ids[:, j] < 8))[:, None], total + row, total)
     got = experts.combine(y, ids.cuda(), 8)
     assert got.shape == (tokens, H) and got.is_contiguous() and torch.equal(got.cpu(), total.to(dtype))
+
+
+@pytest.mark.parametrize("op", ["mxfp4_dequant", "mxfp4_gemm"])
+def test_references_are_captured(gpu, op):
+    """A reference that is timed beside a replayed kernel is replayed itself: its graph gives the eager result, again and
+    again, on what the inputs hold then."""
+    say("reference graph", op)
+    a, w = matrix(40, 352, 1), matrix(24, 352, 2)
+    args = a if op == "mxfp4_dequant" else (*a, *w)
+    ref = dequant_ref if op == "mxfp4_dequant" else gemm_ref
+    want = ref.run(*args)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ref.run(*args)
+    for i in range(4):
+        if i == 2:
+            for t, fresh in zip(a, matrix(40, 352, 9)):
+                t.copy_(fresh)
+            want = ref.run(*args)
+        out.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        assert torch.equal(ref.run(*args), want)

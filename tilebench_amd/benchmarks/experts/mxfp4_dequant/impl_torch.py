@@ -3,13 +3,13 @@ import torch
 
 from tilebench_amd.benchmarks.experts.mxfp4_quant.impl_torch import BLOCK, power
 
-E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
-
 
 def values(codes, scales):
-    """Values [.., K] in 64 bits."""
-    table = torch.tensor(E2M1 + tuple(-v for v in E2M1), dtype=torch.float64, device=codes.device)
-    v = table[torch.stack((codes & 15, codes >> 4), dim=-1).flatten(-2).int()]
+    """Values [.., K] in 64 bits.  No table from the host, so that a call can be captured."""
+    code = torch.stack((codes & 15, codes >> 4), dim=-1).flatten(-2)
+    m = (code & 7).double()
+    v = torch.where(m < 4, m / 2, torch.where(m < 6, m - 2, 2 * m - 8))  # 0, 0.5, 1, 1.5, 2, 3, 4, 6
+    v = torch.where(code > 7, -v, v)
     scale = torch.where(scales == 255, float("nan"), power(scales.long() - 127))
     return (v.unflatten(-1, (-1, BLOCK)) * scale[..., None]).flatten(-2)
 
