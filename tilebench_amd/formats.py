@@ -34,6 +34,12 @@ reference (Tilebench has no quantized checkpoints); their conventions are:
   2^-10 (all below 2^-6) round to nearest even.  Block
   scales (one per 128 x 128 tile, [ceil(N/128), ceil(K/128)]: DeepSeek-V3's
   weight_scale_inv) select the block-scaled GEMM (Fp8BlockWeights).
+* MXFP4 (the OCP microscaling formats): two e2m1 codes a byte, the lower
+  channel in the low four bits, as rows [.., K/2] or in blocks
+  [.., K/32, 16], and E8M0 scales [.., K/32] (biased by 127, 255 is NaN).
+  These are the products' own conventions, but rows of scales have to start on
+  4 bytes and codes on 16: mxfp4_checkpoint_to_tb lays them out once, where a
+  product would copy them in every call.
 * Decode slab layout: not a checkpoint format but the W4A16 decode's own
   weight layout, converted once at load (w4a16_to_slabs below).
 """
@@ -72,6 +78,14 @@ class Fp8BlockWeights:
     wqT: torch.Tensor      # uint8 [N, K]
     sw: torch.Tensor       # fp32 [ceil(N/128), K/128]
     block: int = 128
+
+
+@dataclass
+class Mxfp4Weights:
+    """Operands of the MXFP4 products, [N, K] or experts' [E, N, K], as the kernels take them: dense codes on 16 bytes, rows
+    of scales that start on 4 bytes."""
+    codes: torch.Tensor    # uint8 [.., N, K/2]
+    scales: torch.Tensor   # uint8 [.., N, K/32]
 
 
 # ----------------------------------------------------------------------------- nibbles
@@ -313,6 +327,23 @@ def fp8_checkpoint_to_tb(weight: torch.Tensor, weight_scale: torch.Tensor | floa
         raise ValueError(f"fp8 scale of shape {tuple(s.shape)} for a [{N}, {K}] weight: expected a scalar, [N], "
                          f"[N, 1] or 128 x 128 blocks {blocks}")
     return Fp8Weights(codes.contiguous(), s.contiguous().to(torch.float32))
+
+
+def mxfp4_checkpoint_to_tb(codes: torch.Tensor, scales: torch.Tensor) -> Mxfp4Weights:
+    """A layer's or its experts' MXFP4 weights in the layout that the products take without a copy.
+
+    codes: e2m1 pairs [N, K/2] or [E, N, K/2], or in blocks [.., K/32, 16] (one dimension more than scales); scales E8M0
+    [.., K/32].  uint8, or torch's types of these bytes.  Tensors that already lie so are passed on."""
+    from tilebench_amd import experts
+
+    bytes_of = {getattr(torch, name) for name in ("float4_e2m1fn_x2", "float8_e8m0fnu") if hasattr(torch, name)}
+    codes, scales = (t.view(torch.uint8) if t.dtype in bytes_of else t for t in (codes, scales))
+    if codes.dim() == scales.dim() + 1 and codes.shape[-1] == 16:
+        codes = codes.flatten(-2)
+    if codes.dim() not in (2, 3):
+        raise ValueError(f"mxfp4 weights must be [N, K] or [E, N, K] (got codes {list(codes.shape)})")
+    experts.check_matrix("mxfp4_checkpoint_to_tb", "the weight", codes, scales, codes.dim())
+    return Mxfp4Weights(experts.code_rows(codes), experts.scale_rows(scales)[0])
 
 
 # ----------------------------------------------------------------------------- files
