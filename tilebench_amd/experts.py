@@ -60,12 +60,14 @@ def code_rows(codes):
 
 def scale_rows(scales):
     """(scales, bytes between rows, bytes between matrices) of [rows, S] or [matrices, rows, S], rows on 4 bytes; copied
-    where they lie otherwise."""
+    where they lie otherwise, or so far apart that the kernels' 32-bit offsets do not reach them (rows 4 MiB apart, or gaps
+    between rows that add up to 2 GiB)."""
     *_, n, S = shape = scales.shape
     strides = scales.stride()
     row = strides[-2] if n > 1 else -(-S // 4) * 4
     matrix = strides[0] if len(shape) == 3 and shape[0] > 1 else n * row
-    if (row | matrix | scales.data_ptr()) % 4 or (strides[-1] != 1 and S > 1) or row < S or matrix < (n - 1) * row + S:
+    if (row | matrix | scales.data_ptr()) % 4 or (strides[-1] != 1 and S > 1) or row < S or matrix < (n - 1) * row + S \
+            or row >= 1 << 22 or (n * row >= 1 << 31 and row >= S + 16):
         scales = empty_scales(shape[:-1], S * BLOCK, scales.device).copy_(scales)
         row = -(-S // 16) * 16
         matrix = n * row
