@@ -610,7 +610,9 @@ tb_status tb_mxfp4_dequant(const uint8_t* codes, const uint8_t* scales, void* y,
  *     there times weights[row of Y] (fp32 [R], null: 1) before the rounding.
  *   tb_moe_align's sorted ids are such gather rows of tokens and scatter rows of
  *   pairs.  Rows of Y that no product row goes to are left as they were.
- *   Offsets are held to 0 .. R.
+ *   Offsets are held to 0 .. R; where they descend or segments overlap, an element
+ *   is left as it was or is that row's product with one of the experts whose range
+ *   holds it.
  * Requires K % 32 == 0, K <= 2^22, a and w 16-byte aligned, rows of scales (sa_row, sw_row,
  * sw_expert) on 4 bytes; experts <= 4096; gathered a below 2 GiB.
  * Nearest in the reference: matmul_fp32_fp16_fp8/impl_triton.py:124 run(a, b).
