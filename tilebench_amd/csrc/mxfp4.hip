@@ -15,11 +15,12 @@
 // border computes in 64 bits (about one in a thousand on N(0, 1) gates; zeros are settled like other values).  16008 x 1408
 // bf16, calls replayed over changing inputs: 26 us, with zeros among the values or half of the rows 25, with all in 64 bits 66.
 //
-// Both are bound by memory: 4096 x 7168 bf16 (74 MB) 14.8 us to codes, 5.0 TB/s, and 12.6 back, 5.9.  Four lanes share a block, eight channels each: a
+// Both are bound by memory: 4096 x 7168 bf16 (74 MB) 15.7 us to codes, 4.7 TB/s, and 16.3 back, replayed over changing
+// operands (back from codes just written: 13.0); 16384 x 4096 31 and 30 us, 5.5 and 5.8 TB/s.  Four lanes share a block, eight channels each: a
 // lane's 16-bit channels are one 16-byte load (a wavefront reads 1 KiB runs), its
 // codes one 4-byte store, and the block's largest magnitude takes two exchanges
-// between lanes.  A thread takes four units in turn: loads of all four first hold registers for 16.8 us instead of 14.8,
-// one or two units a thread make no difference.
+// between lanes.  A thread takes four units in turn: loads of all four first hold registers and take a seventh
+// longer, one or two units a thread make no difference.
 #include "tb_common.h"
 
 namespace tb {

@@ -337,8 +337,9 @@ __global__ void __launch_bounds__(64 * KS, KS / 4) mx_skinny(Args p) {
 // through 64 experts' down: 222 us, four of 4 x 4 fragments 237).  8192 x 8192 x 8192: 270 us, 4.1 PFLOP/s; its matrix
 // instructions alone, in this order, 190 (the card then holds 1.8 GHz), without the DMAs 232, without fragment reads 268.
 // Both operands and their scales stream HBM -> LDS by DMA.  Codes: ST stages of one step, rows of 128 bytes, 16-byte chunk
-// c of row i at slot c ^ ((i ^ (i >> 3)) & 7), so that writes and fragment reads are free of conflicts (rows of 64 bytes
-// and twice the stages: 1.3 to 1.4 times slower, a DMA then takes 16 lines for its KiB instead of 8).
+// c of row i at slot c ^ ((i ^ (i >> 3)) & 7), so that their writes and fragment reads are free of conflicts (rows of 64 bytes
+// and twice the stages: 1.3 to 1.4 times slower, a DMA then takes 16 lines for its KiB instead of 8).  Rows of scales lie one
+// after the other: 32 of them 8 CS bytes apart conflict (cycles of it an LDS instruction of any kind: CS = 8 2.9, 4 1.2, 2 0.4).
 // Scales: two buffers of CS steps, 8 CS bytes of a row at once, since a load of a row's 8 bytes takes a whole line's time
 // and, from HBM, a whole line.  A step is four substeps of one MFMA per fragment pair.  While a substep's MFMAs run, the
 // next one's fragments are read (one ds_read_b128 each); the barrier sits before the last substep, when every wavefront

@@ -170,8 +170,9 @@ enum MxTile { MX_256 = 0, MX_256_LONG, MX_32x32, MX_32x128, MX_64x64, MX_128x128
 // The tile of an MXFP4 product of M rows, dense (experts = 0) or over `experts` experts, by estimated time in us: a start,
 // the K steps of 256 channels times what a step of all tiles takes (or reading the weights, if that takes longer), and a
 // share of the weights' MB.  Least-squares fits over 374 sizes (1 - 8192 rows, N 128 - 28672, K 512 - 8192; 8 - 256
-// experts with 1 - 16384 rows between them; cold weights, each tile forced in turn), within a fifth; the picks take 1.2 %
-// (dense) and 2.3 % (experts) more than the best tile.  Measured, us: 1 x 4096 x 4096 5.8 (32 x 32; 64 x 64 7.4), 16 x
+// experts with 1 - 16384 rows between them; cold weights, each tile forced in turn), the deep tiles' over another 70, within a
+// fifth.  Over profiles/mxfp4_tiles.txt (all tiles as they are, 374 sizes) the picks take 2.2 % (dense) and 1.5 % (experts) more
+// than the best tile on average, more than 10 % at 30 sizes; the worst is 192 x 1408 x 8192, 32 x 32 20.8 for 64 x 64 11.7.  Measured, us: 1 x 4096 x 4096 5.8 (32 x 32; 64 x 64 7.4), 16 x
 // 11008 x 4096 8.9 (64 x 64; 32 x 32 11.4), 512 x 11008 x 4096 29 (128 x 128; 64 x 64 42, 256 x 256 37), 8192 x 8192 x
 // 8192 270 (256 x 256; 128 x 128 337); 64 experts, top 8, N 2816, K 4096: 32 tokens 70 (32 x 128; 64 x 64 75, 32 x 32
 // 86), 512 tokens 106 (256 x 256; 32 x 128 128), 4096 tokens 290 (256 x 256; 128 x 128 329).
@@ -196,6 +197,7 @@ inline MxTile pick_mx_tile(int64_t M, int64_t N, int64_t K, int64_t experts) {
   constexpr MxCost s128[2] = {{3.8, 0.61, 0.45, 1.18, 0.71, 0.39, 4.8, 0.052}, {7.1, 0.78, 0.19, 1.23, 1.17, 0.18, 7.3, 0.0}};
   constexpr MxCost s256[2] = {{9.2, 1.10, 1.02, 3.39, 2.27, 0.94, 3.0, 0.024}, {9.4, 1.11, 0.80, 3.63, 3.41, 0.0, 4.6, 0.0}};
   constexpr MxCost deep[2] = {{5.0, 0.355, 0.30, 0.0, 0.0, 0.0, 6.0, 0.0}, {6.3, 0.33, 0.27, 0.0, 0.0, 0.0, 7.5, 0.06}};
+  // fitted to dense products; experts' go by it too
   constexpr MxCost s256x128{7.2, 0.55, 0.56, 0.0, 0.0, 0.0, 6.0, 0.03};
   constexpr MxCost s32x128{4.8, 0.33, 0.08, 0.65, 0.51, 0.06, 9.0, 0.091};
   MxTile best = MX_128x128;
