@@ -1,8 +1,9 @@
-"""Expert layers on the GPU: the steps between the products, and references in graphs."""
+"""Expert layers on the GPU: the steps between the products, references in graphs, a checkpoint's weights."""
 import pytest
 import torch
 
 from tilebench_amd import experts
+from tilebench_amd import formats as F
 from tilebench_amd.benchmarks.experts.mxfp4_dequant import impl_torch as dequant_ref
 from tilebench_amd.benchmarks.experts.mxfp4_gemm import impl_torch as gemm_ref
 from tilebench_amd.benchmarks.experts.mxfp4_quant import impl_torch as quant_ref
@@ -62,3 +63,18 @@ def test_references_are_captured(gpu, op):
         torch.cuda.synchronize()
         assert torch.equal(out, want)
         assert torch.equal(ref.run(*args), want)
+
+
+@pytest.mark.parametrize("shape", [(40, 2912), (3, 24, 736)])
+def test_a_checkpoints_weights_are_laid_out_where_they_are_used(gpu, shape):
+    """Rows of scales keep their padding on the GPU, and a product with them is the one with the dense scales."""
+    from tilebench_amd.benchmarks.experts.mxfp4_gemm import impl_hip
+
+    say("checkpoint", shape)
+    codes, scales = quant_ref.run(torch.randn(shape, generator=gen(1)))
+    w = F.mxfp4_checkpoint_to_tb(codes, scales, "cuda")
+    assert experts.scale_rows(w.scales)[0] is w.scales and experts.code_rows(w.codes) is w.codes
+    assert torch.equal(w.scales.cpu(), scales) and torch.equal(w.codes.cpu(), codes)
+    a = matrix(9, shape[-1], 2)
+    last = lambda c, s: (c, s) if len(shape) == 2 else (c[-1], s[-1])
+    assert torch.equal(impl_hip.run(*a, *last(w.codes, w.scales)), impl_hip.run(*a, *last(codes.cuda(), scales.cuda())))

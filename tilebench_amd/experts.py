@@ -6,7 +6,8 @@ An MXFP4 matrix [.., K] is a pair of uint8 tensors: codes [.., K / 2], channel
 powers of two 2^(scale - 127) of 32 channels each (255: NaN).  A value is its
 code times its scale.  mxfp4_quant makes such pairs; it pads rows of scales to
 16 bytes, so that scales whose K / 32 is no multiple of 4 are a view that the
-products take without a copy.
+products take without a copy (moved to another device they become dense:
+formats.mxfp4_checkpoint_to_tb lays weights out where they are used).
 """
 from __future__ import annotations
 

@@ -329,15 +329,18 @@ def fp8_checkpoint_to_tb(weight: torch.Tensor, weight_scale: torch.Tensor | floa
     return Fp8Weights(codes.contiguous(), s.contiguous().to(torch.float32))
 
 
-def mxfp4_checkpoint_to_tb(codes: torch.Tensor, scales: torch.Tensor) -> Mxfp4Weights:
+def mxfp4_checkpoint_to_tb(codes: torch.Tensor, scales: torch.Tensor, device=None) -> Mxfp4Weights:
     """A layer's or its experts' MXFP4 weights in the layout that the products take without a copy.
 
     codes: e2m1 pairs [N, K/2] or [E, N, K/2], or in blocks [.., K/32, 16] (one dimension more than scales); scales E8M0
-    [.., K/32].  uint8, or torch's types of these bytes.  Tensors that already lie so are passed on."""
+    [.., K/32].  uint8, or torch's types of these bytes.  Tensors that already lie so are passed on.  device: where the
+    weights are used, if elsewhere; they are laid out there, since moving padded rows of scales makes them dense."""
     from tilebench_amd import experts
 
     bytes_of = {getattr(torch, name) for name in ("float4_e2m1fn_x2", "float8_e8m0fnu") if hasattr(torch, name)}
     codes, scales = (t.view(torch.uint8) if t.dtype in bytes_of else t for t in (codes, scales))
+    if device is not None:
+        codes, scales = codes.to(device), scales.to(device)
     if codes.dim() == scales.dim() + 1 and codes.shape[-1] == 16:
         codes = codes.flatten(-2)
     if codes.dim() not in (2, 3):
